@@ -348,6 +348,90 @@ typedef struct tp_grow {
  * src and dst must not overlap. */
 int32_t tp_grow_rows(const tp_grow* bufs, int32_t n_bufs, int64_t rows, void* stream);
 
+/* ---- Serving operators around a cache.  No counterpart in the reference, which leaves a prompt
+ * to the model's own attention and keeps one line of tokens per cache. ---- */
+
+/*
+ * Attention over a whole prompt, causal or not, with grouped query heads:
+ * out[b][h][i] = sum_j p_ij v[b][h / (hq / hkv)][j], p_ij = softmax_j(scale q_i . k_j).
+ * q, out: [batch][hq][tq][128], k, v: [batch][hkv][tk][128], all of dtype 0 (fp16)
+ * or 1 (bf16), 16-byte aligned, the 128 dimensions contiguous; strides: 12 host
+ * values, the (batch, head, token) strides of q, k, v and out in elements, each a
+ * multiple of 8 (0 reads one row for all; out's rows must not overlap).
+ * causal: the queries are the last tq of the tk positions, query i sees keys 0 ..
+ * tk - tq + i.  A query that sees no key gives 0.  Infinities and NaN in keys and
+ * values that a query does not see do not reach it.
+ * n_seq > 0 (batch 1): packed sequences; q_starts and k_starts are device arrays of
+ * n_seq + 1 ascending token positions, the first 0, sequence s being queries
+ * [q_starts[s], q_starts[s + 1]) over keys [k_starts[s], k_starts[s + 1]).  Queries
+ * behind the last sequence give 0, or are left as they are with keep_rest.  Starts
+ * out of range or order give unspecified rows, within the buffers.
+ * workspace: tp_prompt_workspace_bytes(...) bytes, 256-byte aligned (none needed
+ * where that is 0), of any content; calls that share it must not run concurrently.
+ * Sums and softmax statistics are fp32; the weights are rounded to dtype between
+ * the products.
+ */
+int32_t tp_prompt_attention(const void* q, const void* k, const void* v, void* out, int32_t dtype, int64_t batch,
+                            int32_t hq, int32_t hkv, int64_t tq, int64_t tk, const int64_t* strides, int32_t causal,
+                            const int32_t* q_starts, const int32_t* k_starts, int32_t n_seq, int32_t keep_rest,
+                            float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t tp_prompt_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int64_t tq, int64_t tk, int32_t n_seq);
+
+/*
+ * Attention of a tree of `nodes` (1..256) drafted tokens over a cache: node i
+ * attends every stored page, the dense tail and the drafted tokens j whose bit is set
+ * in its mask row.  q, out: fp16 [batch][hq][nodes][128]; draft_k, draft_v: fp16
+ * [batch][hkv][nodes][128]; strides: 12 host values, (batch, head, token) of q,
+ * draft_k, draft_v and out, as for tp_prompt_attention.
+ * mask: device uint64 [nodes][ceil(nodes / 64)], bit j % 64 of word j / 64 of row i;
+ * mask_stride: words between the masks of two batch rows (0: one for all).  A node
+ * whose own bit is clear is padding and gives 0.
+ * pages, tail_k, tail_v, tail_len, tail_stride as for tp_decode_attention, all of them
+ * attended; workspace (tp_tree_workspace_bytes) as for tp_prompt_attention.
+ */
+int32_t tp_tree_attention(const void* q, void* out, int64_t batch, int32_t hq, int32_t hkv, int32_t nodes,
+                          const tp_page_layout* layout, const tp_pages* pages, int32_t n_pages, const void* tail_k,
+                          const void* tail_v, int32_t tail_len, int64_t tail_stride, const void* draft_k,
+                          const void* draft_v, const int64_t* strides, const uint64_t* mask, int64_t mask_stride,
+                          float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t tp_tree_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t nodes, int32_t n_pages);
+
+/* One buffer of tp_copy_pages: pages of page_bytes bytes in [row][capacity] slots. */
+typedef struct tp_page_copy {
+  const void* src;
+  void* dst;
+  int64_t page_bytes;
+} tp_page_copy;
+
+/*
+ * Pages of a store copied into another one, one launch: slot s < keep of batch row i
+ * and head h of every buffer becomes stored page page_index[s] (NULL: s) of row rows[i]
+ * (NULL: i) and head h; slots [keep, dst_capacity) are zeroed.  rows and page_index are
+ * device arrays, their entries clamped to [0, batch_in) and [0, n_stored).  tail_bytes
+ * (a multiple of 16, 0 for none) of each row of the tails, rows tail_row bytes apart, go
+ * along.  Sources and destinations must not overlap.
+ */
+int32_t tp_copy_pages(const tp_page_copy* bufs, int32_t n_bufs, int64_t batch, int32_t heads, int64_t batch_in,
+                      const int32_t* rows, int64_t src_capacity, int64_t dst_capacity, int32_t n_stored,
+                      const int32_t* page_index, int32_t keep, const void* tail_k, const void* tail_v,
+                      void* tail_k_out, void* tail_v_out, int64_t tail_bytes, int64_t tail_row, void* stream);
+
+/*
+ * Tokens index[0 .. n) (a host array; with per_batch one run of n for each batch row;
+ * at most 1024 entries, each in [0, tokens)) of k and v [batch][heads][tokens][128] of
+ * in_dtype (0 fp16, 1 fp32) into rows [out_pos, out_pos + n) of out_k and out_v
+ * [batch][heads][out_tokens][128]; strides: 6 host values, (batch, head, token) of k and
+ * v in elements, multiples of 16 bytes.  check 2: waits for the verdict as
+ * tp_append_stage does, TP_ERR_NONFINITE if a taken value is not finite (k and v are no
+ * longer read then); check 0: returns after the launch.
+ */
+int32_t tp_take_tokens(const void* k, const void* v, int32_t in_dtype, int64_t batch, int32_t heads, int64_t tokens,
+                       const int64_t* strides, const int32_t* index, int32_t n, int32_t per_batch, void* out_k,
+                       void* out_v, int64_t out_tokens, int64_t out_pos, int32_t check, uint32_t* flag, uint32_t epoch,
+                       void* stream);
+
 /* ---- QJL (rejected by TurboPolarConfig, turbo_polar_config.py:46-47, as in
  * the reference; these serve the bridge-level QJL calls the reference's own
  * tests make). ---- */

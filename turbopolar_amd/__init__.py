@@ -9,12 +9,14 @@ behind the C ABI of ``include/turbopolar.h`` (``libturbopolar_hip.so``).
 from .bridge import HipKernelBridge
 from .codecs import GroupedVQuantizer, PolarQuantDecoder, PolarQuantEncoder
 from .config import TurboPolarConfig
+from .draft import DraftTree
 from .fast_attention import TurboPolarFastCache, make_turbo_caches
 from .payload import PolarKeyBlock, QuantizedVBlock
 from .runtime import TurboPolarKVCacheRuntime
 from .storage import PolarKBlockStorage, QuantVBlockStorage
 
 __all__ = [
+    "DraftTree",
     "GroupedVQuantizer",
     "HipKernelBridge",
     "PolarKBlockStorage",

@@ -76,6 +76,12 @@ class TPGrow(ctypes.Structure):
     ]
 
 
+class TPPageCopy(ctypes.Structure):
+    """tp_page_copy: one buffer of tp_copy_pages."""
+
+    _fields_ = [("src", c_vp), ("dst", c_vp), ("page_bytes", c_i64)]
+
+
 class TPBoundsCase(ctypes.Structure):
     """tp_bounds_case: one launch shape for tp_selftest_decode_bounds."""
 
@@ -108,6 +114,7 @@ class TurboPolarHipError(RuntimeError):
 _P_LAYOUT = ctypes.POINTER(TPPageLayout)
 _P_PAGES = ctypes.POINTER(TPPages)
 _P_QJL = ctypes.POINTER(TPQjl)
+_P_STRIDES = ctypes.POINTER(c_i64)
 
 _SIGNATURES = {
     "tp_last_error": (ctypes.c_char_p, []),
@@ -157,6 +164,36 @@ _SIGNATURES = {
         [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp, ctypes.c_uint32, c_vp],
     ),
     "tp_grow_rows": (c_i32, [ctypes.POINTER(TPGrow), c_i32, c_i64, c_vp]),
+    "tp_prompt_attention": (
+        c_i32,
+        [
+            c_vp, c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_i64, c_i64, _P_STRIDES, c_i32, c_vp, c_vp, c_i32,
+            c_i32, c_float, c_vp, c_size, c_vp,
+        ],
+    ),
+    "tp_prompt_workspace_bytes": (c_size, [c_i64, c_i32, c_i32, c_i64, c_i64, c_i32]),
+    "tp_tree_attention": (
+        c_i32,
+        [
+            c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, _P_LAYOUT, _P_PAGES, c_i32, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp,
+            _P_STRIDES, c_vp, c_i64, c_float, c_vp, c_size, c_vp,
+        ],
+    ),
+    "tp_tree_workspace_bytes": (c_size, [c_i64, c_i32, c_i32, c_i32, c_i32]),
+    "tp_copy_pages": (
+        c_i32,
+        [
+            ctypes.POINTER(TPPageCopy), c_i32, c_i64, c_i32, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp, c_i32,
+            c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp,
+        ],
+    ),
+    "tp_take_tokens": (
+        c_i32,
+        [
+            c_vp, c_vp, c_i32, c_i64, c_i32, c_i64, _P_STRIDES, ctypes.POINTER(c_i32), c_i32, c_i32, c_vp, c_vp, c_i64,
+            c_i64, c_i32, c_vp, ctypes.c_uint32, c_vp,
+        ],
+    ),
     "tp_fused_qk_qjl": (c_i32, [c_vp, c_i64, c_i32, c_i32, _P_LAYOUT, _P_PAGES, c_i32, _P_QJL, c_float, c_vp, c_vp]),
     "tp_decode_attention_qjl": (
         c_i32,

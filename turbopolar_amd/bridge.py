@@ -10,6 +10,11 @@ rfsn_v11/kernels/turbo_polar/metal.py:57-792 for the supported path:
 
 * ``execute_fused_qk_qjl(q, block, qjl_payload, q_proj_signs, config)`` (metal.py:532-571)
 
+and, with no counterpart there, attention of a whole prompt and of a drafted tree:
+
+* ``execute_prompt_attention(q, k, v, config, ...) -> (out, trace)``
+* ``execute_tree_attention_quant_v_dense_tail(...) -> (out, trace)``
+
 Differences: there is no silent CPU fallback (unsupported inputs raise), and
 the trace reports ``hip_used`` where the reference reports ``metal_used``.
 ``use_qjl=True`` adds the QJL correction to the page tokens' scores
@@ -25,7 +30,11 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels import PageSet, decode_attention, decode_attention_dense_v, fp16_scale, fused_qk
+from .draft import DraftTree
+from .kernels import (
+    PageSet, _DEFAULT_LAYOUT, decode_attention, decode_attention_dense_v, fp16_scale, fused_qk, prompt_attention,
+    tree_attention,
+)
 from .payload import PolarKeyBlock, QuantizedVBlock, layout_from_metadata
 from .qjl import QJLPages
 
@@ -201,5 +210,74 @@ class HipKernelBridge:
             "tail_length": tail_len,
             "actual_seq_len": actual_seq_len,
             "num_queries_per_kv": q.shape[1] // hkv,
+        }
+        return out, trace
+
+    def execute_prompt_attention(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        config,
+        causal: bool = True,
+        q_starts=None,
+        k_starts=None,
+        out: Optional[torch.Tensor] = None,
+    ) -> Tuple[torch.Tensor, Dict[str, Any]]:
+        """Attention of a whole prompt over dense keys and values (``kernels.prompt_attention``):
+        grouped heads, causal or not, packed sequences."""
+        out = prompt_attention(q, k, v, fp16_scale(config.attention_scale), causal, q_starts, k_starts, out)
+        trace = {
+            "kernel_name": "prompt_attention",
+            "hip_kernel": "tp_prompt_attention",
+            "hip_used": True,
+            "fallback_used": False,
+            "causal": bool(causal),
+            "packed": q_starts is not None,
+            "num_queries_per_kv": q.shape[1] // k.shape[1],
+        }
+        return out, trace
+
+    def execute_tree_attention_quant_v_dense_tail(
+        self,
+        q: torch.Tensor,
+        block: Optional[PolarKeyBlock],
+        quant_v: Optional[QuantizedVBlock],
+        tail_k: Optional[torch.Tensor],
+        tail_v: Optional[torch.Tensor],
+        draft_k: torch.Tensor,
+        draft_v: torch.Tensor,
+        tree: DraftTree,
+        config,
+    ) -> Tuple[torch.Tensor, Dict[str, Any]]:
+        """Attention of a tree of drafted tokens over compressed pages and a dense tail
+        (``kernels.tree_attention``); ``block`` and ``quant_v`` None without pages, the tail None or
+        empty without one."""
+        pages = None
+        if block is not None:
+            self._supports_block(block)
+            pages = _pages_of(block, quant_v, config.head_dim)
+            if (pages.B, pages.H) != (q.shape[0], draft_k.shape[1]):
+                raise ValueError(f"pages of {pages.B} x {pages.H} (batch, heads) do not match q {tuple(q.shape)} and "
+                                 f"the draft {tuple(draft_k.shape)}")
+            if pages.tensors["radii"].device != q.device:
+                raise ValueError(f"q is on {q.device}, the pages on {pages.tensors['radii'].device}")
+        tail_len = int(tail_k.shape[2]) if tail_k is not None else 0
+        if tail_len and (tail_k.device != q.device or tail_v.device != q.device):
+            raise ValueError(f"q is on {q.device}, the tail on {tail_k.device}")
+        out = tree_attention(
+            q, pages.layout if pages is not None else _DEFAULT_LAYOUT, pages.pages if pages is not None else None,
+            pages.S if pages is not None else 0, tail_k if tail_len else None, tail_v if tail_len else None, draft_k,
+            draft_v, tree, fp16_scale(config.attention_scale),
+        )
+        trace = {
+            "kernel_name": "tree_attention_quant_v_dense_tail",
+            "hip_kernel": "tp_tree_attention",
+            "hip_used": True,
+            "fallback_used": False,
+            "quant_v_used": True,
+            "tail_length": tail_len,
+            "nodes": tree.nodes,
+            "num_queries_per_kv": q.shape[1] // draft_k.shape[1],
         }
         return out, trace

@@ -27,7 +27,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 TIMELINE_LIB_PATH = PKG_DIR / "libturbopolar_hip_timeline.so"
 ARCH = os.environ.get("TP_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = ["tp_api.hip", "tp_encode.hip", "tp_attention.hip", "tp_decode.hip", "tp_append.hip", "tp_qjl.hip"]
+SOURCES = ["tp_api.hip", "tp_encode.hip", "tp_attention.hip", "tp_decode.hip", "tp_append.hip", "tp_qjl.hip",
+           "tp_prompt.hip", "tp_tree.hip", "tp_pages.hip"]
 MEASURE_SOURCES = ["tp_measure.hip"]  # measurement library only
 
 # -ffp-contract=off and correctly rounded fp32 divide/sqrt are required for the
@@ -61,7 +62,7 @@ def _hipcc() -> str:
 # 51.10 us, paired); the decoded code angle keeps the reference's separate
 # roundings by its own pragma (code_angle, tp_common.h).  Every other source
 # stays uncontracted for the encoder's and the page decoder's bit-exact rules.
-SOURCE_FLAGS = {"tp_attention.hip": ["-ffp-contract=fast-honor-pragmas"]}
+SOURCE_FLAGS = {name: ["-ffp-contract=fast-honor-pragmas"] for name in ("tp_attention.hip", "tp_prompt.hip", "tp_tree.hip")}
 
 
 def _compile(src: Path, obj: Path, defines=()) -> None:

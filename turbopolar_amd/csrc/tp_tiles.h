@@ -1,0 +1,280 @@
+// tp_tiles.h -- attention over 64-token tiles of keys and values in LDS.
+//
+// Shared by the prompt kernel (tp_prompt.hip, dense keys) and the drafted-tree
+// kernel (tp_tree.hip, decoded pages).  A wave owns 32 query rows; both products
+// run on v_mfma_f32_32x32x16 with the rows as columns:
+//   S^T[t][r] = sum_d K[t][d] Q[r][d]      (A = keys, B = queries)
+//   O^T[d][r] += sum_t V[t][d] P[r][t]     (A = values, B = weights)
+// so a lane's column is one query row from end to end: its maximum, sum and
+// rescaling are plain registers, and one swap of the wave's halves per tile joins
+// the two lanes of a row.  The accumulator of S^T holds tokens
+//   32 nb + 8 (i / 4) + 4 h + i % 4   (register i of block nb, half h = lane / 32),
+// and the second product takes its sum over tokens in that very order, so the
+// weights go from one product to the other without leaving their lane: values are
+// read from LDS by the transposing read (4 tokens of one dimension a lane) at the
+// same tokens.
+//
+// Tiles lie in LDS as rows of 256 bytes, 16-byte chunk c of row t at chunk c ^
+// tile_swizzle(t): the 8 lanes that read 16 bytes of 8 key rows together, and the 16
+// that read a 4-token by 16-dimension block of values, hit all banks once.
+#pragma once
+
+#include "tp_common.h"
+
+namespace tp {
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+
+constexpr int kTileTokens = 64;
+constexpr int kTileBytes = kTileTokens * kHeadDim * 2;
+constexpr int kWaveRows = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__host__ __device__ inline int tile_swizzle(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
+// Byte offset of 16-byte chunk c of token t.
+__host__ __device__ inline int tile_at(int t, int c) { return t * (kHeadDim * 2) + ((c ^ tile_swizzle(t)) << 4); }
+
+// Element types: the product and the rounding of a pair of weights (to nearest: the
+// weights are at most 1, so an output's rounding error stays below half a step of
+// the type relative to the largest value).
+struct F16 {
+  typedef half8v frag;
+  static __device__ __forceinline__ float16v mfma(uint4v a, uint4v b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0,
+                                                  0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{x, y}, half2v));
+  }
+  static constexpr uint32_t kExponent = 0x7c00u;
+};
+struct BF16 {
+  static __device__ __forceinline__ float16v mfma(uint4v a, uint4v b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{x, y}, bf16x2));
+  }
+  static constexpr uint32_t kExponent = 0x7f80u;
+};
+
+// Whether any of the pair's two 16-bit values is infinite or NaN.
+template <class T>
+__device__ __forceinline__ bool pair_nonfinite(uint32_t w) {
+  return (w & T::kExponent) == T::kExponent || (w & (T::kExponent << 16)) == (T::kExponent << 16);
+}
+template <class T>
+__device__ __forceinline__ uint32_t pair_finite(uint32_t w) {  // those set to 0
+  if ((w & T::kExponent) == T::kExponent) w &= 0xffff0000u;
+  if ((w & (T::kExponent << 16)) == (T::kExponent << 16)) w &= 0xffffu;
+  return w;
+}
+template <class T>
+__device__ __forceinline__ float from_bits(uint16_t b);
+template <>
+__device__ __forceinline__ float from_bits<F16>(uint16_t b) {
+  return h2f(b);
+}
+template <>
+__device__ __forceinline__ float from_bits<BF16>(uint16_t b) {
+  return __uint_as_float((uint32_t)b << 16);
+}
+
+__device__ __forceinline__ uint4v lds_read16(const char* p) { return *reinterpret_cast<const uint4v*>(p); }
+
+// 4 tokens of one dimension: lane l gets, of the four rows that lanes 4 j + (l % 16) / 4
+// of its 16 address, element l % 4.
+__device__ __forceinline__ uint2v lds_read_tr(const char* p) {
+  typedef __attribute__((address_space(3))) short4v* lds_ptr;
+  const short4v r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+  return __builtin_bit_cast(uint2v, r);
+}
+
+// The two lanes of a row, combined in both.
+template <class Op>
+__device__ __forceinline__ float across_halves(float x, Op op) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
+struct RowState {
+  float16v o[4];  // O^T, dimensions 32 db + 8 (i / 4) + 4 h + i % 4
+  float m;        // running maximum of scale * score, in log2 units
+  float l;        // this lane's part of the sum of the weights
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+  }
+};
+
+// A wave's lane offsets into a tile.
+struct TileLane {
+  int k;  // key row lane % 32, chunk h
+  int v;  // value rows of the transposing read, dimension block 0
+  __device__ __forceinline__ explicit TileLane(int lane) {
+    const int h = lane >> 5;
+    k = tile_at(lane & 31, h);
+    const int row = 4 * h + ((lane >> 2) & 3);
+    v = tile_at(row, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+  }
+};
+
+// The queries of a row as the B operand: q[ks] holds dimensions 16 ks + 8 h .. + 7.
+__device__ __forceinline__ void load_query(const uint16_t* row, bool live, uint32_t flip, int lane, uint4v* q) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    uint4v w = {0u, 0u, 0u, 0u};
+    if (live) w = *reinterpret_cast<const uint4v*>(row + 16 * ks + 8 * (lane >> 5));
+    q[ks] = w ^ flip;
+  }
+}
+
+// One pass over NB blocks of 32 tokens from token t0 of a tile: scores, running maximum
+// and sum, weights, values.  seen(token): whether the lane's row sees a token of the
+// tile (asked where MASKED only).  c: scale * log2(e), positive.
+template <class T, int NB, bool MASKED, class Seen>
+__device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int t0, const TileLane& at, const uint4v* q,
+                                            float c, RowState& st, int lane, Seen seen) {
+  float16v s[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[nb][i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      const int off = (at.k ^ (32 * (ks & 3))) + 128 * (ks >> 2) + (t0 + 32 * nb) * (kHeadDim * 2);
+      s[nb] = T::mfma(lds_read16(kt + off), q[ks], s[nb]);
+    }
+  }
+  if constexpr (MASKED) {
+    const int h4 = 4 * (lane >> 5);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!seen(t0 + 32 * nb + 8 * (i >> 2) + (i & 3) + h4)) s[nb][i] = -INFINITY;
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
+  top = across_halves(top, [](float x, float y) { return fmaxf(x, y); });
+  const float m = fmaxf(st.m, top * c);
+  const float base = m == -INFINITY ? 0.0f : m;  // a row that has seen nothing yet
+  const float alpha = __builtin_amdgcn_exp2f(st.m - base);
+  float sum = 0.0f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][i], c, -base));
+      sum += s[nb][i];
+    }
+  st.m = m;
+  st.l = st.l * alpha + sum;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint4v p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = T::pack(s[nb][8 * kk + 2 * j], s[nb][8 * kk + 2 * j + 1]);
+      const int row = (t0 + 32 * nb + 16 * kk) * (kHeadDim * 2);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const char* a = vt + (at.v ^ (64 * (db & 1))) + 128 * (db >> 1) + row;
+        const uint2v lo = lds_read_tr(a), hi = lds_read_tr(a + 8 * kHeadDim * 2);
+        st.o[db] = T::mfma(uint4v{lo.x, lo.y, hi.x, hi.y}, p, st.o[db]);
+      }
+    }
+}
+
+// Infinities and NaN among the values of a tile that some rows do not see: a product
+// with a weight of 0 would carry them into those rows, so the tile holds 0 in their
+// place, and the rows that do see the token take the value itself (a positive weight
+// leaves an infinity or NaN what it is).  row(t): the token's values.
+template <class T, class Seen, class Row>
+__device__ __forceinline__ void add_nonfinite(RowState& st, int lane, int tokens, Seen seen, Row row) {
+  for (int t = 0; t < tokens; ++t) {
+    if (!seen(t)) continue;
+    const uint16_t* v = row(t) + 4 * (lane >> 5);
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint16_t x = v[32 * db + 8 * (i >> 2) + (i & 3)];
+        if ((x & T::kExponent) == T::kExponent) st.o[db][i] += from_bits<T>(x);
+      }
+  }
+}
+
+// The row's result, divided by its sum: 16 bytes a store (the halves of a row hold
+// every other four dimensions; one swap gives each lane 8 in a row).
+template <class T>
+__device__ __forceinline__ void store_row(const RowState& st, float inv, uint16_t* row, bool live, int lane) {
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = T::pack(st.o[db][8 * a + 2 * j] * inv, st.o[db][8 * a + 2 * j + 1] * inv);
+        const uint32_t y = T::pack(st.o[db][8 * a + 4 + 2 * j] * inv, st.o[db][8 * a + 5 + 2 * j] * inv);
+        const auto p = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        w[j] = p[0];
+        w[2 + j] = p[1];
+      }
+      if (live)
+        *reinterpret_cast<uint4v*>(row + 32 * db + 16 * a + 8 * (lane >> 5)) = uint4v{w[0], w[1], w[2], w[3]};
+    }
+}
+
+// A split's record of a row: its output divided by its sum, in fp32, with the maximum
+// (log2 units) and the sum.  Splits of a row are joined by join_splits_kernel.
+__device__ __forceinline__ void store_record(const RowState& st, float l, float* o, float* ml, bool live, int lane) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (!live) return;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const float4v x = {st.o[db][4 * a] * inv, st.o[db][4 * a + 1] * inv, st.o[db][4 * a + 2] * inv,
+                         st.o[db][4 * a + 3] * inv};
+      *reinterpret_cast<float4v*>(o + 32 * db + 8 * a + 4 * (lane >> 5)) = x;
+    }
+  if (lane < 32) *reinterpret_cast<float2v*>(ml) = float2v{st.m, l};
+}
+
+// Where the splits' records are and where the joined rows go.  Rows are counted as
+// (token, head of the group) per unit = (batch, kv head).
+struct JoinArgs {
+  const float* o;   // [units][rows][splits][128]
+  const float* ml;  // [units][rows][splits][2]
+  uint16_t* out;
+  int64_t rows;     // per unit
+  int64_t out_b, out_h, out_t;
+  int32_t units, splits, g, hkv;
+  const int32_t* rest_from;  // tokens from *rest_from on are left as they are (NULL: none)
+};
+
+int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s);
+
+}  // namespace tp

@@ -1,0 +1,479 @@
+// tp_tree.hip -- attention of a tree of drafted tokens over a compressed cache.
+//
+//   out[b, h, i] = sum_j p_ij v_j,  p_ij = softmax_j(scale q[b, h, i] . k_j)
+//
+// over every stored page (decoded: k = r (cos a, sin a), v = code x scale), the dense tail, and
+// of the drafted tokens node i itself and its ancestors.  A node that does not see itself is
+// padding: its row is 0.
+//
+// The rows of a workgroup are (node, head of the group) pairs of one kv head, so a page is
+// read and decoded once for up to 256 rows: its codes go through registers into an fp16 tile in
+// LDS (the next page's codes in flight meanwhile), from which the waves multiply.  The cache is
+// split over workgroups, the tail and the drafts go to one of their own, and a second launch
+// joins their records.
+#include <algorithm>
+
+#include "tp_codes.h"
+#include "tp_tiles.h"
+
+namespace tp {
+
+enum TreeKind { kTreeDefault = 0, kTreeFast = 1, kTreeAnyF16 = 2, kTreeAnyI8 = 3 };
+constexpr bool tree_i8(int kind) { return kind == kTreeFast || kind == kTreeAnyI8; }
+constexpr bool tree_any(int kind) { return kind == kTreeAnyF16 || kind == kTreeAnyI8; }
+
+constexpr int kTreeMaxNodes = 256;
+constexpr int kTreeTarget = 512;  // workgroups that fill the GPU, two a CU
+
+struct TreeArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_b, q_h, q_t, out_b, out_h, out_t;
+  int32_t units, hkv, g, nodes, row_blocks;
+  const void* radii;
+  const uint16_t* radii_scales;
+  const uint8_t* angle_l1;
+  const uint8_t* angle_deep;
+  const int8_t* v_codes;
+  const uint16_t* v_scales;
+  int64_t capacity;
+  int32_t n_pages, l1_bits, deep_bits, split_half, l1_row, deep_row;
+  const uint16_t* tail_k;
+  const uint16_t* tail_v;
+  int64_t tail_stride;  // tokens
+  int32_t tail_len;
+  const uint16_t* draft_k;
+  const uint16_t* draft_v;
+  int64_t dk_b, dk_h, dk_t, dv_b, dv_h, dv_t;
+  const uint64_t* mask;  // [batch or 1][nodes][words]: bit j of node i: i sees drafted token j
+  int64_t mask_b;        // words between batch rows (0: one mask for all)
+  int32_t words;
+  float c;
+  uint32_t flip;
+  int32_t pages_per_split, page_splits, records;
+  float* part_o;
+  float* part_ml;
+};
+
+// The codes of one thread's part of a page: N runs of 8 pairs (16 dimensions) of a token,
+// threads 8 to a token.
+template <int KIND, int N>
+struct PageRegs {
+  uint4v r[tree_i8(KIND) ? 1 : N];  // fp16 radii
+  uint2v r8[tree_i8(KIND) ? N : 1];
+  uint2v c8[KIND == kTreeFast ? N : 1];
+  uint32_t c4[KIND == kTreeDefault ? N : 1];
+  uint4v v[N];
+  uint16_t vs[N];
+  uint16_t ls;
+};
+
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void load_page(const TreeArgs& a, int64_t slot, int tid, PageRegs<KIND, N>& p) {
+  const int c = tid & 7;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int64_t row = slot * kPageTokens + (tid >> 3) + (THREADS / 8) * n;
+    if constexpr (tree_i8(KIND))
+      p.r8[n] = *reinterpret_cast<const uint2v*>(static_cast<const int8_t*>(a.radii) + row * kPairs + 8 * c);
+    else
+      p.r[n] = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(a.radii) + row * kPairs + 8 * c);
+    if constexpr (KIND == kTreeFast)
+      p.c8[n] = *reinterpret_cast<const uint2v*>(a.angle_deep + row * kPairs + 8 * c);
+    else if constexpr (KIND == kTreeDefault)
+      p.c4[n] = *reinterpret_cast<const uint32_t*>((c < 4 ? a.angle_l1 : a.angle_deep) + row * 16 + 4 * (c & 3));
+    p.v[n] = *reinterpret_cast<const uint4v*>(a.v_codes + row * kHeadDim + 16 * c);
+    p.vs[n] = a.v_scales[row * kVGroups + (c >> 1)];
+  }
+  if constexpr (tree_i8(KIND)) p.ls = a.radii_scales[slot];
+}
+
+struct TreeLut {
+  uint32_t code[512];  // (cos, sin) of the level-1 codes, then of the deep codes
+  uint2 pair[256];     // default layout: of both nibbles of a code byte
+};
+
+// Decodes them into a tile of keys and one of values.
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void decode_page(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
+                                            const PageRegs<KIND, N>& p, char* kt, char* vt) {
+  const int c = tid & 7;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int t = (tid >> 3) + (THREADS / 8) * n;
+    uint32_t e[8];
+    if constexpr (KIND == kTreeDefault) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 cs = lut.pair[(p.c4[n] >> (8 * i)) & 0xffu];
+        e[2 * i] = pack_h2(lo_lo(p.r[n][i]) * __builtin_bit_cast(half2v, cs.x));
+        e[2 * i + 1] = pack_h2(hi_hi(p.r[n][i]) * __builtin_bit_cast(half2v, cs.y));
+      }
+    } else {
+      const float ls = tree_i8(KIND) ? h2f(p.ls) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t code;
+        if constexpr (KIND == kTreeFast) {
+          code = 256 + ((p.c8[n][i >> 2] >> (8 * (i & 3))) & 0xffu);
+        } else {
+          const int pair = 8 * c + i;
+          const bool l1 = pair < a.split_half;
+          const int bits = l1 ? a.l1_bits : a.deep_bits;
+          const int bit = (l1 ? pair : pair - a.split_half) * bits;
+          const uint8_t* row = l1 ? a.angle_l1 + (slot * kPageTokens + t) * a.l1_row
+                                  : a.angle_deep + (slot * kPageTokens + t) * a.deep_row;
+          code = (l1 ? 0u : 256u) + ((row[bit >> 3] >> (bit & 7)) & ((1u << bits) - 1u));
+        }
+        half2v r;
+        if constexpr (tree_i8(KIND)) {
+          // code x scale is exact in fp32; r = exp(code x scale) rounded to fp16 once.
+          const int rc = (int)(int8_t)(p.r8[n][i >> 2] >> (8 * (i & 3)));
+          const f16 x = (f16)__builtin_amdgcn_exp2f((float)rc * (ls * kLog2e));
+          r = half2v{x, x};
+        } else {
+          const uint32_t w = p.r[n][i >> 1];
+          r = (i & 1) ? hi_hi(w) : lo_lo(w);
+        }
+        e[i] = pack_h2(r * __builtin_bit_cast(half2v, lut.code[code]));
+      }
+    }
+    *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c)) = uint4v{e[0], e[1], e[2], e[3]};
+    *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + 1)) = uint4v{e[4], e[5], e[6], e[7]};
+    const half2v scale = lo_lo(p.vs[n]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4v w;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        half2v lo, hi;
+        i8x4_to_f16(p.v[n][2 * i + j], lo, hi);
+        w[2 * j] = pack_h2(lo * scale);
+        w[2 * j + 1] = pack_h2(hi * scale);
+      }
+      *reinterpret_cast<uint4v*>(vt + tile_at(t, 2 * c + i)) = w;
+    }
+  }
+}
+
+// 64 dense tokens from k, v (t strides in elements) into the tiles; rows from `count` on are 0,
+// infinities and NaN among the values too, and reported.
+template <int THREADS>
+__device__ __forceinline__ bool dense_tile(const uint16_t* k, const uint16_t* v, int64_t k_t, int64_t v_t, int count,
+                                           int tid, char* kt, char* vt) {
+  bool flagged = false;
+#pragma unroll
+  for (int x = tid; x < kTileTokens * 16; x += THREADS) {
+    const int t = x >> 4, c = x & 15;
+    uint4v kw = {0u, 0u, 0u, 0u}, vw = kw;
+    if (t < count) {
+      kw = *reinterpret_cast<const uint4v*>(k + t * k_t + 8 * c);
+      vw = *reinterpret_cast<const uint4v*>(v + t * v_t + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      flagged = flagged || pair_nonfinite<F16>(vw[i]);
+      vw[i] = pair_finite<F16>(vw[i]);
+    }
+    *reinterpret_cast<uint4v*>(kt + tile_at(t, c)) = kw;
+    *reinterpret_cast<uint4v*>(vt + tile_at(t, c)) = vw;
+  }
+  return flagged;
+}
+
+// RW waves of 32 rows each; TW waves share a row block and take a page's tokens in TW parts.
+// At least four waves, so that enough threads load and decode.
+template <int RW, int TW>
+constexpr int kTreeThreads = 64 * (RW * TW < 4 ? 4 : RW * TW);
+
+template <int KIND, int RW, int TW>
+__global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kernel(TreeArgs a) {
+  constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW;
+  __shared__ __align__(16) char tiles[2][2][kTileBytes];
+  __shared__ TreeLut lut;
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units;
+  const int block = rest % a.row_blocks, record = rest / a.row_blocks;
+  const int64_t b = unit / a.hkv, kv = unit % a.hkv;
+  const int rw = wave / TW, tw = wave % TW;
+  const bool works = rw < RW;
+
+  const int row = (block * RW + rw) * kWaveRows + (lane & 31);
+  const int node = row / a.g, head = row - node * a.g;
+  const uint64_t* mask = a.mask + b * a.mask_b + (int64_t)node * a.words;
+  const bool live = works && node < a.nodes;
+  const bool real = live && ((mask[node >> 6] >> (node & 63)) & 1u);
+  uint4v q[8];
+  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + node * a.q_t, real, a.flip, lane, q);
+  const TileLane at(lane);
+  RowState st;
+  st.clear();
+
+  const int64_t slot0 = (int64_t)unit * a.capacity;
+  int page = record * a.pages_per_split;
+  const int page_end = record < a.page_splits ? min(page + a.pages_per_split, a.n_pages) : page;
+  if (tid == 0) flag = 0;
+  if (page < page_end) {
+    PageRegs<KIND, N> p;
+    load_page<KIND, N, THREADS>(a, slot0 + page, tid, p);
+    for (int x = tid; x < 256; x += THREADS) {
+      if constexpr (KIND == kTreeDefault) {
+        lut.pair[x] = make_uint2(make_cs(x & 15u, 4), make_cs(x >> 4, 4));
+      } else if constexpr (KIND == kTreeFast) {
+        lut.code[256 + x] = make_cs(x, 8);
+      } else {
+        if (x < (1 << a.l1_bits)) lut.code[x] = make_cs(x, a.l1_bits);
+        if (x < (1 << a.deep_bits)) lut.code[256 + x] = make_cs(x, a.deep_bits);
+      }
+    }
+    __syncthreads();
+    for (int buf = 0; page < page_end; ++page, buf ^= 1) {
+      decode_page<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, tiles[buf][0], tiles[buf][1]);
+      __syncthreads();
+      if (page + 1 < page_end) load_page<KIND, N, THREADS>(a, slot0 + page + 1, tid, p);
+      if (works)
+        attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, q, a.c, st, lane,
+                                    [](int) { return true; });
+    }
+  }
+  if (record == a.records - 1) {  // the tail and the drafts
+    const int first = a.tail_len > 0 ? -1 : 0;
+    for (int j = first; j < a.words; ++j) {
+      const uint16_t *k, *v;
+      int64_t k_t, v_t;
+      int count;
+      if (j < 0) {
+        k = a.tail_k + unit * a.tail_stride * kHeadDim, v = a.tail_v + unit * a.tail_stride * kHeadDim;
+        k_t = v_t = kHeadDim;
+        count = a.tail_len;
+      } else {
+        k = a.draft_k + b * a.dk_b + kv * a.dk_h + 64 * j * a.dk_t;
+        v = a.draft_v + b * a.dv_b + kv * a.dv_h + 64 * j * a.dv_t;
+        k_t = a.dk_t, v_t = a.dv_t;
+        count = min(a.nodes - 64 * j, kTileTokens);
+      }
+      __syncthreads();  // the tile before is read
+      if (dense_tile<THREADS>(k, v, k_t, v_t, count, tid, tiles[0][0], tiles[0][1])) flag = 1;
+      __syncthreads();
+      if (works) {
+        const uint64_t there = count < 64 ? (1ull << count) - 1ull : ~0ull;
+        const uint64_t sees = !real ? 0ull : j < 0 ? there : mask[j] & there;
+        auto seen = [&](int x) { return ((sees >> x) & 1u) != 0; };
+        attend_tile<F16, NB, true>(tiles[0][0], tiles[0][1], 32 * tw, at, q, a.c, st, lane, seen);
+        if (flag)
+          add_nonfinite<F16>(st, lane, count, [&](int x) { return seen(x) && (TW == 1 || (x >> 5) == tw); },
+                             [&](int x) { return v + x * v_t; });
+      }
+    }
+  }
+  if constexpr (TW == 2) {  // the second half's rows join the first's
+    __syncthreads();
+    float* side = reinterpret_cast<float*>(&tiles[0][0][0]) + rw * 66 * 64 + lane;
+    if (works && tw == 1) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) side[(16 * db + i) * 64] = st.o[db][i];
+      side[64 * 64] = st.m;
+      side[65 * 64] = st.l;
+    }
+    __syncthreads();
+    if (works && tw == 0) {
+      const float m1 = side[64 * 64], l1 = side[65 * 64];
+      const float m = fmaxf(st.m, m1), base = m == -INFINITY ? 0.0f : m;
+      const float w0 = __builtin_amdgcn_exp2f(st.m - base), w1 = __builtin_amdgcn_exp2f(m1 - base);
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[db][i] = st.o[db][i] * w0 + side[(16 * db + i) * 64] * w1;
+      st.l = st.l * w0 + l1 * w1;
+      st.m = m;
+    }
+  }
+  if (!works || tw != 0) return;
+  if (!real) st.clear();  // padding: its queries were 0, its page tokens seen
+  const float l = across_halves(st.l, [](float x, float y) { return x + y; });
+  if (a.records > 1) {
+    const int64_t rec = ((int64_t)unit * a.nodes * a.g + row) * a.records + record;
+    store_record(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
+  } else {
+    store_row<F16>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + node * a.out_t,
+                   live, lane);
+  }
+}
+
+// Rows of a workgroup, and how the pages are split: into as many workgroups as fill the GPU.  The
+// tail and the drafts take one more record, unless there is but one split of pages.
+struct TreePlan {
+  int32_t row_waves, row_blocks, pages_per_split, page_splits, records;
+};
+static TreePlan plan_tree(int64_t units, int64_t rows, int32_t n_pages) {
+  TreePlan p;
+  p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  p.row_blocks = (int32_t)((rows + p.row_waves * kWaveRows - 1) / (p.row_waves * kWaveRows));
+  const int64_t target = p.row_waves == 8 ? kTreeTarget / 2 : kTreeTarget;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(target / (units * p.row_blocks), n_pages));
+  p.pages_per_split = (int32_t)std::max<int64_t>(1, (n_pages + splits - 1) / splits);
+  p.page_splits = (n_pages + p.pages_per_split - 1) / p.pages_per_split;
+  p.records = p.page_splits <= 1 ? 1 : p.page_splits + 1;
+  return p;
+}
+
+template <int KIND>
+static void launch_tree(const TreeArgs& a, int row_waves, dim3 grid, hipStream_t s) {
+  switch (row_waves) {
+    case 1: hipLaunchKernelGGL((tree_attention_kernel<KIND, 1, 2>), grid, dim3(kTreeThreads<1, 2>), 0, s, a); break;
+    case 2: hipLaunchKernelGGL((tree_attention_kernel<KIND, 2, 2>), grid, dim3(kTreeThreads<2, 2>), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((tree_attention_kernel<KIND, 4, 1>), grid, dim3(kTreeThreads<4, 1>), 0, s, a); break;
+    default: hipLaunchKernelGGL((tree_attention_kernel<KIND, 8, 1>), grid, dim3(kTreeThreads<8, 1>), 0, s, a); break;
+  }
+}
+
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" size_t tp_tree_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t nodes, int32_t n_pages) {
+  if (batch < 1 || hkv < 1 || hq < hkv || hq % hkv || nodes < 1 || nodes > kTreeMaxNodes || n_pages < 0) return 0;
+  const TreePlan p = plan_tree(batch * hkv, (int64_t)nodes * (hq / hkv), n_pages);
+  return p.records == 1 ? 0 : (size_t)batch * hq * nodes * p.records * (kHeadDim + 2) * sizeof(float);
+}
+
+extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, int32_t hq, int32_t hkv, int32_t nodes,
+                                     const tp_page_layout* layout, const tp_pages* pages, int32_t n_pages,
+                                     const void* tail_k, const void* tail_v, int32_t tail_len, int64_t tail_stride,
+                                     const void* draft_k, const void* draft_v, const int64_t* strides,
+                                     const uint64_t* mask, int64_t mask_stride, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  clear_error();
+  int l1_row = 0, deep_row = 0;
+  if (!check_layout(layout, &l1_row, &deep_row)) return TP_ERR_UNSUPPORTED;
+  if (batch < 1 || hq < 1 || hkv < 1 || hq % hkv != 0 || batch > INT32_MAX / hkv) {
+    set_error("bad query shape: batch=%lld hq=%d hkv=%d (hq must be a multiple of hkv)", (long long)batch, hq, hkv);
+    return TP_ERR_INVALID;
+  }
+  if (nodes < 1 || nodes > kTreeMaxNodes || (int64_t)nodes * (hq / hkv) > INT32_MAX / 2) {
+    set_error("nodes must be in [1, %d], got %d", kTreeMaxNodes, nodes);
+    return TP_ERR_INVALID;
+  }
+  if (n_pages < 0 || (n_pages > 0 && (!pages || pages->capacity < n_pages))) {
+    set_error("n_pages=%d exceeds page capacity", n_pages);
+    return TP_ERR_INVALID;
+  }
+  if (n_pages > 0) {
+    if (!pages->radii || !pages->v_codes || !pages->v_scales || (l1_row > 0 && !pages->angle_l1) ||
+        (deep_row > 0 && !pages->angle_deep) || (layout->int8_radii && !pages->radii_scales)) {
+      set_error("page buffers missing for this layout");
+      return TP_ERR_INVALID;
+    }
+    if (((uintptr_t)pages->radii & 15u) || ((uintptr_t)pages->v_codes & 15u) || ((uintptr_t)pages->angle_l1 & 7u) ||
+        ((uintptr_t)pages->angle_deep & 15u) || ((uintptr_t)pages->v_scales & 3u)) {
+      set_error("page buffers are not aligned");
+      return TP_ERR_INVALID;
+    }
+  }
+  if (tail_len < 0 || tail_len >= kPageTokens) {
+    set_error("tail_len must be in [0, 64), got %d", tail_len);
+    return TP_ERR_INVALID;
+  }
+  if (tail_len > 0 && (!tail_k || !tail_v || tail_stride < tail_len || ((uintptr_t)tail_k & 15u) ||
+                       ((uintptr_t)tail_v & 15u))) {
+    set_error("tail buffers missing, misaligned or tail_stride < tail_len");
+    return TP_ERR_INVALID;
+  }
+  if (!q || !out || !draft_k || !draft_v || !mask || ((uintptr_t)q & 15u) || ((uintptr_t)out & 15u) ||
+      ((uintptr_t)draft_k & 15u) || ((uintptr_t)draft_v & 15u) || ((uintptr_t)mask & 7u) || mask_stride < 0) {
+    set_error("q, out, draft_k and draft_v must be non-NULL 16-byte aligned buffers, mask an 8-byte aligned one");
+    return TP_ERR_INVALID;
+  }
+  if (!strides) {
+    set_error("strides is NULL");
+    return TP_ERR_INVALID;
+  }
+  for (int i = 0; i < 12; ++i)
+    if (strides[i] < 0 || (strides[i] & 7)) {
+      set_error("strides must be non-negative multiples of 8 elements");
+      return TP_ERR_INVALID;
+    }
+  if (!(scale == scale) || scale - scale != 0.0f) {
+    set_error("scale must be finite");
+    return TP_ERR_INVALID;
+  }
+  const int64_t units = batch * hkv, rows = (int64_t)nodes * (hq / hkv);
+  const TreePlan p = plan_tree(units, rows, n_pages);
+  if ((double)units * p.row_blocks * p.records > (double)INT32_MAX) {
+    set_error("too many workgroups for one launch");
+    return TP_ERR_INVALID;
+  }
+  TreeArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  int64_t* const to[12] = {&a.q_b, &a.q_h, &a.q_t, &a.dk_b, &a.dk_h, &a.dk_t, &a.dv_b, &a.dv_h, &a.dv_t, &a.out_b, &a.out_h, &a.out_t};
+  for (int i = 0; i < 12; ++i) *to[i] = strides[i];
+  a.units = (int32_t)units;
+  a.hkv = hkv;
+  a.g = hq / hkv;
+  a.nodes = nodes;
+  a.row_blocks = p.row_blocks;
+  if (n_pages > 0) {
+    a.radii = pages->radii;
+    a.radii_scales = static_cast<const uint16_t*>(pages->radii_scales);
+    a.angle_l1 = pages->angle_l1;
+    a.angle_deep = pages->angle_deep;
+    a.v_codes = pages->v_codes;
+    a.v_scales = static_cast<const uint16_t*>(pages->v_scales);
+    a.capacity = pages->capacity;
+  }
+  a.n_pages = n_pages;
+  a.l1_bits = layout->l1_bits;
+  a.deep_bits = layout->deep_bits;
+  a.split_half = layout->split_dim / 2;
+  a.l1_row = l1_row;
+  a.deep_row = deep_row;
+  a.tail_k = static_cast<const uint16_t*>(tail_k);
+  a.tail_v = static_cast<const uint16_t*>(tail_v);
+  a.tail_stride = tail_stride;
+  a.tail_len = tail_len;
+  a.draft_k = static_cast<const uint16_t*>(draft_k);
+  a.draft_v = static_cast<const uint16_t*>(draft_v);
+  a.mask = mask;
+  a.mask_b = mask_stride;
+  a.words = (nodes + 63) / 64;
+  a.c = std::max(fabsf(scale) * kLog2e, 1.17549435e-38f);  // 2^-126 stands for 0: see tp_prompt_attention
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.pages_per_split = p.pages_per_split;
+  a.page_splits = p.page_splits;
+  a.records = p.records;
+  if (a.records > 1) {
+    const size_t need = tp_tree_workspace_bytes(batch, hq, hkv, nodes, n_pages);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u)) {
+      set_error("workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace_bytes);
+      return TP_ERR_WORKSPACE;
+    }
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)units * rows * a.records * kHeadDim;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(units * p.row_blocks * p.records));
+  const bool is_default = !layout->int8_radii && layout->l1_bits == 4 && layout->deep_bits == 4 && layout->split_dim == 64;
+  const bool is_fast = layout->int8_radii && layout->deep_bits == 8 && layout->split_dim == 0;
+  if (is_default)
+    launch_tree<kTreeDefault>(a, p.row_waves, grid, s);
+  else if (is_fast)
+    launch_tree<kTreeFast>(a, p.row_waves, grid, s);
+  else if (layout->int8_radii)
+    launch_tree<kTreeAnyI8>(a, p.row_waves, grid, s);
+  else
+    launch_tree<kTreeAnyF16>(a, p.row_waves, grid, s);
+  const int32_t st = launch_status("tp_tree_attention");
+  if (st != TP_OK || a.records == 1) return st;
+  JoinArgs j{};
+  j.o = a.part_o;
+  j.ml = a.part_ml;
+  j.out = a.out;
+  j.rows = rows;
+  j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
+  j.units = a.units, j.splits = a.records, j.g = a.g, j.hkv = hkv;
+  return launch_join(j, false, s);
+}

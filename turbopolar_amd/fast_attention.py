@@ -23,14 +23,18 @@ builds (:207-229).  The mechanism is this library's own:
 
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from .bridge import HipKernelBridge
 from .codecs import GroupedVQuantizer, PolarQuantDecoder
 from .config import TurboPolarConfig
-from .kernels import HEAD_DIM, PAGE, decode_attention_store, decode_pages_into, fp16_scale
+from .draft import DraftTree
+from .kernels import (
+    HEAD_DIM, PAGE, _check_draft, _no_grad, decode_attention_store, decode_pages_into, fp16_scale, prompt_attention,
+    tree_attention,
+)
 from .runtime import TurboPolarKVCacheRuntime
 from .storage import pages_of
 
@@ -143,6 +147,74 @@ class TurboPolarFastCache:
         pages = self._store_pages() if n_pages else None
         return decode_attention_store(q[:, :, 0], layout, pages, n_pages, rt._num_kv_heads, tail_k, tail_v,
                                       rt.actual_seq_len, scale)
+
+    # ------------------------------------------------------------------ prompts, drafts, branches
+    def prompt_attention(self, q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
+                         causal: bool = True) -> torch.Tensor:
+        """A prompt's, or a chunk's, attention without its score matrix: append ``keys`` /
+        ``values`` ``[B, H_kv, T, 128]`` and attend the chunk's ``q`` ``[B, H_q, T, 128]`` over the
+        whole history as ``update_and_fetch`` decompresses it (tp_prompt_attention; the scale in
+        32 bits, as the model's own attention takes it).  Returns ``[B, H_q, T, 128]`` of q's
+        type.  No counterpart in the reference, which hands the history to the model's attention."""
+        for name, t in (("q", q), ("keys", keys), ("values", values)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[-1] != HEAD_DIM:
+                raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ()))}")
+            if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+                raise ValueError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+        if keys.shape != values.shape or q.shape[0] != keys.shape[0] or q.shape[2] != keys.shape[2]:
+            raise ValueError(f"q {tuple(q.shape)}, keys {tuple(keys.shape)} and values {tuple(values.shape)} differ")
+        if q.shape[1] < 1 or keys.shape[1] < 1 or q.shape[1] % keys.shape[1]:
+            raise ValueError(f"H_q={q.shape[1]} is not a multiple of H_kv={keys.shape[1]}")
+        if not (q.device == keys.device == values.device and q.is_cuda):
+            raise ValueError(f"q is on {q.device}, keys on {keys.device}, values on {values.device}; need one HIP device")
+        _no_grad(q, keys, values)
+        k, v = self.update_and_fetch(keys.to(torch.float16), values.to(torch.float16))
+        return prompt_attention(q.to(torch.float16), k, v, scale, causal=causal).to(q.dtype)
+
+    def tree_attention(self, q: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor, tree: DraftTree,
+                       scale: float) -> torch.Tensor:
+        """Attention of a tree of drafted tokens: the queries ``q`` ``[B, H_q, T, 128]`` of its nodes
+        over every cached token, their ancestors among the drafted ``k_draft`` / ``v_draft`` ``[B,
+        H_kv, T, 128]`` and themselves (tp_tree_attention; ``scale`` taken as fp16, as for
+        ``decode_attention``).  The cache does not change; ``accept`` takes the nodes that the
+        verification keeps.  Returns fp16 ``[B, H_q, T, 128]``."""
+        _check_draft(q, k_draft, v_draft, tree)
+        rt = self.runtime
+        rt.resolve_deferred_check()
+        if int(k_draft.shape[1]) != self.config.num_kv_heads:
+            raise ValueError(f"draft has {k_draft.shape[1]} KV heads but config expects {self.config.num_kv_heads}")
+        if rt._initialized and q.shape[0] != rt._batch_size:
+            raise ValueError(f"batch of q ({q.shape[0]}) and cache ({rt._batch_size}) differ")
+        n_pages = rt.k_storage.block_count
+        tail_k, tail_v = rt._tail_views()
+        held = rt.k_storage.radii if n_pages else tail_k
+        if held is not None and held.device != q.device:
+            raise ValueError(f"q is on {q.device}, the cache on {held.device}")
+        return tree_attention(q, rt.polar_encoder.layout, self._store_pages() if n_pages else None, n_pages, tail_k,
+                              tail_v, k_draft, v_draft, tree, fp16_scale(scale))
+
+    def accept(self, k_draft: torch.Tensor, v_draft: torch.Tensor, path: Sequence) -> None:
+        """Appends the drafted tokens ``path`` (node indices, root first; ``DraftTree.path_to``)."""
+        self.runtime.accept(k_draft.to(torch.float16), v_draft.to(torch.float16), path)
+
+    def truncate(self, tokens: int) -> None:
+        """Keeps the first ``tokens`` tokens (``TurboPolarKVCacheRuntime.truncate``)."""
+        self.runtime.truncate(tokens)
+
+    def fork(self, tokens: Optional[int] = None, rows: Optional[Sequence[int]] = None,
+             pages: Optional[Sequence[int]] = None) -> "TurboPolarFastCache":
+        """An independent copy of this cache or a part of it (``TurboPolarKVCacheRuntime.fork``)."""
+        other = TurboPolarFastCache(self.config)
+        other.runtime = self.runtime.fork(tokens, rows, pages)
+        return other
+
+    def select_rows(self, rows: Sequence[int]) -> None:
+        """Makes batch row i what row ``rows[i]`` was."""
+        self.runtime.select_rows(rows)
+
+    def keep_pages(self, pages: Sequence[int]) -> None:
+        """Compacts the cache to the stored pages ``pages`` and the tail."""
+        self.runtime.keep_pages(pages)
 
     # ------------------------------------------------------------------ mlx_lm cache protocol
     def size(self) -> int:

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 from functools import lru_cache
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -542,3 +542,254 @@ def _tail_pair(tail_k: torch.Tensor, tail_v: torch.Tensor):
     if stride_v != stride:
         tk, tv, stride = _fresh(tk), _fresh(tv), tk.shape[2]
     return tk, tv, stride
+
+
+# --------------------------------------------------------------------------
+# prompts and drafts
+# --------------------------------------------------------------------------
+
+_Strides12, _Strides6 = ctypes.c_int64 * 12, ctypes.c_int64 * 6
+
+
+def _no_grad(*tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("the TurboPolar kernels compute no gradients; call them under torch.no_grad()")
+
+
+def _strided(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """``t`` ``[B, H, T, 128]`` as a kernel reads it in place, and its (batch, head, token)
+    strides: rows of 128 contiguous elements, 16 bytes aligned.  Anything else is copied."""
+    B, H, T, _ = t.shape
+    s0, s1, s2, s3 = t.stride()
+    s0, s1, s2 = s0 if B > 1 else 0, s1 if H > 1 else 0, s2 if T > 1 else 0
+    if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15:
+        t = _fresh(t)
+        s0, s1, s2, _ = t.stride()
+    return t, (s0, s1, s2)
+
+
+def _token_major(B: int, H: int, T: int, dtype, device) -> torch.Tensor:
+    """An output ``[B, H, T, 128]`` that lies token by token, as the output projection reads it."""
+    return torch.empty((B, T, H, HEAD_DIM), dtype=dtype, device=device).transpose(1, 2)
+
+
+def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
+    """Workspace of one call.  Not kept: its content is any, and the caching allocator orders its
+    reuse on the stream, inside a captured graph too (graphs never share it)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+@lru_cache(maxsize=1024)
+def _prompt_workspace(B: int, Hq: int, Hkv: int, Tq: int, Tk: int, n_seq: int) -> int:
+    return int(lib().tp_prompt_workspace_bytes(B, Hq, Hkv, Tq, Tk, n_seq))
+
+
+def _starts(starts, name: str, tokens: int, device: torch.device) -> torch.Tensor:
+    """Starts of packed sequences as a device int32 array.  A device tensor is taken as it is
+    (its values are not read here); a host one or a sequence of ints is checked and copied."""
+    if isinstance(starts, torch.Tensor) and starts.is_cuda:
+        if starts.dtype is not torch.int32 or starts.dim() != 1 or not starts.is_contiguous() or starts.shape[0] < 2:
+            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor of at least 2 starts")
+        if starts.device != device:
+            raise ValueError(f"{name} is on {starts.device}, q on {device}")
+        return starts
+    values = [int(x) for x in (starts.tolist() if isinstance(starts, torch.Tensor) else starts)]
+    if len(values) < 2 or values[0] != 0 or any(b < a for a, b in zip(values, values[1:])) or values[-1] > tokens:
+        raise ValueError(f"{name} must ascend from 0 to at most {tokens} tokens, got {values[:8]}")
+    return torch.tensor(values, dtype=torch.int32).to(device)
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float,
+    causal: bool = True,
+    q_starts=None,
+    k_starts=None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """tp_prompt_attention: attention of ``q`` ``[B, H_q, Tq, 128]`` over ``k`` / ``v`` ``[B, H_kv,
+    Tk, 128]``, all float16 or all bfloat16, any strides with contiguous rows of 128 (others are
+    copied).  ``causal``: the queries are the last ``Tq`` of the ``Tk`` positions.  A query that
+    sees no key gives 0.
+
+    ``q_starts`` / ``k_starts`` (together, batch 1): packed sequences, the ``n + 1`` ascending
+    token positions between them, as sequences of ints or host tensors, which are checked, or as
+    int32 device tensors, which are not read here (values out of order give unspecified rows).
+    Query rows behind the last sequence are 0, or left as they are where ``out`` is given.
+
+    Returns ``out``, or a new ``[B, H_q, Tq, 128]`` of q's type that lies token by token."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[-1] != HEAD_DIM:
+            raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ()))}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError(f"q, k and v must all be float16 or all bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, Hq, Tq, _ = q.shape
+    Hkv, Tk = int(k.shape[1]), int(k.shape[2])
+    if v.shape != k.shape or k.shape[0] != B:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match each other and q's batch of {B}")
+    if B < 1 or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"H_q={Hq} is not a multiple of H_kv={Hkv}, or the batch is empty")
+    require_hip(q, "q")
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"q is on {dev}, k on {k.device}, v on {v.device}")
+    _no_grad(q, k, v)
+    n_seq = 0
+    if (q_starts is None) != (k_starts is None):
+        raise ValueError("q_starts and k_starts come together")
+    if q_starts is not None:
+        if B != 1:
+            raise ValueError(f"packed sequences take a batch of 1, got {B}")
+        same = k_starts is q_starts and Tq == Tk
+        q_starts = _starts(q_starts, "q_starts", Tq, dev)
+        k_starts = q_starts if same else _starts(k_starts, "k_starts", Tk, dev)
+        if q_starts.shape != k_starts.shape:
+            raise ValueError(f"{q_starts.shape[0]} q_starts, {k_starts.shape[0]} k_starts")
+        n_seq = int(q_starts.shape[0]) - 1
+    keep_rest = out is not None
+    if out is None:
+        out = _token_major(B, Hq, Tq, q.dtype, dev)
+    else:
+        if out.shape != q.shape or out.dtype is not q.dtype or out.device != dev:
+            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev}")
+        _no_grad(out)
+        view, strides = _strided(out)
+        if view is not out or _overlaps(out):
+            raise ValueError("out must have distinct, contiguous rows of 128 elements, 16 bytes aligned")
+    if Tq == 0:
+        return out
+    (q, qs), (k, ks), (v, vs), (_, os_) = _strided(q), _strided(k), _strided(v), _strided(out)
+    L = lib()
+    ws = _scratch(_prompt_workspace(B, Hq, Hkv, Tq, Tk, n_seq), dev)
+    st = call_on(
+        dev, L.tp_prompt_attention, q.data_ptr(), ptr(k), ptr(v), out.data_ptr(), 1 if q.dtype is torch.bfloat16 else 0,
+        B, Hq, Hkv, Tq, Tk, _Strides12(*qs, *ks, *vs, *os_), 1 if causal else 0, ptr(q_starts), ptr(k_starts), n_seq,
+        1 if keep_rest else 0, float(scale), ptr(ws), 0 if ws is None else ws.numel(), stream_handle(dev),
+    )
+    check(st, "tp_prompt_attention")
+    return out
+
+
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether two rows of ``t`` share memory (sizes and strides sorted, each step past the last)."""
+    dims = sorted((s, n) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
+    reach = t.shape[-1]
+    for s, n in dims:
+        if s < reach:
+            return True
+        reach = s * (n - 1) + reach
+    return False
+
+
+@lru_cache(maxsize=1024)
+def _tree_workspace(B: int, Hq: int, Hkv: int, nodes: int, n_pages: int) -> int:
+    return int(lib().tp_tree_workspace_bytes(B, Hq, Hkv, nodes, n_pages))
+
+
+def tree_attention(q: torch.Tensor, layout, pages: Optional[TPPages], n_pages: int,
+                   tail_k: Optional[torch.Tensor], tail_v: Optional[torch.Tensor], draft_k: torch.Tensor,
+                   draft_v: torch.Tensor, tree, scale: float) -> torch.Tensor:
+    """tp_tree_attention: the drafted tokens ``draft_k`` / ``draft_v`` ``[B, H_kv, T, 128]`` of a
+    ``DraftTree`` and their queries ``q`` ``[B, H_q, T, 128]`` over the first ``n_pages`` slots of a
+    page store and a dense tail ``[B, H_kv, < 64, 128]`` (None for none).  Float types other than
+    float16 are converted to it, as the cache and the decode step do.  Returns fp16 ``[B, H_q, T,
+    128]`` that lies token by token."""
+    _check_draft(q, draft_k, draft_v, tree)
+    B, Hq, T, _ = q.shape
+    Hkv = int(draft_k.shape[1])
+    dev = q.device
+    tk = tv = None
+    tail_len = tail_stride = 0
+    if tail_k is not None and tail_k.shape[2]:
+        if tail_k.shape != tail_v.shape or tuple(tail_k.shape[:2]) != (B, Hkv) or tail_k.shape[3] != HEAD_DIM:
+            raise ValueError(f"tail shape {tuple(tail_k.shape)} does not match [B={B}, H_kv={Hkv}, T, {HEAD_DIM}]")
+        tail_len = int(tail_k.shape[2])
+        tk, tv, tail_stride = _tail_pair(tail_k, tail_v)
+    (q, qs), (dk, ks), (dv, vs) = (_strided(t if t.dtype is torch.float16 else t.to(torch.float16))
+                                   for t in (q, draft_k, draft_v))
+    mask = tree.mask_on(dev)
+    out = _token_major(B, Hq, T, torch.float16, dev)
+    _, os_ = _strided(out)
+    if pages is None:
+        pages, n_pages = _NO_PAGES, 0
+    ws = _scratch(_tree_workspace(B, Hq, Hkv, T, n_pages), dev)
+    st = call_on(
+        dev, lib().tp_tree_attention, q.data_ptr(), out.data_ptr(), B, Hq, Hkv, T, ctypes.byref(layout),
+        ctypes.byref(pages), n_pages, ptr(tk), ptr(tv), tail_len, tail_stride, dk.data_ptr(), dv.data_ptr(),
+        _Strides12(*qs, *ks, *vs, *os_), mask.data_ptr(), 0 if tree.shared else mask.stride(0), float(scale), ptr(ws),
+        0 if ws is None else ws.numel(), stream_handle(dev),
+    )
+    check(st, "tp_tree_attention")
+    return out
+
+
+def _check_draft(q, draft_k, draft_v, tree) -> None:
+    """The checks of a draft's tensors against each other and its tree."""
+    for name, t in (("q", q), ("k", draft_k), ("v", draft_v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[-1] != HEAD_DIM:
+            raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ()))}")
+        if not t.is_floating_point():
+            raise ValueError(f"{name} must be a float tensor, got {t.dtype}")
+    B, Hq, T, _ = q.shape
+    if draft_k.shape != draft_v.shape or draft_k.shape[0] != B or draft_k.shape[2] != T:
+        raise ValueError(f"drafted k {tuple(draft_k.shape)} and v {tuple(draft_v.shape)} do not match q {tuple(q.shape)}")
+    Hkv = int(draft_k.shape[1])
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"H_q={Hq} is not a multiple of H_kv={Hkv}")
+    if tree.nodes != T or (tree.batch is not None and tree.batch != B):
+        raise ValueError(f"a tree of {tree.nodes} nodes for {tree.batch or 'every'} batch rows does not match q {tuple(q.shape)}")
+    require_hip(q, "q")
+    if draft_k.device != q.device or draft_v.device != q.device:
+        raise ValueError(f"q is on {q.device}, k on {draft_k.device}, v on {draft_v.device}")
+    _no_grad(q, draft_k, draft_v)
+
+
+def take_tokens(k: torch.Tensor, v: torch.Tensor, index: Union[Sequence[int], Sequence[Sequence[int]]], n: int,
+                out_k: torch.Tensor, out_v: torch.Tensor, out_pos: int, flag: Optional[torch.Tensor] = None,
+                epoch: int = 0) -> None:
+    """tp_take_tokens: tokens ``index`` of ``k`` / ``v`` ``[B, H, T, 128]`` (fp16 or fp32; one list of
+    ``n`` for every batch row, or one each) into rows ``[out_pos, out_pos + n)`` of ``out_k`` /
+    ``out_v`` ``[B, H, tokens, 128]`` of the same type, contiguous.  With ``flag`` and ``epoch`` (as for
+    an append) the call waits for the verdict and raises the append's ValueError."""
+    B, H, T, _ = k.shape
+    per_batch = isinstance(index[0], (list, tuple))
+    flat = [i for row in index for i in row] if per_batch else list(index)
+    item_mask = 3 if k.dtype is torch.float32 else 7
+    views = []
+    for t in (k, v):
+        t, s = _strided(t)
+        if any(x & item_mask for x in s):
+            t = _fresh(t)
+            s = t.stride()[:3]
+        views.append((t, s))
+    (k, ks), (v, vs) = views
+    dev = k.device
+    st = call_on(
+        dev, lib().tp_take_tokens, k.data_ptr(), v.data_ptr(), 1 if k.dtype is torch.float32 else 0, B, H, T,
+        _Strides6(*ks, *vs), (ctypes.c_int32 * len(flat))(*flat), n, 1 if per_batch else 0, out_k.data_ptr(),
+        out_v.data_ptr(), int(out_k.shape[2]), out_pos, 0 if flag is None else 2, ptr(flag), epoch, stream_handle(dev),
+    )
+    if st == _lib.TP_ERR_NONFINITE:
+        raise ValueError("append() inputs must contain finite values")
+    check(st, "tp_take_tokens")
+
+
+def copy_pages(buffers, batch: int, heads: int, batch_in: int, rows: Optional[torch.Tensor], src_capacity: int,
+               dst_capacity: int, n_stored: int, page_index: Optional[torch.Tensor], keep: int,
+               tails: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]], tail_tokens: int,
+               device: torch.device) -> None:
+    """tp_copy_pages: ``buffers`` is a list of (source, destination, bytes of a page), sources and
+    destinations contiguous ``[batch, heads, capacity, ...]``; ``tails`` (k, v, their copies), each
+    ``[batch, heads, 64, 128]`` and contiguous, of which ``tail_tokens`` rows are copied."""
+    bufs = (_lib.TPPageCopy * max(1, len(buffers)))(*[_lib.TPPageCopy(ptr(s), ptr(d), n) for s, d, n in buffers])
+    tail_ptrs, tail_bytes, tail_row = (None,) * 4, 0, 0
+    if tails is not None and tail_tokens:
+        token = HEAD_DIM * tails[0].element_size()
+        tail_ptrs, tail_bytes, tail_row = tuple(t.data_ptr() for t in tails), tail_tokens * token, PAGE * token
+    st = call_on(
+        device, lib().tp_copy_pages, bufs, len(buffers), batch, heads, batch_in, ptr(rows), src_capacity, dst_capacity,
+        n_stored, ptr(page_index), keep, *tail_ptrs, tail_bytes, tail_row, stream_handle(device),
+    )
+    check(st, "tp_copy_pages")

@@ -15,7 +15,12 @@ Mirrors the reference's mlx_lm hook (benchmarks/turbopolar_fast_attention.py:
 * ``patch_llama_attention`` swaps ``LlamaAttention.forward`` for one that sends
   single-token decode steps with a standard causal mask through
   ``TurboPolarFastCache.decode_attention`` (the fused HIP kernel over the
-  compressed pages) and everything else through the original forward.
+  compressed pages) and everything else through the original forward.  With
+  ``prompt_kernel=True`` prompts and chunks of them go through
+  ``TurboPolarFastCache.prompt_attention``, which needs no score matrix.
+* The cache protocol's ``crop``, ``reorder_cache``, ``batch_select_indices`` and
+  ``batch_repeat_interleave`` (assisted generation and beams) truncate and
+  re-order the compressed cache.
 
 The model's weights are untouched; any Llama checkpoint loaded from a local
 path works, and tests use randomly initialised models.
@@ -76,6 +81,28 @@ class TurboPolarLayer(CacheLayerMixin):
     def get_max_length(self) -> int:
         return -1
 
+    def crop(self, tokens_to_remove: int) -> None:
+        """Removes the last ``-tokens_to_remove`` tokens; a positive number is the length to
+        keep (the protocol's older meaning; nothing happens where the cache is shorter)."""
+        held = self.fast.offset
+        tokens_to_remove = int(tokens_to_remove)  # generation hands over a tensor
+        keep = tokens_to_remove if tokens_to_remove > 0 else held + tokens_to_remove
+        if keep < held:
+            self.fast.truncate(max(0, keep))
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        self.batch_select_indices(beam_idx)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        if self.fast.offset:
+            if indices.dtype is torch.bool:
+                indices = indices.nonzero().flatten()
+            self.fast.select_rows(indices)
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        if self.fast.offset:
+            self.fast.select_rows([b for b in range(self.fast.runtime._batch_size) for _ in range(repeats)])
+
     def reset(self) -> None:
         self.fast = TurboPolarFastCache(self.fast.config)
         self.is_initialized = False
@@ -128,11 +155,11 @@ def make_turbo_cache(model, config: Optional[TurboPolarConfig] = None) -> TurboP
 _mask_verdict = None  # (mask, its version, seq_len, cache_len, verdict) of the last check
 
 
-def _is_standard_causal_mask(mask: Optional[torch.Tensor], seq_len: int, cache_len: int) -> bool:
+def _is_standard_causal_mask(mask: Optional[torch.Tensor], seq_len: int, cache_len: int, batch: int = 1) -> bool:
     """True for no mask or the full-history causal mask ``[1, 1, seq_len, cache_len]``
     (turbopolar_fast_attention.py:235-244), boolean (True = attend) or additive
     (0 = attend).  Query i (at position cache_len - seq_len + i) sees keys
-    0 .. cache_len - seq_len + i.
+    0 .. cache_len - seq_len + i.  ``batch``: rows that a mask may hold, all alike.
 
     A forward pass hands the same mask tensor to every layer; the verdict is
     kept for that tensor (held, so its memory cannot be reused, and keyed on
@@ -142,14 +169,14 @@ def _is_standard_causal_mask(mask: Optional[torch.Tensor], seq_len: int, cache_l
     global _mask_verdict
     if mask is None:
         return True
-    if tuple(mask.shape) != (1, 1, seq_len, cache_len):
+    if tuple(mask.shape) not in ((1, 1, seq_len, cache_len), (batch, 1, seq_len, cache_len)):
         return False
     hit = _mask_verdict
     if hit is not None and hit[0] is mask and hit[1] == mask._version and hit[2] == seq_len and hit[3] == cache_len:
         return hit[4]
-    allowed = mask[0, 0] if mask.dtype == torch.bool else mask[0, 0] == 0
+    allowed = mask[:, 0] if mask.dtype == torch.bool else mask[:, 0] == 0
     expected = torch.ones((seq_len, cache_len), dtype=torch.bool, device=mask.device).tril(cache_len - seq_len)
-    ok = bool(torch.equal(allowed, expected))
+    ok = bool((allowed == expected).all())
     _mask_verdict = (mask, mask._version, seq_len, cache_len, ok)
     return ok
 
@@ -186,8 +213,36 @@ def _turbo_llama_attention_forward(
         out = fast.decode_attention(q, k, v, self.scaling, defer_check=_model_wrapped())  # [B, H_q, D] fp16
         out = out.to(hidden_states.dtype).reshape(B, L, -1)
         return self.o_proj(out), None
+    if _prompt_kernel and isinstance(past_key_values, TurboPolarCache) and _takes_prompt(
+        self, hidden_states, attention_mask, past_key_values.fast(self.layer_idx)
+    ):
+        B, L, _ = hidden_states.shape
+        q, k, v = (
+            proj(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2)
+            for proj in (self.q_proj, self.k_proj, self.v_proj)
+        )
+        q, k = _llama.apply_rotary_pos_emb(q, k, *position_embeddings)
+        out = past_key_values.fast(self.layer_idx).prompt_attention(q, k, v, self.scaling)
+        past_key_values.layers[self.layer_idx].is_initialized = True
+        return self.o_proj(out.transpose(1, 2).reshape(B, L, -1)), None
     return _orig_llama_attention_forward(
         self, hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs
+    )
+
+
+_prompt_kernel = False
+
+
+def _takes_prompt(attention, hidden_states, mask, fast) -> bool:
+    """Whether a step of several tokens is one for the prompt kernel: half precision, the full-history
+    causal mask, no dropout and no gradients; anything else is the original forward's."""
+    return (
+        hidden_states.is_cuda
+        and hidden_states.dtype in (torch.float16, torch.bfloat16)
+        and not torch.is_grad_enabled()
+        and not (attention.training and attention.attention_dropout)
+        and _is_standard_causal_mask(mask, hidden_states.shape[1], fast.offset + hidden_states.shape[1],
+                                     hidden_states.shape[0])
     )
 
 
@@ -211,12 +266,15 @@ def _turbo_llama_model_forward(self, *args, **kwargs):
     return out
 
 
-def patch_llama_attention(model=None) -> None:
+def patch_llama_attention(model=None, prompt_kernel: bool = False) -> None:
     """Route Llama decode steps on a ``TurboPolarCache`` through the fused kernel
     (turbopolar_fast_attention.py:283-290).  Patches the class, like the
     reference; ``model`` is accepted for the same signature.  LlamaModel.forward
-    is wrapped too, to read the steps' non-finite verdicts once per forward."""
-    global _orig_llama_attention_forward, _orig_llama_model_forward
+    is wrapped too, to read the steps' non-finite verdicts once per forward.
+    ``prompt_kernel``: steps of several tokens run tp_prompt_attention over the
+    decompressed history instead of the model's own attention."""
+    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel
+    _prompt_kernel = bool(prompt_kernel)
     if _orig_llama_attention_forward is None:
         _orig_llama_attention_forward = _llama.LlamaAttention.forward
     _llama.LlamaAttention.forward = _turbo_llama_attention_forward
@@ -227,7 +285,8 @@ def patch_llama_attention(model=None) -> None:
 
 def unpatch_llama_attention(model=None) -> None:
     """Restore the original forward (turbopolar_fast_attention.py:293-298)."""
-    global _orig_llama_attention_forward, _orig_llama_model_forward
+    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel
+    _prompt_kernel = False
     if _orig_llama_attention_forward is not None:
         _llama.LlamaAttention.forward = _orig_llama_attention_forward
         _orig_llama_attention_forward = None

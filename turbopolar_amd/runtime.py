@@ -22,20 +22,53 @@ rfsn_v11/generation/turbo_polar_cache.py:18-395.  Differences of mechanism
 from __future__ import annotations
 
 import ctypes
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
 from .codecs import GroupedVQuantizer, PolarQuantDecoder, PolarQuantEncoder
 from .config import TurboPolarConfig
-from .kernels import PAGE, decode_pages_gather, decode_step, encode_pages, step_flag_words
+from .kernels import (
+    PAGE, copy_pages, decode_pages_gather, decode_pages_into, decode_step, encode_pages, step_flag_words, take_tokens,
+)
 from .payload import PolarKeyBlock, QuantizedVBlock
-from .storage import Growth, PolarKBlockStorage, QuantVBlockStorage, pages_of
+from .storage import Growth, PolarKBlockStorage, QuantVBlockStorage, capacity_for, pages_of
 
 
 def _nbytes(x: torch.Tensor) -> int:
     return int(x.numel() * x.element_size())
+
+
+def _whole(x, name: str) -> int:
+    if isinstance(x, bool) or not isinstance(x, int):
+        raise TypeError(f"{name} must be an int, got {type(x).__name__}")
+    return x
+
+
+def _indices(values, n: int, name: str, of: str) -> list:
+    """A list of ints in [0, n) from a sequence or a tensor."""
+    if isinstance(values, torch.Tensor):
+        if values.dim() != 1 or values.is_floating_point() or values.dtype is torch.bool:
+            raise ValueError(f"{name} must be a 1-D tensor of whole numbers")
+        values = values.tolist()
+    values = [_whole(x, name) for x in values]
+    bad = [x for x in values if not 0 <= x < n]
+    if bad:
+        raise IndexError(f"{name} {bad[:8]} outside the {n} {of}")
+    return values
+
+
+def _path_of(path, batch: int, tokens: int):
+    """(whether there is one path per batch row, the path or paths as lists)."""
+    if isinstance(path, torch.Tensor):
+        path = path.tolist()
+    path = list(path)
+    if path and isinstance(path[0], (list, tuple)):
+        if len(path) != batch or len({len(row) for row in path}) != 1:
+            raise ValueError(f"accept() takes one path, or one of equal length for each of the {batch} batch rows")
+        return True, [_indices(row, tokens, "path", "drafted tokens") for row in path]
+    return False, _indices(path, tokens, "path", "drafted tokens")
 
 
 class TurboPolarKVCacheRuntime:
@@ -235,15 +268,7 @@ class TurboPolarKVCacheRuntime:
         v_new = v_new.contiguous()
         if self._tail_k is not None and self._tail_k.device != k_new.device:
             raise ValueError(f"append() inputs moved from {self._tail_k.device} to {k_new.device}")
-        if self._tail_k is None:
-            # Rows past the tail's length are never read, so they are not cleared.
-            self._tail_k = torch.empty((B, H, PAGE, D), dtype=k_new.dtype, device=k_new.device)
-            self._tail_v = torch.empty((B, H, PAGE, D), dtype=k_new.dtype, device=k_new.device)
-        if self._flag is None:
-            # Written by the append launches and read here, with no device-to-host
-            # copy; the words past the first are a one-launch step's.
-            words = step_flag_words(B, max(self.config.num_q_heads, H), H)
-            self._flag = torch.zeros(words, dtype=torch.int32, pin_memory=True)
+        self._make_tail(B, H, D, k_new.dtype, k_new.device)
         if self._tail_len:
             n_head, head_dst = min(PAGE - self._tail_len, T), self._tail_len
         elif T < PAGE:
@@ -270,6 +295,18 @@ class TurboPolarKVCacheRuntime:
         if n_head < T:
             self._stage(k_new, v_new, n_head, T - n_head, 0, check=0)
             self._tail_len = T - n_head
+
+    def _make_tail(self, B: int, H: int, D: int, dtype, device) -> None:
+        """The tail's buffers and the launches' flag, if they are not there yet."""
+        if self._tail_k is None:
+            # Rows past the tail's length are never read, so they are not cleared.
+            self._tail_k = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
+            self._tail_v = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
+        if self._flag is None:
+            # Written by the append launches and read here, with no device-to-host
+            # copy; the words past the first are a one-launch step's.
+            words = step_flag_words(B, max(self.config.num_q_heads, H), H)
+            self._flag = torch.zeros(words, dtype=torch.int32, pin_memory=True)
 
     def append_and_attend(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, scale: float, pages,
                           layout, defer_check: bool = False) -> Optional[torch.Tensor]:
@@ -587,6 +624,175 @@ class TurboPolarKVCacheRuntime:
             "k_storage_reallocs": self.k_storage.reallocation_count,
             "v_storage_reallocs": self.v_storage.reallocation_count,
         }
+
+    # ------------------------------------------------------------------
+    # Drafts and branches (no counterpart in the reference)
+    # ------------------------------------------------------------------
+    def accept(self, k: torch.Tensor, v: torch.Tensor, path: Sequence) -> None:
+        """Appends tokens ``path`` of the drafted ``k`` / ``v`` ``[B, H_kv, T, D]``, in that
+        order: one list of node indices for every batch row, or one of equal length for
+        each.  One launch gathers them, checks them and writes them to the dense tail
+        (tp_take_tokens) where they leave it at a page at most; a longer path is gathered and
+        appended.  An empty path changes nothing.  Errors are ``append``'s and leave the
+        cache unchanged."""
+        if self._pending:
+            self.resolve_deferred_check()
+        self._validate_shapes(k, v)
+        per_batch, path = _path_of(path, int(k.shape[0]), int(k.shape[2]))
+        n = len(path[0]) if per_batch else len(path)
+        if n == 0:
+            return
+        B, H, _, D = k.shape
+        err = self._invariant_error(k)
+        if err is not None:
+            raise err
+        if not (k.is_cuda and v.is_cuda):
+            rows = path if per_batch else [path] * B
+            self.append(*(torch.stack([t[b, :, rows[b]] for b in range(B)]) for t in (k, v)))
+            return
+        if v.device != k.device or (self._tail_k is not None and self._tail_k.device != k.device):
+            raise ValueError(f"accept() inputs are on {k.device} and {v.device}, not where the cache is")
+        flat = n * B if per_batch else n
+        if self._initialized and self._tail_len + n <= PAGE and flat <= 1024:
+            self._make_tail(B, H, D, k.dtype, k.device)
+            self._epoch = ((self._epoch + 2) & 0xFFFFFFFE) or 2
+            take_tokens(k, v, path, n, self._tail_k, self._tail_v, self._tail_len, self._flag, self._epoch)
+            self.actual_seq_len += n
+            self._tail_len += n
+            if self._tail_len == PAGE:
+                self._encode_into_storage(self._tail_k, self._tail_v, 0, 1)
+                self._tail_len = 0
+            return
+        taken = [torch.empty((B, H, n, D), dtype=k.dtype, device=k.device) for _ in range(2)]
+        for rows, row in [(slice(b, b + 1), x) for b, x in enumerate(path)] if per_batch else [(slice(0, B), path)]:
+            for at in range(0, n, 1024):
+                part = row[at:at + 1024]
+                take_tokens(k[rows], v[rows], part, len(part), taken[0][rows], taken[1][rows], at)
+        self.append(*taken)
+
+    def truncate(self, tokens: int) -> None:
+        """Keeps the first ``tokens`` tokens.  Freed page slots take the next pages; the
+        memory stays the cache's.  Where the cut falls inside a stored page, that page's
+        first tokens are decoded to the dense tail, with the values that attention read
+        from it."""
+        if self._pending:
+            self.resolve_deferred_check()
+        tokens = _whole(tokens, "tokens")
+        if not 0 <= tokens <= self.actual_seq_len:
+            raise ValueError(f"cannot keep {tokens} of {self.actual_seq_len} tokens")
+        if tokens == self.actual_seq_len:
+            return
+        S = self.k_storage.block_count
+        pages, left = min(tokens // PAGE, S), tokens - min(tokens // PAGE, S) * PAGE
+        if pages < S:
+            if left:
+                self._make_tail(self._batch_size, self._num_kv_heads, self._head_dim, self._input_dtype,
+                                self.k_storage.radii.device)
+                self._decode_to_tail(self, pages)
+            self.k_storage.block_count = self.v_storage.block_count = pages
+            self.total_blocks = max(0, self.total_blocks - (S - pages))
+            self.bytes_written = max(0, self.bytes_written - (S - pages) * self._page_bytes())
+            self._fused_views = None
+        self._tail_len = left
+        self.actual_seq_len = tokens
+
+    def _decode_to_tail(self, source: "TurboPolarKVCacheRuntime", page: int) -> None:
+        """``source``'s stored page decoded into the dense tail's buffers."""
+        k, v = self._tail_k, self._tail_v
+        if k.dtype is not torch.float16:
+            k, v = torch.empty_like(k, dtype=torch.float16), torch.empty_like(v, dtype=torch.float16)
+        decode_pages_into(source.polar_encoder.layout, pages_of(source.k_storage, source.v_storage),
+                          self._batch_size * self._num_kv_heads, page, 1, k, v, 0)
+        if k is not self._tail_k:
+            self._tail_k.copy_(k)
+            self._tail_v.copy_(v)
+
+    def fork(self, tokens: Optional[int] = None, rows: Optional[Sequence[int]] = None,
+             pages: Optional[Sequence[int]] = None) -> "TurboPolarKVCacheRuntime":
+        """An independent copy of this cache, or of a part of it: its first ``tokens`` tokens
+        (as ``truncate`` keeps them), batch rows ``rows`` in that order (one may come
+        more than once), or the stored pages ``pages`` in that order, followed by the tail.
+        One launch copies every buffer (tp_copy_pages); the growth counters of the copy start
+        at 0.  ``rows`` and ``pages`` are ints; a tensor of them is read back from its device."""
+        if self._pending:
+            self.resolve_deferred_check()
+        if tokens is not None and pages is not None:
+            raise ValueError("fork() takes tokens or pages, not both")
+        other = TurboPolarKVCacheRuntime(self.config)
+        B, H, D, S = self._batch_size, self._num_kv_heads, self._head_dim, self.k_storage.block_count
+        rows = None if rows is None else _indices(rows, B or 0, "rows", "batch rows")
+        pages = None if pages is None else _indices(pages, S, "pages", "stored pages")
+        if rows is not None and not rows:
+            raise ValueError("fork() needs at least one batch row")
+        keep, left, cut = (S if pages is None else len(pages)), self._tail_len, None
+        if tokens is not None:
+            tokens = _whole(tokens, "tokens")
+            if not 0 <= tokens <= self.actual_seq_len:
+                raise ValueError(f"cannot keep {tokens} of {self.actual_seq_len} tokens")
+            keep = min(tokens // PAGE, S)
+            left = tokens - keep * PAGE
+            cut = keep if keep < S and left else None
+        if not self._initialized:
+            return other
+        n = B if rows is None else len(rows)
+        other._batch_size, other._num_kv_heads, other._head_dim, other._input_dtype = n, H, D, self._input_dtype
+        other._initialized = True
+        device = self._tail_k.device if S == 0 else self.k_storage.radii.device
+        if self._tail_k is not None and not device.type == "cuda":
+            at = list(range(B)) if rows is None else rows
+            other._tail_k, other._tail_v = self._tail_k[at].clone(), self._tail_v[at].clone()
+        else:
+            if left:
+                other._make_tail(n, H, D, self._input_dtype, device)
+            self._copy_into(other, n, rows, pages, keep, cut, left, device)
+        other.k_storage.block_count = other.v_storage.block_count = other.total_blocks = keep
+        other._tail_len = left
+        other.actual_seq_len = keep * PAGE + left
+        other.bytes_written = keep * other._page_bytes() if keep else 0
+        return other
+
+    def _copy_into(self, other, n, rows, pages, keep, cut, left, device) -> None:
+        """The launches of ``fork``: the kept pages (and the one that the cut falls in, which is
+        then decoded) into stores of their own, and the tail."""
+        stored = keep + (cut is not None)
+        capacity, moves = (capacity_for(stored), []) if stored else (0, [([], 0)])
+        if stored:
+            stores = ((self.k_storage, other.k_storage), (self.v_storage, other.v_storage))
+            moves = [(theirs.like(mine, n, capacity), mine.capacity) for mine, theirs in stores]
+            if moves[0][1] == moves[1][1]:
+                moves = [(moves[0][0] + moves[1][0], moves[0][1])]
+            other.k_storage.metadata = dict(self.k_storage.metadata)
+        row_index = page_index = None
+        if rows is not None or pages:
+            index = torch.tensor((rows or []) + (pages or []), dtype=torch.int32).to(device, non_blocking=True)
+            row_index = None if rows is None else index[: len(rows)]
+            page_index = index[len(rows or []):] if pages else None
+        tails = None
+        if left and cut is None:
+            tails = (self._tail_k, self._tail_v, other._tail_k, other._tail_v)
+        for i, (buffers, held) in enumerate(moves):
+            tail = tails if i == 0 else None
+            if buffers or tail:
+                copy_pages(buffers, n, self._num_kv_heads, self._batch_size, row_index, held, capacity,
+                           self.k_storage.block_count if stored else 0, page_index, stored, tail, left, device)
+        if cut is not None:
+            other._decode_to_tail(other, cut)
+
+    def _adopt(self, other: "TurboPolarKVCacheRuntime") -> None:
+        read, spent = self.bytes_read, self.compression_time_ns
+        flag = self._flag if other._batch_size == self._batch_size else None
+        vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch,
+                           "_flag": flag if flag is not None else other._flag})
+
+    def select_rows(self, rows: Sequence[int]) -> None:
+        """Makes batch row i what row ``rows[i]`` was (beams re-ordered, or a batch that grows or
+        shrinks)."""
+        self._adopt(self.fork(rows=rows))
+
+    def keep_pages(self, pages: Sequence[int]) -> None:
+        """Compacts the cache to the stored pages ``pages``, in that order, and the tail; the
+        others' memory is freed.  ``actual_seq_len`` becomes the tokens held."""
+        self._adopt(self.fork(pages=pages))
 
     def reset(self) -> None:
         """turbo_polar_cache.py:379-395."""

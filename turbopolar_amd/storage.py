@@ -31,6 +31,29 @@ def _doublings(capacity: int, needed: int):
     return caps, capacity
 
 
+def capacity_for(needed: int, initial_capacity: int = 4) -> int:
+    """The capacity that the doublings reach for ``needed`` pages."""
+    return _doublings(initial_capacity, needed)[1]
+
+
+def _like(store, names, source, B: int, capacity: int) -> list:
+    """Gives ``store`` buffers of ``source``'s forms for ``B`` batch rows and ``capacity`` pages, on
+    ``source``'s device, their content any.  Returns (source buffer, new one, bytes of a page) of
+    each that holds something, sources made contiguous."""
+    out = []
+    for name in names:
+        old = getattr(source, name)
+        if old is None:
+            continue
+        new = torch.empty((B, old.shape[1], capacity, *old.shape[3:]), dtype=old.dtype, device=old.device)
+        setattr(store, name, new)
+        page = prod(old.shape[3:]) * old.element_size()
+        if page:
+            out.append((old.contiguous(), new, page))
+    store.capacity = capacity
+    return out
+
+
 def _regrow(t: Optional[torch.Tensor], new_cap: int) -> Optional[torch.Tensor]:
     if t is None:
         return None
@@ -170,6 +193,9 @@ class PolarKBlockStorage:
         growth.fill()
         growth.commit()
 
+    def like(self, source: "PolarKBlockStorage", B: int, capacity: int) -> list:
+        return _like(self, _KEY_BUFFERS, source, B, capacity)
+
     def append(self, block: PolarKeyBlock, initial_capacity: int = 4) -> None:
         """Copy one 4-D page into the next slot (storage.py:75-87)."""
         B, H = block.radii.shape[:2]
@@ -237,6 +263,10 @@ class QuantVBlockStorage:
         self.plan(growth, needed, B, H, torch.device(device), initial_capacity)
         growth.fill()
         growth.commit()
+
+    def like(self, source: "QuantVBlockStorage", B: int, capacity: int) -> list:
+        self.group_size = source.group_size
+        return _like(self, _VALUE_BUFFERS, source, B, capacity)
 
     def append(self, block: QuantizedVBlock, initial_capacity: int = 4) -> None:
         """Copy one page ``codes [B,H,1,64,128]`` into the next slot (storage.py:149-158)."""
