@@ -357,7 +357,8 @@ int32_t tp_grow_rows(const tp_grow* bufs, int32_t n_bufs, int64_t rows, void* st
  * q, out: [batch][hq][tq][128], k, v: [batch][hkv][tk][128], all of dtype 0 (fp16)
  * or 1 (bf16), 16-byte aligned, the 128 dimensions contiguous; strides: 12 host
  * values, the (batch, head, token) strides of q, k, v and out in elements, each a
- * multiple of 8 (0 reads one row for all; out's rows must not overlap).
+ * multiple of 8, the token strides of k and v below 2^23 (0 reads one row for all;
+ * out's rows must not overlap).
  * causal: the queries are the last tq of the tk positions, query i sees keys 0 ..
  * tk - tq + i.  A query that sees no key gives 0.  Infinities and NaN in keys and
  * values that a query does not see do not reach it.

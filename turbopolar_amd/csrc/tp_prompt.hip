@@ -73,16 +73,18 @@ __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, i
     }
     const uint64_t found = __ballot(before + upto > tile);
     if (found) {
-      const int w = __ffsll((unsigned long long)found) - 1;
-      t.q0 = __shfl(q0, w);
-      t.nq = __shfl(q1, w) - t.q0;
-      const int first = before + __shfl(upto, w) - __shfl(mine, w), count = __shfl(mine, w);
+      const int w = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)found) - 1);
+      // Values of one lane for all: scalar from here on.
+      t.q0 = __builtin_amdgcn_readlane(q0, w);
+      t.nq = __builtin_amdgcn_readlane(q1, w) - t.q0;
+      const int count = __builtin_amdgcn_readlane(mine, w);
+      const int first = before + __builtin_amdgcn_readlane(upto, w) - count;
       t.k0 = min(max(a.k_starts[base + w], 0), a.tk);
       t.nk = min(max(a.k_starts[base + w + 1], t.k0), a.tk) - t.k0;
       t.row0 = (a.causal ? count - 1 - (tile - first) : tile - first) * kPromptRows;
       return t;
     }
-    before += __shfl(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   t.rest = true;
   t.q0 = min(max(a.q_starts[a.n_seq], 0), a.tq);
@@ -92,140 +94,221 @@ __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, i
   return t;
 }
 
-// A tile's loads of one thread: 16-byte chunks tid + 512 j of 64 rows of 16, keys, then values.
+// A thread's part of a tile of keys or values: 16-byte chunks tid + threads j of 64 rows of 16.
 constexpr int kChunksPerThread = kTileTokens * 16 / kPromptThreads;
-struct PromptLoads {
-  uint4v k[kChunksPerThread], v[kChunksPerThread];
-};
 
-__device__ __forceinline__ void load_tile(const uint16_t* k, const uint16_t* v, int64_t k_t, int64_t v_t, int t0,
-                                          int nk, int tid, PromptLoads& r) {
-#pragma unroll
-  for (int j = 0; j < kChunksPerThread; ++j) {
-    const int x = tid + kPromptThreads * j, c = x & 15;
-    const int64_t t = min(t0 + (x >> 4), nk - 1);
-    r.k[j] = *reinterpret_cast<const uint4v*>(k + t * k_t + 8 * c);
-    r.v[j] = *reinterpret_cast<const uint4v*>(v + t * v_t + 8 * c);
-  }
+// Chunk i of tile j of the n tokens of x, `stride` bytes (below 2^24) apart.  Tiles past the last one
+// repeat it and rows past the last token repeat that: no load is under a branch, at whose join it would
+// be waited for.  The base is scalar, a lane's offset one 24-bit multiply-add.
+__device__ __forceinline__ uint4v load_chunk(const uint16_t* x, uint32_t stride, int j, int n, int tid, int i) {
+  const int t0 = min(j, (n - 1) / kTileTokens) * kTileTokens, last = min(n - 1 - t0, kTileTokens - 1);
+  const char* base = reinterpret_cast<const char*>(x) + (int64_t)t0 * stride;
+  const uint32_t row = min((tid + kPromptThreads * i) >> 4, last);
+  return *reinterpret_cast<const uint4v*>(base + (__umul24(row, stride) + 16u * (tid & 15)));
 }
 
-// Into LDS.  Values past the last key are 0 (their weights are 0, and 0 times an infinity is
-// not); BORDER: infinities and NaN of the others are 0 too, and flagged.
-template <class T, bool BORDER>
-__device__ __forceinline__ bool store_tile(char* kt, char* vt, int t0, int nk, int tid, PromptLoads& r) {
+__device__ __forceinline__ void store_chunk(char* tile, int tid, int i, uint4v x) {
+  const int at = tid + kPromptThreads * i;
+  *reinterpret_cast<uint4v*>(tile + tile_at(at >> 4, at & 15)) = x;
+}
+
+// Values of a tile that some row does not see whole: 0 past the last key (their weights are 0, and
+// 0 times an infinity is not), and for infinities and NaN, which are reported.
+template <class T>
+__device__ __forceinline__ bool clean_part(int t0, int n, int tid, uint4v* r) {
   bool flagged = false;
 #pragma unroll
-  for (int j = 0; j < kChunksPerThread; ++j) {
-    const int x = tid + kPromptThreads * j, at = tile_at(x >> 4, x & 15);
-    *reinterpret_cast<uint4v*>(kt + at) = r.k[j];
-    if constexpr (BORDER) {
-      const bool in = t0 + (x >> 4) < nk;
+  for (int j = 0; j < kChunksPerThread; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = in ? r.v[j][i] : 0u;
-        flagged = flagged || pair_nonfinite<T>(w);
-        r.v[j][i] = pair_finite<T>(w);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = t0 + ((tid + kPromptThreads * j) >> 4) < n ? r[j][i] : 0u;
+      flagged = flagged || pair_nonfinite<T>(w);
+      r[j][i] = pair_finite<T>(w);
     }
-    *reinterpret_cast<uint4v*>(vt + at) = r.v[j];
-  }
   return flagged;
+}
+
+// A barrier that waits for this wave's LDS accesses, not for its loads from memory.
+__device__ __forceinline__ void phase_barrier() { lds_barrier(); }
+
+// The products of a step: the next tile's scores in turn with a tile's weights and values, so that four
+// products lie between two that add to the same registers.  Reads from LDS go out kAhead pairs before the
+// products that take them; the order is held by scheduling barriers (left to itself the compiler puts each
+// read right before its product, which then waits for the LDS every time).  Past the last tile the scores
+// are of whatever the LDS holds, and not used: a second form without them would cost 64 registers more,
+// where the two meet.  beside(i): what is issued under the products of pair i.
+template <class T, class Beside>
+__device__ __forceinline__ void multiply_tile(const char* kt, const char* vt, const TileLane& at, const uint4v* q,
+                                              const uint4v* p, float16v* s, RowState& st, Beside beside) {
+  constexpr int kAhead = 3;
+  auto key = [&](int i) { return lds_read16(kt + (at.k ^ (32 * (i >> 1))) + 32 * (i & 1) * (kHeadDim * 2)); };
+  auto value = [&](int i) {  // 16 tokens of block i % 4 of the dimensions
+    const char* row = vt + 16 * (i >> 2) * (kHeadDim * 2);
+    const uint2v lo = lds_read_tr(row + (at.v ^ (64 * (i & 3))));
+    const uint2v hi = lds_read_tr(row + (at.v ^ (64 * (i & 3) + 32)) + 8 * kHeadDim * 2);
+    return uint4v{lo.x, lo.y, hi.x, hi.y};
+  };
+  uint4v k[kAhead], v[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) k[i] = key(i), v[i] = value(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float16v& sum = s[i & 1];
+    if (i < 2)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[j] = 0.0f;
+    sum = T::mfma(k[i % kAhead], q[i >> 1], sum);
+    if (i + kAhead < 16) k[i % kAhead] = key(i + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+    st.o[i & 3] = T::mfma(v[i % kAhead], p[i >> 2], st.o[i & 3]);
+    if (i + kAhead < 16) v[i % kAhead] = value(i + kAhead);
+    beside(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 template <class T>
 __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(PromptArgs a) {
-  __shared__ __align__(16) char tiles[2][2][kTileBytes];
-  __shared__ int flags[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) char kts[2][kTileBytes], vts[2][kTileBytes];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units;
   const int split = rest % a.splits;
   const PromptTile t = find_tile(a, rest / a.splits, lane);
   const int64_t b = unit / a.hkv, kv = unit % a.hkv;
 
   // The lane's row, and how many keys of its sequence it sees.
-  const int row = t.row0 + kWaveRows * wave + (lane & 31);
-  const int tok = row / a.g, head = row - tok * a.g;
-  const bool live = tok < t.nq;
   auto keys_of = [&](int i) { return i >= t.nq ? 0 : a.causal ? min(max(t.nk - t.nq + i + 1, 0), t.nk) : t.nk; };
+  const int wave_row = t.row0 + kWaveRows * wave, row = wave_row + (lane & 31);
+  const int tok = row / a.g, head = row - tok * a.g;
   const int limit = keys_of(tok);
-  // Of the workgroup's rows: the fewest and the most (the last live row's).
+  // Of the workgroup's rows: the fewest and the most (the last live row's).  Rows past the last
+  // query compute what they like and are not stored.
   const int last_tok = min((t.row0 + kPromptRows - 1) / a.g, t.nq - 1);
   const int most = last_tok < 0 ? 0 : keys_of(last_tok), fewest = keys_of(t.row0 / a.g);
   // Of the wave's.
-  const int wave_row = t.row0 + kWaveRows * wave;
-  const int wave_last = min((wave_row + kWaveRows - 1) / a.g, t.nq - 1);
-  const int wave_most = wave_row / a.g >= t.nq ? 0 : keys_of(wave_last);
-  const int wave_fewest = (wave_row + kWaveRows - 1) / a.g >= t.nq ? 0 : keys_of(wave_row / a.g);
+  const int wave_most = wave_row / a.g >= t.nq ? 0 : keys_of(min((wave_row + kWaveRows - 1) / a.g, t.nq - 1));
+  const int wave_fewest = keys_of(wave_row / a.g);
 
-  // This split's tiles of keys, of those that the whole sequence has.
+  // This split's tiles of keys, of those that the whole sequence has; the wave's end of them.
   const int all = (t.nk + kTileTokens - 1) / kTileTokens, each = (all + a.splits - 1) / a.splits;
   const int first = split * each, end = min(min(first + each, all), (most + kTileTokens - 1) / kTileTokens);
+  const int wave_end = min(end, (wave_most + kTileTokens - 1) / kTileTokens);
 
-  RowState st;
+  RowState rows[1];
+  RowState& st = rows[0];
   st.clear();
   if (first < end) {
     const uint16_t* k = a.k + b * a.k_b + kv * a.k_h + (int64_t)t.k0 * a.k_t;
     const uint16_t* v = a.v + b * a.v_b + kv * a.v_h + (int64_t)t.k0 * a.v_t;
-    uint4v q[8];
-    const int64_t qt = t.q0 + (live ? tok : 0);
-    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, live, a.flip, lane, q);
+    const uint32_t k_t = (uint32_t)a.k_t * 2, v_t = (uint32_t)a.v_t * 2;
+    static_assert(kChunksPerThread == 2, "two chunks of keys and two of values a thread");
+    uint4v kr[4], vr[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kr[i] = load_chunk(k, k_t, first + (i >> 1), t.nk, tid, i & 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) vr[i] = load_chunk(v, v_t, first, t.nk, tid, i);
+    uint4v q[1][8];
+    const int64_t qt = t.q0 + min(tok, t.nq - 1);  // first < end: there is a query
+    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, tok < t.nq, a.flip, lane, q[0]);
     const TileLane at(lane);
-    if (tid < 2) flags[tid] = 0;
-    PromptLoads r;
-    load_tile(k, v, a.k_t, a.v_t, first * kTileTokens, t.nk, tid, r);
+    auto clean = [&](int j) {  // where some row does not see all of tile j
+      if ((j + 1) * kTileTokens > fewest && clean_part<T>(j * kTileTokens, t.nk, tid, vr)) flag = 1;
+    };
+    // Tile j + 2's keys and j + 1's values to LDS, and the loads of those after them: piece i of 8.
+    auto stage = [&](int j, int i) {
+      const int c = i & 1;
+      if (i < 2)
+        store_chunk(kts[j & 1], tid, c, kr[c]);
+      else if (i < 4)
+        store_chunk(vts[(j + 1) & 1], tid, c, vr[c]);
+      else if (i < 6)
+        kr[c] = load_chunk(k, k_t, j + 3, t.nk, tid, c);
+      else
+        vr[c] = load_chunk(v, v_t, j + 2, t.nk, tid, c);
+    };
+    // The waves of a SIMD are w and w + 4: the second four run one phase behind the first.
+    const int behind = __builtin_amdgcn_readfirstlane(tid / (kPromptThreads / 2));
+    if (tid == 0) flag = 0;
     __syncthreads();
+    clean(first);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_chunk(kts[(first + (i >> 1)) & 1], tid, i & 1, kr[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      store_chunk(vts[first & 1], tid, i, vr[i]);
+      kr[i] = load_chunk(k, k_t, first + 2, t.nk, tid, i);
+      vr[i] = load_chunk(v, v_t, first + 1, t.nk, tid, i);
+    }
+    __syncthreads();
+    float16v s[1][2];
+    if (first < wave_end) score_tile<T, 1, 2>(kts[first & 1], 0, at, q, s);
+    if (behind) phase_barrier();
+    // Two phases a tile, a barrier after each: the softmax, and the products.  While one wave of a SIMD
+    // multiplies, the other runs its softmax (in step, 41 % of the time went to products and almost all of
+    // the rest to softmax).  The next tiles go to LDS under the products, into the buffers that both
+    // halves of the waves have left by then.
     for (int j = first; j < end; ++j) {
-      const int t0 = j * kTileTokens, buf = j & 1;
-      char *kt = tiles[buf][0], *vt = tiles[buf][1];
-      const bool border = t0 + kTileTokens > fewest;  // some row of the workgroup does not see all of it
-      if (border) {
-        if (store_tile<T, true>(kt, vt, t0, t.nk, tid, r)) flags[buf] = 1;
+      uint4v p[4];
+      if (j < wave_end) {
+        if ((j + 1) * kTileTokens > wave_fewest) mask_scores<2>(s[0], limit - 4 * (lane >> 5) - j * kTileTokens);
+        rescale<1, 2>(s, a.c, rows);
+        weigh<T, 2>(s[0], a.c, p, st);
+      }
+      clean(j + 1);
+      phase_barrier();
+      if (j < wave_end) {
+        __builtin_amdgcn_s_setprio(1);
+        multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q[0], p, s[0], st, [&](int i) {
+          if (i >= 2 && i < 10) stage(j, i - 2);
+        });
+        __builtin_amdgcn_s_setprio(0);
       } else {
-        store_tile<T, false>(kt, vt, t0, t.nk, tid, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) stage(j, i);
       }
-      __syncthreads();
-      if (j + 1 < end) load_tile(k, v, a.k_t, a.v_t, t0 + kTileTokens, t.nk, tid, r);
-      if (t0 < wave_most) {
-        if (t0 + kTileTokens <= wave_fewest)
-          attend_tile<T, 2, false>(kt, vt, 0, at, q, a.c, st, lane, [](int) { return true; });
-        else
-          attend_tile<T, 2, true>(kt, vt, 0, at, q, a.c, st, lane, [&](int x) { return t0 + x < limit; });
-        if (border && flags[buf])
-          add_nonfinite<T>(st, lane, min(kTileTokens, t.nk - t0), [&](int x) { return t0 + x < limit; },
-                           [&](int x) { return v + (int64_t)(t0 + x) * a.v_t; });
-      }
+      phase_barrier();
+    }
+    if (!behind) phase_barrier();
+    if (flag) {
+      const int t0 = max(fewest / kTileTokens, first) * kTileTokens;  // the first tile with a border
+      add_nonfinite<T>(st, lane, min(end * kTileTokens, t.nk) - t0, [&](int x) { return t0 + x < limit; },
+                       [&](int x) { return v + (int64_t)(t0 + x) * a.v_t; });
     }
   }
   const float l = across_halves(st.l, [](float x, float y) { return x + y; });
   const int64_t out_t = t.q0 + tok;
+  const bool live = tok < t.nq;
   if (a.splits > 1) {
     const int64_t rec = (((int64_t)unit * a.tq + out_t) * a.g + head) * a.splits + split;
-    store_record(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
+    store_record<false>(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
   } else if (!(t.rest && a.keep_rest)) {
     store_row<T>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + out_t * a.out_t,
                  live, lane);
   }
 }
 
-// Joins the splits of a row: weights l_s 2^(m_s - max) over their sum, two dimensions a lane, a
-// wave a row.  Records with a sum of 0 (nothing seen) are not read.
-template <class T>
+// Joins the splits of a row: weights l_s 2^(m_s - max) over their sum, a wave a row.  A record's 16
+// bytes a lane: 16 lanes (fp16) or 32 (fp32) take one, so 4 or 2 records go by side by side and are
+// folded at the end, 8 such steps in flight.
+template <class T, bool HALF>
 __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
-  const int lane = threadIdx.x & 63;
+  constexpr int kLanes = HALF ? 16 : 32, kSide = 64 / kLanes, kDims = kHeadDim / kLanes, kAhead = 8;
+  const int lane = threadIdx.x & 63, part = lane / kLanes, d0 = lane % kLanes * kDims;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= (int64_t)a.units * a.rows) return;
   const int64_t unit = i / a.rows, row = i - unit * a.rows;
   const int64_t tok = row / a.g, head = row - tok * a.g;
   if (a.rest_from && tok >= *a.rest_from) return;
   const float* ml = a.ml + i * a.splits * 2;
-  const float* o = a.o + i * a.splits * kHeadDim + 2 * lane;
-  float m = -INFINITY, l = 0.0f;
-  float2v acc = {0.0f, 0.0f};
+  const char* o = static_cast<const char*>(a.o) + (i * a.splits * kHeadDim + d0) * (HALF ? 2 : 4);
+  float m = -INFINITY, l = 0.0f, acc[kDims] = {};
   for (int base = 0; base < a.splits; base += 64) {
     const int n = min(64, a.splits - base);
     float2v mine = {-INFINITY, 0.0f};
     if (lane < n) mine = *reinterpret_cast<const float2v*>(ml + 2 * (base + lane));
-    if (mine.y == 0.0f) mine.x = -INFINITY;
+    if (mine.y == 0.0f) mine.x = -INFINITY;  // saw nothing
     float top = mine.x;
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -235,26 +318,58 @@ __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     const float alpha = __builtin_amdgcn_exp2f(m - to);
-    acc *= alpha;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] *= alpha;
     l = l * alpha + sum;
     m = next;
-    for (int s = 0; s < n; ++s) {
-      const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
-      if (ws != 0.0f) acc += ws * *reinterpret_cast<const float2v*>(o + (int64_t)(base + s) * kHeadDim);
+    for (int s0 = 0; s0 < n; s0 += kAhead * kSide) {
+      uint4v x[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int s = min(s0 + kSide * j + part, n - 1);
+        x[j] = *reinterpret_cast<const uint4v*>(o + (int64_t)(base + s) * kHeadDim * (HALF ? 2 : 4));
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int s = s0 + kSide * j + part;
+        const float ws = s < n ? __shfl(w, s & 63) : 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          float v;
+          if constexpr (HALF)
+            v = h2f((uint16_t)(x[j][d >> 1] >> (16 * (d & 1))));
+          else
+            v = __uint_as_float(x[j][d]);
+          acc[d] += ws != 0.0f ? ws * v : 0.0f;
+        }
+      }
     }
   }
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int step = kLanes; step < 64; step <<= 1) acc[d] += __shfl_xor(acc[d], step);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* out = a.out + (unit / a.hkv) * a.out_b + ((unit % a.hkv) * a.g + head) * a.out_h + tok * a.out_t;
-  *reinterpret_cast<uint32_t*>(out + 2 * lane) = T::pack(acc.x * inv, acc.y * inv);
+  if (part != 0) return;
+  uint16_t* out = a.out + (unit / a.hkv) * a.out_b + ((unit % a.hkv) * a.g + head) * a.out_h + tok * a.out_t + d0;
+  uint32_t y[kDims / 2];
+#pragma unroll
+  for (int d = 0; d < kDims / 2; ++d) y[d] = T::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+  if constexpr (HALF)
+    *reinterpret_cast<uint4v*>(out) = uint4v{y[0], y[1], y[2], y[3]};
+  else
+    *reinterpret_cast<uint2v*>(out) = uint2v{y[0], y[1]};
 }
 
-int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s) {
+int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s) {
   const int64_t rows = (int64_t)a.units * a.rows;
   const dim3 grid((unsigned)((rows + 3) / 4));
-  if (bf16)
-    hipLaunchKernelGGL((join_splits_kernel<BF16>), grid, dim3(256), 0, s, a);
+  if (half_records)
+    hipLaunchKernelGGL((join_splits_kernel<F16, true>), grid, dim3(256), 0, s, a);
+  else if (bf16)
+    hipLaunchKernelGGL((join_splits_kernel<BF16, false>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((join_splits_kernel<F16>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_splits_kernel<F16, false>), grid, dim3(256), 0, s, a);
   return launch_status("join of the splits");
 }
 
@@ -321,8 +436,9 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
     set_error("q, k, v and out must be non-NULL 16-byte aligned buffers");
     return TP_ERR_INVALID;
   }
-  if (!strides || !strides_ok(strides, 12)) {
-    set_error("strides must be non-negative multiples of 8 elements");
+  // Keys' and values' offsets within a tile are 24-bit products.
+  if (!strides || !strides_ok(strides, 12) || strides[5] >= (1 << 23) || strides[8] >= (1 << 23)) {
+    set_error("strides must be non-negative multiples of 8 elements, the token strides of k and v below 2^23");
     return TP_ERR_INVALID;
   }
   if (!(scale == scale) || scale - scale != 0.0f) {
@@ -381,5 +497,5 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.splits, j.g = g, j.hkv = hkv;
   j.rest_from = n_seq && keep_rest ? q_starts + n_seq : nullptr;
-  return launch_join(j, dtype != 0, s);
+  return launch_join(j, dtype != 0, false, s);
 }

@@ -15,8 +15,10 @@
 // same tokens.
 //
 // Tiles lie in LDS as rows of 256 bytes, 16-byte chunk c of row t at chunk c ^
-// tile_swizzle(t): the 8 lanes that read 16 bytes of 8 key rows together, and the 16
-// that read a 4-token by 16-dimension block of values, hit all banks once.
+// tile_swizzle(t), which is another one for each 16 rows in turn (16 lanes read one chunk
+// of 16 key rows together) and moves 4 rows in turn by 4 chunks (32 lanes read 4 chunks of
+// 4 value rows together), so that both reads hit every bank once.  With 8 chunks in turn
+// both took twice the cycles (42 % of the prompt kernel's LDS time was conflicts).
 #pragma once
 
 #include "tp_common.h"
@@ -36,7 +38,7 @@ constexpr int kTileBytes = kTileTokens * kHeadDim * 2;
 constexpr int kWaveRows = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-__host__ __device__ inline int tile_swizzle(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
+__host__ __device__ inline int tile_swizzle(int t) { return ((t & 3) << 2) | ((t >> 2) & 3); }
 // Byte offset of 16-byte chunk c of token t.
 __host__ __device__ inline int tile_at(int t, int c) { return t * (kHeadDim * 2) + ((c ^ tile_swizzle(t)) << 4); }
 
@@ -131,79 +133,131 @@ struct TileLane {
   }
 };
 
-// The queries of a row as the B operand: q[ks] holds dimensions 16 ks + 8 h .. + 7.
+// The queries of a row as the B operand: q[ks] holds dimensions 16 ks + 8 h .. + 7; zeros where
+// the row is not live (`row` is then some other row's: the loads are not under a branch, whose
+// join would wait for each of them in turn).
 __device__ __forceinline__ void load_query(const uint16_t* row, bool live, uint32_t flip, int lane, uint4v* q) {
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) {
-    uint4v w = {0u, 0u, 0u, 0u};
-    if (live) w = *reinterpret_cast<const uint4v*>(row + 16 * ks + 8 * (lane >> 5));
-    q[ks] = w ^ flip;
+  for (int ks = 0; ks < 8; ++ks) q[ks] = *reinterpret_cast<const uint4v*>(row + 16 * ks + 8 * (lane >> 5));
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) q[ks] = live ? q[ks] ^ flip : uint4v{0u, 0u, 0u, 0u};
+}
+
+// Scores of NB blocks of 32 tokens from token t0 of a tile of keys with RB blocks of 32 rows.
+template <class T, int RB, int NB>
+__device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLane& at, const uint4v (&q)[RB][8],
+                                           float16v (&s)[RB][NB]) {
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[rb][nb][i] = 0.0f;
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int off = (at.k ^ (32 * ks)) + (t0 + 32 * nb) * (kHeadDim * 2);
+      const uint4v key = lds_read16(kt + off);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb][nb] = T::mfma(key, q[rb][ks], s[rb][nb]);
+    }
+}
+
+// Scores of tokens from `limit` on masked; limit counts from the lane's first token of the tile (4 (lane /
+// 32)), so that the tokens it is compared with are constants.
+template <int NB>
+__device__ __forceinline__ void mask_scores(float16v* s, int limit) {
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[nb][i] = 32 * nb + 8 * (i >> 2) + (i & 3) < limit ? s[nb][i] : -INFINITY;
+}
+
+// The running maximum (of c times the scores, c > 0) moved to hold a tile's scores.  It moves only
+// where some row of the wave grew by more than kSlack, so that most tiles need no rescaling: a weight
+// is then at most 2^kSlack, which neither its 16 bits nor the sums in fp32 mind (their roundings are
+// relative).
+constexpr float kSlack = 8.0f;
+template <int RB, int NB>
+__device__ __forceinline__ void rescale(const float16v (&s)[RB][NB], float c, RowState (&st)[RB]) {
+  float top[RB];
+  bool grown = false;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    float x = s[rb][0][0];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x = fmaxf(x, s[rb][nb][i]);
+    top[rb] = across_halves(x, [](float u, float w) { return fmaxf(u, w); }) * c;
+    grown = grown || top[rb] > st[rb].m + kSlack;  // -inf: a row that has seen nothing yet
+  }
+  if (__any(grown)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float m = fmaxf(st[rb].m, top[rb]);
+      const float alpha = __builtin_amdgcn_exp2f(st[rb].m - (m == -INFINITY ? 0.0f : m));
+      st[rb].m = m;
+      st[rb].l *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[rb].o[db][i] *= alpha;
+    }
   }
 }
 
-// One pass over NB blocks of 32 tokens from token t0 of a tile: scores, running maximum
-// and sum, weights, values.  seen(token): whether the lane's row sees a token of the
-// tile (asked where MASKED only).  c: scale * log2(e), positive.
-template <class T, int NB, bool MASKED, class Seen>
-__device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int t0, const TileLane& at, const uint4v* q,
-                                            float c, RowState& st, int lane, Seen seen) {
-  float16v s[NB];
+// The product of packed weights with NK runs of 16 values from token t0.
+template <class T, int NK>
+__device__ __forceinline__ void add_values(const char* vt, int t0, const TileLane& at, const uint4v (&p)[NK],
+                                           RowState& st) {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
+  for (int k = 0; k < NK; ++k)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[nb][i] = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      const int off = (at.k ^ (32 * (ks & 3))) + 128 * (ks >> 2) + (t0 + 32 * nb) * (kHeadDim * 2);
-      s[nb] = T::mfma(lds_read16(kt + off), q[ks], s[nb]);
+    for (int db = 0; db < 4; ++db) {
+      // 8 rows on, the swizzle differs by 2 chunks.
+      const char* row = vt + (t0 + 16 * k) * (kHeadDim * 2);
+      const uint2v lo = lds_read_tr(row + (at.v ^ (64 * db)));
+      const uint2v hi = lds_read_tr(row + (at.v ^ (64 * db + 32)) + 8 * kHeadDim * 2);
+      st.o[db] = T::mfma(uint4v{lo.x, lo.y, hi.x, hi.y}, p[k], st.o[db]);
     }
+}
+
+// Weights of a tile's scores, packed as the second product takes them, and their sum.
+template <class T, int NB>
+__device__ __forceinline__ void weigh(const float16v* s, float c, uint4v* p, RowState& st) {
+  const float base = st.m == -INFINITY ? 0.0f : st.m;
+#pragma unroll
+  for (int i = 0; i < 8 * NB; ++i) {
+    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 3][2 * (i & 7)], c, -base));
+    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 3][2 * (i & 7) + 1], c, -base));
+    st.l += x;
+    st.l += y;
+    p[i >> 2][i & 3] = T::pack(x, y);
+    if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // scores give way to weights four pairs at a time
   }
+}
+
+// One pass over NB blocks of 32 tokens from token t0 of a tile.  seen(token): whether the lane's row sees
+// a token of the tile (asked where MASKED only).
+template <class T, int NB, bool MASKED, class Seen>
+__device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int t0, const TileLane& at,
+                                            const uint4v (&q)[1][8], float c, RowState (&st)[1], int lane, Seen seen) {
+  float16v s[1][NB];
+  score_tile<T, 1, NB>(kt, t0, at, q, s);
   if constexpr (MASKED) {
     const int h4 = 4 * (lane >> 5);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (!seen(t0 + 32 * nb + 8 * (i >> 2) + (i & 3) + h4)) s[nb][i] = -INFINITY;
+        if (!seen(t0 + 32 * nb + 8 * (i >> 2) + (i & 3) + h4)) s[0][nb][i] = -INFINITY;
   }
-  float top = s[0][0];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
-  top = across_halves(top, [](float x, float y) { return fmaxf(x, y); });
-  const float m = fmaxf(st.m, top * c);
-  const float base = m == -INFINITY ? 0.0f : m;  // a row that has seen nothing yet
-  const float alpha = __builtin_amdgcn_exp2f(st.m - base);
-  float sum = 0.0f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][i], c, -base));
-      sum += s[nb][i];
-    }
-  st.m = m;
-  st.l = st.l * alpha + sum;
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      uint4v p;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = T::pack(s[nb][8 * kk + 2 * j], s[nb][8 * kk + 2 * j + 1]);
-      const int row = (t0 + 32 * nb + 16 * kk) * (kHeadDim * 2);
-#pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        const char* a = vt + (at.v ^ (64 * (db & 1))) + 128 * (db >> 1) + row;
-        const uint2v lo = lds_read_tr(a), hi = lds_read_tr(a + 8 * kHeadDim * 2);
-        st.o[db] = T::mfma(uint4v{lo.x, lo.y, hi.x, hi.y}, p, st.o[db]);
-      }
-    }
+  rescale<1, NB>(s, c, st);
+  uint4v p[2 * NB];
+  weigh<T, NB>(s[0], c, p, st[0]);
+  add_values<T>(vt, t0, at, p, st[0]);
 }
 
 // Infinities and NaN among the values of a tile that some rows do not see: a product
@@ -247,26 +301,32 @@ __device__ __forceinline__ void store_row(const RowState& st, float inv, uint16_
     }
 }
 
-// A split's record of a row: its output divided by its sum, in fp32, with the maximum
-// (log2 units) and the sum.  Splits of a row are joined by join_splits_kernel.
-__device__ __forceinline__ void store_record(const RowState& st, float l, float* o, float* ml, bool live, int lane) {
+// A split's record of a row: its output divided by its sum, with the maximum (log2 units) and the
+// sum in fp32.  Splits of a row are joined by join_splits_kernel.  HALF: the output in fp16, for
+// half the bytes written and read back; each record's rounding (half a step, 2^-11) is weighted
+// by the record's share, so it stays below the result's own.
+template <bool HALF>
+__device__ __forceinline__ void store_record(const RowState& st, float l, void* o, float* ml, bool live, int lane) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (!live) return;
+  if constexpr (HALF) {
+    store_row<F16>(st, inv, static_cast<uint16_t*>(o), live, lane);
+  } else if (live) {
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const float4v x = {st.o[db][4 * a] * inv, st.o[db][4 * a + 1] * inv, st.o[db][4 * a + 2] * inv,
-                         st.o[db][4 * a + 3] * inv};
-      *reinterpret_cast<float4v*>(o + 32 * db + 8 * a + 4 * (lane >> 5)) = x;
-    }
-  if (lane < 32) *reinterpret_cast<float2v*>(ml) = float2v{st.m, l};
+      for (int a = 0; a < 4; ++a) {
+        const float4v x = {st.o[db][4 * a] * inv, st.o[db][4 * a + 1] * inv, st.o[db][4 * a + 2] * inv,
+                           st.o[db][4 * a + 3] * inv};
+        *reinterpret_cast<float4v*>(static_cast<float*>(o) + 32 * db + 8 * a + 4 * (lane >> 5)) = x;
+      }
+  }
+  if (live && lane < 32) *reinterpret_cast<float2v*>(ml) = float2v{st.m, l};
 }
 
 // Where the splits' records are and where the joined rows go.  Rows are counted as
 // (token, head of the group) per unit = (batch, kv head).
 struct JoinArgs {
-  const float* o;   // [units][rows][splits][128]
+  const void* o;    // [units][rows][splits][128], fp16 or fp32
   const float* ml;  // [units][rows][splits][2]
   uint16_t* out;
   int64_t rows;     // per unit
@@ -275,6 +335,6 @@ struct JoinArgs {
   const int32_t* rest_from;  // tokens from *rest_from on are left as they are (NULL: none)
 };
 
-int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s);
+int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s);
 
 }  // namespace tp

@@ -51,7 +51,7 @@ struct TreeArgs {
   float c;
   uint32_t flip;
   int32_t pages_per_split, page_splits, records;
-  float* part_o;
+  uint16_t* part_o;
   float* part_ml;
 };
 
@@ -64,8 +64,8 @@ struct PageRegs {
   uint2v c8[KIND == kTreeFast ? N : 1];
   uint32_t c4[KIND == kTreeDefault ? N : 1];
   uint4v v[N];
-  uint16_t vs[N];
-  uint16_t ls;
+  uint32_t vs[N];  // fp16 scale of the run's group
+  uint32_t ls;     // fp16 page scale
 };
 
 template <int KIND, int N, int THREADS>
@@ -110,7 +110,7 @@ __device__ __forceinline__ void decode_page(const TreeArgs& a, const TreeLut& lu
         e[2 * i + 1] = pack_h2(hi_hi(p.r[n][i]) * __builtin_bit_cast(half2v, cs.y));
       }
     } else {
-      const float ls = tree_i8(KIND) ? h2f(p.ls) : 0.0f;
+      const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t code;
@@ -156,27 +156,32 @@ __device__ __forceinline__ void decode_page(const TreeArgs& a, const TreeLut& lu
   }
 }
 
-// 64 dense tokens from k, v (t strides in elements) into the tiles; rows from `count` on are 0,
-// infinities and NaN among the values too, and reported.
+// 64 dense tokens from k, v (t strides in elements) into the tiles; rows from `count` on repeat the
+// last key (masked) and hold values of 0, as infinities and NaN among the values do, which are
+// reported.
 template <int THREADS>
 __device__ __forceinline__ bool dense_tile(const uint16_t* k, const uint16_t* v, int64_t k_t, int64_t v_t, int count,
                                            int tid, char* kt, char* vt) {
+  constexpr int N = kTileTokens * 16 / THREADS;
+  uint4v kw[N], vw[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int x = tid + THREADS * n, t = min(x >> 4, count - 1), c = x & 15;
+    kw[n] = *reinterpret_cast<const uint4v*>(k + t * k_t + 8 * c);
+    vw[n] = *reinterpret_cast<const uint4v*>(v + t * v_t + 8 * c);
+  }
   bool flagged = false;
 #pragma unroll
-  for (int x = tid; x < kTileTokens * 16; x += THREADS) {
-    const int t = x >> 4, c = x & 15;
-    uint4v kw = {0u, 0u, 0u, 0u}, vw = kw;
-    if (t < count) {
-      kw = *reinterpret_cast<const uint4v*>(k + t * k_t + 8 * c);
-      vw = *reinterpret_cast<const uint4v*>(v + t * v_t + 8 * c);
-    }
+  for (int n = 0; n < N; ++n) {
+    const int x = tid + THREADS * n, t = x >> 4, c = x & 15;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      flagged = flagged || pair_nonfinite<F16>(vw[i]);
-      vw[i] = pair_finite<F16>(vw[i]);
+      const uint32_t w = t < count ? vw[n][i] : 0u;
+      flagged = flagged || pair_nonfinite<F16>(w);
+      vw[n][i] = pair_finite<F16>(w);
     }
-    *reinterpret_cast<uint4v*>(kt + tile_at(t, c)) = kw;
-    *reinterpret_cast<uint4v*>(vt + tile_at(t, c)) = vw;
+    *reinterpret_cast<uint4v*>(kt + tile_at(t, c)) = kw[n];
+    *reinterpret_cast<uint4v*>(vt + tile_at(t, c)) = vw[n];
   }
   return flagged;
 }
@@ -201,13 +206,15 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
 
   const int row = (block * RW + rw) * kWaveRows + (lane & 31);
   const int node = row / a.g, head = row - node * a.g;
-  const uint64_t* mask = a.mask + b * a.mask_b + (int64_t)node * a.words;
   const bool live = works && node < a.nodes;
-  const bool real = live && ((mask[node >> 6] >> (node & 63)) & 1u);
-  uint4v q[8];
-  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + node * a.q_t, real, a.flip, lane, q);
+  const int at_node = min(node, a.nodes - 1);  // loads of rows past the last node repeat it
+  const uint64_t* mask = a.mask + b * a.mask_b + (int64_t)at_node * a.words;
+  const bool real = live && ((mask[at_node >> 6] >> (at_node & 63)) & 1u);
+  uint4v qs[1][8];
+  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, real, a.flip, lane, qs[0]);
   const TileLane at(lane);
-  RowState st;
+  RowState rows[1];
+  RowState& st = rows[0];
   st.clear();
 
   const int64_t slot0 = (int64_t)unit * a.capacity;
@@ -231,9 +238,10 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
     for (int buf = 0; page < page_end; ++page, buf ^= 1) {
       decode_page<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, tiles[buf][0], tiles[buf][1]);
       __syncthreads();
-      if (page + 1 < page_end) load_page<KIND, N, THREADS>(a, slot0 + page + 1, tid, p);
+      // The last page again rather than none: a load under a branch is waited for at its join.
+      load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
       if (works)
-        attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, q, a.c, st, lane,
+        attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, qs, a.c, rows, lane,
                                     [](int) { return true; });
     }
   }
@@ -260,7 +268,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         const uint64_t there = count < 64 ? (1ull << count) - 1ull : ~0ull;
         const uint64_t sees = !real ? 0ull : j < 0 ? there : mask[j] & there;
         auto seen = [&](int x) { return ((sees >> x) & 1u) != 0; };
-        attend_tile<F16, NB, true>(tiles[0][0], tiles[0][1], 32 * tw, at, q, a.c, st, lane, seen);
+        attend_tile<F16, NB, true>(tiles[0][0], tiles[0][1], 32 * tw, at, qs, a.c, rows, lane, seen);
         if (flag)
           add_nonfinite<F16>(st, lane, count, [&](int x) { return seen(x) && (TW == 1 || (x >> 5) == tw); },
                              [&](int x) { return v + x * v_t; });
@@ -296,7 +304,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   const float l = across_halves(st.l, [](float x, float y) { return x + y; });
   if (a.records > 1) {
     const int64_t rec = ((int64_t)unit * a.nodes * a.g + row) * a.records + record;
-    store_record(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
+    store_record<true>(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
   } else {
     store_row<F16>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + node * a.out_t,
                    live, lane);
@@ -337,7 +345,7 @@ using namespace tp;
 extern "C" size_t tp_tree_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t nodes, int32_t n_pages) {
   if (batch < 1 || hkv < 1 || hq < hkv || hq % hkv || nodes < 1 || nodes > kTreeMaxNodes || n_pages < 0) return 0;
   const TreePlan p = plan_tree(batch * hkv, (int64_t)nodes * (hq / hkv), n_pages);
-  return p.records == 1 ? 0 : (size_t)batch * hq * nodes * p.records * (kHeadDim + 2) * sizeof(float);
+  return p.records == 1 ? 0 : (size_t)batch * hq * nodes * p.records * (kHeadDim * sizeof(uint16_t) + 2 * sizeof(float));
 }
 
 extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, int32_t hq, int32_t hkv, int32_t nodes,
@@ -451,8 +459,8 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
       set_error("workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace_bytes);
       return TP_ERR_WORKSPACE;
     }
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)units * rows * a.records * kHeadDim;
+    a.part_o = static_cast<uint16_t*>(workspace);
+    a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)units * rows * a.records * kHeadDim);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(units * p.row_blocks * p.records));
@@ -475,5 +483,5 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
   j.rows = rows;
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.records, j.g = a.g, j.hkv = hkv;
-  return launch_join(j, false, s);
+  return launch_join(j, false, true, s);
 }

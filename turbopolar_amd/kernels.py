@@ -558,11 +558,12 @@ def _no_grad(*tensors: torch.Tensor) -> None:
 
 def _strided(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
     """``t`` ``[B, H, T, 128]`` as a kernel reads it in place, and its (batch, head, token)
-    strides: rows of 128 contiguous elements, 16 bytes aligned.  Anything else is copied."""
+    strides: rows of 128 contiguous elements, 16 bytes aligned, tokens less than 2^23
+    elements apart.  Anything else is copied."""
     B, H, T, _ = t.shape
     s0, s1, s2, s3 = t.stride()
     s0, s1, s2 = s0 if B > 1 else 0, s1 if H > 1 else 0, s2 if T > 1 else 0
-    if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15:
+    if s3 != 1 or (s0 | s1 | s2) & 7 or s2 >= 1 << 23 or t.data_ptr() & 15:
         t = _fresh(t)
         s0, s1, s2, _ = t.stride()
     return t, (s0, s1, s2)
