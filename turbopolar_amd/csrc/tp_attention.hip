@@ -78,27 +78,6 @@ __device__ unsigned long long g_timeline[kTimelineGroups][kTimelineStamps];
 enum LayoutKind { kKindDefault = 0, kKindFast = 1, kKindAnyF16 = 2, kKindDefaultHR = 3, kKindAnyI8 = 4, kKindNone = 5 };
 constexpr bool any_kind(int kind) { return kind == kKindAnyF16 || kind == kKindAnyI8; }
 
-// Division by a launch constant d as a multiply and a shift: for n < 2^31,
-// l = ceil(log2 d) and m = floor(2^(31+l) / d) + 1 (< 2^32), floor(n / d) =
-// (n * m) >> (31 + l) (Granlund and Montgomery, PLDI 1994, theorem 4.2:
-// 2^(31+l) < m d <= 2^(31+l) + 2^l).  Three scalar instructions instead of
-// the ~30-instruction integer division, on the decode kernel's critical
-// path before its first page load.
-struct FastDiv {
-  uint32_t m;
-  uint32_t sh;
-};
-
-static inline FastDiv make_fastdiv(uint32_t d) {
-  uint32_t l = 0;
-  while ((1ull << l) < d) ++l;
-  return FastDiv{(uint32_t)(((1ull << (31 + l)) / d) + 1), 31 + l};
-}
-
-__host__ __device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv f) {
-  return (uint32_t)(((uint64_t)n * f.m) >> f.sh);
-}
-
 struct AttnArgs {
   const uint16_t* q;
   uint16_t* out;

@@ -13,14 +13,12 @@
 // Few tiles of rows: the keys are split over workgroups too, and joined by a second
 // launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "tp_tiles.h"
 
 namespace tp {
 
-constexpr int kPromptWaves = 8;
-constexpr int kPromptRows = kPromptWaves * kWaveRows;
-constexpr int kPromptThreads = kPromptWaves * 64;
 constexpr int kPromptTarget = 256;  // workgroups that fill the GPU
 
 struct PromptArgs {
@@ -36,9 +34,10 @@ struct PromptArgs {
   int32_t n_seq;  // 0: one sequence a batch row
   int32_t keep_rest;
   int32_t tiles, splits;
+  FastDiv div_units, div_splits, div_hkv, div_g;
   float c;        // |scale| log2(e)
   uint32_t flip;  // sign bits of a pair where the scale is negative
-  float* part_o;
+  float* part_o;  // fp16 or fp32 records (store_record)
   float* part_ml;
 };
 
@@ -48,12 +47,13 @@ struct PromptTile {
   bool rest;  // tokens behind the last sequence
 };
 
+template <int ROWS>
 __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, int lane) {
   PromptTile t;
   t.rest = false;
   if (a.n_seq == 0) {
     t.q0 = 0, t.nq = a.tq, t.k0 = 0, t.nk = a.tk;
-    t.row0 = (a.causal ? a.tiles - 1 - tile : tile) * kPromptRows;  // the longest first
+    t.row0 = (a.causal ? a.tiles - 1 - tile : tile) * ROWS;  // the longest first
     return t;
   }
   int before = 0;  // tiles of the sequences before
@@ -64,7 +64,7 @@ __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, i
       q0 = min(max(a.q_starts[i], 0), a.tq);
       q1 = min(max(a.q_starts[i + 1], q0), a.tq);
     }
-    const int mine = (int)(((int64_t)(q1 - q0) * a.g + kPromptRows - 1) / kPromptRows);
+    const int mine = (int)(((int64_t)(q1 - q0) * a.g + ROWS - 1) / ROWS);
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -81,7 +81,7 @@ __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, i
       const int first = before + __builtin_amdgcn_readlane(upto, w) - count;
       t.k0 = min(max(a.k_starts[base + w], 0), a.tk);
       t.nk = min(max(a.k_starts[base + w + 1], t.k0), a.tk) - t.k0;
-      t.row0 = (a.causal ? count - 1 - (tile - first) : tile - first) * kPromptRows;
+      t.row0 = (a.causal ? count - 1 - (tile - first) : tile - first) * ROWS;
       return t;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -90,38 +90,38 @@ __device__ __forceinline__ PromptTile find_tile(const PromptArgs& a, int tile, i
   t.q0 = min(max(a.q_starts[a.n_seq], 0), a.tq);
   t.nq = a.tq - t.q0;
   t.k0 = 0, t.nk = 0;
-  t.row0 = (tile - before) * kPromptRows;
+  t.row0 = (tile - before) * ROWS;
   return t;
 }
 
-// A thread's part of a tile of keys or values: 16-byte chunks tid + threads j of 64 rows of 16.
-constexpr int kChunksPerThread = kTileTokens * 16 / kPromptThreads;
-
+// A thread's part of a tile of keys or values is 16-byte chunks tid + THREADS i of 64 rows of 16.
 // Chunk i of tile j of the n tokens of x, `stride` bytes (below 2^24) apart.  Tiles past the last one
 // repeat it and rows past the last token repeat that: no load is under a branch, at whose join it would
 // be waited for.  The base is scalar, a lane's offset one 24-bit multiply-add.
+template <int THREADS>
 __device__ __forceinline__ uint4v load_chunk(const uint16_t* x, uint32_t stride, int j, int n, int tid, int i) {
   const int t0 = min(j, (n - 1) / kTileTokens) * kTileTokens, last = min(n - 1 - t0, kTileTokens - 1);
   const char* base = reinterpret_cast<const char*>(x) + (int64_t)t0 * stride;
-  const uint32_t row = min((tid + kPromptThreads * i) >> 4, last);
+  const uint32_t row = min((tid + THREADS * i) >> 4, last);
   return *reinterpret_cast<const uint4v*>(base + (__umul24(row, stride) + 16u * (tid & 15)));
 }
 
+template <int THREADS>
 __device__ __forceinline__ void store_chunk(char* tile, int tid, int i, uint4v x) {
-  const int at = tid + kPromptThreads * i;
+  const int at = tid + THREADS * i;
   *reinterpret_cast<uint4v*>(tile + tile_at(at >> 4, at & 15)) = x;
 }
 
 // Values of a tile that some row does not see whole: 0 past the last key (their weights are 0, and
 // 0 times an infinity is not), and for infinities and NaN, which are reported.
-template <class T>
+template <class T, int THREADS>
 __device__ __forceinline__ bool clean_part(int t0, int n, int tid, uint4v* r) {
   bool flagged = false;
 #pragma unroll
-  for (int j = 0; j < kChunksPerThread; ++j)
+  for (int j = 0; j < kTileTokens * 16 / THREADS; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = t0 + ((tid + kPromptThreads * j) >> 4) < n ? r[j][i] : 0u;
+      const uint32_t w = t0 + ((tid + THREADS * j) >> 4) < n ? r[j][i] : 0u;
       flagged = flagged || pair_nonfinite<T>(w);
       r[j][i] = pair_finite<T>(w);
     }
@@ -168,28 +168,31 @@ __device__ __forceinline__ void multiply_tile(const char* kt, const char* vt, co
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(PromptArgs a) {
+template <class T, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptArgs a) {
+  constexpr int ROWS = WAVES * kWaveRows, THREADS = WAVES * 64;
   __shared__ __align__(16) char kts[2][kTileBytes], vts[2][kTileBytes];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units;
-  const int split = rest % a.splits;
-  const PromptTile t = find_tile(a, rest / a.splits, lane);
-  const int64_t b = unit / a.hkv, kv = unit % a.hkv;
+  const int rest = fast_div(blockIdx.x, a.div_units), unit = blockIdx.x - rest * a.units;
+  const int tile = fast_div(rest, a.div_splits), split = rest - tile * a.splits;
+  const PromptTile t = find_tile<ROWS>(a, tile, lane);
+  const int batch = fast_div(unit, a.div_hkv);
+  const int64_t b = batch, kv = unit - batch * a.hkv;
+  auto token_of = [&](int row) { return (int)fast_div(row, a.div_g); };
 
   // The lane's row, and how many keys of its sequence it sees.
   auto keys_of = [&](int i) { return i >= t.nq ? 0 : a.causal ? min(max(t.nk - t.nq + i + 1, 0), t.nk) : t.nk; };
   const int wave_row = t.row0 + kWaveRows * wave, row = wave_row + (lane & 31);
-  const int tok = row / a.g, head = row - tok * a.g;
+  const int tok = token_of(row), head = row - tok * a.g;
   const int limit = keys_of(tok);
   // Of the workgroup's rows: the fewest and the most (the last live row's).  Rows past the last
   // query compute what they like and are not stored.
-  const int last_tok = min((t.row0 + kPromptRows - 1) / a.g, t.nq - 1);
-  const int most = last_tok < 0 ? 0 : keys_of(last_tok), fewest = keys_of(t.row0 / a.g);
+  const int last_tok = min(token_of(t.row0 + ROWS - 1), t.nq - 1);
+  const int most = last_tok < 0 ? 0 : keys_of(last_tok), fewest = keys_of(token_of(t.row0));
   // Of the wave's.
-  const int wave_most = wave_row / a.g >= t.nq ? 0 : keys_of(min((wave_row + kWaveRows - 1) / a.g, t.nq - 1));
-  const int wave_fewest = keys_of(wave_row / a.g);
+  const int wave_most = token_of(wave_row) >= t.nq ? 0 : keys_of(min(token_of(wave_row + kWaveRows - 1), t.nq - 1));
+  const int wave_fewest = keys_of(token_of(wave_row));
 
   // This split's tiles of keys, of those that the whole sequence has; the wave's end of them.
   const int all = (t.nk + kTileTokens - 1) / kTileTokens, each = (all + a.splits - 1) / a.splits;
@@ -203,45 +206,46 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(Pro
     const uint16_t* k = a.k + b * a.k_b + kv * a.k_h + (int64_t)t.k0 * a.k_t;
     const uint16_t* v = a.v + b * a.v_b + kv * a.v_h + (int64_t)t.k0 * a.v_t;
     const uint32_t k_t = (uint32_t)a.k_t * 2, v_t = (uint32_t)a.v_t * 2;
-    static_assert(kChunksPerThread == 2, "two chunks of keys and two of values a thread");
-    uint4v kr[4], vr[2];
+    constexpr int C = kTileTokens * 16 / THREADS;
+    uint4v kr[2 * C], vr[C];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kr[i] = load_chunk(k, k_t, first + (i >> 1), t.nk, tid, i & 1);
+    for (int i = 0; i < 2 * C; ++i) kr[i] = load_chunk<THREADS>(k, k_t, first + i / C, t.nk, tid, i % C);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vr[i] = load_chunk(v, v_t, first, t.nk, tid, i);
+    for (int i = 0; i < C; ++i) vr[i] = load_chunk<THREADS>(v, v_t, first, t.nk, tid, i);
     uint4v q[1][8];
     const int64_t qt = t.q0 + min(tok, t.nq - 1);  // first < end: there is a query
-    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, tok < t.nq, a.flip, lane, q[0]);
+    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, lane, q[0]);
     const TileLane at(lane);
     auto clean = [&](int j) {  // where some row does not see all of tile j
-      if ((j + 1) * kTileTokens > fewest && clean_part<T>(j * kTileTokens, t.nk, tid, vr)) flag = 1;
+      if ((j + 1) * kTileTokens > fewest && clean_part<T, THREADS>(j * kTileTokens, t.nk, tid, vr)) flag = 1;
     };
-    // Tile j + 2's keys and j + 1's values to LDS, and the loads of those after them: piece i of 8.
+    // Tile j + 2's keys and j + 1's values to LDS, and the loads of those after them: piece i of 4 C.
     auto stage = [&](int j, int i) {
-      const int c = i & 1;
-      if (i < 2)
-        store_chunk(kts[j & 1], tid, c, kr[c]);
-      else if (i < 4)
-        store_chunk(vts[(j + 1) & 1], tid, c, vr[c]);
-      else if (i < 6)
-        kr[c] = load_chunk(k, k_t, j + 3, t.nk, tid, c);
+      const int c = i % C;
+      if (i < C)
+        store_chunk<THREADS>(kts[j & 1], tid, c, kr[c]);
+      else if (i < 2 * C)
+        store_chunk<THREADS>(vts[(j + 1) & 1], tid, c, vr[c]);
+      else if (i < 3 * C)
+        kr[c] = load_chunk<THREADS>(k, k_t, j + 3, t.nk, tid, c);
       else
-        vr[c] = load_chunk(v, v_t, j + 2, t.nk, tid, c);
+        vr[c] = load_chunk<THREADS>(v, v_t, j + 2, t.nk, tid, c);
     };
-    // The waves of a SIMD are w and w + 4: the second four run one phase behind the first.
-    const int behind = __builtin_amdgcn_readfirstlane(tid / (kPromptThreads / 2));
+    // Of 8 waves, w and w + 4 share a SIMD: the second four run one phase behind the first.
+    const int behind = WAVES == 8 ? __builtin_amdgcn_readfirstlane(tid / (THREADS / 2)) : 0;
     if (tid == 0) flag = 0;
     __syncthreads();
     clean(first);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_chunk(kts[(first + (i >> 1)) & 1], tid, i & 1, kr[i]);
+    for (int i = 0; i < 2 * C; ++i) store_chunk<THREADS>(kts[(first + i / C) & 1], tid, i % C, kr[i]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      store_chunk(vts[first & 1], tid, i, vr[i]);
-      kr[i] = load_chunk(k, k_t, first + 2, t.nk, tid, i);
-      vr[i] = load_chunk(v, v_t, first + 1, t.nk, tid, i);
+    for (int i = 0; i < C; ++i) {
+      store_chunk<THREADS>(vts[first & 1], tid, i, vr[i]);
+      kr[i] = load_chunk<THREADS>(k, k_t, first + 2, t.nk, tid, i);
+      vr[i] = load_chunk<THREADS>(v, v_t, first + 1, t.nk, tid, i);
     }
     __syncthreads();
+    flip_query(a.flip, q[0]);
     float16v s[1][2];
     if (first < wave_end) score_tile<T, 1, 2>(kts[first & 1], 0, at, q, s);
     if (behind) phase_barrier();
@@ -261,12 +265,14 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(Pro
       if (j < wave_end) {
         __builtin_amdgcn_s_setprio(1);
         multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q[0], p, s[0], st, [&](int i) {
-          if (i >= 2 && i < 10) stage(j, i - 2);
+          if (i * C / 2 < 4 * C)
+#pragma unroll
+            for (int x = i * C / 2; x < (i + 1) * C / 2; ++x) stage(j, x);
         });
         __builtin_amdgcn_s_setprio(0);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) stage(j, i);
+        for (int i = 0; i < 4 * C; ++i) stage(j, i);
       }
       phase_barrier();
     }
@@ -282,7 +288,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(Pro
   const bool live = tok < t.nq;
   if (a.splits > 1) {
     const int64_t rec = (((int64_t)unit * a.tq + out_t) * a.g + head) * a.splits + split;
-    store_record<false>(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
+    constexpr bool kHalf = std::is_same<T, F16>::value;
+    store_record<kHalf>(st, l, a.part_o + rec * (kHalf ? kHeadDim / 2 : kHeadDim), a.part_ml + rec * 2, live, lane);
   } else if (!(t.rest && a.keep_rest)) {
     store_row<T>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + out_t * a.out_t,
                  live, lane);
@@ -291,10 +298,11 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attention_kernel(Pro
 
 // Joins the splits of a row: weights l_s 2^(m_s - max) over their sum, a wave a row.  A record's 16
 // bytes a lane: 16 lanes (fp16) or 32 (fp32) take one, so 4 or 2 records go by side by side and are
-// folded at the end, 8 such steps in flight.
-template <class T, bool HALF>
+// folded at the end, kAhead such steps in flight (8 at most: 16 took 6.4 us instead of 5.5 for 65
+// records of 256 rows).
+template <class T, bool HALF, int kAhead>
 __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
-  constexpr int kLanes = HALF ? 16 : 32, kSide = 64 / kLanes, kDims = kHeadDim / kLanes, kAhead = 8;
+  constexpr int kLanes = HALF ? 16 : 32, kSide = 64 / kLanes, kDims = kHeadDim / kLanes;
   const int lane = threadIdx.x & 63, part = lane / kLanes, d0 = lane % kLanes * kDims;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= (int64_t)a.units * a.rows) return;
@@ -361,29 +369,46 @@ __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
     *reinterpret_cast<uint2v*>(out) = uint2v{y[0], y[1]};
 }
 
-int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s) {
+template <class T, bool HALF>
+static void launch_join_of(const JoinArgs& a, dim3 grid, hipStream_t s) {
+  const int steps = (std::min(a.splits, 64) + (HALF ? 3 : 1)) / (HALF ? 4 : 2);
+  if (steps <= 2)
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 2>), grid, dim3(256), 0, s, a);
+  else if (steps <= 5)
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 5>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 8>), grid, dim3(256), 0, s, a);
+}
+
+int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s) {
   const int64_t rows = (int64_t)a.units * a.rows;
   const dim3 grid((unsigned)((rows + 3) / 4));
-  if (half_records)
-    hipLaunchKernelGGL((join_splits_kernel<F16, true>), grid, dim3(256), 0, s, a);
-  else if (bf16)
-    hipLaunchKernelGGL((join_splits_kernel<BF16, false>), grid, dim3(256), 0, s, a);
+  if (bf16)
+    launch_join_of<BF16, false>(a, grid, s);
   else
-    hipLaunchKernelGGL((join_splits_kernel<F16, false>), grid, dim3(256), 0, s, a);
+    launch_join_of<F16, true>(a, grid, s);
   return launch_status("join of the splits");
 }
 
-// Tiles of rows per unit (an upper bound where sequences are packed: each has one that it does
-// not fill, and so have the tokens behind them) and splits of the keys: few tiles leave most of
-// the GPU idle, so each is given to as many workgroups as fill it, of two tiles of keys at least.
+// Waves a workgroup, tiles of rows per unit (an upper bound where sequences are packed: each has one that
+// it does not fill, and so have the tokens behind them) and splits of the keys.  256 rows (8 waves) read
+// keys and values half as often as 128; where they leave part of the GPU idle, 128 rows do not, start
+// sooner and fit a CU twice.  Few tiles all the same: each is given to as many workgroups as fill the GPU,
+// of 8 tiles of keys at least
+// (the join takes as long as some 5 of them).  32/8 heads: PLACEHOLDER
 struct PromptPlan {
-  int64_t tiles, splits;
+  int64_t waves, tiles, splits;
 };
+static int64_t prompt_tiles(int64_t rows, int64_t tile, int32_t n_seq) {
+  return n_seq ? rows / tile + n_seq + 1 : (rows + tile - 1) / tile;
+}
 static PromptPlan plan_prompt(int64_t units, int32_t g, int64_t tq, int64_t tk, int32_t n_seq) {
   PromptPlan p;
-  p.tiles = n_seq ? tq * g / kPromptRows + n_seq + 1 : (tq * g + kPromptRows - 1) / kPromptRows;
+  p.waves = units * prompt_tiles(tq * g, 256, n_seq) < kPromptTarget ? 4 : 8;
+  p.tiles = prompt_tiles(tq * g, p.waves * kWaveRows, n_seq);
   const int64_t all = units * p.tiles, key_tiles = (tk + kTileTokens - 1) / kTileTokens;
-  p.splits = std::max<int64_t>(1, std::min<int64_t>(kPromptTarget / std::max<int64_t>(all, 1), key_tiles / 2));
+  const int64_t target = p.waves == 8 ? kPromptTarget : 2 * kPromptTarget;
+  p.splits = std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(all, 1), key_tiles / 8));
   return p;
 }
 
@@ -422,7 +447,7 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
   }
   const int32_t g = hq / hkv;
   // Rows, tokens and workgroups are counted in 32 bits.
-  if (tk > INT32_MAX - 2 * kTileTokens || tq > (INT32_MAX - 2 * kPromptRows) / g || batch > INT32_MAX / hkv) {
+  if (tk > INT32_MAX - 2 * kTileTokens || tq > (INT32_MAX - 512) / g || batch > INT32_MAX / hkv) {
     set_error("tq=%lld x %d heads a group, tk=%lld or batch * hkv exceeds 2^31 rows", (long long)tq, g, (long long)tk);
     return TP_ERR_INVALID;
   }
@@ -482,11 +507,19 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
     a.part_ml = a.part_o + (size_t)batch * hq * tq * a.splits * kHeadDim;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(a.units * p.tiles * p.splits));
-  if (dtype)
-    hipLaunchKernelGGL((prompt_attention_kernel<BF16>), grid, dim3(kPromptThreads), 0, s, a);
+  a.div_units = make_fastdiv((uint32_t)a.units);
+  a.div_splits = make_fastdiv((uint32_t)a.splits);
+  a.div_hkv = make_fastdiv((uint32_t)hkv);
+  a.div_g = make_fastdiv((uint32_t)g);
+  const dim3 grid((unsigned)(a.units * p.tiles * p.splits)), threads((unsigned)p.waves * 64);
+  if (dtype && p.waves == 8)
+    hipLaunchKernelGGL((prompt_attention_kernel<BF16, 8>), grid, threads, 0, s, a);
+  else if (dtype)
+    hipLaunchKernelGGL((prompt_attention_kernel<BF16, 4>), grid, threads, 0, s, a);
+  else if (p.waves == 8)
+    hipLaunchKernelGGL((prompt_attention_kernel<F16, 8>), grid, threads, 0, s, a);
   else
-    hipLaunchKernelGGL((prompt_attention_kernel<F16>), grid, dim3(kPromptThreads), 0, s, a);
+    hipLaunchKernelGGL((prompt_attention_kernel<F16, 4>), grid, threads, 0, s, a);
   const int32_t st = launch_status("tp_prompt_attention");
   if (st != TP_OK || a.splits == 1) return st;
   JoinArgs j{};
@@ -497,5 +530,5 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.splits, j.g = g, j.hkv = hkv;
   j.rest_from = n_seq && keep_rest ? q_starts + n_seq : nullptr;
-  return launch_join(j, dtype != 0, false, s);
+  return launch_join(j, dtype != 0, s);
 }

@@ -133,14 +133,18 @@ struct TileLane {
   }
 };
 
-// The queries of a row as the B operand: q[ks] holds dimensions 16 ks + 8 h .. + 7; zeros where
-// the row is not live (`row` is then some other row's: the loads are not under a branch, whose
-// join would wait for each of them in turn).
-__device__ __forceinline__ void load_query(const uint16_t* row, bool live, uint32_t flip, int lane, uint4v* q) {
+// The queries of a row as the B operand: q[ks] holds dimensions 16 ks + 8 h .. + 7.  Where the row is not
+// a query's, `row` is some other one: the loads are not under a branch, whose join would wait for each of
+// them in turn.
+__device__ __forceinline__ void load_query(const uint16_t* row, int lane, uint4v* q) {
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) q[ks] = *reinterpret_cast<const uint4v*>(row + 16 * ks + 8 * (lane >> 5));
+}
+// Negative scales: the queries' signs turned.
+__device__ __forceinline__ void flip_query(uint32_t flip, uint4v* q) {
+  if (flip)
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) q[ks] = live ? q[ks] ^ flip : uint4v{0u, 0u, 0u, 0u};
+    for (int ks = 0; ks < 8; ++ks) q[ks] ^= flip;
 }
 
 // Scores of NB blocks of 32 tokens from token t0 of a tile of keys with RB blocks of 32 rows.
@@ -302,9 +306,9 @@ __device__ __forceinline__ void store_row(const RowState& st, float inv, uint16_
 }
 
 // A split's record of a row: its output divided by its sum, with the maximum (log2 units) and the
-// sum in fp32.  Splits of a row are joined by join_splits_kernel.  HALF: the output in fp16, for
-// half the bytes written and read back; each record's rounding (half a step, 2^-11) is weighted
-// by the record's share, so it stays below the result's own.
+// sum in fp32.  Splits of a row are joined by join_splits_kernel.  HALF, for fp16 results: the output in
+// fp16 too (it lies within the values' range), for half the bytes written and read back; each record's
+// rounding (half a step, 2^-11) is weighted by the record's share, so it stays below the result's own.
 template <bool HALF>
 __device__ __forceinline__ void store_record(const RowState& st, float l, void* o, float* ml, bool live, int lane) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -335,6 +339,7 @@ struct JoinArgs {
   const int32_t* rest_from;  // tokens from *rest_from on are left as they are (NULL: none)
 };
 
-int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s);
+// Records in fp32 and results in bf16, or both in fp16.
+int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s);
 
 }  // namespace tp

@@ -30,6 +30,7 @@ struct TreeArgs {
   uint16_t* out;
   int64_t q_b, q_h, q_t, out_b, out_h, out_t;
   int32_t units, hkv, g, nodes, row_blocks;
+  FastDiv div_units, div_blocks, div_hkv, div_g;
   const void* radii;
   const uint16_t* radii_scales;
   const uint8_t* angle_l1;
@@ -197,33 +198,35 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   __shared__ __align__(16) char tiles[2][2][kTileBytes];
   __shared__ TreeLut lut;
   __shared__ int flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units;
-  const int block = rest % a.row_blocks, record = rest / a.row_blocks;
-  const int64_t b = unit / a.hkv, kv = unit % a.hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rest = fast_div(blockIdx.x, a.div_units), unit = blockIdx.x - rest * a.units;
+  const int record = fast_div(rest, a.div_blocks), block = rest - record * a.row_blocks;
+  const int64_t slot0 = (int64_t)unit * a.capacity;
+  int page = record * a.pages_per_split;
+  const int page_end = record < a.page_splits ? min(page + a.pages_per_split, a.n_pages) : page;
+  // The first page's loads before anything else; a record without pages has none to wait for.
+  PageRegs<KIND, N> p;
+  if (page < page_end) load_page<KIND, N, THREADS>(a, slot0 + page, tid, p);
+
+  const int batch = fast_div(unit, a.div_hkv);
+  const int64_t b = batch, kv = unit - batch * a.hkv;
   const int rw = wave / TW, tw = wave % TW;
   const bool works = rw < RW;
-
   const int row = (block * RW + rw) * kWaveRows + (lane & 31);
-  const int node = row / a.g, head = row - node * a.g;
+  const int node = fast_div(row, a.div_g), head = row - node * a.g;
   const bool live = works && node < a.nodes;
   const int at_node = min(node, a.nodes - 1);  // loads of rows past the last node repeat it
   const uint64_t* mask = a.mask + b * a.mask_b + (int64_t)at_node * a.words;
-  const bool real = live && ((mask[at_node >> 6] >> (at_node & 63)) & 1u);
   uint4v qs[1][8];
-  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, real, a.flip, lane, qs[0]);
+  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, lane, qs[0]);
+  const uint64_t self = mask[at_node >> 6];
   const TileLane at(lane);
   RowState rows[1];
   RowState& st = rows[0];
   st.clear();
 
-  const int64_t slot0 = (int64_t)unit * a.capacity;
-  int page = record * a.pages_per_split;
-  const int page_end = record < a.page_splits ? min(page + a.pages_per_split, a.n_pages) : page;
   if (tid == 0) flag = 0;
   if (page < page_end) {
-    PageRegs<KIND, N> p;
-    load_page<KIND, N, THREADS>(a, slot0 + page, tid, p);
     for (int x = tid; x < 256; x += THREADS) {
       if constexpr (KIND == kTreeDefault) {
         lut.pair[x] = make_uint2(make_cs(x & 15u, 4), make_cs(x >> 4, 4));
@@ -234,6 +237,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         if (x < (1 << a.deep_bits)) lut.code[256 + x] = make_cs(x, a.deep_bits);
       }
     }
+    flip_query(a.flip, qs[0]);
     __syncthreads();
     for (int buf = 0; page < page_end; ++page, buf ^= 1) {
       decode_page<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, tiles[buf][0], tiles[buf][1]);
@@ -245,7 +249,9 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
                                     [](int) { return true; });
     }
   }
+  const bool real = live && ((self >> (at_node & 63)) & 1u);
   if (record == a.records - 1) {  // the tail and the drafts
+    if (record >= a.page_splits) flip_query(a.flip, qs[0]);  // not turned above
     const int first = a.tail_len > 0 ? -1 : 0;
     for (int j = first; j < a.words; ++j) {
       const uint16_t *k, *v;
@@ -462,6 +468,10 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
     a.part_o = static_cast<uint16_t*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)units * rows * a.records * kHeadDim);
   }
+  a.div_units = make_fastdiv((uint32_t)units);
+  a.div_blocks = make_fastdiv((uint32_t)p.row_blocks);
+  a.div_hkv = make_fastdiv((uint32_t)hkv);
+  a.div_g = make_fastdiv((uint32_t)a.g);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(units * p.row_blocks * p.records));
   const bool is_default = !layout->int8_radii && layout->l1_bits == 4 && layout->deep_bits == 4 && layout->split_dim == 64;
@@ -483,5 +493,5 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
   j.rows = rows;
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.records, j.g = a.g, j.hkv = hkv;
-  return launch_join(j, false, true, s);
+  return launch_join(j, false, s);
 }
