@@ -133,21 +133,14 @@ __device__ __forceinline__ void phase_barrier() { lds_barrier(); }
 
 // The products of a step: the next tile's scores in turn with a tile's weights and values, so that four
 // products lie between two that add to the same registers.  Reads from LDS go out kAhead pairs before the
-// products that take them; the order is held by scheduling barriers (left to itself the compiler puts each
-// read right before its product, which then waits for the LDS every time).  Past the last tile the scores
-// are of whatever the LDS holds, and not used: a second form without them would cost 64 registers more,
-// where the two meet.  beside(i): what is issued under the products of pair i.
+// products that take them.  Past the last tile the scores are of whatever the LDS holds, and not used: a
+// second form without them would cost 64 registers more, where the two meet.  beside(i): what is issued under the products of pair i.
 template <class T, class Beside>
 __device__ __forceinline__ void multiply_tile(const char* kt, const char* vt, const TileLane& at, const uint4v* q,
                                               const uint4v* p, float16v* s, RowState& st, Beside beside) {
-  constexpr int kAhead = 3;
-  auto key = [&](int i) { return lds_read16(kt + (at.k ^ (32 * (i >> 1))) + 32 * (i & 1) * (kHeadDim * 2)); };
-  auto value = [&](int i) {  // 16 tokens of block i % 4 of the dimensions
-    const char* row = vt + 16 * (i >> 2) * (kHeadDim * 2);
-    const uint2v lo = lds_read_tr(row + (at.v ^ (64 * (i & 3))));
-    const uint2v hi = lds_read_tr(row + (at.v ^ (64 * (i & 3) + 32)) + 8 * kHeadDim * 2);
-    return uint4v{lo.x, lo.y, hi.x, hi.y};
-  };
+  constexpr int kAhead = 3;  // 4 would take 8 registers more than there are
+  auto key = [&](int i) { return read_key<2>(kt, 0, at, i); };
+  auto value = [&](int i) { return read_value(vt, 0, at, i); };
   uint4v k[kAhead], v[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) k[i] = key(i), v[i] = value(i);
@@ -212,9 +205,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
     for (int i = 0; i < 2 * C; ++i) kr[i] = load_chunk<THREADS>(k, k_t, first + i / C, t.nk, tid, i % C);
 #pragma unroll
     for (int i = 0; i < C; ++i) vr[i] = load_chunk<THREADS>(v, v_t, first, t.nk, tid, i);
-    uint4v q[1][8];
+    uint4v q[8];
     const int64_t qt = t.q0 + min(tok, t.nq - 1);  // first < end: there is a query
-    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, lane, q[0]);
+    load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + qt * a.q_t, lane, q);
     const TileLane at(lane);
     auto clean = [&](int j) {  // where some row does not see all of tile j
       if ((j + 1) * kTileTokens > fewest && clean_part<T, THREADS>(j * kTileTokens, t.nk, tid, vr)) flag = 1;
@@ -245,9 +238,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
       vr[i] = load_chunk<THREADS>(v, v_t, first + 1, t.nk, tid, i);
     }
     __syncthreads();
-    flip_query(a.flip, q[0]);
+    flip_query(a.flip, q);
     float16v s[1][2];
-    if (first < wave_end) score_tile<T, 1, 2>(kts[first & 1], 0, at, q, s);
+    if (first < wave_end) score_tile<T, 2>(kts[first & 1], 0, at, q, s[0]);
     if (behind) phase_barrier();
     // Two phases a tile, a barrier after each: the softmax, and the products.  While one wave of a SIMD
     // multiplies, the other runs its softmax (in step, 41 % of the time went to products and almost all of
@@ -264,7 +257,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
       phase_barrier();
       if (j < wave_end) {
         __builtin_amdgcn_s_setprio(1);
-        multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q[0], p, s[0], st, [&](int i) {
+        multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q, p, s[0], st, [&](int i) {
           if (i * C / 2 < 4 * C)
 #pragma unroll
             for (int x = i * C / 2; x < (i + 1) * C / 2; ++x) stage(j, x);
@@ -296,24 +289,27 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
   }
 }
 
-// Joins the splits of a row: weights l_s 2^(m_s - max) over their sum, a wave a row.  A record's 16
-// bytes a lane: 16 lanes (fp16) or 32 (fp32) take one, so 4 or 2 records go by side by side and are
-// folded at the end, kAhead such steps in flight (8 at most: 16 took 6.4 us instead of 5.5 for 65
-// records of 256 rows).
-template <class T, bool HALF, int kAhead>
+// Joins the splits of a row: weights l_s 2^(m_s - max) over their sum.  A record's 16 bytes a lane: 16 lanes
+// (fp16) or 32 (fp32) take one, so 4 or 2 records go by side by side and are folded at the end, kAhead such
+// steps in flight.  WAVES waves a row, each a part of its records: one, or four where there are few rows of
+// many records (65 records of 1,024 rows: PLACEHOLDER us).
+template <class T, bool HALF, int kAhead, int WAVES>
 __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
   constexpr int kLanes = HALF ? 16 : 32, kSide = 64 / kLanes, kDims = kHeadDim / kLanes;
-  const int lane = threadIdx.x & 63, part = lane / kLanes, d0 = lane % kLanes * kDims;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ float part_acc[WAVES > 1 ? WAVES : 1][kHeadDim], part_ml[WAVES][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane / kLanes, d0 = lane % kLanes * kDims;
+  const int64_t i = WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (i >= (int64_t)a.units * a.rows) return;
   const int64_t unit = i / a.rows, row = i - unit * a.rows;
   const int64_t tok = row / a.g, head = row - tok * a.g;
   if (a.rest_from && tok >= *a.rest_from) return;
+  const int each = (a.splits + WAVES - 1) / WAVES;
+  const int first = WAVES > 1 ? min(wave * each, a.splits) : 0, end = min(first + each, a.splits);
   const float* ml = a.ml + i * a.splits * 2;
   const char* o = static_cast<const char*>(a.o) + (i * a.splits * kHeadDim + d0) * (HALF ? 2 : 4);
   float m = -INFINITY, l = 0.0f, acc[kDims] = {};
-  for (int base = 0; base < a.splits; base += 64) {
-    const int n = min(64, a.splits - base);
+  for (int base = first; base < end; base += 64) {
+    const int n = min(64, end - base);
     float2v mine = {-INFINITY, 0.0f};
     if (lane < n) mine = *reinterpret_cast<const float2v*>(ml + 2 * (base + lane));
     if (mine.y == 0.0f) mine.x = -INFINITY;  // saw nothing
@@ -340,7 +336,8 @@ __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int s = s0 + kSide * j + part;
-        const float ws = s < n ? __shfl(w, s & 63) : 0.0f;
+        const float of_lane = __shfl(w, s & 63);  // with every lane taking part
+        const float ws = s < n ? of_lane : 0.0f;
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
           float v;
@@ -357,6 +354,28 @@ __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int step = kLanes; step < 64; step <<= 1) acc[d] += __shfl_xor(acc[d], step);
+  if constexpr (WAVES > 1) {
+    if (part == 0)
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) part_acc[wave][d0 + d] = acc[d];
+    if (lane == 0) part_ml[wave][0] = m, part_ml[wave][1] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, part_ml[w][0]);
+    if (top == -INFINITY) top = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float scale = __builtin_amdgcn_exp2f(part_ml[w][0] - top);
+      l += part_ml[w][1] * scale;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) acc[d] += part_acc[w][d0 + d] * scale;
+    }
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (part != 0) return;
   uint16_t* out = a.out + (unit / a.hkv) * a.out_b + ((unit % a.hkv) * a.g + head) * a.out_h + tok * a.out_t + d0;
@@ -370,23 +389,23 @@ __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
 }
 
 template <class T, bool HALF>
-static void launch_join_of(const JoinArgs& a, dim3 grid, hipStream_t s) {
-  const int steps = (std::min(a.splits, 64) + (HALF ? 3 : 1)) / (HALF ? 4 : 2);
+static void launch_join_of(const JoinArgs& a, hipStream_t s) {
+  const int64_t rows = (int64_t)a.units * a.rows;
+  const int steps = (a.splits + (HALF ? 3 : 1)) / (HALF ? 4 : 2);
+  const dim3 grid((unsigned)((rows + 3) / 4));
   if (steps <= 2)
-    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 2>), grid, dim3(256), 0, s, a);
-  else if (steps <= 5)
-    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 5>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 2, 1>), grid, dim3(256), 0, s, a);
+  else if (steps > 5 && rows <= 4096)
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 5, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 8>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_splits_kernel<T, HALF, 5, 1>), grid, dim3(256), 0, s, a);
 }
 
 int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s) {
-  const int64_t rows = (int64_t)a.units * a.rows;
-  const dim3 grid((unsigned)((rows + 3) / 4));
   if (bf16)
-    launch_join_of<BF16, false>(a, grid, s);
+    launch_join_of<BF16, false>(a, s);
   else
-    launch_join_of<F16, true>(a, grid, s);
+    launch_join_of<F16, true>(a, s);
   return launch_status("join of the splits");
 }
 

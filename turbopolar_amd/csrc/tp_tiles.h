@@ -147,25 +147,42 @@ __device__ __forceinline__ void flip_query(uint32_t flip, uint4v* q) {
     for (int ks = 0; ks < 8; ++ks) q[ks] ^= flip;
 }
 
-// Scores of NB blocks of 32 tokens from token t0 of a tile of keys with RB blocks of 32 rows.
-template <class T, int RB, int NB>
-__device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLane& at, const uint4v (&q)[RB][8],
-                                           float16v (&s)[RB][NB]) {
+// Product reads: 16 bytes of a key row (run i / NB of the dimensions of block i % NB of the tokens), and 16
+// tokens of the values (run i / 4 of the tokens of block i % 4 of the dimensions; 8 rows on, the swizzle
+// differs by 2 chunks).
+template <int NB>
+__device__ __forceinline__ uint4v read_key(const char* kt, int t0, const TileLane& at, int i) {
+  return lds_read16(kt + (at.k ^ (32 * (i / NB))) + (t0 + 32 * (i % NB)) * (kHeadDim * 2));
+}
+__device__ __forceinline__ uint4v read_value(const char* vt, int t0, const TileLane& at, int i) {
+  const char* row = vt + (t0 + 16 * (i >> 2)) * (kHeadDim * 2);
+  const uint2v lo = lds_read_tr(row + (at.v ^ (64 * (i & 3))));
+  const uint2v hi = lds_read_tr(row + (at.v ^ (64 * (i & 3) + 32)) + 8 * kHeadDim * 2);
+  return uint4v{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Products take what was read from LDS kReadAhead products before; the order is held by scheduling barriers
+// (left to itself the compiler puts each read right before its product, which then waits for the LDS every
+// time).
+constexpr int kReadAhead = 4;
+
+// Scores of NB blocks of 32 tokens from token t0 of a tile of keys.
+template <class T, int NB>
+__device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLane& at, const uint4v* q, float16v* s) {
+  uint4v k[kReadAhead];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
+  for (int i = 0; i < kReadAhead; ++i) k[i] = read_key<NB>(kt, t0, at, i);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+  for (int i = 0; i < 8 * NB; ++i) {
+    float16v& sum = s[i % NB];
+    if (i < NB)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[rb][nb][i] = 0.0f;
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int off = (at.k ^ (32 * ks)) + (t0 + 32 * nb) * (kHeadDim * 2);
-      const uint4v key = lds_read16(kt + off);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb][nb] = T::mfma(key, q[rb][ks], s[rb][nb]);
-    }
+      for (int j = 0; j < 16; ++j) sum[j] = 0.0f;
+    sum = T::mfma(k[i % kReadAhead], q[i / NB], sum);
+    if (i + kReadAhead < 8 * NB) k[i % kReadAhead] = read_key<NB>(kt, t0, at, i + kReadAhead);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // Scores of tokens from `limit` on masked; limit counts from the lane's first token of the tile (4 (lane /
@@ -212,20 +229,16 @@ __device__ __forceinline__ void rescale(const float16v (&s)[RB][NB], float c, Ro
   }
 }
 
-// The product of packed weights with NK runs of 16 values from token t0.
+// The product of packed weights with NK runs of 16 values from token t0; v holds the first reads.
 template <class T, int NK>
-__device__ __forceinline__ void add_values(const char* vt, int t0, const TileLane& at, const uint4v (&p)[NK],
+__device__ __forceinline__ void add_values(const char* vt, int t0, const TileLane& at, const uint4v* p, uint4v* v,
                                            RowState& st) {
 #pragma unroll
-  for (int k = 0; k < NK; ++k)
-#pragma unroll
-    for (int db = 0; db < 4; ++db) {
-      // 8 rows on, the swizzle differs by 2 chunks.
-      const char* row = vt + (t0 + 16 * k) * (kHeadDim * 2);
-      const uint2v lo = lds_read_tr(row + (at.v ^ (64 * db)));
-      const uint2v hi = lds_read_tr(row + (at.v ^ (64 * db + 32)) + 8 * kHeadDim * 2);
-      st.o[db] = T::mfma(uint4v{lo.x, lo.y, hi.x, hi.y}, p[k], st.o[db]);
-    }
+  for (int i = 0; i < 4 * NK; ++i) {
+    st.o[i & 3] = T::mfma(v[i % kReadAhead], p[i >> 2], st.o[i & 3]);
+    if (i + kReadAhead < 4 * NK) v[i % kReadAhead] = read_value(vt, t0, at, i + kReadAhead);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // Weights of a tile's scores, packed as the second product takes them, and their sum.
@@ -247,9 +260,9 @@ __device__ __forceinline__ void weigh(const float16v* s, float c, uint4v* p, Row
 // a token of the tile (asked where MASKED only).
 template <class T, int NB, bool MASKED, class Seen>
 __device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int t0, const TileLane& at,
-                                            const uint4v (&q)[1][8], float c, RowState (&st)[1], int lane, Seen seen) {
+                                            const uint4v* q, float c, RowState (&st)[1], int lane, Seen seen) {
   float16v s[1][NB];
-  score_tile<T, 1, NB>(kt, t0, at, q, s);
+  score_tile<T, NB>(kt, t0, at, q, s[0]);
   if constexpr (MASKED) {
     const int h4 = 4 * (lane >> 5);
 #pragma unroll
@@ -259,9 +272,16 @@ __device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int 
         if (!seen(t0 + 32 * nb + 8 * (i >> 2) + (i & 3) + h4)) s[0][nb][i] = -INFINITY;
   }
   rescale<1, NB>(s, c, st);
-  uint4v p[2 * NB];
+  uint4v p[2 * NB], v[kReadAhead];
+  // The first values are read under the softmax; of two blocks, whose scores leave no registers, after it.
+  if (NB == 1)
+#pragma unroll
+    for (int i = 0; i < kReadAhead; ++i) v[i] = read_value(vt, t0, at, i);
   weigh<T, NB>(s[0], c, p, st[0]);
-  add_values<T>(vt, t0, at, p, st[0]);
+  if (NB != 1)
+#pragma unroll
+    for (int i = 0; i < kReadAhead; ++i) v[i] = read_value(vt, t0, at, i);
+  add_values<T, 2 * NB>(vt, t0, at, p, v, st[0]);
 }
 
 // Infinities and NaN among the values of a tile that some rows do not see: a product

@@ -23,7 +23,7 @@ constexpr bool tree_i8(int kind) { return kind == kTreeFast || kind == kTreeAnyI
 constexpr bool tree_any(int kind) { return kind == kTreeAnyF16 || kind == kTreeAnyI8; }
 
 constexpr int kTreeMaxNodes = 256;
-constexpr int kTreeTarget = 512;  // workgroups that fill the GPU, two a CU
+constexpr int kTreeTarget = 2048;  // waves that fill the GPU, two a SIMD
 
 struct TreeArgs {
   const uint16_t* q;
@@ -89,7 +89,7 @@ __device__ __forceinline__ void load_page(const TreeArgs& a, int64_t slot, int t
   if constexpr (tree_i8(KIND)) p.ls = a.radii_scales[slot];
 }
 
-struct TreeLut {
+union TreeLut {
   uint32_t code[512];  // (cos, sin) of the level-1 codes, then of the deep codes
   uint2 pair[256];     // default layout: of both nibbles of a code byte
 };
@@ -187,15 +187,15 @@ __device__ __forceinline__ bool dense_tile(const uint16_t* k, const uint16_t* v,
   return flagged;
 }
 
-// RW waves of 32 rows each; TW waves share a row block and take a page's tokens in TW parts.
-// At least four waves, so that enough threads load and decode.
+// RW waves of 32 rows each; TW waves share a row block and take a page's tokens in TW parts.  Two waves
+// keep one tile in LDS, so that four such workgroups share a CU; more keep two.
 template <int RW, int TW>
-constexpr int kTreeThreads = 64 * (RW * TW < 4 ? 4 : RW * TW);
+constexpr int kTreeThreads = 64 * RW * TW;
 
 template <int KIND, int RW, int TW>
 __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kernel(TreeArgs a) {
-  constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW;
-  __shared__ __align__(16) char tiles[2][2][kTileBytes];
+  constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW, BUFS = RW * TW > 2 ? 2 : 1;
+  __shared__ __align__(16) char tiles[BUFS][2][kTileBytes];
   __shared__ TreeLut lut;
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -211,14 +211,13 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   const int batch = fast_div(unit, a.div_hkv);
   const int64_t b = batch, kv = unit - batch * a.hkv;
   const int rw = wave / TW, tw = wave % TW;
-  const bool works = rw < RW;
   const int row = (block * RW + rw) * kWaveRows + (lane & 31);
   const int node = fast_div(row, a.div_g), head = row - node * a.g;
-  const bool live = works && node < a.nodes;
+  const bool live = node < a.nodes;
   const int at_node = min(node, a.nodes - 1);  // loads of rows past the last node repeat it
   const uint64_t* mask = a.mask + b * a.mask_b + (int64_t)at_node * a.words;
-  uint4v qs[1][8];
-  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, lane, qs[0]);
+  uint4v qs[8];
+  load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, lane, qs);
   const uint64_t self = mask[at_node >> 6];
   const TileLane at(lane);
   RowState rows[1];
@@ -237,21 +236,21 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         if (x < (1 << a.deep_bits)) lut.code[256 + x] = make_cs(x, a.deep_bits);
       }
     }
-    flip_query(a.flip, qs[0]);
+    flip_query(a.flip, qs);
     __syncthreads();
-    for (int buf = 0; page < page_end; ++page, buf ^= 1) {
+    for (int buf = 0; page < page_end; ++page, buf ^= BUFS - 1) {
       decode_page<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, tiles[buf][0], tiles[buf][1]);
       __syncthreads();
       // The last page again rather than none: a load under a branch is waited for at its join.
       load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
-      if (works)
-        attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, qs, a.c, rows, lane,
-                                    [](int) { return true; });
+      attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, qs, a.c, rows, lane,
+                                  [](int) { return true; });
+      if (BUFS == 1) __syncthreads();
     }
   }
   const bool real = live && ((self >> (at_node & 63)) & 1u);
   if (record == a.records - 1) {  // the tail and the drafts
-    if (record >= a.page_splits) flip_query(a.flip, qs[0]);  // not turned above
+    if (record >= a.page_splits) flip_query(a.flip, qs);  // not turned above
     const int first = a.tail_len > 0 ? -1 : 0;
     for (int j = first; j < a.words; ++j) {
       const uint16_t *k, *v;
@@ -270,7 +269,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
       __syncthreads();  // the tile before is read
       if (dense_tile<THREADS>(k, v, k_t, v_t, count, tid, tiles[0][0], tiles[0][1])) flag = 1;
       __syncthreads();
-      if (works) {
+      {
         const uint64_t there = count < 64 ? (1ull << count) - 1ull : ~0ull;
         const uint64_t sees = !real ? 0ull : j < 0 ? there : mask[j] & there;
         auto seen = [&](int x) { return ((sees >> x) & 1u) != 0; };
@@ -284,7 +283,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   if constexpr (TW == 2) {  // the second half's rows join the first's
     __syncthreads();
     float* side = reinterpret_cast<float*>(&tiles[0][0][0]) + rw * 66 * 64 + lane;
-    if (works && tw == 1) {
+    if (tw == 1) {
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -293,7 +292,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
       side[65 * 64] = st.l;
     }
     __syncthreads();
-    if (works && tw == 0) {
+    if (tw == 0) {
       const float m1 = side[64 * 64], l1 = side[65 * 64];
       const float m = fmaxf(st.m, m1), base = m == -INFINITY ? 0.0f : m;
       const float w0 = __builtin_amdgcn_exp2f(st.m - base), w1 = __builtin_amdgcn_exp2f(m1 - base);
@@ -305,7 +304,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
       st.m = m;
     }
   }
-  if (!works || tw != 0) return;
+  if (tw != 0) return;
   if (!real) st.clear();  // padding: its queries were 0, its page tokens seen
   const float l = across_halves(st.l, [](float x, float y) { return x + y; });
   if (a.records > 1) {
@@ -326,7 +325,7 @@ static TreePlan plan_tree(int64_t units, int64_t rows, int32_t n_pages) {
   TreePlan p;
   p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   p.row_blocks = (int32_t)((rows + p.row_waves * kWaveRows - 1) / (p.row_waves * kWaveRows));
-  const int64_t target = p.row_waves == 8 ? kTreeTarget / 2 : kTreeTarget;
+  const int64_t target = kTreeTarget / (p.row_waves == 8 ? 8 : p.row_waves == 1 ? 2 : 4);
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(target / (units * p.row_blocks), n_pages));
   p.pages_per_split = (int32_t)std::max<int64_t>(1, (n_pages + splits - 1) / splits);
   p.page_splits = (n_pages + p.pages_per_split - 1) / p.pages_per_split;
