@@ -240,7 +240,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
     __syncthreads();
     flip_query(a.flip, q);
     float16v s[1][2];
-    if (first < wave_end) score_tile<T, 2>(kts[first & 1], 0, at, q, s[0]);
+    if (first < wave_end) score_tile<T, 2>(kts[first & 1], 0, at, q, s[0], [](int) {});
     if (behind) phase_barrier();
     // Two phases a tile, a barrier after each: the softmax, and the products.  While one wave of a SIMD
     // multiplies, the other runs its softmax (in step, 41 % of the time went to products and almost all of

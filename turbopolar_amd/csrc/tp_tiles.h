@@ -166,9 +166,10 @@ __device__ __forceinline__ uint4v read_value(const char* vt, int t0, const TileL
 // time).
 constexpr int kReadAhead = 4;
 
-// Scores of NB blocks of 32 tokens from token t0 of a tile of keys.
-template <class T, int NB>
-__device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLane& at, const uint4v* q, float16v* s) {
+// Scores of NB blocks of 32 tokens from token t0 of a tile of keys.  beside(i): what is issued under product i.
+template <class T, int NB, class Beside>
+__device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLane& at, const uint4v* q, float16v* s,
+                                           Beside beside) {
   uint4v k[kReadAhead];
 #pragma unroll
   for (int i = 0; i < kReadAhead; ++i) k[i] = read_key<NB>(kt, t0, at, i);
@@ -181,6 +182,7 @@ __device__ __forceinline__ void score_tile(const char* kt, int t0, const TileLan
       for (int j = 0; j < 16; ++j) sum[j] = 0.0f;
     sum = T::mfma(k[i % kReadAhead], q[i / NB], sum);
     if (i + kReadAhead < 8 * NB) k[i % kReadAhead] = read_key<NB>(kt, t0, at, i + kReadAhead);
+    beside(i);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -256,21 +258,10 @@ __device__ __forceinline__ void weigh(const float16v* s, float c, uint4v* p, Row
   }
 }
 
-// One pass over NB blocks of 32 tokens from token t0 of a tile.  seen(token): whether the lane's row sees
-// a token of the tile (asked where MASKED only).
-template <class T, int NB, bool MASKED, class Seen>
-__device__ __forceinline__ void attend_tile(const char* kt, const char* vt, int t0, const TileLane& at,
-                                            const uint4v* q, float c, RowState (&st)[1], int lane, Seen seen) {
-  float16v s[1][NB];
-  score_tile<T, NB>(kt, t0, at, q, s[0]);
-  if constexpr (MASKED) {
-    const int h4 = 4 * (lane >> 5);
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!seen(t0 + 32 * nb + 8 * (i >> 2) + (i & 3) + h4)) s[0][nb][i] = -INFINITY;
-  }
+// The rest of a pass over NB blocks of 32 tokens from token t0 of a tile, from its scores on.
+template <class T, int NB>
+__device__ __forceinline__ void finish_tile(const char* vt, int t0, const TileLane& at, float c, float16v (&s)[1][NB],
+                                            RowState (&st)[1]) {
   rescale<1, NB>(s, c, st);
   uint4v p[2 * NB], v[kReadAhead];
   // The first values are read under the softmax; of two blocks, whose scores leave no registers, after it.

@@ -94,67 +94,75 @@ union TreeLut {
   uint2 pair[256];     // default layout: of both nibbles of a code byte
 };
 
-// Decodes them into a tile of keys and one of values.
+// Decodes half h of run n into a tile of keys: 4 pairs, 16 bytes.
 template <int KIND, int N, int THREADS>
-__device__ __forceinline__ void decode_page(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
-                                            const PageRegs<KIND, N>& p, char* kt, char* vt) {
-  const int c = tid & 7;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int t = (tid >> 3) + (THREADS / 8) * n;
-    uint32_t e[8];
-    if constexpr (KIND == kTreeDefault) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint2 cs = lut.pair[(p.c4[n] >> (8 * i)) & 0xffu];
-        e[2 * i] = pack_h2(lo_lo(p.r[n][i]) * __builtin_bit_cast(half2v, cs.x));
-        e[2 * i + 1] = pack_h2(hi_hi(p.r[n][i]) * __builtin_bit_cast(half2v, cs.y));
-      }
-    } else {
-      const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t code;
-        if constexpr (KIND == kTreeFast) {
-          code = 256 + ((p.c8[n][i >> 2] >> (8 * (i & 3))) & 0xffu);
-        } else {
-          const int pair = 8 * c + i;
-          const bool l1 = pair < a.split_half;
-          const int bits = l1 ? a.l1_bits : a.deep_bits;
-          const int bit = (l1 ? pair : pair - a.split_half) * bits;
-          const uint8_t* row = l1 ? a.angle_l1 + (slot * kPageTokens + t) * a.l1_row
-                                  : a.angle_deep + (slot * kPageTokens + t) * a.deep_row;
-          code = (l1 ? 0u : 256u) + ((row[bit >> 3] >> (bit & 7)) & ((1u << bits) - 1u));
-        }
-        half2v r;
-        if constexpr (tree_i8(KIND)) {
-          // code x scale is exact in fp32; r = exp(code x scale) rounded to fp16 once.
-          const int rc = (int)(int8_t)(p.r8[n][i >> 2] >> (8 * (i & 3)));
-          const f16 x = (f16)__builtin_amdgcn_exp2f((float)rc * (ls * kLog2e));
-          r = half2v{x, x};
-        } else {
-          const uint32_t w = p.r[n][i >> 1];
-          r = (i & 1) ? hi_hi(w) : lo_lo(w);
-        }
-        e[i] = pack_h2(r * __builtin_bit_cast(half2v, lut.code[code]));
-      }
-    }
-    *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c)) = uint4v{e[0], e[1], e[2], e[3]};
-    *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + 1)) = uint4v{e[4], e[5], e[6], e[7]};
-    const half2v scale = lo_lo(p.vs[n]);
+__device__ __forceinline__ void decode_keys(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
+                                            const PageRegs<KIND, N>& p, int n, int h, char* kt) {
+  const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
+  uint32_t e[4];
+  if constexpr (KIND == kTreeDefault) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint4v w;
+      const uint2 cs = lut.pair[(p.c4[n] >> (16 * h + 8 * i)) & 0xffu];
+      e[2 * i] = pack_h2(lo_lo(p.r[n][2 * h + i]) * __builtin_bit_cast(half2v, cs.x));
+      e[2 * i + 1] = pack_h2(hi_hi(p.r[n][2 * h + i]) * __builtin_bit_cast(half2v, cs.y));
+    }
+  } else {
+    const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        half2v lo, hi;
-        i8x4_to_f16(p.v[n][2 * i + j], lo, hi);
-        w[2 * j] = pack_h2(lo * scale);
-        w[2 * j + 1] = pack_h2(hi * scale);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t code;
+      if constexpr (KIND == kTreeFast) {
+        code = 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
+      } else {
+        const int pair = 8 * c + 4 * h + i;
+        const bool l1 = pair < a.split_half;
+        const int bits = l1 ? a.l1_bits : a.deep_bits;
+        const int bit = (l1 ? pair : pair - a.split_half) * bits;
+        const uint8_t* row = l1 ? a.angle_l1 + (slot * kPageTokens + t) * a.l1_row
+                                : a.angle_deep + (slot * kPageTokens + t) * a.deep_row;
+        code = (l1 ? 0u : 256u) + ((row[bit >> 3] >> (bit & 7)) & ((1u << bits) - 1u));
       }
-      *reinterpret_cast<uint4v*>(vt + tile_at(t, 2 * c + i)) = w;
+      half2v r;
+      if constexpr (tree_i8(KIND)) {
+        // code x scale is exact in fp32; r = exp(code x scale) rounded to fp16 once.
+        const int rc = (int)(int8_t)(p.r8[n][h] >> (8 * i));
+        const f16 x = (f16)__builtin_amdgcn_exp2f((float)rc * ls);
+        r = half2v{x, x};
+      } else {
+        const uint32_t w = p.r[n][2 * h + (i >> 1)];
+        r = (i & 1) ? hi_hi(w) : lo_lo(w);
+      }
+      e[i] = pack_h2(r * __builtin_bit_cast(half2v, lut.code[code]));
     }
   }
+  *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + h)) = uint4v{e[0], e[1], e[2], e[3]};
+}
+
+// And into a tile of values: 8 codes.
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void decode_values(int tid, const PageRegs<KIND, N>& p, int n, int h, char* vt) {
+  const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
+  const half2v scale = lo_lo(p.vs[n]);
+  uint4v w;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    half2v lo, hi;
+    i8x4_to_f16(p.v[n][2 * h + j], lo, hi);
+    w[2 * j] = pack_h2(lo * scale);
+    w[2 * j + 1] = pack_h2(hi * scale);
+  }
+  *reinterpret_cast<uint4v*>(vt + tile_at(t, 2 * c + h)) = w;
+}
+
+// Piece i of the 4 N that a page takes.
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void decode_piece(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
+                                             const PageRegs<KIND, N>& p, int i, char* kt, char* vt) {
+  if (i & 2)
+    decode_values<KIND, N, THREADS>(tid, p, i >> 2, i & 1, vt);
+  else
+    decode_keys<KIND, N, THREADS>(a, lut, slot, tid, p, i >> 2, i & 1, kt);
 }
 
 // 64 dense tokens from k, v (t strides in elements) into the tiles; rows from `count` on repeat the
@@ -238,14 +246,38 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
     }
     flip_query(a.flip, qs);
     __syncthreads();
-    for (int buf = 0; page < page_end; ++page, buf ^= BUFS - 1) {
-      decode_page<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, tiles[buf][0], tiles[buf][1]);
-      __syncthreads();
-      // The last page again rather than none: a load under a branch is waited for at its join.
+    float16v s[1][NB];
+    if constexpr (BUFS == 1) {
+      for (; page < page_end; ++page) {
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i)
+          decode_piece<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, i, tiles[0][0], tiles[0][1]);
+        __syncthreads();
+        // The last page again rather than none: a load under a branch is waited for at its join.
+        load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
+        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s[0], [](int) {});
+        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, rows);
+        __syncthreads();
+      }
+    } else {
+      // The next page is decoded under this one's first products.
+#pragma unroll
+      for (int i = 0; i < 4 * N; ++i)
+        decode_piece<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, i, tiles[0][0], tiles[0][1]);
       load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
-      attend_tile<F16, NB, false>(tiles[buf][0], tiles[buf][1], 32 * tw, at, qs, a.c, rows, lane,
-                                  [](int) { return true; });
-      if (BUFS == 1) __syncthreads();
+      for (int buf = 0; page < page_end; ++page, buf ^= 1) {
+        char *kt = tiles[buf ^ 1][0], *vt = tiles[buf ^ 1][1];
+        const int next = min(page + 1, page_end - 1);
+        __syncthreads();
+        score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s[0], [&](int i) {
+          constexpr int kProducts = 8 * NB, kPieces = 4 * N;
+#pragma unroll
+          for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x)
+            decode_piece<KIND, N, THREADS>(a, lut, slot0 + next, tid, p, x, kt, vt);
+        });
+        load_page<KIND, N, THREADS>(a, slot0 + min(page + 2, page_end - 1), tid, p);
+        finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, rows);
+      }
     }
   }
   const bool real = live && ((self >> (at_node & 63)) & 1u);
@@ -273,7 +305,12 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         const uint64_t there = count < 64 ? (1ull << count) - 1ull : ~0ull;
         const uint64_t sees = !real ? 0ull : j < 0 ? there : mask[j] & there;
         auto seen = [&](int x) { return ((sees >> x) & 1u) != 0; };
-        attend_tile<F16, NB, true>(tiles[0][0], tiles[0][1], 32 * tw, at, qs, a.c, rows, lane, seen);
+        float16v s[1][NB];
+        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s[0], [](int) {});
+#pragma unroll
+        for (int x = 0; x < 16 * NB; ++x)
+          if (!seen(32 * (tw + (x >> 4)) + 8 * ((x & 15) >> 2) + (x & 3) + 4 * (lane >> 5))) s[0][x >> 4][x & 15] = -INFINITY;
+        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, rows);
         if (flag)
           add_nonfinite<F16>(st, lane, count, [&](int x) { return seen(x) && (TW == 1 || (x >> 5) == tw); },
                              [&](int x) { return v + x * v_t; });
