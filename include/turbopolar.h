@@ -410,14 +410,15 @@ typedef struct tp_page_copy {
  * Pages of a store copied into another one, one launch: slot s < keep of batch row i
  * and head h of every buffer becomes stored page page_index[s] (NULL: s) of row rows[i]
  * (NULL: i) and head h; slots [keep, dst_capacity) are zeroed.  rows and page_index are
- * device arrays, their entries clamped to [0, batch_in) and [0, n_stored).  tail_bytes
+ * device arrays, their entries clamped to [0, batch_in) and [0, n_stored), or, with
+ * host_index, host arrays of at most 768 entries together, which are checked.  tail_bytes
  * (a multiple of 16, 0 for none) of each row of the tails, rows tail_row bytes apart, go
  * along.  Sources and destinations must not overlap.
  */
 int32_t tp_copy_pages(const tp_page_copy* bufs, int32_t n_bufs, int64_t batch, int32_t heads, int64_t batch_in,
                       const int32_t* rows, int64_t src_capacity, int64_t dst_capacity, int32_t n_stored,
-                      const int32_t* page_index, int32_t keep, const void* tail_k, const void* tail_v,
-                      void* tail_k_out, void* tail_v_out, int64_t tail_bytes, int64_t tail_row, void* stream);
+                      const int32_t* page_index, int32_t keep, int32_t host_index, const void* tail_k,
+                      const void* tail_v, void* tail_k_out, void* tail_v_out, int64_t tail_bytes, int64_t tail_row, void* stream);
 
 /*
  * Tokens index[0 .. n) (a host array; with per_batch one run of n for each batch row;

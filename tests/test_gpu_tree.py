@@ -313,8 +313,27 @@ def test_fork_rows_and_pages(device):
         other = cache.fork(pages=pages)
         same_pages(other.runtime, cache.runtime, pages=pages)
         assert other.offset == 64 * len(pages) + 9 and torch.equal(other.runtime.partial_k, cache.runtime.partial_k)
+    many = [i % 6 for i in range(800)]  # past what travels with a launch
+    other = cache.fork(rows=[2], pages=many)
+    for name, t in buffers(other.runtime).items():
+        assert torch.equal(t, buffers(cache.runtime)[name][[2]][:, :, many]), name
     both = cache.fork(rows=[1, 1], pages=[4])
     same_pages(both.runtime, cache.runtime, rows=[1, 1], pages=[4])
+
+
+def test_fork_keeps_a_set_encoder(device):
+    """A cache whose encoder was given another layout forks with it."""
+    cache = TurboPolarFastCache(config("default", 4, 2))
+    cache.runtime.polar_encoder.k_angle_bits_deep = 8
+    k, v = (torch.from_numpy(x).to(device) for x in gen_kv(1, 1, 2, 200))
+    cache.runtime.append(k, v)
+    other = cache.fork(tokens=150)
+    other.runtime.append(k[:, :, 150:].contiguous(), v[:, :, 150:].contiguous())
+    assert other.runtime.k_storage.angle_codes_deep.shape == cache.runtime.k_storage.angle_codes_deep.shape
+    q, dk, dv = draft(device, 1, 4, 2, 3, seed=1)
+    tree = DraftTree([-1, 0, 1])
+    got = other.tree_attention(q, dk, dv, tree, 0.09)
+    check(got, q, dk, dv, tree, history(other.runtime), fp16_scale(0.09), "set encoder")
 
 
 @pytest.mark.parametrize("layout", ["default", "fast", "odd_split"])

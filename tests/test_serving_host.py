@@ -113,13 +113,20 @@ def test_copy_abi():
     buf = _lib.TPPageCopy(4096, 8192, 512)
     call = lambda **c: L.tp_copy_pages(*{**dict(  # noqa: E731
         bufs=ctypes.byref(buf), n=1, batch=1, heads=2, batch_in=1, rows=None, src=8, dst=4, stored=4, index=None, keep=4,
-        tk=None, tv=None, tko=None, tvo=None, tail=0, row=0, stream=None), **c}.values())
+        host=0, tk=None, tv=None, tko=None, tvo=None, tail=0, row=0, stream=None), **c}.values())
     for change, message in [
         (dict(n=9), b"up to"), (dict(batch=40000), b"up to"), (dict(batch=2), b"row index"), (dict(keep=5), b"do not fit"),
         (dict(stored=9), b"do not fit"), (dict(keep=3, stored=2), b"do not fit"), (dict(tail=8, row=16), b"tails"),
         (dict(tail=32, row=16), b"tails"), (dict(tail=16, row=16), b"tails"), (dict(rows=4097), b"aligned"),
     ]:
         assert call(**change) == _lib.TP_ERR_INVALID and message in L.tp_last_error(), change
+    for rows, pages, message in [([1], None, b"batch row 1"), (None, [0, 4, 1, 2], b"page 4"), (None, [0, -1, 1, 2], b"page -1")]:
+        held = [None if x is None else (ctypes.c_int32 * len(x))(*x) for x in (rows, pages)]
+        at = [None if x is None else ctypes.addressof(x) for x in held]
+        assert call(rows=at[0], index=at[1], host=1) == _lib.TP_ERR_INVALID and message in L.tp_last_error()
+    many = (ctypes.c_int32 * 769)()
+    assert call(dst=1024, keep=769, index=ctypes.addressof(many), host=1) == _lib.TP_ERR_INVALID
+    assert b"at most 768" in L.tp_last_error()
     none = _lib.TPPageCopy(None, 8192, 512)
     assert call(bufs=ctypes.byref(none)) == _lib.TP_ERR_INVALID and b"missing" in L.tp_last_error()
 

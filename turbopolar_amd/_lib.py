@@ -183,7 +183,7 @@ _SIGNATURES = {
     "tp_copy_pages": (
         c_i32,
         [
-            ctypes.POINTER(TPPageCopy), c_i32, c_i64, c_i32, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp, c_i32,
+            ctypes.POINTER(TPPageCopy), c_i32, c_i64, c_i32, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp, c_i32, c_i32,
             c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp,
         ],
     ),

@@ -11,6 +11,7 @@ namespace tp {
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int kCopyBuffers = 8;
+constexpr int kCopyIndex = 768;  // index entries that travel with the launch
 struct CopyArgs {
   struct Buffer {
     const char* src;
@@ -23,6 +24,8 @@ struct CopyArgs {
   int32_t heads, batch_in, n_stored, keep;
   const int32_t* rows;   // source batch row of each copied one (NULL: the same)
   const int32_t* pages;  // source page of each copied one (NULL: the same)
+  int32_t rows_at, pages_at;  // where they begin in `index` instead (-1: they do not)
+  int32_t index[kCopyIndex];
   const char* tail_k;
   const char* tail_v;
   char* tail_k_out;
@@ -36,7 +39,9 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int tid = threadIdx.x;
   const int64_t bh = blockIdx.y, slot = blockIdx.x;
   const int batch = (int)(bh / a.heads);
-  const int from = a.rows ? min(max(a.rows[batch], 0), a.batch_in - 1) : batch;
+  const int from = a.rows_at >= 0 ? a.index[a.rows_at + batch]
+                   : a.rows       ? min(max(a.rows[batch], 0), a.batch_in - 1)
+                                  : batch;
   const int64_t src_bh = (int64_t)from * a.heads + (bh - (int64_t)batch * a.heads);
   if (slot == a.dst_capacity) {
     for (int64_t i = 16 * tid; i < a.tail_bytes; i += 16 * 256) {
@@ -49,7 +54,10 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   }
   const bool kept = slot < a.keep;
   int64_t page = slot;
-  if (kept && a.pages) page = min(max(a.pages[slot], 0), a.n_stored - 1);
+  if (kept && a.pages_at >= 0)
+    page = a.index[a.pages_at + slot];
+  else if (kept && a.pages)
+    page = min(max(a.pages[slot], 0), a.n_stored - 1);
   const int64_t src_page = src_bh * a.src_capacity + page, dst_page = bh * a.dst_capacity + slot;
   constexpr int kUnroll = 5;
   const int total = a.first[a.n_wide];
@@ -135,8 +143,8 @@ using namespace tp;
 
 extern "C" int32_t tp_copy_pages(const tp_page_copy* bufs, int32_t n_bufs, int64_t batch, int32_t heads,
                                  int64_t batch_in, const int32_t* rows, int64_t src_capacity, int64_t dst_capacity,
-                                 int32_t n_stored, const int32_t* page_index, int32_t keep, const void* tail_k,
-                                 const void* tail_v, void* tail_k_out, void* tail_v_out, int64_t tail_bytes,
+                                 int32_t n_stored, const int32_t* page_index, int32_t keep, int32_t host_index,
+                                 const void* tail_k, const void* tail_v, void* tail_k_out, void* tail_v_out, int64_t tail_bytes,
                                  int64_t tail_row, void* stream) {
   clear_error();
   if (n_bufs < 0 || n_bufs > kCopyBuffers || (n_bufs && !bufs) || batch < 1 || heads < 1 || batch_in < 1 ||
@@ -185,6 +193,27 @@ extern "C" int32_t tp_copy_pages(const tp_page_copy* bufs, int32_t n_bufs, int64
     } else {
       a.narrow[a.n_narrow++] = to;
     }
+  }
+  a.rows_at = a.pages_at = -1;
+  if (host_index && (rows || page_index)) {
+    const int64_t n_rows = rows ? batch : 0, n_pages = page_index ? keep : 0;
+    if (n_rows + n_pages > kCopyIndex) {
+      set_error("host indices hold at most %d entries, got %lld", kCopyIndex, (long long)(n_rows + n_pages));
+      return TP_ERR_INVALID;
+    }
+    for (int64_t i = 0; i < n_rows + n_pages; ++i) {
+      const bool row = i < n_rows;
+      const int32_t x = row ? rows[i] : page_index[i - n_rows];
+      const int64_t end = row ? batch_in : n_stored;
+      if (x < 0 || x >= end) {
+        set_error("%s %d outside the %lld there are", row ? "batch row" : "page", x, (long long)end);
+        return TP_ERR_INVALID;
+      }
+      a.index[i] = x;
+    }
+    if (rows) a.rows_at = 0;
+    if (page_index) a.pages_at = (int32_t)n_rows;
+    rows = page_index = nullptr;
   }
   a.src_capacity = src_capacity;
   a.dst_capacity = dst_capacity;

@@ -23,6 +23,7 @@ builds (:207-229).  The mechanism is this library's own:
 
 from __future__ import annotations
 
+import copy
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -204,8 +205,8 @@ class TurboPolarFastCache:
     def fork(self, tokens: Optional[int] = None, rows: Optional[Sequence[int]] = None,
              pages: Optional[Sequence[int]] = None) -> "TurboPolarFastCache":
         """An independent copy of this cache or a part of it (``TurboPolarKVCacheRuntime.fork``)."""
-        other = TurboPolarFastCache(self.config)
-        other.runtime = self.runtime.fork(tokens, rows, pages)
+        other = copy.copy(self)
+        other.runtime, other._store = self.runtime.fork(tokens, rows, pages), None
         return other
 
     def select_rows(self, rows: Sequence[int]) -> None:

@@ -777,20 +777,28 @@ def take_tokens(k: torch.Tensor, v: torch.Tensor, index: Union[Sequence[int], Se
     check(st, "tp_take_tokens")
 
 
-def copy_pages(buffers, batch: int, heads: int, batch_in: int, rows: Optional[torch.Tensor], src_capacity: int,
-               dst_capacity: int, n_stored: int, page_index: Optional[torch.Tensor], keep: int,
+def copy_pages(buffers, batch: int, heads: int, batch_in: int, rows: Optional[list], src_capacity: int,
+               dst_capacity: int, n_stored: int, page_index: Optional[list], keep: int,
                tails: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]], tail_tokens: int,
                device: torch.device) -> None:
     """tp_copy_pages: ``buffers`` is a list of (source, destination, bytes of a page), sources and
-    destinations contiguous ``[batch, heads, capacity, ...]``; ``tails`` (k, v, their copies), each
-    ``[batch, heads, 64, 128]`` and contiguous, of which ``tail_tokens`` rows are copied."""
+    destinations contiguous ``[batch, heads, capacity, ...]``; ``rows`` and ``page_index`` lists of
+    ints (the caller has checked them); ``tails`` (k, v, their copies), each ``[batch, heads, 64,
+    128]`` and contiguous, of which ``tail_tokens`` rows are copied."""
     bufs = (_lib.TPPageCopy * max(1, len(buffers)))(*[_lib.TPPageCopy(ptr(s), ptr(d), n) for s, d, n in buffers])
     tail_ptrs, tail_bytes, tail_row = (None,) * 4, 0, 0
     if tails is not None and tail_tokens:
         token = HEAD_DIM * tails[0].element_size()
         tail_ptrs, tail_bytes, tail_row = tuple(t.data_ptr() for t in tails), tail_tokens * token, PAGE * token
+    # Short indices travel with the launch; longer ones are copied to the device first.
+    on_host = len(rows or ()) + len(page_index or ()) <= 768
+    held = [
+        None if not x else (ctypes.c_int32 * len(x))(*x) if on_host else torch.tensor(x, dtype=torch.int32).to(device)
+        for x in (rows, page_index)
+    ]
+    row_ptr, page_ptr = (x if x is None else ctypes.addressof(x) if on_host else x.data_ptr() for x in held)
     st = call_on(
-        device, lib().tp_copy_pages, bufs, len(buffers), batch, heads, batch_in, ptr(rows), src_capacity, dst_capacity,
-        n_stored, ptr(page_index), keep, *tail_ptrs, tail_bytes, tail_row, stream_handle(device),
+        device, lib().tp_copy_pages, bufs, len(buffers), batch, heads, batch_in, row_ptr, src_capacity, dst_capacity,
+        n_stored, page_ptr, keep, 1 if on_host else 0, *tail_ptrs, tail_bytes, tail_row, stream_handle(device),
     )
     check(st, "tp_copy_pages")

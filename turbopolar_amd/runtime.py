@@ -21,6 +21,7 @@ rfsn_v11/generation/turbo_polar_cache.py:18-395.  Differences of mechanism
 
 from __future__ import annotations
 
+import copy
 import ctypes
 from typing import Any, Dict, Optional, Sequence, Tuple
 
@@ -298,15 +299,18 @@ class TurboPolarKVCacheRuntime:
 
     def _make_tail(self, B: int, H: int, D: int, dtype, device) -> None:
         """The tail's buffers and the launches' flag, if they are not there yet."""
-        if self._tail_k is None:
-            # Rows past the tail's length are never read, so they are not cleared.
-            self._tail_k = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
-            self._tail_v = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
+        self._make_tail_buffers(B, H, D, dtype, device)
         if self._flag is None:
             # Written by the append launches and read here, with no device-to-host
             # copy; the words past the first are a one-launch step's.
             words = step_flag_words(B, max(self.config.num_q_heads, H), H)
             self._flag = torch.zeros(words, dtype=torch.int32, pin_memory=True)
+
+    def _make_tail_buffers(self, B: int, H: int, D: int, dtype, device) -> None:
+        if self._tail_k is None:
+            # Rows past the tail's length are never read, so they are not cleared.
+            self._tail_k = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
+            self._tail_v = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
 
     def append_and_attend(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, scale: float, pages,
                           layout, defer_check: bool = False) -> Optional[torch.Tensor]:
@@ -686,8 +690,8 @@ class TurboPolarKVCacheRuntime:
         pages, left = min(tokens // PAGE, S), tokens - min(tokens // PAGE, S) * PAGE
         if pages < S:
             if left:
-                self._make_tail(self._batch_size, self._num_kv_heads, self._head_dim, self._input_dtype,
-                                self.k_storage.radii.device)
+                self._make_tail_buffers(self._batch_size, self._num_kv_heads, self._head_dim, self._input_dtype,
+                                        self.k_storage.radii.device)
                 self._decode_to_tail(self, pages)
             self.k_storage.block_count = self.v_storage.block_count = pages
             self.total_blocks = max(0, self.total_blocks - (S - pages))
@@ -718,7 +722,7 @@ class TurboPolarKVCacheRuntime:
             self.resolve_deferred_check()
         if tokens is not None and pages is not None:
             raise ValueError("fork() takes tokens or pages, not both")
-        other = TurboPolarKVCacheRuntime(self.config)
+        other = self._emptied()
         B, H, D, S = self._batch_size, self._num_kv_heads, self._head_dim, self.k_storage.block_count
         rows = None if rows is None else _indices(rows, B or 0, "rows", "batch rows")
         pages = None if pages is None else _indices(pages, S, "pages", "stored pages")
@@ -743,12 +747,22 @@ class TurboPolarKVCacheRuntime:
             other._tail_k, other._tail_v = self._tail_k[at].clone(), self._tail_v[at].clone()
         else:
             if left:
-                other._make_tail(n, H, D, self._input_dtype, device)
+                other._make_tail_buffers(n, H, D, self._input_dtype, device)
             self._copy_into(other, n, rows, pages, keep, cut, left, device)
         other.k_storage.block_count = other.v_storage.block_count = other.total_blocks = keep
         other._tail_len = left
         other.actual_seq_len = keep * PAGE + left
         other.bytes_written = keep * other._page_bytes() if keep else 0
+        return other
+
+    def _emptied(self) -> "TurboPolarKVCacheRuntime":
+        """A cache of this one's kind and codecs that holds nothing."""
+        other = type(self).__new__(type(self))
+        vars(other).update(vars(self))
+        # The encoder's layout follows its attributes, which may have been set: a copy of it.
+        other.polar_encoder = copy.copy(self.polar_encoder)
+        other._flag, other._epoch = None, 0
+        other.reset()
         return other
 
     def _copy_into(self, other, n, rows, pages, keep, cut, left, device) -> None:
@@ -762,26 +776,21 @@ class TurboPolarKVCacheRuntime:
             if moves[0][1] == moves[1][1]:
                 moves = [(moves[0][0] + moves[1][0], moves[0][1])]
             other.k_storage.metadata = dict(self.k_storage.metadata)
-        row_index = page_index = None
-        if rows is not None or pages:
-            index = torch.tensor((rows or []) + (pages or []), dtype=torch.int32).to(device, non_blocking=True)
-            row_index = None if rows is None else index[: len(rows)]
-            page_index = index[len(rows or []):] if pages else None
         tails = None
         if left and cut is None:
             tails = (self._tail_k, self._tail_v, other._tail_k, other._tail_v)
         for i, (buffers, held) in enumerate(moves):
             tail = tails if i == 0 else None
             if buffers or tail:
-                copy_pages(buffers, n, self._num_kv_heads, self._batch_size, row_index, held, capacity,
-                           self.k_storage.block_count if stored else 0, page_index, stored, tail, left, device)
+                copy_pages(buffers, n, self._num_kv_heads, self._batch_size, rows, held, capacity,
+                           self.k_storage.block_count if stored else 0, pages, stored, tail, left, device)
         if cut is not None:
             other._decode_to_tail(other, cut)
 
     def _adopt(self, other: "TurboPolarKVCacheRuntime") -> None:
         read, spent = self.bytes_read, self.compression_time_ns
         flag = self._flag if other._batch_size == self._batch_size else None
-        vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch,
+        vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch, "polar_encoder": self.polar_encoder,
                            "_flag": flag if flag is not None else other._flag})
 
     def select_rows(self, rows: Sequence[int]) -> None:
