@@ -13,7 +13,6 @@
 // Few tiles of rows: the keys are split over workgroups too, and joined by a second
 // launch.
 #include <algorithm>
-#include <type_traits>
 
 #include "tp_tiles.h"
 
@@ -37,7 +36,7 @@ struct PromptArgs {
   FastDiv div_units, div_splits, div_hkv, div_g;
   float c;        // |scale| log2(e)
   uint32_t flip;  // sign bits of a pair where the scale is negative
-  float* part_o;  // fp16 or fp32 records (store_record)
+  float* part_o;
   float* part_ml;
 };
 
@@ -281,8 +280,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
   const bool live = tok < t.nq;
   if (a.splits > 1) {
     const int64_t rec = (((int64_t)unit * a.tq + out_t) * a.g + head) * a.splits + split;
-    constexpr bool kHalf = std::is_same<T, F16>::value;
-    store_record<kHalf>(st, l, a.part_o + rec * (kHalf ? kHeadDim / 2 : kHeadDim), a.part_ml + rec * 2, live, lane);
+    store_record<false>(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
   } else if (!(t.rest && a.keep_rest)) {
     store_row<T>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + out_t * a.out_t,
                  live, lane);
@@ -292,7 +290,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
 // Joins the splits of a row: weights l_s 2^(m_s - max) over their sum.  A record's 16 bytes a lane: 16 lanes
 // (fp16) or 32 (fp32) take one, so 4 or 2 records go by side by side and are folded at the end, kAhead such
 // steps in flight.  WAVES waves a row, each a part of its records: one, or four where there are few rows of
-// many records (65 records of 1,024 rows: PLACEHOLDER us).
+// many records (129 records of 256 rows 8.4 -> 5.1 us, 65 of 1,024 7.4 -> 6.2).
 template <class T, bool HALF, int kAhead, int WAVES>
 __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
   constexpr int kLanes = HALF ? 16 : 32, kSide = 64 / kLanes, kDims = kHeadDim / kLanes;
@@ -401,20 +399,23 @@ static void launch_join_of(const JoinArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((join_splits_kernel<T, HALF, 5, 1>), grid, dim3(256), 0, s, a);
 }
 
-int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s) {
-  if (bf16)
+int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s) {
+  if (half_records)
+    launch_join_of<F16, true>(a, s);
+  else if (bf16)
     launch_join_of<BF16, false>(a, s);
   else
-    launch_join_of<F16, true>(a, s);
+    launch_join_of<F16, false>(a, s);
   return launch_status("join of the splits");
 }
 
 // Waves a workgroup, tiles of rows per unit (an upper bound where sequences are packed: each has one that
 // it does not fill, and so have the tokens behind them) and splits of the keys.  256 rows (8 waves) read
 // keys and values half as often as 128; where they leave part of the GPU idle, 128 rows do not, start
-// sooner and fit a CU twice.  Few tiles all the same: each is given to as many workgroups as fill the GPU,
-// of 8 tiles of keys at least
-// (the join takes as long as some 5 of them).  32/8 heads: PLACEHOLDER
+// sooner and fit a CU twice: 32/8 heads, 64 queries of 64 tokens 8.7 us (256 rows 10.9), but 8,192 causal tokens
+// 609 (256 rows 549).  Few tiles all the same: each is given to as many workgroups as fill the GPU, of 4 tiles of
+// keys at least, since the join takes as long as some 4 of them: 64 queries over 1,024 keys, us with the join,
+// at least 2, 4 or 8 tiles: 18.2, 18.2, 22.1; over 4,096 keys 32.8, 26.8, 25.0; over 512 keys (4 or 8) 17.1, 16.4.
 struct PromptPlan {
   int64_t waves, tiles, splits;
 };
@@ -427,7 +428,7 @@ static PromptPlan plan_prompt(int64_t units, int32_t g, int64_t tq, int64_t tk, 
   p.tiles = prompt_tiles(tq * g, p.waves * kWaveRows, n_seq);
   const int64_t all = units * p.tiles, key_tiles = (tk + kTileTokens - 1) / kTileTokens;
   const int64_t target = p.waves == 8 ? kPromptTarget : 2 * kPromptTarget;
-  p.splits = std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(all, 1), key_tiles / 8));
+  p.splits = std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(all, 1), key_tiles / 4));
   return p;
 }
 
@@ -549,5 +550,5 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.splits, j.g = g, j.hkv = hkv;
   j.rest_from = n_seq && keep_rest ? q_starts + n_seq : nullptr;
-  return launch_join(j, dtype != 0, s);
+  return launch_join(j, dtype != 0, false, s);
 }

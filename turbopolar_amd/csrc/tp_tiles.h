@@ -317,9 +317,10 @@ __device__ __forceinline__ void store_row(const RowState& st, float inv, uint16_
 }
 
 // A split's record of a row: its output divided by its sum, with the maximum (log2 units) and the
-// sum in fp32.  Splits of a row are joined by join_splits_kernel.  HALF, for fp16 results: the output in
-// fp16 too (it lies within the values' range), for half the bytes written and read back; each record's
-// rounding (half a step, 2^-11) is weighted by the record's share, so it stays below the result's own.
+// sum in fp32.  Splits of a row are joined by join_splits_kernel.  HALF: the output in fp16 (it lies
+// within the values' range), for half the bytes written and read back, where a row has dozens of records:
+// each one's rounding (half a step, 2^-11) is weighted by its share, so their sum stays below the result's
+// own.
 template <bool HALF>
 __device__ __forceinline__ void store_record(const RowState& st, float l, void* o, float* ml, bool live, int lane) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -350,7 +351,6 @@ struct JoinArgs {
   const int32_t* rest_from;  // tokens from *rest_from on are left as they are (NULL: none)
 };
 
-// Records in fp32 and results in bf16, or both in fp16.
-int32_t launch_join(const JoinArgs& a, bool bf16, hipStream_t s);
+int32_t launch_join(const JoinArgs& a, bool bf16, bool half_records, hipStream_t s);
 
 }  // namespace tp

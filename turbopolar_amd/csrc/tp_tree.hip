@@ -64,6 +64,7 @@ struct PageRegs {
   uint2v r8[tree_i8(KIND) ? N : 1];
   uint2v c8[KIND == kTreeFast ? N : 1];
   uint32_t c4[KIND == kTreeDefault ? N : 1];
+  uint32_t rows[tree_any(KIND) ? 2 * N : 1];  // dwords of the page's code rows, tid + threads i of them
   uint4v v[N];
   uint32_t vs[N];  // fp16 scale of the run's group
   uint32_t ls;     // fp16 page scale
@@ -87,6 +88,23 @@ __device__ __forceinline__ void load_page(const TreeArgs& a, int64_t slot, int t
     p.vs[n] = a.v_scales[row * kVGroups + (c >> 1)];
   }
   if constexpr (tree_i8(KIND)) p.ls = a.radii_scales[slot];
+  if constexpr (tree_any(KIND)) {  // at most 64 bytes of codes a token: 1,024 dwords, the level-1 rows first
+    const int l1 = kPageTokens / 4 * a.l1_row, all = l1 + kPageTokens / 4 * a.deep_row;
+    const uint32_t* l1_rows = reinterpret_cast<const uint32_t*>(a.angle_l1 + slot * kPageTokens * a.l1_row);
+    const uint32_t* deep_rows = reinterpret_cast<const uint32_t*>(a.angle_deep + slot * kPageTokens * a.deep_row);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      const int x = min(tid + THREADS * i, all - 1);  // threads past the last dword reread it
+      p.rows[i] = *(x < l1 ? l1_rows + x : deep_rows + (x - l1));
+    }
+  }
+}
+
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void stage_rows(int tid, const PageRegs<KIND, N>& p, uint32_t* codes) {
+  if constexpr (tree_any(KIND))
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) codes[tid + THREADS * i] = p.rows[i];
 }
 
 union TreeLut {
@@ -96,7 +114,7 @@ union TreeLut {
 
 // Decodes half h of run n into a tile of keys: 4 pairs, 16 bytes.
 template <int KIND, int N, int THREADS>
-__device__ __forceinline__ void decode_keys(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
+__device__ __forceinline__ void decode_keys(const TreeArgs& a, const TreeLut& lut, const uint32_t* codes, int tid,
                                             const PageRegs<KIND, N>& p, int n, int h, char* kt) {
   const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
   uint32_t e[4];
@@ -109,19 +127,21 @@ __device__ __forceinline__ void decode_keys(const TreeArgs& a, const TreeLut& lu
     }
   } else {
     const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;
+    int c0 = c;  // where a pair's code lies is computed anew: kept over the pages, it costs 30 registers
+    if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t code;
       if constexpr (KIND == kTreeFast) {
         code = 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
       } else {
-        const int pair = 8 * c + 4 * h + i;
+        const int pair = 8 * c0 + 4 * h + i;
         const bool l1 = pair < a.split_half;
         const int bits = l1 ? a.l1_bits : a.deep_bits;
         const int bit = (l1 ? pair : pair - a.split_half) * bits;
-        const uint8_t* row = l1 ? a.angle_l1 + (slot * kPageTokens + t) * a.l1_row
-                                : a.angle_deep + (slot * kPageTokens + t) * a.deep_row;
-        code = (l1 ? 0u : 256u) + ((row[bit >> 3] >> (bit & 7)) & ((1u << bits) - 1u));
+        const int row = l1 ? t * a.l1_row : kPageTokens * a.l1_row + t * a.deep_row;
+        const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
+        code = (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
       }
       half2v r;
       if constexpr (tree_i8(KIND)) {
@@ -157,12 +177,12 @@ __device__ __forceinline__ void decode_values(int tid, const PageRegs<KIND, N>& 
 
 // Piece i of the 4 N that a page takes.
 template <int KIND, int N, int THREADS>
-__device__ __forceinline__ void decode_piece(const TreeArgs& a, const TreeLut& lut, int64_t slot, int tid,
+__device__ __forceinline__ void decode_piece(const TreeArgs& a, const TreeLut& lut, const uint32_t* codes, int tid,
                                              const PageRegs<KIND, N>& p, int i, char* kt, char* vt) {
   if (i & 2)
     decode_values<KIND, N, THREADS>(tid, p, i >> 2, i & 1, vt);
   else
-    decode_keys<KIND, N, THREADS>(a, lut, slot, tid, p, i >> 2, i & 1, kt);
+    decode_keys<KIND, N, THREADS>(a, lut, codes, tid, p, i >> 2, i & 1, kt);
 }
 
 // 64 dense tokens from k, v (t strides in elements) into the tiles; rows from `count` on repeat the
@@ -205,6 +225,8 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW, BUFS = RW * TW > 2 ? 2 : 1;
   __shared__ __align__(16) char tiles[BUFS][2][kTileBytes];
   __shared__ TreeLut lut;
+  __shared__ uint32_t codes[tree_any(KIND) ? BUFS : 1][tree_any(KIND) ? 1024 : 1];  // any layout's code rows
+  __shared__ float side_ml[TW == 2 ? RW : 1][2][64];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rest = fast_div(blockIdx.x, a.div_units), unit = blockIdx.x - rest * a.units;
@@ -249,9 +271,13 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
     float16v s[1][NB];
     if constexpr (BUFS == 1) {
       for (; page < page_end; ++page) {
+        if constexpr (tree_any(KIND)) {
+          stage_rows<KIND, N, THREADS>(tid, p, codes[0]);
+          __syncthreads();
+        }
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i)
-          decode_piece<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, i, tiles[0][0], tiles[0][1]);
+          decode_piece<KIND, N, THREADS>(a, lut, codes[0], tid, p, i, tiles[0][0], tiles[0][1]);
         __syncthreads();
         // The last page again rather than none: a load under a branch is waited for at its join.
         load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
@@ -261,19 +287,24 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
       }
     } else {
       // The next page is decoded under this one's first products.
+      if constexpr (tree_any(KIND)) {
+        stage_rows<KIND, N, THREADS>(tid, p, codes[0]);
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < 4 * N; ++i)
-        decode_piece<KIND, N, THREADS>(a, lut, slot0 + page, tid, p, i, tiles[0][0], tiles[0][1]);
+        decode_piece<KIND, N, THREADS>(a, lut, codes[0], tid, p, i, tiles[0][0], tiles[0][1]);
       load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
       for (int buf = 0; page < page_end; ++page, buf ^= 1) {
         char *kt = tiles[buf ^ 1][0], *vt = tiles[buf ^ 1][1];
-        const int next = min(page + 1, page_end - 1);
+        const uint32_t* rows_of = codes[tree_any(KIND) ? buf ^ 1 : 0];
+        stage_rows<KIND, N, THREADS>(tid, p, codes[tree_any(KIND) ? buf ^ 1 : 0]);
         __syncthreads();
         score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s[0], [&](int i) {
           constexpr int kProducts = 8 * NB, kPieces = 4 * N;
 #pragma unroll
           for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x)
-            decode_piece<KIND, N, THREADS>(a, lut, slot0 + next, tid, p, x, kt, vt);
+            decode_piece<KIND, N, THREADS>(a, lut, rows_of, tid, p, x, kt, vt);
         });
         load_page<KIND, N, THREADS>(a, slot0 + min(page + 2, page_end - 1), tid, p);
         finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, rows);
@@ -319,18 +350,19 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   }
   if constexpr (TW == 2) {  // the second half's rows join the first's
     __syncthreads();
-    float* side = reinterpret_cast<float*>(&tiles[0][0][0]) + rw * 66 * 64 + lane;
+    static_assert(RW * 64 * 64 * sizeof(float) <= sizeof(tiles), "the second half's rows lie over the tiles");
+    float* side = reinterpret_cast<float*>(&tiles[0][0][0]) + rw * 64 * 64 + lane;
     if (tw == 1) {
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) side[(16 * db + i) * 64] = st.o[db][i];
-      side[64 * 64] = st.m;
-      side[65 * 64] = st.l;
+      side_ml[rw][0][lane] = st.m;
+      side_ml[rw][1][lane] = st.l;
     }
     __syncthreads();
     if (tw == 0) {
-      const float m1 = side[64 * 64], l1 = side[65 * 64];
+      const float m1 = side_ml[rw][0][lane], l1 = side_ml[rw][1][lane];
       const float m = fmaxf(st.m, m1), base = m == -INFINITY ? 0.0f : m;
       const float w0 = __builtin_amdgcn_exp2f(st.m - base), w1 = __builtin_amdgcn_exp2f(m1 - base);
 #pragma unroll
@@ -353,16 +385,22 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   }
 }
 
-// Rows of a workgroup, and how the pages are split: into as many workgroups as fill the GPU.  The
-// tail and the drafts take one more record, unless there is but one split of pages.
+// Rows of a workgroup, and how the pages are split: into as many workgroups as fill the GPU (two waves a
+// SIMD).  Measured with 32/8 heads, us without the join:
+//   up to 32 rows: two waves, four workgroups a CU, 58 over 131,072 tokens (four waves, two of them decoding only,
+//     67); layouts whose codes go through LDS take the four of 64 rows, since a thread of two waves decodes four
+//     runs, for which they have no registers (2-bit deep codes over 32,768 tokens 32 instead of 54);
+//   up to 128 rows: four waves, 31 over 32,768 tokens (eight, each with half of a page's tokens, 37); the layouts
+//     through LDS, which spill at four, the eight (split at pair 23: 48 instead of 88).
+// The tail and the drafts take one more record, unless there is but one split of pages.
 struct TreePlan {
   int32_t row_waves, row_blocks, pages_per_split, page_splits, records;
 };
-static TreePlan plan_tree(int64_t units, int64_t rows, int32_t n_pages) {
+static TreePlan plan_tree(int64_t units, int64_t rows, int32_t n_pages, bool any) {
   TreePlan p;
-  p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  p.row_waves = rows <= 32 && !any ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   p.row_blocks = (int32_t)((rows + p.row_waves * kWaveRows - 1) / (p.row_waves * kWaveRows));
-  const int64_t target = kTreeTarget / (p.row_waves == 8 ? 8 : p.row_waves == 1 ? 2 : 4);
+  const int64_t target = kTreeTarget / (p.row_waves == 8 || (p.row_waves == 4 && any) ? 8 : p.row_waves == 1 ? 2 : 4);
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(target / (units * p.row_blocks), n_pages));
   p.pages_per_split = (int32_t)std::max<int64_t>(1, (n_pages + splits - 1) / splits);
   p.page_splits = (n_pages + p.pages_per_split - 1) / p.pages_per_split;
@@ -373,9 +411,17 @@ static TreePlan plan_tree(int64_t units, int64_t rows, int32_t n_pages) {
 template <int KIND>
 static void launch_tree(const TreeArgs& a, int row_waves, dim3 grid, hipStream_t s) {
   switch (row_waves) {
-    case 1: hipLaunchKernelGGL((tree_attention_kernel<KIND, 1, 2>), grid, dim3(kTreeThreads<1, 2>), 0, s, a); break;
+    case 1:
+      if constexpr (!tree_any(KIND))
+        hipLaunchKernelGGL((tree_attention_kernel<KIND, 1, 2>), grid, dim3(kTreeThreads<1, 2>), 0, s, a);
+      break;
     case 2: hipLaunchKernelGGL((tree_attention_kernel<KIND, 2, 2>), grid, dim3(kTreeThreads<2, 2>), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((tree_attention_kernel<KIND, 4, 1>), grid, dim3(kTreeThreads<4, 1>), 0, s, a); break;
+    case 4:
+      if constexpr (tree_any(KIND))
+        hipLaunchKernelGGL((tree_attention_kernel<KIND, 4, 2>), grid, dim3(kTreeThreads<4, 2>), 0, s, a);
+      else
+        hipLaunchKernelGGL((tree_attention_kernel<KIND, 4, 1>), grid, dim3(kTreeThreads<4, 1>), 0, s, a);
+      break;
     default: hipLaunchKernelGGL((tree_attention_kernel<KIND, 8, 1>), grid, dim3(kTreeThreads<8, 1>), 0, s, a); break;
   }
 }
@@ -386,7 +432,8 @@ using namespace tp;
 
 extern "C" size_t tp_tree_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t nodes, int32_t n_pages) {
   if (batch < 1 || hkv < 1 || hq < hkv || hq % hkv || nodes < 1 || nodes > kTreeMaxNodes || n_pages < 0) return 0;
-  const TreePlan p = plan_tree(batch * hkv, (int64_t)nodes * (hq / hkv), n_pages);
+  // Of the layouts, those with workgroups of two waves have the most splits.
+  const TreePlan p = plan_tree(batch * hkv, (int64_t)nodes * (hq / hkv), n_pages, false);
   return p.records == 1 ? 0 : (size_t)batch * hq * nodes * p.records * (kHeadDim * sizeof(uint16_t) + 2 * sizeof(float));
 }
 
@@ -451,7 +498,9 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
     return TP_ERR_INVALID;
   }
   const int64_t units = batch * hkv, rows = (int64_t)nodes * (hq / hkv);
-  const TreePlan p = plan_tree(units, rows, n_pages);
+  const bool is_default = !layout->int8_radii && layout->l1_bits == 4 && layout->deep_bits == 4 && layout->split_dim == 64;
+  const bool is_fast = layout->int8_radii && layout->deep_bits == 8 && layout->split_dim == 0;
+  const TreePlan p = plan_tree(units, rows, n_pages, !is_default && !is_fast);
   if ((double)units * p.row_blocks * p.records > (double)INT32_MAX) {
     set_error("too many workgroups for one launch");
     return TP_ERR_INVALID;
@@ -510,8 +559,6 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
   a.div_g = make_fastdiv((uint32_t)a.g);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(units * p.row_blocks * p.records));
-  const bool is_default = !layout->int8_radii && layout->l1_bits == 4 && layout->deep_bits == 4 && layout->split_dim == 64;
-  const bool is_fast = layout->int8_radii && layout->deep_bits == 8 && layout->split_dim == 0;
   if (is_default)
     launch_tree<kTreeDefault>(a, p.row_waves, grid, s);
   else if (is_fast)
@@ -529,5 +576,5 @@ extern "C" int32_t tp_tree_attention(const void* q, void* out, int64_t batch, in
   j.rows = rows;
   j.out_b = a.out_b, j.out_h = a.out_h, j.out_t = a.out_t;
   j.units = a.units, j.splits = a.records, j.g = a.g, j.hkv = hkv;
-  return launch_join(j, false, s);
+  return launch_join(j, false, true, s);
 }
