@@ -15,7 +15,7 @@ import torch
 import oracle
 from common import ATOL, LAYOUTS, PAGE, RTOL_L2, gen_kv, rel_l2
 from turbopolar_amd import DraftTree, HipKernelBridge, TurboPolarConfig, TurboPolarFastCache, wire
-from turbopolar_amd.kernels import fp16_scale
+from turbopolar_amd.kernels import fp16_scale, prompt_attention
 
 pytestmark = pytest.mark.gpu
 EPS = 2.0 ** -11
@@ -483,3 +483,42 @@ def test_prompt_through_the_cache(device, dtype):
     with pytest.raises(ValueError):
         cache.prompt_attention(q, k[:, :, :5], v[:, :, :5], 0.088)
     assert cache.offset == 201
+
+
+def test_emptied_branches(device):
+    """A branch that never had a tail, cut to nothing, is forked, filled and forked again."""
+    cache = filled(device, "default", 2, 8, 2, 64 * 3, seed=4)
+    branch = cache.fork()
+    branch.truncate(0)
+    again = branch.fork(rows=[1])
+    assert again.offset == 0 and branch.fork(pages=[]).offset == 0
+    k, v = (torch.from_numpy(x).to(device) for x in gen_kv(5, 1, 2, 70))
+    again.runtime.append(k, v)
+    fresh = TurboPolarFastCache(config("default", 8, 2))
+    fresh.runtime.append(k, v)
+    same_pages(again.runtime, fresh.runtime)
+    assert torch.equal(again.fork().runtime.partial_k, fresh.runtime.partial_k) and cache.offset == 192
+
+
+def test_trees_on_another_stream(device):
+    """A tree that is dropped while another stream still reads it keeps its masks' memory until then."""
+    cache = filled(device, "default", 1, 8, 2, 64 * 100, seed=5)
+    q, dk, dv = draft(device, 1, 8, 2, 60, seed=5)
+    parents = random_parents(60, 5)
+    want = cache.tree_attention(q, dk, dv, DraftTree(parents), 0.1)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        tree = DraftTree(parents, device=device)
+        with torch.cuda.stream(side):
+            got = [cache.tree_attention(q, dk, dv, tree, 0.1) for _ in range(4)]
+        del tree
+        over = [torch.zeros((1, 60, 1), dtype=torch.int64, device=device) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got) and len(over) == 4
+
+
+def test_prompt_in_place(device):
+    q, k, v = draft(device, 1, 8, 2, 300, seed=6)
+    want = prompt_attention(q, k, v, 0.1)
+    assert torch.equal(prompt_attention(q, k, v, 0.1, out=q), want)

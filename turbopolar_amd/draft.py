@@ -10,7 +10,7 @@ every step keeps it.
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -21,7 +21,7 @@ class DraftTree:
     """``parents``: one parent per node, or one such list per batch row.  Lists of
     different lengths are padded; a padding node's output row is 0.  ``device``: where
     the masks are put at once (otherwise at the first call on a device, by a copy that
-    waits)."""
+    waits).  A captured graph reads the masks: keep the tree as long as the graph."""
 
     def __init__(self, parents: Sequence, device=None):
         rows = list(parents)
@@ -53,7 +53,7 @@ class DraftTree:
             sees += [0] * (self.nodes - len(sees))
             table.append([[_signed((s >> (64 * w)) & (2 ** 64 - 1)) for w in range(words)] for s in sees])
         self._mask = torch.tensor(table, dtype=torch.int64)  # [1 or batch, nodes, words]
-        self._on: Dict[torch.device, torch.Tensor] = {}
+        self._on: Dict[torch.device, Tuple[torch.Tensor, Optional[torch.cuda.Stream]]] = {}
         if device is not None:
             self.mask_on(torch.device(device))
 
@@ -63,8 +63,14 @@ class DraftTree:
         if hit is None:
             if device.type == "cuda" and device.index is None:
                 return self.mask_on(torch.device("cuda", torch.cuda.current_device()))
-            hit = self._on[device] = self._mask.to(device)
-        return hit
+            stream = torch.cuda.current_stream(device) if device.type == "cuda" else None
+            hit = self._on[device] = (self._mask.to(device), stream)
+        mask, stream = hit
+        if stream is not None and not torch.cuda.is_current_stream_capturing():
+            now = torch.cuda.current_stream(device)
+            if now != stream:
+                mask.record_stream(now)  # the tree may go while a call on that stream still reads
+        return mask
 
     def depths(self, row: int = 0) -> List[int]:
         """Tokens between the cache's last one and each node: node i sits at position

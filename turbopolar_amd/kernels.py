@@ -619,6 +619,7 @@ def prompt_attention(
     token positions between them, as sequences of ints or host tensors, which are checked, or as
     int32 device tensors, which are not read here (values out of order give unspecified rows).
     Query rows behind the last sequence are 0, or left as they are where ``out`` is given.
+    ``out`` shares no memory with k or v, nor with q unless it is q.
 
     Returns ``out``, or a new ``[B, H_q, Tq, 128]`` of q's type that lies token by token."""
     for name, t in (("q", q), ("k", k), ("v", v)):

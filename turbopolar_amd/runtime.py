@@ -741,7 +741,7 @@ class TurboPolarKVCacheRuntime:
         n = B if rows is None else len(rows)
         other._batch_size, other._num_kv_heads, other._head_dim, other._input_dtype = n, H, D, self._input_dtype
         other._initialized = True
-        device = self._tail_k.device if S == 0 else self.k_storage.radii.device
+        device = (self._tail_k if self.k_storage.radii is None else self.k_storage.radii).device
         if self._tail_k is not None and not device.type == "cuda":
             at = list(range(B)) if rows is None else rows
             other._tail_k, other._tail_v = self._tail_k[at].clone(), self._tail_v[at].clone()
@@ -790,8 +790,8 @@ class TurboPolarKVCacheRuntime:
     def _adopt(self, other: "TurboPolarKVCacheRuntime") -> None:
         read, spent = self.bytes_read, self.compression_time_ns
         flag = self._flag if other._batch_size == self._batch_size else None
-        vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch, "polar_encoder": self.polar_encoder,
-                           "_flag": flag if flag is not None else other._flag})
+        vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch,
+                           "polar_encoder": self.polar_encoder, "_flag": flag if flag is not None else other._flag})
 
     def select_rows(self, rows: Sequence[int]) -> None:
         """Makes batch row i what row ``rows[i]`` was (beams re-ordered, or a batch that grows or
