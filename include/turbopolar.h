@@ -418,7 +418,8 @@ typedef struct tp_page_copy {
 int32_t tp_copy_pages(const tp_page_copy* bufs, int32_t n_bufs, int64_t batch, int32_t heads, int64_t batch_in,
                       const int32_t* rows, int64_t src_capacity, int64_t dst_capacity, int32_t n_stored,
                       const int32_t* page_index, int32_t keep, int32_t host_index, const void* tail_k,
-                      const void* tail_v, void* tail_k_out, void* tail_v_out, int64_t tail_bytes, int64_t tail_row, void* stream);
+                      const void* tail_v, void* tail_k_out, void* tail_v_out, int64_t tail_bytes, int64_t tail_row,
+                      void* stream);
 
 /*
  * Tokens index[0 .. n) (a host array; with per_batch one run of n for each batch row;

@@ -160,6 +160,11 @@ __device__ __forceinline__ void multiply_tile(const char* kt, const char* vt, co
   }
 }
 
+// S^T = K Q^T and O^T += V^T P^T, so that a query is a column: its scores, maximum, sum and output stay with one
+// pair of lanes, and P goes from the first product to the second in registers.  The work is 4 x 128 operations a
+// query and key; the matrix units bind long prompts (32/8 heads, causal, fp16 4,096 tokens 151 us, 0.91 PFLOP/s;
+// bf16 16,384 tokens 1.9 to 2.1 ms, 1.05 to 1.15, where the clock falls to 1.7 GHz; a large library product 1.2 to
+// 1.3).  Where one wave of a SIMD computes its softmax, its partner multiplies (8 waves in two phases a tile).
 template <class T, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptArgs a) {
   constexpr int ROWS = WAVES * kWaveRows, THREADS = WAVES * 64;

@@ -42,9 +42,9 @@ __host__ __device__ inline int tile_swizzle(int t) { return ((t & 3) << 2) | ((t
 // Byte offset of 16-byte chunk c of token t.
 __host__ __device__ inline int tile_at(int t, int c) { return t * (kHeadDim * 2) + ((c ^ tile_swizzle(t)) << 4); }
 
-// Element types: the product and the rounding of a pair of weights (to nearest: the
-// weights are at most 1, so an output's rounding error stays below half a step of
-// the type relative to the largest value).
+// Element types: the product and the rounding of a pair of weights (to nearest: each
+// is off by at most half a step of itself, so an output's rounding error stays below
+// half a step of the type relative to the largest value).
 struct F16 {
   typedef half8v frag;
   static __device__ __forceinline__ float16v mfma(uint4v a, uint4v b, float16v c) {
