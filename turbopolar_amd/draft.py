@@ -14,6 +14,8 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ._lib import stream_handle
+
 MAX_NODES = 256
 
 
@@ -53,23 +55,24 @@ class DraftTree:
             sees += [0] * (self.nodes - len(sees))
             table.append([[_signed((s >> (64 * w)) & (2 ** 64 - 1)) for w in range(words)] for s in sees])
         self._mask = torch.tensor(table, dtype=torch.int64)  # [1 or batch, nodes, words]
-        self._on: Dict[torch.device, Tuple[torch.Tensor, Optional[torch.cuda.Stream]]] = {}
+        self._on: Dict[torch.device, Tuple[torch.Tensor, int]] = {}
         if device is not None:
             self.mask_on(torch.device(device))
 
     def mask_on(self, device: torch.device) -> torch.Tensor:
-        """The masks on ``device``, int64 ``[1 or batch, nodes, words]``."""
+        """The masks on ``device``, int64 ``[1 or batch, nodes, words]``, for a call on its current
+        stream."""
         hit = self._on.get(device)
         if hit is None:
-            if device.type == "cuda" and device.index is None:
+            if device.type != "cuda":
+                return self._mask
+            if device.index is None:
                 return self.mask_on(torch.device("cuda", torch.cuda.current_device()))
-            stream = torch.cuda.current_stream(device) if device.type == "cuda" else None
-            hit = self._on[device] = (self._mask.to(device), stream)
+            hit = self._on[device] = (self._mask.to(device), stream_handle(device))
         mask, stream = hit
-        if stream is not None and not torch.cuda.is_current_stream_capturing():
-            now = torch.cuda.current_stream(device)
-            if now != stream:
-                mask.record_stream(now)  # the tree may go while a call on that stream still reads
+        if stream_handle(device) != stream and not torch.cuda.is_current_stream_capturing():
+            # The tree may go while that call still reads.
+            mask.record_stream(torch.cuda.current_stream(device))
         return mask
 
     def depths(self, row: int = 0) -> List[int]:

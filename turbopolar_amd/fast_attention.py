@@ -33,8 +33,8 @@ from .codecs import GroupedVQuantizer, PolarQuantDecoder
 from .config import TurboPolarConfig
 from .draft import DraftTree
 from .kernels import (
-    HEAD_DIM, PAGE, _check_draft, _no_grad, decode_attention_store, decode_pages_into, fp16_scale, prompt_attention,
-    tree_attention,
+    HEAD_DIM, PAGE, _check_draft, _no_grad, _tree_attention, decode_attention_store, decode_pages_into, fp16_scale,
+    prompt_attention,
 )
 from .runtime import TurboPolarKVCacheRuntime
 from .storage import pages_of
@@ -191,8 +191,8 @@ class TurboPolarFastCache:
         held = rt.k_storage.radii if n_pages else tail_k
         if held is not None and held.device != q.device:
             raise ValueError(f"q is on {q.device}, the cache on {held.device}")
-        return tree_attention(q, rt.polar_encoder.layout, self._store_pages() if n_pages else None, n_pages, tail_k,
-                              tail_v, k_draft, v_draft, tree, fp16_scale(scale))
+        return _tree_attention(q, rt.polar_encoder.layout, self._store_pages() if n_pages else None, n_pages, tail_k,
+                               tail_v, k_draft, v_draft, tree, fp16_scale(scale))
 
     def accept(self, k_draft: torch.Tensor, v_draft: torch.Tensor, path: Sequence) -> None:
         """Appends the drafted tokens ``path`` (node indices, root first; ``DraftTree.path_to``)."""

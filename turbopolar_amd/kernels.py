@@ -571,7 +571,7 @@ def _strided(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
 
 def _token_major(B: int, H: int, T: int, dtype, device) -> torch.Tensor:
     """An output ``[B, H, T, 128]`` that lies token by token, as the output projection reads it."""
-    return torch.empty((B, T, H, HEAD_DIM), dtype=dtype, device=device).transpose(1, 2)
+    return torch.empty_strided((B, H, T, HEAD_DIM), (T * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, 1), dtype=dtype, device=device)
 
 
 def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -699,6 +699,11 @@ def tree_attention(q: torch.Tensor, layout, pages: Optional[TPPages], n_pages: i
     float16 are converted to it, as the cache and the decode step do.  Returns fp16 ``[B, H_q, T,
     128]`` that lies token by token."""
     _check_draft(q, draft_k, draft_v, tree)
+    return _tree_attention(q, layout, pages, n_pages, tail_k, tail_v, draft_k, draft_v, tree, scale)
+
+
+def _tree_attention(q, layout, pages, n_pages, tail_k, tail_v, draft_k, draft_v, tree, scale) -> torch.Tensor:
+    """``tree_attention`` of a checked draft."""
     B, Hq, T, _ = q.shape
     Hkv = int(draft_k.shape[1])
     dev = q.device
@@ -712,8 +717,7 @@ def tree_attention(q: torch.Tensor, layout, pages: Optional[TPPages], n_pages: i
     (q, qs), (dk, ks), (dv, vs) = (_strided(t if t.dtype is torch.float16 else t.to(torch.float16))
                                    for t in (q, draft_k, draft_v))
     mask = tree.mask_on(dev)
-    out = _token_major(B, Hq, T, torch.float16, dev)
-    _, os_ = _strided(out)
+    out, os_ = _token_major(B, Hq, T, torch.float16, dev), (T * Hq * HEAD_DIM, HEAD_DIM, Hq * HEAD_DIM)
     if pages is None:
         pages, n_pages = _NO_PAGES, 0
     ws = _scratch(_tree_workspace(B, Hq, Hkv, T, n_pages), dev)
