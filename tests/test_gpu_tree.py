@@ -522,3 +522,28 @@ def test_prompt_in_place(device):
     q, k, v = draft(device, 1, 8, 2, 300, seed=6)
     want = prompt_attention(q, k, v, 0.1)
     assert torch.equal(prompt_attention(q, k, v, 0.1, out=q), want)
+
+
+def test_branches_cut_to_nothing(device):
+    """Forks of no tokens or pages own no buffers: they are forked, re-ordered, attended and filled all the same."""
+    cache = filled(device, "fast", 2, 8, 2, 64 * 3, seed=8)
+    kept = cache.fork()
+    kept.keep_pages([])
+    k, v = (torch.from_numpy(x).to(device) for x in gen_kv(9, 2, 2, 70))
+    fresh = TurboPolarFastCache(cache.config)
+    fresh.runtime.append(k, v)
+    q, dk, dv = draft(device, 2, 8, 2, 3, seed=9)
+    tree = DraftTree([-1, 0, 0])
+    alone = TurboPolarFastCache(cache.config).tree_attention(q, dk, dv, tree, 0.1)
+    for branch in (cache.fork(tokens=0), cache.fork(pages=[]), kept):
+        assert branch.offset == 0 and branch.runtime.k_storage.radii is None and branch.runtime._tail_k is None
+        for again in (branch.fork(), branch.fork(tokens=0, rows=[1, 0]), branch.fork(pages=[])):
+            assert torch.equal(again.tree_attention(q, dk, dv, tree, 0.1), alone)
+            again.runtime.append(k, v)
+            same_pages(again.runtime, fresh.runtime)
+            assert torch.equal(again.runtime.partial_v, fresh.runtime.partial_v)
+        branch.select_rows([0])
+        branch.keep_pages([])
+        branch.runtime.append(k[:1], v[:1])
+        same_pages(branch.runtime, fresh.runtime, rows=[0])
+    assert cache.offset == 192

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from turbopolar_amd import DraftTree, TurboPolarConfig, TurboPolarFastCache, TurboPolarKVCacheRuntime, _lib
+from turbopolar_amd import DraftTree, TurboPolarConfig, TurboPolarFastCache, TurboPolarKVCacheRuntime, _lib, wire
 from turbopolar_amd.kernels import _overlaps, _starts, prompt_attention
 
 H = torch.float16
@@ -265,3 +265,27 @@ def test_empty_cache():
         rt.fork(rows=[0])
     with pytest.raises(ValueError):
         rt.truncate(1)
+
+
+def emptied(B=2):
+    """A cache that was cut to nothing and holds no buffers, as a fork of no tokens does on a device."""
+    rt, _, _ = host_cache(B)
+    rt.truncate(0)
+    rt = wire.load_state_dict(*wire.state_dict(rt), "cpu")
+    assert rt._initialized and rt._tail_k is None and rt.k_storage.radii is None
+    return rt
+
+
+def test_branches_of_a_cache_without_buffers():
+    rt = emptied()
+    for other, B in ((rt.fork(), 2), (rt.fork(tokens=0), 2), (rt.fork(pages=[]), 2), (rt.fork(rows=[1, 0, 0]), 3)):
+        assert other.actual_seq_len == 0 and other._batch_size == B and other._initialized
+        k = torch.randn(B, 2, 3, 128).half()
+        other.append(k, k)
+        assert torch.equal(other.fork().partial_k, k)
+    rt.select_rows([1])
+    rt.keep_pages([])
+    with pytest.raises(ValueError, match="batch size"):
+        rt.append(k, k)
+    rt.append(k[:1], k[:1])
+    assert rt.actual_seq_len == 3

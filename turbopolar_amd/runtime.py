@@ -741,7 +741,10 @@ class TurboPolarKVCacheRuntime:
         n = B if rows is None else len(rows)
         other._batch_size, other._num_kv_heads, other._head_dim, other._input_dtype = n, H, D, self._input_dtype
         other._initialized = True
-        device = (self._tail_k if self.k_storage.radii is None else self.k_storage.radii).device
+        held = self._tail_k if self.k_storage.radii is None else self.k_storage.radii
+        if held is None:  # a branch cut to nothing has no buffers either
+            return other
+        device = held.device
         if self._tail_k is not None and not device.type == "cuda":
             at = list(range(B)) if rows is None else rows
             other._tail_k, other._tail_v = self._tail_k[at].clone(), self._tail_v[at].clone()
