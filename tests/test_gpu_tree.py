@@ -547,3 +547,15 @@ def test_branches_cut_to_nothing(device):
         branch.runtime.append(k[:1], v[:1])
         same_pages(branch.runtime, fresh.runtime, rows=[0])
     assert cache.offset == 192
+
+
+def test_prompt_refused_leaves_the_cache(device):
+    """A scale that is not finite in 32 bits is refused before the chunk is appended."""
+    cache = filled(device, "fast", 1, 8, 2, 100, seed=2)
+    q, k, v = draft(device, 1, 8, 2, 5, seed=2)
+    for scale in (float("nan"), float("-inf"), 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            cache.prompt_attention(q, k, v, scale)
+        assert cache.offset == 100
+    cache.prompt_attention(q, k, v, 0.1)
+    assert cache.offset == 105

@@ -289,3 +289,13 @@ def test_branches_of_a_cache_without_buffers():
         rt.append(k, k)
     rt.append(k[:1], k[:1])
     assert rt.actual_seq_len == 3
+
+
+@pytest.mark.parametrize("scale,error", [(float("nan"), ValueError), (float("inf"), ValueError), (1e300, ValueError),
+                                         (None, TypeError)])
+def test_prompt_scale_is_checked_first(scale, error):
+    """Before the device, and so before the append."""
+    c = cache()
+    with pytest.raises(error, match="scale|float"):
+        c.prompt_attention(x(1, 4, 3, 128), x(1, 2, 3, 128), x(1, 2, 3, 128), scale)
+    assert c.offset == 0

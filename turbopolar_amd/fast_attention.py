@@ -24,6 +24,8 @@ builds (:207-229).  The mechanism is this library's own:
 from __future__ import annotations
 
 import copy
+import math
+from ctypes import c_float
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -166,6 +168,10 @@ class TurboPolarFastCache:
             raise ValueError(f"q {tuple(q.shape)}, keys {tuple(keys.shape)} and values {tuple(values.shape)} differ")
         if q.shape[1] < 1 or keys.shape[1] < 1 or q.shape[1] % keys.shape[1]:
             raise ValueError(f"H_q={q.shape[1]} is not a multiple of H_kv={keys.shape[1]}")
+        # Before the append: a refused call leaves the cache as it was.
+        scale = float(scale)
+        if not math.isfinite(c_float(scale).value):
+            raise ValueError(f"scale must be finite in 32 bits, got {scale}")
         if not (q.device == keys.device == values.device and q.is_cuda):
             raise ValueError(f"q is on {q.device}, keys on {keys.device}, values on {values.device}; need one HIP device")
         _no_grad(q, keys, values)
