@@ -559,3 +559,25 @@ def test_prompt_refused_leaves_the_cache(device):
         assert cache.offset == 100
     cache.prompt_attention(q, k, v, 0.1)
     assert cache.offset == 105
+
+
+@pytest.mark.parametrize("use,pages,rows", [
+    (lambda c: c.select_rows([1, 1, 0]), list(range(6)), [1, 1, 0]), (lambda c: c.keep_pages([5, 0]), [5, 0], [0, 1])])
+def test_replaced_buffers_outlive_their_copy(device, use, pages, rows):
+    """Rows selected and pages kept on a stream other than the buffers' own: what another stream allocates
+    while the copy still waits does not lie over what it reads."""
+    side = torch.cuda.Stream()
+    for seed in range(3):
+        cache = filled(device, "fast", 2, 8, 2, 64 * 6 + 20, seed=seed)
+        rt = cache.runtime
+        before, tail = buffers(rt), rt.partial_k
+        sizes = [(t.shape, t.dtype) for t in (*rt.k_storage._buffers(), rt.v_storage.codes, rt.v_storage.scales, rt._tail_k,
+                                              rt._tail_v)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            use(cache)
+        over = [torch.full(shape, 7, dtype=dtype, device=device) for shape, dtype in sizes for _ in range(2)]
+        torch.cuda.synchronize()
+        same_pages(rt, before, rows=rows, pages=pages)
+        assert torch.equal(rt.partial_k, tail[rows]) and len(over) == 2 * len(sizes)

@@ -791,6 +791,12 @@ class TurboPolarKVCacheRuntime:
             other._decode_to_tail(other, cut)
 
     def _adopt(self, other: "TurboPolarKVCacheRuntime") -> None:
+        # The buffers replaced here were just read on the current stream, which need not be theirs: the
+        # allocator hands their memory out again only after that copy.
+        ks, vs = self.k_storage, self.v_storage
+        for t in (*ks._buffers(), vs.codes, vs.scales, self._tail_k, self._tail_v):
+            if t is not None and t.is_cuda:
+                t.record_stream(torch.cuda.current_stream(t.device))
         read, spent = self.bytes_read, self.compression_time_ns
         flag = self._flag if other._batch_size == self._batch_size else None
         vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch,
