@@ -581,3 +581,28 @@ def test_replaced_buffers_outlive_their_copy(device, use, pages, rows):
         torch.cuda.synchronize()
         same_pages(rt, before, rows=rows, pages=pages)
         assert torch.equal(rt.partial_k, tail[rows]) and len(over) == 2 * len(sizes)
+
+
+def test_growth_on_another_stream(device):
+    """A page completed on a stream other than the store's: the outgrown buffers are not allocated anew while
+    they are still copied."""
+    side = torch.cuda.Stream()
+    k, v = (torch.from_numpy(x).to(device) for x in gen_kv(1, 2, 2, 64 * 5))
+    cut = 64 * 4 + 63
+    whole = TurboPolarFastCache(config("fast", 8, 2)).runtime
+    whole.append(k, v)
+    for _ in range(3):
+        rt = TurboPolarFastCache(config("fast", 8, 2)).runtime
+        rt.append(k[:, :, :64 * 4].contiguous(), v[:, :, :64 * 4].contiguous())
+        rt.append(k[:, :, 64 * 4:cut].contiguous(), v[:, :, 64 * 4:cut].contiguous())
+        sizes = [(t.shape, t.dtype) for t in (*rt.k_storage._buffers(), rt.v_storage.codes, rt.v_storage.scales)]
+        last = k[:, :, cut:].contiguous(), v[:, :, cut:].contiguous()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            rt.append(*last, defer_check=True)
+        over = [torch.full(shape, 7, dtype=dtype, device=device) for shape, dtype in sizes for _ in range(2)]
+        torch.cuda.synchronize()
+        rt.resolve_deferred_check()
+        assert rt.k_storage.reallocation_count == whole.k_storage.reallocation_count == 1 and len(over) == 2 * len(sizes)
+        same_pages(rt, whole)

@@ -158,6 +158,10 @@ class Growth:
     def commit(self) -> None:
         for storage, made, cap, reallocs, grown in self._sets:
             for name, new in made.items():
+                old = getattr(storage, name)
+                if old is not None and old.is_cuda:
+                    # ``fill`` reads it on the current stream, which need not be its own.
+                    old.record_stream(torch.cuda.current_stream(old.device))
                 setattr(storage, name, new)
             storage.capacity = cap
             storage.reallocation_count += reallocs
