@@ -606,3 +606,20 @@ def test_growth_on_another_stream(device):
         rt.resolve_deferred_check()
         assert rt.k_storage.reallocation_count == whole.k_storage.reallocation_count == 1 and len(over) == 2 * len(sizes)
         same_pages(rt, whole)
+
+
+def test_compaction_frees_what_it_drops(device):
+    """Nothing of a cache that was attended keeps the buffers that select_rows or keep_pages replaced."""
+    import weakref
+
+    q, dk, dv = draft(device, 2, 8, 2, 3, seed=3)
+    tree = DraftTree([-1, 0, 1])
+    for use in (lambda c: c.keep_pages([]), lambda c: c.keep_pages([2]), lambda c: c.select_rows([1, 0])):
+        cache = filled(device, "fast", 2, 8, 2, 64 * 4, seed=3)
+        cache.tree_attention(q, dk, dv, tree, 0.1)
+        cache.runtime.get_fused_attention_inputs()
+        held = [weakref.ref(t) for t in (*cache.runtime.k_storage._buffers(), cache.runtime.v_storage.codes,
+                                         cache.runtime.v_storage.scales)]
+        use(cache)
+        assert [r() is None for r in held] == [True] * len(held)
+        cache.tree_attention(q, dk, dv, tree, 0.1)

@@ -299,3 +299,12 @@ def test_prompt_scale_is_checked_first(scale, error):
     with pytest.raises(error, match="scale|float"):
         c.prompt_attention(x(1, 4, 3, 128), x(1, 2, 3, 128), x(1, 2, 3, 128), scale)
     assert c.offset == 0
+
+
+def test_replaced_stores_are_let_go():
+    for use in (lambda c: c.select_rows([0, 1]), lambda c: c.keep_pages([])):
+        c = cache()
+        c.runtime.append(x(2, 2, 5, 128), x(2, 2, 5, 128))
+        c._store = (x(1), x(1), None)  # as a call on the store leaves it
+        use(c)
+        assert c._store is None and c.offset == 5

@@ -218,10 +218,12 @@ class TurboPolarFastCache:
     def select_rows(self, rows: Sequence[int]) -> None:
         """Makes batch row i what row ``rows[i]`` was."""
         self.runtime.select_rows(rows)
+        self._store = None  # holds the replaced buffers
 
     def keep_pages(self, pages: Sequence[int]) -> None:
         """Compacts the cache to the stored pages ``pages`` and the tail."""
         self.runtime.keep_pages(pages)
+        self._store = None
 
     # ------------------------------------------------------------------ mlx_lm cache protocol
     def size(self) -> int:
