@@ -125,3 +125,37 @@ def test_assisted_generation(model):
     finally:
         tl.unpatch_llama_attention(model)
     assert out.shape[0] == 1 and 61 <= out.shape[1] <= 72 and torch.equal(out[:, :60], ids)
+
+
+@pytest.mark.parametrize("by", ["call", "config"])
+def test_attention_weights_are_the_models(model, by, monkeypatch):
+    """A step that asks for the attention's weights, by its call or by the configuration, gets them."""
+    ids = _tokens(1, 20, 6)
+    asked = dict(output_attentions=True) if by == "call" else {}
+    if by == "config":
+        monkeypatch.setattr(model.config, "output_attentions", True)
+    try:
+        tl.patch_llama_attention(model, prompt_kernel=True)
+        cache = tl.make_turbo_cache(model)
+        with torch.no_grad():
+            out = model(ids[:, :13], past_key_values=cache, use_cache=True, **asked)
+            more = model(ids[:, 13:], past_key_values=cache, use_cache=True, **asked)
+    finally:
+        tl.unpatch_llama_attention(model)
+    for weights, T, held in ((out.attentions, 13, 13), (more.attentions, 7, 20)):
+        assert [w.shape for w in weights] == [(1, 8, T, held)] * 2
+        assert all(((w.float().sum(-1) - 1).abs() <= held * 2.0 ** -8).all() for w in weights)  # bf16 weights of at most 1
+
+
+def test_other_keywords_are_the_models(model, monkeypatch):
+    """Sequences packed by their lengths, and attention without the causal mask, are not the kernel's."""
+    monkeypatch.setattr(TurboPolarFastCache, "prompt_attention", lambda *a, **k: pytest.fail("called"))
+    ids = _tokens(1, 12, 7)
+    try:
+        tl.patch_llama_attention(model, prompt_kernel=True)
+        starts = torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda:0")
+        for asked in (dict(is_causal=False), dict(cu_seq_lens_q=starts, cu_seq_lens_k=starts)):
+            with torch.no_grad():
+                model(ids, past_key_values=tl.make_turbo_cache(model), use_cache=True, **asked)
+    finally:
+        tl.unpatch_llama_attention(model)

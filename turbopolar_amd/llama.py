@@ -214,7 +214,7 @@ def _turbo_llama_attention_forward(
         out = out.to(hidden_states.dtype).reshape(B, L, -1)
         return self.o_proj(out), None
     if _prompt_kernel and isinstance(past_key_values, TurboPolarCache) and _takes_prompt(
-        self, hidden_states, attention_mask, past_key_values.fast(self.layer_idx)
+        self, hidden_states, attention_mask, past_key_values.fast(self.layer_idx), kwargs
     ):
         B, L, _ = hidden_states.shape
         q, k, v = (
@@ -233,11 +233,16 @@ def _turbo_llama_attention_forward(
 _prompt_kernel = False
 
 
-def _takes_prompt(attention, hidden_states, mask, fast) -> bool:
+def _takes_prompt(attention, hidden_states, mask, fast, asked) -> bool:
     """Whether a step of several tokens is one for the prompt kernel: half precision, the full-history
-    causal mask, no dropout and no gradients; anything else is the original forward's."""
+    causal mask, no dropout, no gradients, and nothing ``asked`` for that the kernel does not give (the weights,
+    from the call or the model's configuration; packed sequences; no causal mask); anything else is the
+    original forward's."""
     return (
         hidden_states.is_cuda
+        and not asked.get("output_attentions", getattr(attention.config, "output_attentions", False))
+        and asked.get("is_causal") in (None, True)
+        and all(asked.get(name) is None for name in ("cu_seq_lens_q", "cu_seq_lens_k"))
         and hidden_states.dtype in (torch.float16, torch.bfloat16)
         and not torch.is_grad_enabled()
         and not (attention.training and attention.attention_dropout)
