@@ -236,3 +236,15 @@ def test_refuses_gradients(device):
         prompt_attention(q.requires_grad_(), k, v, SCALE)
     with torch.no_grad():
         prompt_attention(q, k, v, SCALE)
+
+
+def test_refuses_tangents(device):
+    import torch.autograd.forward_ad as fw
+
+    q, k, v = make(device, F16, 1, 4, 2, 3, 3)
+    with fw.dual_level():
+        for i in range(3):
+            args = [fw.make_dual(t, t) if j == i else t for j, t in enumerate((q, k, v))]
+            with pytest.raises(ValueError, match="no gradients"):
+                prompt_attention(*args, SCALE)
+        assert torch.equal(prompt_attention(q, k, v, SCALE), prompt_attention(q, k, v, SCALE, out=torch.empty_like(q)))

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from turbopolar_amd import DraftTree, TurboPolarConfig, TurboPolarFastCache, TurboPolarKVCacheRuntime, _lib, wire
-from turbopolar_amd.kernels import _overlaps, _starts, prompt_attention
+from turbopolar_amd.kernels import _no_grad, _overlaps, _starts, prompt_attention
 
 H = torch.float16
 
@@ -308,3 +308,26 @@ def test_replaced_stores_are_let_go():
         c._store = (x(1), x(1), None)  # as a call on the store leaves it
         use(c)
         assert c._store is None and c.offset == 5
+
+
+def test_no_grad_sees_tangents():
+    """Forward-mode duals are refused, with gradients recorded or not; plain tensors beside them are not."""
+    import torch.autograd.forward_ad as fw
+
+    a, b = x(3), x(3)
+    _no_grad(a, b)
+    with pytest.raises(ValueError, match="no gradients"):
+        _no_grad(a, b.clone().requires_grad_())
+    with torch.no_grad():
+        _no_grad(a, b.clone().requires_grad_())
+    with fw.dual_level():
+        _no_grad(a, b)
+        dual = fw.make_dual(b, a)
+        with pytest.raises(ValueError, match="no gradients"):
+            _no_grad(a, dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="no gradients"):
+            _no_grad(dual, a)
+    with pytest.raises(ValueError, match="no gradients"):
+        torch.func.jvp(lambda t: (_no_grad(t), t)[1], (a,), (b,))
+    with torch.inference_mode():
+        _no_grad(a, b, x(2))
