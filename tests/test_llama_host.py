@@ -99,3 +99,23 @@ def test_load_local_llama(tmp_path):
     assert not tl.is_patched()
     with pytest.raises(OSError):
         tl.load_local_llama(tmp_path / "missing", device="cpu", patch=False)
+
+
+def test_batch_changes_of_a_cropped_cache():
+    """A layer cropped to nothing follows changes of its batch as one that holds tokens does."""
+    layer = tl.make_turbo_cache(_tiny_model()).layers[0]
+    layer.batch_repeat_interleave(2)  # holds nothing yet: any batch may come
+    layer.batch_select_indices(torch.tensor([0]))
+    k = torch.randn(2, 1, 5, 128).half()
+    layer.fast.runtime.append(k, k)
+    layer.crop(-5)
+    assert layer.get_seq_length() == 0
+    layer.batch_repeat_interleave(2)
+    layer.fast.runtime.append(k.repeat_interleave(2, 0), k.repeat_interleave(2, 0))
+    layer.crop(-5)
+    layer.batch_select_indices(torch.tensor([True, False, False, False]))
+    layer.fast.runtime.append(k[:1], k[:1])
+    layer.crop(-5)
+    layer.reorder_cache(torch.tensor([0, 0]))
+    layer.fast.runtime.append(k, k)
+    assert layer.get_seq_length() == 5 and torch.equal(layer.fast.runtime.partial_k, k)

@@ -94,13 +94,13 @@ class TurboPolarLayer(CacheLayerMixin):
         self.batch_select_indices(beam_idx)
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
-        if self.fast.offset:
+        if self.fast.runtime._initialized:  # also one cut to nothing, whose batch stays
             if indices.dtype is torch.bool:
                 indices = indices.nonzero().flatten()
             self.fast.select_rows(indices)
 
     def batch_repeat_interleave(self, repeats: int) -> None:
-        if self.fast.offset:
+        if self.fast.runtime._initialized:
             self.fast.select_rows([b for b in range(self.fast.runtime._batch_size) for _ in range(repeats)])
 
     def reset(self) -> None:
