@@ -248,3 +248,21 @@ def test_refuses_tangents(device):
             with pytest.raises(ValueError, match="no gradients"):
                 prompt_attention(*args, SCALE)
         assert torch.equal(prompt_attention(q, k, v, SCALE), prompt_attention(q, k, v, SCALE, out=torch.empty_like(q)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("at", [0, 20_000, 32_767])
+def test_many_small_weights(device, at, dtype):
+    """One key of weight 1 beside 32,767 of e^-18, in one workgroup's run of keys: 5e-4 of the result.  fp16 weights
+    lie up to 2^7 above 1, so each is off by 2^-32 at most (they are below the type's least normal number)."""
+    n, w = 32768, 1.5229979744712628e-08
+    q = torch.zeros((1, 64, 1024, 128), dtype=dtype, device=device)
+    k = torch.zeros((1, 1, n, 128), dtype=dtype, device=device)
+    v = torch.ones((1, 1, n, 128), dtype=dtype, device=device)
+    q[..., 0], k[:, :, at, 0], v[:, :, at] = 1.0, 18.0, 0.0
+    got = prompt_attention(q, k.expand(1, 64, n, 128), v.expand(1, 64, n, 128), 1.0, causal=False)
+    want = (n - 1) * w / (1 + (n - 1) * w)
+    eps = torch.finfo(dtype).eps / 2
+    tol = want * (2 * eps + 2 * 18 * 129 * 2.0 ** -24 + (n + 16) * 2.0 ** -23) + (n * 2.0 ** -32 + 2.0 ** -25 if dtype is F16 else 0)
+    print(f"[prompt] small weights at {at} {dtype}: {got.double().sub(want).abs().max().item():.3g} of {tol:.3g}", flush=True)
+    assert (got.double() - want).abs().max() <= tol

@@ -623,3 +623,25 @@ def test_compaction_frees_what_it_drops(device):
         use(cache)
         assert [r() is None for r in held] == [True] * len(held)
         cache.tree_attention(q, dk, dv, tree, 0.1)
+
+
+def test_many_small_weights(device):
+    """One stored key of weight 1 beside 2,560 of e^-18, three pages of them in its workgroup.  Weights lie up to 2^7
+    above 1, so each is off by 2^-32 at most; a record and the result are fp16, subnormal here."""
+    B, H, T = 8, 8, 64 * 40
+    cache = TurboPolarFastCache(config("default", H, H))
+    k = torch.zeros((B, H, T, 128), dtype=torch.float16, device=device)
+    v = torch.ones_like(k)
+    k[:, :, 5, 0], v[:, :, 5] = -18.0, 0.0
+    cache.runtime.append(k, v)
+    q, dk = torch.zeros((2, B, H, 1, 128), dtype=torch.float16, device=device)
+    q[..., 0] = -1.0
+    got = cache.tree_attention(q, dk, torch.ones_like(dk), DraftTree([-1]), 1.0).double().cpu()
+    keys, values = pages64(cache.runtime)
+    assert (keys[0, 0, 5, 0], keys[0, 0, 6, 0], values[0, 0, 5, 0]) == (-18.0, 0.0, 0.0)
+    w = np.exp(-18.0)
+    want = (w * values[0, 0].sum(0) + w) / (1 + T * w)
+    tol = want * (2 * EPS + 2 * 18 * 129 * 2.0 ** -24 + (T + 16) * 2.0 ** -23) + T * 2.0 ** -32 + 2 * 2.0 ** -25
+    off = np.abs(got[:, :, 0].numpy() - want)
+    print(f"[tree] small weights: {off.max():.3g} of {tol.max():.3g}", flush=True)
+    assert (off <= tol).all()

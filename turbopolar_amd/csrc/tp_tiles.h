@@ -55,6 +55,10 @@ struct F16 {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{x, y}, half2v));
   }
   static constexpr uint32_t kExponent = 0x7c00u;
+  // Weights lie 2^kHeadroom higher than the largest being 1 (2^kSlack more at most, 2^15 in all): the smallest
+  // that keeps all of its bits is then 2^-21 of the row's largest instead of 2^-14, and what vanishes 2^-32
+  // instead of 2^-25 (32,767 keys of weight 2^-26 beside one of 1 are 5e-4 of the result, and were lost).
+  static constexpr float kHeadroom = 7.0f;
 };
 struct BF16 {
   static __device__ __forceinline__ float16v mfma(uint4v a, uint4v b, float16v c) {
@@ -65,6 +69,7 @@ struct BF16 {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{x, y}, bf16x2));
   }
   static constexpr uint32_t kExponent = 0x7f80u;
+  static constexpr float kHeadroom = 0.0f;  // fp32's exponents
 };
 
 // Whether any of the pair's two 16-bit values is infinite or NaN.
@@ -109,7 +114,7 @@ __device__ __forceinline__ float across_halves(float x, Op op) {
 struct RowState {
   float16v o[4];  // O^T, dimensions 32 db + 8 (i / 4) + 4 h + i % 4
   float m;        // running maximum of scale * score, in log2 units
-  float l;        // this lane's part of the sum of the weights
+  float l;        // this lane's part of the sum of the weights (2^kHeadroom times it, as o)
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -199,8 +204,8 @@ __device__ __forceinline__ void mask_scores(float16v* s, int limit) {
 
 // The running maximum (of c times the scores, c > 0) moved to hold a tile's scores.  It moves only
 // where some row of the wave grew by more than kSlack, so that most tiles need no rescaling: a weight
-// is then at most 2^kSlack, which neither its 16 bits nor the sums in fp32 mind (their roundings are
-// relative).
+// is then at most 2^(kHeadroom + kSlack), which neither its 16 bits nor the sums in fp32 mind (their roundings
+// are relative).
 constexpr float kSlack = 8.0f;
 template <int RB, int NB>
 __device__ __forceinline__ void rescale(const float16v (&s)[RB][NB], float c, RowState (&st)[RB]) {
@@ -246,7 +251,7 @@ __device__ __forceinline__ void add_values(const char* vt, int t0, const TileLan
 // Weights of a tile's scores, packed as the second product takes them, and their sum.
 template <class T, int NB>
 __device__ __forceinline__ void weigh(const float16v* s, float c, uint4v* p, RowState& st) {
-  const float base = st.m == -INFINITY ? 0.0f : st.m;
+  const float base = st.m == -INFINITY ? 0.0f : st.m - T::kHeadroom;
 #pragma unroll
   for (int i = 0; i < 8 * NB; ++i) {
     const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 3][2 * (i & 7)], c, -base));
