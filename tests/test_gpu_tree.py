@@ -645,3 +645,34 @@ def test_many_small_weights(device):
     off = np.abs(got[:, :, 0].numpy() - want)
     print(f"[tree] small weights: {off.max():.3g} of {tol.max():.3g}", flush=True)
     assert (off <= tol).all()
+
+
+@pytest.mark.parametrize("layout,hkv,n", [("default", 2, 5), ("default", 2, 16), ("default", 1, 16), ("deep2", 2, 16),
+                                          ("l1_8bit", 1, 20)])
+def test_keys_are_the_page_decoders(device, layout, hkv, n):
+    """The keys attended are those that the page decoder hands out, each component rounded to fp16 once: queries of
+    four large components tell scores of a few steps apart.  A score is then a sum of four products, off by
+    5 2^-24 sum|q||k|, a weight by twice that and its rounding, and records and the result are rounded once."""
+    cache = filled(device, layout, 1, 8, hkv, 64 * 6, seed=n)
+    q, dk, dv = draft(device, 1, 8, hkv, n, seed=n + 50)
+    q[..., 4:] = 0
+    q *= 8
+    got = cache.tree_attention(q, dk, dv, DraftTree(list(range(-1, n - 1))), 1.0).double().cpu().numpy()
+    keys = cache.runtime.fetch_blocks().double().cpu().numpy()
+    values = pages64(cache.runtime)[1]
+    q64, k64, v64 = (t.double().cpu().numpy() for t in (q, dk, dv))
+    worst = 0.0
+    for i in range(n):
+        for h in range(8):
+            kv = h // (8 // hkv)
+            k = np.concatenate((keys[0, kv], k64[0, kv, : i + 1]))
+            v = np.concatenate((values[0, kv], v64[0, kv, : i + 1]))
+            s = k @ q64[0, h, i]
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            ds = 5 * 2.0 ** -24 * (np.abs(k) @ np.abs(q64[0, h, i])).max()
+            tol = (p @ np.abs(v)) * (3 * EPS + np.expm1(2 * ds) + (len(s) + 16) * 2.0 ** -23)
+            tol += (len(s) + 2) * 2.0 ** -25 * np.abs(v).max()
+            worst = max(worst, (np.abs(got[0, h, i] - p @ v) / tol).max())
+    print(f"[tree] page decoder's keys, {layout}: {worst:.3g} of the bound", flush=True)
+    assert worst <= 1

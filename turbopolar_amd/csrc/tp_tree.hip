@@ -107,10 +107,20 @@ __device__ __forceinline__ void stage_rows(int tid, const PageRegs<KIND, N>& p, 
     for (int i = 0; i < 2 * N; ++i) codes[tid + THREADS * i] = p.rows[i];
 }
 
-union TreeLut {
-  uint32_t code[512];  // (cos, sin) of the level-1 codes, then of the deep codes
-  uint2 pair[256];     // default layout: of both nibbles of a code byte
+// (cos, sin) in fp32 of the level-1 codes, then of the deep codes (the default layout's codes are of one width: the
+// first 16).
+struct TreeLut {
+  float2v code[512];
 };
+
+// Of a code's decoded angle, the reference's (code_angle); an infinite radius meets no zero, as make_cs explains.
+__device__ __forceinline__ float2v angle_pair(uint32_t code, int bits) {
+  const float th = code_angle(code, bits);
+  return float2v{cosf(th), sinf(th)};
+}
+
+// A pair's key, r (cos a, sin a), each rounded once.
+__device__ __forceinline__ uint32_t key_pair(float r, float2v cs) { return F16::pack(r * cs.x, r * cs.y); }
 
 // Decodes half h of run n into a tile of keys: 4 pairs, 16 bytes.
 template <int KIND, int N, int THREADS>
@@ -118,43 +128,31 @@ __device__ __forceinline__ void decode_keys(const TreeArgs& a, const TreeLut& lu
                                             const PageRegs<KIND, N>& p, int n, int h, char* kt) {
   const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
   uint32_t e[4];
-  if constexpr (KIND == kTreeDefault) {
+  const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;  // rounded in fp32, as its products below
+  int c0 = c;  // where a pair's code lies is computed anew: kept over the pages, it costs 30 registers
+  if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint2 cs = lut.pair[(p.c4[n] >> (16 * h + 8 * i)) & 0xffu];
-      e[2 * i] = pack_h2(lo_lo(p.r[n][2 * h + i]) * __builtin_bit_cast(half2v, cs.x));
-      e[2 * i + 1] = pack_h2(hi_hi(p.r[n][2 * h + i]) * __builtin_bit_cast(half2v, cs.y));
+  for (int i = 0; i < 4; ++i) {
+    uint32_t code;
+    if constexpr (KIND == kTreeDefault) {
+      code = (p.c4[n] >> (16 * h + 4 * i)) & 15u;
+    } else if constexpr (KIND == kTreeFast) {
+      code = 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
+    } else {
+      const int pair = 8 * c0 + 4 * h + i;
+      const bool l1 = pair < a.split_half;
+      const int bits = l1 ? a.l1_bits : a.deep_bits;
+      const int bit = (l1 ? pair : pair - a.split_half) * bits;
+      const int row = l1 ? t * a.l1_row : kPageTokens * a.l1_row + t * a.deep_row;
+      const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
+      code = (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
     }
-  } else {
-    const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;
-    int c0 = c;  // where a pair's code lies is computed anew: kept over the pages, it costs 30 registers
-    if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t code;
-      if constexpr (KIND == kTreeFast) {
-        code = 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
-      } else {
-        const int pair = 8 * c0 + 4 * h + i;
-        const bool l1 = pair < a.split_half;
-        const int bits = l1 ? a.l1_bits : a.deep_bits;
-        const int bit = (l1 ? pair : pair - a.split_half) * bits;
-        const int row = l1 ? t * a.l1_row : kPageTokens * a.l1_row + t * a.deep_row;
-        const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
-        code = (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
-      }
-      half2v r;
-      if constexpr (tree_i8(KIND)) {
-        // code x scale is exact in fp32; r = exp(code x scale) rounded to fp16 once.
-        const int rc = (int)(int8_t)(p.r8[n][h] >> (8 * i));
-        const f16 x = (f16)__builtin_amdgcn_exp2f((float)rc * ls);
-        r = half2v{x, x};
-      } else {
-        const uint32_t w = p.r[n][2 * h + (i >> 1)];
-        r = (i & 1) ? hi_hi(w) : lo_lo(w);
-      }
-      e[i] = pack_h2(r * __builtin_bit_cast(half2v, lut.code[code]));
-    }
+    float r;
+    if constexpr (tree_i8(KIND))
+      r = __builtin_amdgcn_exp2f((float)(int)(int8_t)(p.r8[n][h] >> (8 * i)) * ls);
+    else
+      r = h2f((uint16_t)(p.r[n][2 * h + (i >> 1)] >> (16 * (i & 1))));
+    e[i] = key_pair(r, lut.code[code]);
   }
   *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + h)) = uint4v{e[0], e[1], e[2], e[3]};
 }
@@ -225,10 +223,11 @@ constexpr int kTreeThreads = 64 * RW * TW;
 // layout: 60 us, 4.6 TB/s), 128 rows by decode and products alike (32 nodes over 32,805 tokens: 35 us, 2.2 TB/s and
 // 0.49 PFLOP/s).
 //
-// A key component is rounded three times (cosine, the radius of an int8 layout, their product: fp16, as the fp16
-// products take it), a weight and the result once each; 32-bit sums.  An output's error, relative in L2, is 5.9e-4
-// (default layout) to 8.7e-4 (int8 radii) by that; one rounding of a key instead of three would leave an estimated
-// 4.5e-4, and products of wider keys cost the matrix units twice the work or more.
+// A key component is rounded to fp16 once, from fp32 angles and radii, as the page decoder rounds it, so that what is
+// attended is what the decoder hands out; a value, a weight, a record and the result once each; 32-bit sums.  An
+// output's error, relative in L2, is 5.2e-4 (default layout, 1,000 tokens) to 6.4e-4 (fast layout, 131,072) by that,
+// of which the keys alone give 3.7e-4 to 5.1e-4 (scores of a spread of 1.8).  Cosines, int8 radii and products in fp16
+// gave 5.9e-4 to 8.7e-4 for 2 % less time (32 nodes over 32,805 tokens 40.6 us instead of 41.5).
 template <int KIND, int RW, int TW>
 __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kernel(TreeArgs a) {
   constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW, BUFS = RW * TW > 2 ? 2 : 1;
@@ -267,12 +266,12 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   if (page < page_end) {
     for (int x = tid; x < 256; x += THREADS) {
       if constexpr (KIND == kTreeDefault) {
-        lut.pair[x] = make_uint2(make_cs(x & 15u, 4), make_cs(x >> 4, 4));
+        if (x < 16) lut.code[x] = angle_pair(x, 4);
       } else if constexpr (KIND == kTreeFast) {
-        lut.code[256 + x] = make_cs(x, 8);
+        lut.code[256 + x] = angle_pair(x, 8);
       } else {
-        if (x < (1 << a.l1_bits)) lut.code[x] = make_cs(x, a.l1_bits);
-        if (x < (1 << a.deep_bits)) lut.code[256 + x] = make_cs(x, a.deep_bits);
+        if (x < (1 << a.l1_bits)) lut.code[x] = angle_pair(x, a.l1_bits);
+        if (x < (1 << a.deep_bits)) lut.code[256 + x] = angle_pair(x, a.deep_bits);
       }
     }
     flip_query(a.flip, qs);
@@ -387,6 +386,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   const float l = across_halves(st.l, [](float x, float y) { return x + y; });
   if (a.records > 1) {
     const int64_t rec = ((int64_t)unit * a.nodes * a.g + row) * a.records + record;
+    // fp16: records of 32 bits lower the error from 6.1e-4 to 5.7e-4 and cost a tenth of the time (41.5 -> 45.2 us).
     store_record<true>(st, l, a.part_o + rec * kHeadDim, a.part_ml + rec * 2, live, lane);
   } else {
     store_row<F16>(st, l == 0.0f ? 0.0f : 1.0f / l, a.out + b * a.out_b + (kv * a.g + head) * a.out_h + node * a.out_t,
