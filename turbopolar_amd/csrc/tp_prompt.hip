@@ -127,9 +127,6 @@ __device__ __forceinline__ bool clean_part(int t0, int n, int tid, uint4v* r) {
   return flagged;
 }
 
-// A barrier that waits for this wave's LDS accesses, not for its loads from memory.
-__device__ __forceinline__ void phase_barrier() { lds_barrier(); }
-
 // The products of a step: the next tile's scores in turn with a tile's weights and values, so that four
 // products lie between two that add to the same registers.  Reads from LDS go out kAhead pairs before the
 // products that take them.  Past the last tile the scores are of whatever the LDS holds, and not used: a
@@ -196,8 +193,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
   const int first = split * each, end = min(min(first + each, all), (most + kTileTokens - 1) / kTileTokens);
   const int wave_end = min(end, (wave_most + kTileTokens - 1) / kTileTokens);
 
-  RowState rows[1];
-  RowState& st = rows[0];
+  RowState st;
   st.clear();
   if (first < end) {
     const uint16_t* k = a.k + b * a.k_b + kv * a.k_h + (int64_t)t.k0 * a.k_t;
@@ -243,25 +239,26 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
     }
     __syncthreads();
     flip_query(a.flip, q);
-    float16v s[1][2];
-    if (first < wave_end) score_tile<T, 2>(kts[first & 1], 0, at, q, s[0], [](int) {});
-    if (behind) phase_barrier();
-    // Two phases a tile, a barrier after each: the softmax, and the products.  While one wave of a SIMD
+    float16v s[2];
+    if (first < wave_end) score_tile<T, 2>(kts[first & 1], 0, at, q, s, [](int) {});
+    if (behind) lds_barrier();
+    // Two phases a tile, a barrier after each (which waits for LDS accesses, not for loads from memory): the softmax,
+    // and the products.  While one wave of a SIMD
     // multiplies, the other runs its softmax (in step, 41 % of the time went to products and almost all of
     // the rest to softmax).  The next tiles go to LDS under the products, into the buffers that both
     // halves of the waves have left by then.
     for (int j = first; j < end; ++j) {
       uint4v p[4];
       if (j < wave_end) {
-        if ((j + 1) * kTileTokens > wave_fewest) mask_scores<2>(s[0], limit - 4 * (lane >> 5) - j * kTileTokens);
-        rescale<1, 2>(s, a.c, rows);
-        weigh<T, 2>(s[0], a.c, p, st);
+        if ((j + 1) * kTileTokens > wave_fewest) mask_scores<2>(s, limit - 4 * (lane >> 5) - j * kTileTokens);
+        rescale<2>(s, a.c, st);
+        weigh<T, 2>(s, a.c, p, st);
       }
       clean(j + 1);
-      phase_barrier();
+      lds_barrier();
       if (j < wave_end) {
         __builtin_amdgcn_s_setprio(1);
-        multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q, p, s[0], st, [&](int i) {
+        multiply_tile<T>(kts[(j + 1) & 1], vts[j & 1], at, q, p, s, st, [&](int i) {
           if (i * C / 2 < 4 * C)
 #pragma unroll
             for (int x = i * C / 2; x < (i + 1) * C / 2; ++x) stage(j, x);
@@ -271,9 +268,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_attention_kernel(PromptA
 #pragma unroll
         for (int i = 0; i < 4 * C; ++i) stage(j, i);
       }
-      phase_barrier();
+      lds_barrier();
     }
-    if (!behind) phase_barrier();
+    if (!behind) lds_barrier();
     if (flag) {
       const int t0 = max(fewest / kTileTokens, first) * kTileTokens;  // the first tile with a border
       add_nonfinite<T>(st, lane, min(end * kTileTokens, t.nk) - t0, [&](int x) { return t0 + x < limit; },

@@ -46,7 +46,6 @@ __host__ __device__ inline int tile_at(int t, int c) { return t * (kHeadDim * 2)
 // is off by at most half a step of itself, so an output's rounding error stays below
 // half a step of the type relative to the largest value).
 struct F16 {
-  typedef half8v frag;
   static __device__ __forceinline__ float16v mfma(uint4v a, uint4v b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0,
                                                   0, 0);
@@ -207,32 +206,23 @@ __device__ __forceinline__ void mask_scores(float16v* s, int limit) {
 // is then at most 2^(kHeadroom + kSlack), which neither its 16 bits nor the sums in fp32 mind (their roundings
 // are relative).
 constexpr float kSlack = 8.0f;
-template <int RB, int NB>
-__device__ __forceinline__ void rescale(const float16v (&s)[RB][NB], float c, RowState (&st)[RB]) {
-  float top[RB];
-  bool grown = false;
+template <int NB>
+__device__ __forceinline__ void rescale(const float16v* s, float c, RowState& st) {
+  float x = s[0][0];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    float x = s[rb][0][0];
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int i = 0; i < 16; ++i) x = fmaxf(x, s[nb][i]);
+  const float top = across_halves(x, [](float u, float w) { return fmaxf(u, w); }) * c;
+  if (__any(top > st.m + kSlack)) {  // -inf: a row that has seen nothing yet
+    const float m = fmaxf(st.m, top);
+    const float alpha = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.0f : m));
+    st.m = m;
+    st.l *= alpha;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x = fmaxf(x, s[rb][nb][i]);
-    top[rb] = across_halves(x, [](float u, float w) { return fmaxf(u, w); }) * c;
-    grown = grown || top[rb] > st[rb].m + kSlack;  // -inf: a row that has seen nothing yet
-  }
-  if (__any(grown)) {
+    for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float m = fmaxf(st[rb].m, top[rb]);
-      const float alpha = __builtin_amdgcn_exp2f(st[rb].m - (m == -INFINITY ? 0.0f : m));
-      st[rb].m = m;
-      st[rb].l *= alpha;
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[rb].o[db][i] *= alpha;
-    }
+      for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
   }
 }
 
@@ -265,19 +255,19 @@ __device__ __forceinline__ void weigh(const float16v* s, float c, uint4v* p, Row
 
 // The rest of a pass over NB blocks of 32 tokens from token t0 of a tile, from its scores on.
 template <class T, int NB>
-__device__ __forceinline__ void finish_tile(const char* vt, int t0, const TileLane& at, float c, float16v (&s)[1][NB],
-                                            RowState (&st)[1]) {
-  rescale<1, NB>(s, c, st);
+__device__ __forceinline__ void finish_tile(const char* vt, int t0, const TileLane& at, float c, const float16v* s,
+                                            RowState& st) {
+  rescale<NB>(s, c, st);
   uint4v p[2 * NB], v[kReadAhead];
   // The first values are read under the softmax; of two blocks, whose scores leave no registers, after it.
   if (NB == 1)
 #pragma unroll
     for (int i = 0; i < kReadAhead; ++i) v[i] = read_value(vt, t0, at, i);
-  weigh<T, NB>(s[0], c, p, st[0]);
+  weigh<T, NB>(s, c, p, st);
   if (NB != 1)
 #pragma unroll
     for (int i = 0; i < kReadAhead; ++i) v[i] = read_value(vt, t0, at, i);
-  add_values<T, 2 * NB>(vt, t0, at, p, v, st[0]);
+  add_values<T, 2 * NB>(vt, t0, at, p, v, st);
 }
 
 // Infinities and NaN among the values of a tile that some rows do not see: a product

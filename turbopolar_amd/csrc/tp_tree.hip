@@ -258,8 +258,7 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
   load_query(a.q + b * a.q_b + (kv * a.g + head) * a.q_h + at_node * a.q_t, lane, qs);
   const uint64_t self = mask[at_node >> 6];
   const TileLane at(lane);
-  RowState rows[1];
-  RowState& st = rows[0];
+  RowState st;
   st.clear();
 
   if (tid == 0) flag = 0;
@@ -276,21 +275,18 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
     }
     flip_query(a.flip, qs);
     __syncthreads();
-    float16v s[1][NB];
+    float16v s[NB];
     if constexpr (BUFS == 1) {
+      static_assert(!tree_any(KIND), "any layout's codes are staged in the other form");
       for (; page < page_end; ++page) {
-        if constexpr (tree_any(KIND)) {
-          stage_rows<KIND, N, THREADS>(tid, p, codes[0]);
-          __syncthreads();
-        }
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i)
           decode_piece<KIND, N, THREADS>(a, lut, codes[0], tid, p, i, tiles[0][0], tiles[0][1]);
         __syncthreads();
         // The last page again rather than none: a load under a branch is waited for at its join.
         load_page<KIND, N, THREADS>(a, slot0 + min(page + 1, page_end - 1), tid, p);
-        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s[0], [](int) {});
-        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, rows);
+        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s, [](int) {});
+        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, st);
         __syncthreads();
       }
     } else {
@@ -308,14 +304,14 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         const uint32_t* rows_of = codes[tree_any(KIND) ? buf ^ 1 : 0];
         stage_rows<KIND, N, THREADS>(tid, p, codes[tree_any(KIND) ? buf ^ 1 : 0]);
         __syncthreads();
-        score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s[0], [&](int i) {
+        score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s, [&](int i) {
           constexpr int kProducts = 8 * NB, kPieces = 4 * N;
 #pragma unroll
           for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x)
             decode_piece<KIND, N, THREADS>(a, lut, rows_of, tid, p, x, kt, vt);
         });
         load_page<KIND, N, THREADS>(a, slot0 + min(page + 2, page_end - 1), tid, p);
-        finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, rows);
+        finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, st);
       }
     }
   }
@@ -344,12 +340,12 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
         const uint64_t there = count < 64 ? (1ull << count) - 1ull : ~0ull;
         const uint64_t sees = !real ? 0ull : j < 0 ? there : mask[j] & there;
         auto seen = [&](int x) { return ((sees >> x) & 1u) != 0; };
-        float16v s[1][NB];
-        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s[0], [](int) {});
+        float16v s[NB];
+        score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s, [](int) {});
 #pragma unroll
         for (int x = 0; x < 16 * NB; ++x)
-          if (!seen(32 * (tw + (x >> 4)) + 8 * ((x & 15) >> 2) + (x & 3) + 4 * (lane >> 5))) s[0][x >> 4][x & 15] = -INFINITY;
-        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, rows);
+          if (!seen(32 * (tw + (x >> 4)) + 8 * ((x & 15) >> 2) + (x & 3) + 4 * (lane >> 5))) s[x >> 4][x & 15] = -INFINITY;
+        finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, st);
         if (flag)
           add_nonfinite<F16>(st, lane, count, [&](int x) { return seen(x) && (TW == 1 || (x >> 5) == tw); },
                              [&](int x) { return v + x * v_t; });

@@ -768,15 +768,7 @@ def take_tokens(k: torch.Tensor, v: torch.Tensor, index: Union[Sequence[int], Se
     B, H, T, _ = k.shape
     per_batch = isinstance(index[0], (list, tuple))
     flat = [i for row in index for i in row] if per_batch else list(index)
-    item_mask = 3 if k.dtype is torch.float32 else 7
-    views = []
-    for t in (k, v):
-        t, s = _strided(t)
-        if any(x & item_mask for x in s):
-            t = _fresh(t)
-            s = t.stride()[:3]
-        views.append((t, s))
-    (k, ks), (v, vs) = views
+    (k, ks), (v, vs) = _strided(k), _strided(v)
     dev = k.device
     st = call_on(
         dev, lib().tp_take_tokens, k.data_ptr(), v.data_ptr(), 1 if k.dtype is torch.float32 else 0, B, H, T,
