@@ -159,3 +159,21 @@ def test_other_keywords_are_the_models(model, monkeypatch):
                 model(ids, past_key_values=tl.make_turbo_cache(model), use_cache=True, **asked)
     finally:
         tl.unpatch_llama_attention(model)
+
+
+def test_inference_mode(model):
+    """A prompt, a chunk, a step and a crop in inference mode are those of no_grad."""
+    ids = _tokens(1, 80, 8)
+    try:
+        tl.patch_llama_attention(model, prompt_kernel=True)
+        got, want = [], []
+        for mode, out in ((torch.inference_mode, got), (torch.no_grad, want)):
+            cache = tl.make_turbo_cache(model)
+            with mode():
+                for a, b in ((0, 60), (60, 75), (75, 76)):
+                    out.append(model(ids[:, a:b], past_key_values=cache, use_cache=True).logits.clone())
+                cache.crop(-70)
+                out.append(model(ids[:, 6:], past_key_values=cache, use_cache=True).logits.clone())
+    finally:
+        tl.unpatch_llama_attention(model)
+    assert cache.get_seq_length() == 80 and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -119,3 +119,18 @@ def test_batch_changes_of_a_cropped_cache():
     layer.reorder_cache(torch.tensor([0, 0]))
     layer.fast.runtime.append(k, k)
     assert layer.get_seq_length() == 5 and torch.equal(layer.fast.runtime.partial_k, k)
+
+
+def test_masks_of_inference_mode():
+    """They have no version: each is compared anew, and none is taken for one that was seen before."""
+    with torch.inference_mode():
+        mask = torch.ones((1, 1, 3, 5), dtype=torch.bool).tril(2)
+        assert tl._is_standard_causal_mask(mask, 3, 5) and tl._is_standard_causal_mask(mask, 3, 5)
+        mask[0, 0, 0, 4] = True
+        assert not tl._is_standard_causal_mask(mask, 3, 5)
+        mask[0, 0, 0, 4] = False
+        assert tl._is_standard_causal_mask(mask, 3, 5)
+    plain = torch.ones((1, 1, 3, 5), dtype=torch.bool).tril(2)
+    assert tl._is_standard_causal_mask(plain, 3, 5) and tl._is_standard_causal_mask(plain, 3, 5)
+    plain[0, 0, 0, 4] = True
+    assert not tl._is_standard_causal_mask(plain, 3, 5)

@@ -165,19 +165,20 @@ def _is_standard_causal_mask(mask: Optional[torch.Tensor], seq_len: int, cache_l
     kept for that tensor (held, so its memory cannot be reused, and keyed on
     its version counter, so an in-place change is seen), which makes the
     comparison, a device-to-host read, once per forward instead of once per
-    layer."""
+    layer.  A mask made in inference mode has no version, so no verdict is kept for it."""
     global _mask_verdict
     if mask is None:
         return True
     if tuple(mask.shape) not in ((1, 1, seq_len, cache_len), (batch, 1, seq_len, cache_len)):
         return False
+    version = None if mask.is_inference() else mask._version
     hit = _mask_verdict
-    if hit is not None and hit[0] is mask and hit[1] == mask._version and hit[2] == seq_len and hit[3] == cache_len:
+    if hit is not None and hit[0] is mask and hit[1] == version and hit[2] == seq_len and hit[3] == cache_len:
         return hit[4]
     allowed = mask[:, 0] if mask.dtype == torch.bool else mask[:, 0] == 0
     expected = torch.ones((seq_len, cache_len), dtype=torch.bool, device=mask.device).tril(cache_len - seq_len)
     ok = bool((allowed == expected).all())
-    _mask_verdict = (mask, mask._version, seq_len, cache_len, ok)
+    _mask_verdict = None if version is None else (mask, version, seq_len, cache_len, ok)
     return ok
 
 
