@@ -676,3 +676,20 @@ def test_keys_are_the_page_decoders(device, layout, hkv, n):
             worst = max(worst, (np.abs(got[0, h, i] - p @ v) / tol).max())
     print(f"[tree] page decoder's keys, {layout}: {worst:.3g} of the bound", flush=True)
     assert worst <= 1
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_caches_filled_in_inference_mode(device, dtype):
+    """They are cut, forked, re-ordered and extended outside of it like any other."""
+    with torch.inference_mode():
+        cache = filled(device, "default", 2, 8, 2, 64 * 3 + 9, seed=7, dtype=dtype)
+    plain = filled(device, "default", 2, 8, 2, 64 * 3 + 9, seed=7, dtype=dtype)
+    k, v = (torch.from_numpy(x).to(device) for x in gen_kv(8, 2, 2, 7, dtype=dtype))
+    for c in (cache, plain):
+        c.truncate(64 * 2 + 30)
+        c.select_rows([1, 0])
+        c.runtime.accept(k, v, [2, 0])
+    other = cache.fork(tokens=64 + 5)
+    same_pages(cache.runtime, plain.runtime)
+    for a, b in ((cache, plain), (other, plain.fork(tokens=64 + 5))):
+        assert a.offset == b.offset and torch.equal(a.runtime.partial_k, b.runtime.partial_k)

@@ -708,8 +708,9 @@ class TurboPolarKVCacheRuntime:
         decode_pages_into(source.polar_encoder.layout, pages_of(source.k_storage, source.v_storage),
                           self._batch_size * self._num_kv_heads, page, 1, k, v, 0)
         if k is not self._tail_k:
-            self._tail_k.copy_(k)
-            self._tail_v.copy_(v)
+            with torch.inference_mode():  # in which the tail's buffers may have been made
+                self._tail_k.copy_(k)
+                self._tail_v.copy_(v)
 
     def fork(self, tokens: Optional[int] = None, rows: Optional[Sequence[int]] = None,
              pages: Optional[Sequence[int]] = None) -> "TurboPolarKVCacheRuntime":
