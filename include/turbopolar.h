@@ -362,7 +362,7 @@ int32_t tp_grow_rows(const tp_grow* bufs, int32_t n_bufs, int64_t rows, void* st
  * causal: the queries are the last tq of the tk positions, query i sees keys 0 ..
  * tk - tq + i.  A query that sees no key gives 0.  Infinities and NaN in keys and
  * values that a query does not see do not reach it.
- * n_seq > 0 (batch 1): packed sequences; q_starts and k_starts are device arrays of
+ * n_seq > 0 (batch 1, at most 65,536): packed sequences; q_starts and k_starts are device arrays of
  * n_seq + 1 ascending token positions, the first 0, sequence s being queries
  * [q_starts[s], q_starts[s + 1]) over keys [k_starts[s], k_starts[s + 1]).  Queries
  * behind the last sequence give 0, or are left as they are with keep_rest.  Starts

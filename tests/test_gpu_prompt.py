@@ -266,3 +266,17 @@ def test_many_small_weights(device, at, dtype):
     tol = want * (2 * eps + 2 * 18 * 129 * 2.0 ** -24 + (n + 16) * 2.0 ** -23) + (n * 2.0 ** -32 + 2.0 ** -25 if dtype is F16 else 0)
     print(f"[prompt] small weights at {at} {dtype}: {got.double().sub(want).abs().max().item():.3g} of {tol:.3g}", flush=True)
     assert (got.double() - want).abs().max() <= tol
+
+
+@pytest.mark.parametrize("last", [65536, 100])
+def test_most_sequences(device, last):
+    """65,536 sequences of a token, or as many of which most are empty: each token sees itself alone, whose weight
+    is 1."""
+    n = 65536
+    q, k, v = make(device, F16, 1, 4, 2, n, n, seed=17)
+    starts = torch.arange(n + 1, dtype=torch.int32, device=device).clamp(max=last)
+    got = prompt_attention(q, k, v, SCALE, q_starts=starts, k_starts=starts)
+    assert torch.equal(got[:, :, :last], v.repeat_interleave(2, 1)[:, :, :last]) and not got[:, :, last:].any()
+    with pytest.raises(ValueError, match="at most 65536"):
+        more = torch.zeros(n + 2, dtype=torch.int32, device=device)
+        prompt_attention(q, k, v, SCALE, q_starts=more, k_starts=more)

@@ -331,3 +331,11 @@ def test_no_grad_sees_tangents():
         torch.func.jvp(lambda t: (_no_grad(t), t)[1], (a,), (b,))
     with torch.inference_mode():
         _no_grad(a, b, x(2))
+
+
+def test_prompt_counts_stay_in_32_bits():
+    """Sequences whose tiles, empty ones among them, would be counted past 2^31 rows, and more than a call takes."""
+    packed = dict(q_starts=4096, k_starts=4096)
+    for change, message in [(dict(n_seq=65537), b"at most 65536"), (dict(n_seq=10_000_000), b"at most 65536"),
+                            (dict(n_seq=65536, tq=(2 ** 31 - 513) // 2), b"too many tiles")]:
+        assert prompt_call(**packed, **change) == _lib.TP_ERR_INVALID and message in _lib.lib().tp_last_error(), change

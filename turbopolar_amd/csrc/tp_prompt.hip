@@ -19,6 +19,9 @@
 namespace tp {
 
 constexpr int kPromptTarget = 256;  // workgroups that fill the GPU
+// Packed sequences of a call.  Each adds a workgroup a kv head, and every workgroup looks its own up in the list, so
+// their time grows with the square of their number.
+constexpr int kMaxSequences = 65536;
 
 struct PromptArgs {
   const uint16_t* q;
@@ -477,6 +480,10 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
     set_error("packed sequences need a batch of 1 and both start arrays");
     return TP_ERR_INVALID;
   }
+  if (n_seq > kMaxSequences) {
+    set_error("a call takes at most %d packed sequences, got %d", kMaxSequences, n_seq);
+    return TP_ERR_INVALID;
+  }
   if (tq == 0) return TP_OK;
   if (!q || !out || (tk && (!k || !v)) || ((uintptr_t)q & 15u) || ((uintptr_t)k & 15u) || ((uintptr_t)v & 15u) ||
       ((uintptr_t)out & 15u)) {
@@ -493,7 +500,9 @@ extern "C" int32_t tp_prompt_attention(const void* q, const void* k, const void*
     return TP_ERR_INVALID;
   }
   const PromptPlan p = plan_prompt(batch * hkv, g, tq, std::max<int64_t>(tk, 1), n_seq);
-  if ((double)batch * hkv * (double)p.tiles * (double)p.splits > (double)INT32_MAX) {
+  // Rows are counted in 32 bits up to the end of the last tile, workgroups too.
+  if (p.tiles * p.waves * kWaveRows > INT32_MAX ||
+      (double)batch * hkv * (double)p.tiles * (double)p.splits > (double)INT32_MAX) {
     set_error("too many tiles of rows for one launch");
     return TP_ERR_INVALID;
   }

@@ -621,8 +621,8 @@ def prompt_attention(
     copied).  ``causal``: the queries are the last ``Tq`` of the ``Tk`` positions.  A query that
     sees no key gives 0.
 
-    ``q_starts`` / ``k_starts`` (together, batch 1): packed sequences, the ``n + 1`` ascending
-    token positions between them, as sequences of ints or host tensors, which are checked, or as
+    ``q_starts`` / ``k_starts`` (together, batch 1): packed sequences, at most 65,536, the ``n + 1``
+    ascending token positions between them, as sequences of ints or host tensors, which are checked, or as
     int32 device tensors, which are not read here (values out of order give unspecified rows).
     Query rows behind the last sequence are 0, or left as they are where ``out`` is given.
     ``out`` shares no memory with k or v, nor with q unless it is q.
