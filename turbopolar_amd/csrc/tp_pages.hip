@@ -35,7 +35,7 @@ struct CopyArgs {
 
 // One workgroup a page slot of a (batch, head) row, over all of its buffers as one run of 16-byte
 // chunks; slots past the kept ones are cleared.  The last workgroups of a row copy its tail.  Bound by
-// HBM: 78 MB read and written in 27 to 35 us, 4.4 to 5.8 TB/s (a copy of 1 GiB 5.1).
+// HBM: 78 MB read and written in 27 to 36 us, 4.4 to 5.8 TB/s (a copy of 1 GiB 5.1).
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int tid = threadIdx.x;
   const int64_t bh = blockIdx.y, slot = blockIdx.x;

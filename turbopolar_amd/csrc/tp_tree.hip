@@ -220,14 +220,15 @@ constexpr int kTreeThreads = 64 * RW * TW;
 
 // The decode of a page (one product a pair of dimensions, one a pair of values) and the two products over it go
 // on side by side: few rows are bound by the reads and the decode (5 nodes, 32 heads, 131,072 tokens of the fast
-// layout: 60 us, 4.6 TB/s), 128 rows by decode and products alike (32 nodes over 32,805 tokens: 35 us, 2.2 TB/s and
-// 0.49 PFLOP/s).
+// layout: 63 us, 4.4 TB/s), 128 rows by decode and products alike (32 nodes over 32,805 tokens: 36.7 us, 2.1 TB/s and
+// 0.46 PFLOP/s).
 //
 // A key component is rounded to fp16 once, from fp32 angles and radii, as the page decoder rounds it, so that what is
 // attended is what the decoder hands out; a value, a weight, a record and the result once each; 32-bit sums.  An
-// output's error, relative in L2, is 5.2e-4 (default layout, 1,000 tokens) to 6.4e-4 (fast layout, 131,072) by that,
-// of which the keys alone give 3.7e-4 to 5.1e-4 (scores of a spread of 1.8).  Cosines, int8 radii and products in fp16
-// gave 5.9e-4 to 8.7e-4 for 2 % less time (32 nodes over 32,805 tokens 40.6 us instead of 41.5).
+// output's error, relative in L2, is 5.2e-4 (default layout, 1,000 tokens) to 7.0e-4 (fast layout, 131,072) by that,
+// of which the keys alone give 3.7e-4 to 5.1e-4 (scores of a spread of 1.8); against attention in 64 bits over the
+// decoder's numbers it is 3.5e-4.  Cosines, int8 radii and products in fp16 gave 5.9e-4 to 8.7e-4 for 2 % less time
+// (32 nodes over 32,805 tokens with the join 40.6 us instead of 41.5).
 template <int KIND, int RW, int TW>
 __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kernel(TreeArgs a) {
   constexpr int THREADS = kTreeThreads<RW, TW>, N = 512 / THREADS, NB = 2 / TW, BUFS = RW * TW > 2 ? 2 : 1;
@@ -392,11 +393,11 @@ __global__ __launch_bounds__((kTreeThreads<RW, TW>), 2) void tree_attention_kern
 
 // Rows of a workgroup, and how the pages are split: into as many workgroups as fill the GPU (two waves a
 // SIMD).  Measured with 32/8 heads, us without the join:
-//   up to 32 rows: two waves, four workgroups a CU, 58 over 131,072 tokens (four waves, two of them decoding only,
-//     67); layouts whose codes go through LDS take the four of 64 rows, since a thread of two waves decodes four
-//     runs, for which they have no registers (2-bit deep codes over 32,768 tokens 32 instead of 54);
-//   up to 128 rows: four waves, 31 over 32,768 tokens (eight, each with half of a page's tokens, 37); the layouts
-//     through LDS, which spill at four, the eight (split at pair 23: 48 instead of 88).
+//   up to 32 rows: two waves, four workgroups a CU, 63 over 131,072 tokens (four waves, two of them decoding only,
+//     77); layouts whose codes go through LDS take the four of 64 rows, since a thread of two waves decodes four
+//     runs, for which they have no registers (2-bit deep codes over 32,768 tokens 33 instead of 54);
+//   up to 128 rows: four waves, 35 over 32,768 tokens (eight, each with half of a page's tokens, 40); the layouts
+//     through LDS, which spill at four, the eight (split at pair 23: 51 instead of 88).
 // The tail and the drafts take one more record, unless there is but one split of pages.
 struct TreePlan {
   int32_t row_waves, row_blocks, pages_per_split, page_splits, records;

@@ -17,7 +17,8 @@ Mirrors the reference's mlx_lm hook (benchmarks/turbopolar_fast_attention.py:
   ``TurboPolarFastCache.decode_attention`` (the fused HIP kernel over the
   compressed pages) and everything else through the original forward.  With
   ``prompt_kernel=True`` prompts and chunks of them go through
-  ``TurboPolarFastCache.prompt_attention``, which needs no score matrix.
+  ``TurboPolarFastCache.prompt_attention``, which forms no scores in memory (the
+  model's mask is still compared with the causal one).
 * The cache protocol's ``crop``, ``reorder_cache``, ``batch_select_indices`` and
   ``batch_repeat_interleave`` (assisted generation and beams) truncate and
   re-order the compressed cache.
