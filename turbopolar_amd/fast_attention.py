@@ -158,7 +158,8 @@ class TurboPolarFastCache:
         ``values`` ``[B, H_kv, T, 128]`` and attend the chunk's ``q`` ``[B, H_q, T, 128]`` over the
         whole history as ``update_and_fetch`` decompresses it (tp_prompt_attention in fp16, the
         cache's type, in which ``q`` is taken too; the scale in 32 bits, as the model's own attention
-        takes it).  Returns ``[B, H_q, T, 128]`` of q's type.  No counterpart in the reference, which hands the history to the model's attention."""
+        takes it).  Returns ``[B, H_q, T, 128]`` of q's type.  No counterpart in the reference, which
+        hands the history to the model's attention."""
         for name, t in (("q", q), ("keys", keys), ("values", values)):
             if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[-1] != HEAD_DIM:
                 raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ()))}")
