@@ -6,7 +6,10 @@ for the prompt kernel (weights and result rounded once each, eps = 2^-11, and fp
 keys: the kernel rounds the cosine, an int8 layout's radius and their product, the oracle the
 product, so a key component differs by at most 4 eps of itself (and r 2^-23 for subnormal cosines
 and the fp32 angle), a score by ds = scale (4 eps + 129 2^-24) sum|q||k| + scale 2^-23 sum|q| r, a
-weight by exp(2 ds) - 1 (its own and the sum's).  Values are the same numbers on both sides."""
+weight by exp(2 ds) - 1 (its own and the sum's).  Values are the same numbers on both sides.
+
+The key's part is more than is needed since the kernel rounds the product alone, as the oracle does;
+test_keys_are_the_page_decoders holds it to that."""
 
 import numpy as np
 import pytest
