@@ -435,6 +435,79 @@ int32_t tp_take_tokens(const void* k, const void* v, int32_t in_dtype, int64_t b
                        void* out_v, int64_t out_tokens, int64_t out_pos, int32_t check, uint32_t* flag, uint32_t epoch,
                        void* stream);
 
+/*
+ * Queries and keys turned by their positions, and keys and values handed on: y_a = x_a cos_a -
+ * x_b sin_a, y_b = x_b cos_b + x_a sin_b over the pairs (a, b) = (d, d + 64), or (2d, 2d + 1) with
+ * `interleaved`.  q [batch][hq][tokens][128], k, v [batch][hkv][tokens][128] of dtype 0 (fp16), 1
+ * (fp32) or 2 (bf16); strides: 9 host values, (batch, head, token) of q, k and v in elements.  cos, sin
+ * [batch][tokens][columns] of table_dtype (dtype, or 1), columns 128 (one a dimension) or 64 (one a pair),
+ * contiguous; table_strides: (batch, token), 0 for one table for all rows.  q_out fp16 with
+ * q_out_strides (batch, head, token); k_out, v_out fp16 [batch][hkv][out_tokens][128], tokens [out_pos,
+ * out_pos + tokens) written, of v as cast.  Strides are non-negative multiples of 8, buffers 16-byte
+ * aligned; outputs share no memory with inputs or each other.
+ * A result is the exact sum rounded to fp32 (by way of fp64 where an input or the tables are fp32), then to
+ * fp16.  check 2: waits for the verdict as tp_append_stage does, TP_ERR_NONFINITE if a key or value written
+ * is not finite (k and v are no longer read then); flag: pinned host memory of flag_words words, of which up to 16 a
+ * token are written; epoch even.  check 0: returns after the launch.
+ */
+int32_t tp_rotate_tokens(const void* q, const void* k, const void* v, int32_t dtype, int64_t batch, int32_t hq,
+                         int32_t hkv, int64_t tokens, const int64_t* strides, const void* cos, const void* sin,
+                         int32_t table_dtype, int32_t columns, const int64_t* table_strides, int32_t interleaved,
+                         void* q_out, const int64_t* q_out_strides, void* k_out, void* v_out, int64_t out_tokens,
+                         int64_t out_pos, int32_t check, uint32_t* flag, int64_t flag_words, uint32_t epoch,
+                         void* stream);
+
+/*
+ * One decode step's attention of a batch behind a common prefix: q, out fp16 [batch][hq][128]; every row
+ * attends the prefix, one cache of batch 1 (its pages, prefix_pages of them, and its dense tail), and then its
+ * own cache's pages and tail (batch rows).  Both caches have `layout`; pages and tails as for
+ * tp_tree_attention, either cache may be empty, not both.  strides: 4 host values, (batch, head) of q and of
+ * out.  workspace (tp_shared_workspace_bytes) as for tp_prompt_attention.
+ */
+int32_t tp_shared_attention(const void* q, void* out, int64_t batch, int32_t hq, int32_t hkv,
+                            const tp_page_layout* layout, const tp_pages* prefix, int32_t prefix_pages,
+                            const void* prefix_tail_k, const void* prefix_tail_v, int32_t prefix_tail,
+                            int64_t prefix_tail_stride, const tp_pages* pages, int32_t n_pages, const void* tail_k,
+                            const void* tail_v, int32_t tail_len, int64_t tail_stride, const int64_t* strides,
+                            float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t tp_shared_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, const tp_page_layout* layout,
+                                 int32_t prefix_pages, int32_t prefix_tail, int32_t n_pages, int32_t tail_len);
+
+/*
+ * The bounds of pages [page_begin, page_begin + n_pages): the smallest and the largest of each key component
+ * over a page's 64 tokens, of the decoded keys (those of tp_decode_pages up to a step of fp16).  bounds: fp16
+ * [bh][bounds_capacity][2][128], 16-byte aligned; bh at most 65535.
+ */
+int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* pages, int64_t bh, int32_t page_begin,
+                       int32_t n_pages, void* bounds, int64_t bounds_capacity, void* stream);
+
+/*
+ * The pages that a query is likely to need.  A page's score for (batch, kv head) is the largest of
+ * sum_d max(q_d lo_d, q_d hi_d) over the query heads of the group (of -q where scale < 0): no key of the page has a
+ * larger product with q.  selected: int32 [batch][hkv][count], ascending: the first `first` and the last `last` of
+ * the n_pages pages and those of the others with the largest scores, ties to the lower index.  Scores are fp64 sums
+ * of exact products; one that is NaN counts as infinite.
+ * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages.
+ * workspace (tp_select_workspace_bytes) as for tp_prompt_attention.
+ */
+int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int32_t hkv, const void* bounds,
+                        int64_t bounds_capacity, int32_t n_pages, int32_t first, int32_t last, int32_t count,
+                        float scale, int32_t* selected, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t tp_select_workspace_bytes(int64_t batch, int32_t hkv, int32_t n_pages);
+
+/*
+ * tp_decode_attention over `count` of the n_pages stored pages, each (batch, kv head) its own (selected: device
+ * int32 [batch][hkv][count], entries clamped to the stored pages), and the whole dense tail.  workspace:
+ * tp_decode_workspace_bytes(batch, hq, hkv, count, tail_len, 0) bytes, its counter area as for
+ * tp_decode_attention.
+ */
+int32_t tp_selected_attention(const void* q, int64_t batch, int32_t hq, int32_t hkv, const tp_page_layout* layout,
+                              const tp_pages* pages, int32_t n_pages, const int32_t* selected, int32_t count,
+                              const void* tail_k, const void* tail_v, int32_t tail_len, int64_t tail_stride, float scale,
+                              void* workspace, size_t workspace_bytes, void* out, void* stream);
+
 /* ---- QJL (rejected by TurboPolarConfig, turbo_polar_config.py:46-47, as in
  * the reference; these serve the bridge-level QJL calls the reference's own
  * tests make). ---- */

@@ -13,6 +13,7 @@ from .draft import DraftTree
 from .fast_attention import TurboPolarFastCache, make_turbo_caches
 from .payload import PolarKeyBlock, QuantizedVBlock
 from .runtime import TurboPolarKVCacheRuntime
+from .shared import SharedPrefixCache
 from .storage import PolarKBlockStorage, QuantVBlockStorage
 
 __all__ = [
@@ -25,6 +26,7 @@ __all__ = [
     "PolarQuantEncoder",
     "QuantVBlockStorage",
     "QuantizedVBlock",
+    "SharedPrefixCache",
     "TurboPolarConfig",
     "TurboPolarFastCache",
     "TurboPolarKVCacheRuntime",

@@ -194,6 +194,34 @@ _SIGNATURES = {
             c_i64, c_i32, c_vp, ctypes.c_uint32, c_vp,
         ],
     ),
+    "tp_rotate_tokens": (
+        c_i32,
+        [
+            c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_i64, _P_STRIDES, c_vp, c_vp, c_i32, c_i32, _P_STRIDES,
+            c_i32, c_vp, _P_STRIDES, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp, c_i64, ctypes.c_uint32, c_vp,
+        ],
+    ),
+    "tp_shared_attention": (
+        c_i32,
+        [
+            c_vp, c_vp, c_i64, c_i32, c_i32, _P_LAYOUT, _P_PAGES, c_i32, c_vp, c_vp, c_i32, c_i64, _P_PAGES, c_i32,
+            c_vp, c_vp, c_i32, c_i64, _P_STRIDES, c_float, c_vp, c_size, c_vp,
+        ],
+    ),
+    "tp_shared_workspace_bytes": (c_size, [c_i64, c_i32, c_i32, _P_LAYOUT, c_i32, c_i32, c_i32, c_i32]),
+    "tp_page_bounds": (c_i32, [_P_LAYOUT, _P_PAGES, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "tp_select_pages": (
+        c_i32,
+        [c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_float, c_vp, c_vp, c_size, c_vp],
+    ),
+    "tp_select_workspace_bytes": (c_size, [c_i64, c_i32, c_i32]),
+    "tp_selected_attention": (
+        c_i32,
+        [
+            c_vp, c_i64, c_i32, c_i32, _P_LAYOUT, _P_PAGES, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_i64, c_float,
+            c_vp, c_size, c_vp, c_vp,
+        ],
+    ),
     "tp_fused_qk_qjl": (c_i32, [c_vp, c_i64, c_i32, c_i32, _P_LAYOUT, _P_PAGES, c_i32, _P_QJL, c_float, c_vp, c_vp]),
     "tp_decode_attention_qjl": (
         c_i32,

@@ -15,6 +15,11 @@ and, with no counterpart there, attention of a whole prompt and of a drafted tre
 * ``execute_prompt_attention(q, k, v, config, ...) -> (out, trace)``
 * ``execute_tree_attention_quant_v_dense_tail(...) -> (out, trace)``
 
+and attention over the pages that a cheap score selects:
+
+* ``execute_page_bounds(block) -> (bounds, trace)``
+* ``execute_selected_attention_quant_v_dense_tail(...) -> (out, trace)``
+
 Differences: there is no silent CPU fallback (unsupported inputs raise), and
 the trace reports ``hip_used`` where the reference reports ``metal_used``.
 ``use_qjl=True`` adds the QJL correction to the page tokens' scores
@@ -32,8 +37,8 @@ import torch
 from . import _lib
 from .draft import DraftTree
 from .kernels import (
-    PageSet, _DEFAULT_LAYOUT, decode_attention, decode_attention_dense_v, fp16_scale, fused_qk, prompt_attention,
-    tree_attention,
+    HEAD_DIM, PageSet, _DEFAULT_LAYOUT, _no_grad, check_selection, decode_attention, decode_attention_dense_v, fp16_scale,
+    fused_qk, page_bounds_into, prompt_attention, selected_attention, tree_attention,
 )
 from .payload import PolarKeyBlock, QuantizedVBlock, layout_from_metadata
 from .qjl import QJLPages
@@ -279,5 +284,64 @@ class HipKernelBridge:
             "tail_length": tail_len,
             "nodes": tree.nodes,
             "num_queries_per_kv": q.shape[1] // draft_k.shape[1],
+        }
+        return out, trace
+
+    def execute_page_bounds(self, block: PolarKeyBlock) -> Tuple[torch.Tensor, Dict[str, Any]]:
+        """The smallest and the largest of each key component over every page of ``block`` (tp_page_bounds): fp16
+        ``[B, H_kv, S, 2, 128]``."""
+        self._supports_block(block)
+        pages = _key_pages_of(block, HEAD_DIM)
+        bounds = torch.empty((pages.B, pages.H, pages.S, 2, HEAD_DIM), dtype=torch.float16,
+                             device=pages.tensors["radii"].device)
+        page_bounds_into(pages.layout, pages.pages, pages.B * pages.H, 0, pages.S, bounds)
+        return bounds, {"kernel_name": "page_bounds", "hip_kernel": "tp_page_bounds", "hip_used": True,
+                        "fallback_used": False, "pages": pages.S}
+
+    def execute_selected_attention_quant_v_dense_tail(
+        self,
+        q: torch.Tensor,
+        block: PolarKeyBlock,
+        quant_v: QuantizedVBlock,
+        bounds: torch.Tensor,
+        tail_k: Optional[torch.Tensor],
+        tail_v: Optional[torch.Tensor],
+        config,
+        pages: int,
+        first: int = 1,
+        last: int = 1,
+    ) -> Tuple[torch.Tensor, Dict[str, Any]]:
+        """Attention of ``q`` ``[B, H_q, 128]`` over ``pages`` of the block's pages (all of them if there are no more)
+        and the dense tail (None or empty without one): for each kv head the first ``first``, the last ``last`` and
+        those whose ``bounds`` (``execute_page_bounds``) allow the largest scores (``kernels.selected_attention``).
+        The trace's ``selected`` holds them, int32 ``[B, H_kv, pages]``."""
+        check_selection(pages, first, last)
+        self._supports_block(block)
+        held = _pages_of(block, quant_v, config.head_dim)
+        dev = held.tensors["radii"].device
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[0] != held.B or q.shape[1] < 1 or q.shape[1] % held.H:
+            raise ValueError(f"q {tuple(getattr(q, 'shape', ()))} does not match pages of {held.B} x {held.H} (batch, heads)")
+        tail_len = int(tail_k.shape[2]) if tail_k is not None else 0
+        if q.device != dev or (tail_len and (tail_k.device != dev or tail_v.device != dev)):
+            raise ValueError(f"q is on {q.device}, the pages on {dev}; the tail must be there too")
+        if tail_len and (tail_k.shape != tail_v.shape or tuple(tail_k.shape[:2]) != (held.B, held.H)
+                         or tail_k.shape[3] != HEAD_DIM):
+            raise ValueError(f"tail shape {tuple(tail_k.shape)} does not match [B={held.B}, H_kv={held.H}, T, {HEAD_DIM}]")
+        _no_grad(q, *((tail_k, tail_v) if tail_len else ()))
+        count = min(pages, held.S)
+        if count < pages:  # every page: none needs a place of its own
+            first = last = 0
+        out, selected = selected_attention(q, held.layout, held.pages, held.S, held.H, bounds, tail_k if tail_len else None,
+                                           tail_v if tail_len else None, fp16_scale(config.attention_scale), count, first,
+                                           last)
+        trace = {
+            "kernel_name": "selected_attention_quant_v_dense_tail",
+            "hip_kernel": "tp_selected_attention",
+            "hip_used": True,
+            "fallback_used": False,
+            "quant_v_used": True,
+            "tail_length": tail_len,
+            "selected": selected,
+            "num_queries_per_kv": q.shape[1] // held.H,
         }
         return out, trace

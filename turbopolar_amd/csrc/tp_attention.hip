@@ -144,6 +144,9 @@ struct AttnArgs {
   int32_t check;     // 2 reports the verdict, 3 only a non-finite value, 4 the verdict and the reads (take_new_row)
   uint32_t* flag;
   uint32_t epoch;
+  // The stored pages that are attended (tp_selected_attention): [bkv][n_pages] of n_stored.
+  const int32_t* list;
+  int32_t n_stored;
 };
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -1372,6 +1375,7 @@ constexpr int kFlNoAcquire = 2;  // no acquire fence in the combining workgroup
 constexpr int kFlTiers = 4;      // two-tier combine (launched only when tier_splits > 0)
 constexpr int kFlBatch16 = 8;    // one-tier combine of exactly 16 splits (4-wave launches)
 constexpr int kFlStep = 16;      // tp_decode_step: the tail's last row is the launch's own token
+constexpr int kFlList = 32;      // tp_selected_attention: page p is stored page list[p] of its row
 
 // One thread draws a ticket of a counter that `count` workgroups increment:
 // relaxed agent-scope add; the workgroup that draws the last ticket issues an
@@ -1769,6 +1773,11 @@ __device__ __forceinline__ void finish_merged(Merge& sh, const AttnArgs& a, int 
 
 // ---- decode attention kernel ---------------------------------------------------
 
+// The stored page of a row's listed page p; an entry out of range reads a page that is there.
+__device__ __forceinline__ int stored_page(const AttnArgs& a, int64_t bkv, int p) {
+  return min(max(a.list[bkv * a.n_pages + p], 0), a.n_stored - 1);
+}
+
 template <int KIND, int WAVES, int FL = 0, int QJL = kQjlOff, bool DV = false>
 __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a) {
   // The fold maps the threads onto heads x 128 dims at 4 dims per thread (512
@@ -1780,6 +1789,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
   // blocks of at most 8 query heads.
   constexpr bool HR = KIND == kKindDefaultHR;
   constexpr bool STEP = (FL & kFlStep) != 0;
+  constexpr bool LIST = (FL & kFlList) != 0;
   __shared__ AttnShared<WAVES> sh;
   if constexpr (STEP) {
     if (blockIdx.z == 0) {
@@ -1825,6 +1835,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
   load_q<HR>(a, b, kv, h0, nh, l16, l4, qb);
   TP_STAMP(60);
   int page = p_begin + wave;
+  [[maybe_unused]] int next_page = 0;  // LIST: the stored page of the wave's next page, read one page ahead
   KRegs<KIND> kr;
   // V: the page store's codes, or the dense V planes' rows (DV).
   typename std::conditional<DV, DenseVRegs, VRegs>::type vr;
@@ -1839,6 +1850,10 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
     // wait for all loads in flight.
     int p_load, lane_e;
     first_page_load(page, p_begin, p_end, lane, p_load, lane_e);
+    if constexpr (LIST) {
+      p_load = stored_page(a, bkv, p_load);
+      next_page = stored_page(a, bkv, min(page + WAVES, a.n_pages - 1));
+    }
     load_k<KIND>(a, bkv * a.capacity + p_load, lane_e & 15, lane_e >> 4, kr);
     if constexpr (DV)
       load_v<HR>(a, bkv * a.v_capacity + p_load, lane_e & 15, lane_e >> 4, lane_e, vr);
@@ -1884,14 +1899,16 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
       if constexpr (QJL == kQjlAny)
         qjl_correct_any<HR>(a, bkv * a.qjl_capacity + page, l4, qjl_qw, HR ? (l16 & 7) : l16, qnorm, qjl_sin, s);
       if (it < 12) TP_STAMP(4 + 4 * it);
-      load_k<KIND>(a, bkv * a.capacity + page + WAVES, l16, l4, kr);
+      const int at_next = LIST ? next_page : page + WAVES;
+      load_k<KIND>(a, bkv * a.capacity + at_next, l16, l4, kr);
       half8v pb[2];
       softmax_page<HR>(s, kPageTokens, a.scale_log2, l4, m_run, l_run, acc, pb);
       pv_regs<HR>(vr, sbase4, ssel, pb, acc);
       if constexpr (DV)
         load_v<HR>(a, bkv * a.v_capacity + page + WAVES, l16, l4, lane, vr);
       else
-        load_v<HR>(a, bkv * a.capacity + page + WAVES, l16, l4, lane, vr);
+        load_v<HR>(a, bkv * a.capacity + at_next, l16, l4, lane, vr);
+      if constexpr (LIST) next_page = stored_page(a, bkv, min(page + 2 * WAVES, a.n_pages - 1));
       if (it < 12) TP_STAMP(5 + 4 * it);
     }
     if (page < p_end) {
@@ -2277,6 +2294,13 @@ template <int KIND, int W, int QJL, bool DV = false>
 static void launch_decode_w(const AttnArgs& a, dim3 grid, hipStream_t s) {
   const dim3 block(W * 64);
   if constexpr (QJL == kQjlOff && !DV) {
+    if (a.list) {
+      if (a.tier_splits > 0)
+        hipLaunchKernelGGL((decode_attention_kernel<KIND, W, kFlList | kFlTiers>), grid, block, 0, s, a);
+      else
+        hipLaunchKernelGGL((decode_attention_kernel<KIND, W, kFlList>), grid, block, 0, s, a);
+      return;
+    }
     if (a.new_k) {  // a step: one z layer more, for stage_new_rows
       const dim3 g(grid.x, grid.y, grid.z + 1);
       if (a.tier_splits > 0)
@@ -2411,7 +2435,8 @@ static int32_t decode_attention_impl(const void* q, int64_t batch, int32_t hq, i
                                      int64_t tail_stride, int64_t actual_seq_len, float scale,
                                      int32_t pages_per_split, void* workspace, size_t workspace_bytes, void* out,
                                      void* stream, bool use_qjl, const void* v_dense = nullptr,
-                                     int64_t v_capacity = 0, const AttnArgs* step = nullptr) {
+                                     int64_t v_capacity = 0, const AttnArgs* step = nullptr,
+                                     const int32_t* list = nullptr, int32_t n_stored = 0) {
   clear_error();
   AttnArgs a{};
   if (!fill_common(a, q, batch, hq, hkv, layout, pages, n_pages, v_dense == nullptr)) return TP_ERR_INVALID;
@@ -2483,6 +2508,10 @@ static int32_t decode_attention_impl(const void* q, int64_t batch, int32_t hq, i
     a.flag = step->flag;
     a.epoch = step->epoch;
   }
+  if (list) {
+    a.list = list;
+    a.n_stored = n_stored;
+  }
   if (n_splits > 1) {
     const size_t need = tp_decode_workspace_bytes(batch, hq, hkv, n_pages, tail_len, pages_per_split);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u)) {
@@ -2531,7 +2560,7 @@ static int32_t decode_attention_impl(const void* q, int64_t batch, int32_t hq, i
     return launch_status("tp_decode_attention_qjl");
   }
 #ifdef TP_TIMELINE
-  if (g_measure_variant != 0 && !step) {
+  if (g_measure_variant != 0 && !step && !list) {
     // The measurement variants combine in one tier (any split count).
     a.tier_splits = 0;
     a.tier_groups = 0;
@@ -2609,6 +2638,29 @@ int32_t tp_decode_attention_dense_v(const void* q, int64_t batch, int32_t hq, in
   return decode_attention_impl(q, batch, hq, hkv, layout, pages, n_pages, qjl, nullptr, nullptr, 0, 0,
                                actual_seq_len, scale, pages_per_split, workspace, workspace_bytes, out, stream,
                                qjl != nullptr, v_dense, v_capacity);
+}
+
+int32_t tp_selected_attention(const void* q, int64_t batch, int32_t hq, int32_t hkv, const tp_page_layout* layout,
+                              const tp_pages* pages, int32_t n_pages, const int32_t* selected, int32_t count,
+                              const void* tail_k, const void* tail_v, int32_t tail_len, int64_t tail_stride, float scale,
+                              void* workspace, size_t workspace_bytes, void* out, void* stream) {
+  clear_error();
+  if (!selected || ((uintptr_t)selected & 3u) || count < 1 || n_pages < 1 || !pages || pages->capacity < n_pages) {
+    set_error("tp_selected_attention needs selected pages of a store, got %d of %d pages", count, n_pages);
+    return TP_ERR_INVALID;
+  }
+  if (!(scale == scale) || scale - scale != 0.0f) {
+    set_error("scale must be finite");
+    return TP_ERR_INVALID;
+  }
+  // The same page may be listed more than once (its tokens then count as often), but not more pages than are stored.
+  if (count > n_pages) {
+    set_error("%d pages selected of %d", count, n_pages);
+    return TP_ERR_INVALID;
+  }
+  return decode_attention_impl(q, batch, hq, hkv, layout, pages, count, nullptr, tail_k, tail_v, tail_len,
+                               tail_stride, INT64_MAX, scale, 0, workspace, workspace_bytes, out, stream, false,
+                               nullptr, 0, nullptr, selected, n_pages);
 }
 
 }  // extern "C"

@@ -35,8 +35,8 @@ from .codecs import GroupedVQuantizer, PolarQuantDecoder
 from .config import TurboPolarConfig
 from .draft import DraftTree
 from .kernels import (
-    HEAD_DIM, PAGE, _check_draft, _no_grad, _tree_attention, decode_attention_store, decode_pages_into, fp16_scale,
-    prompt_attention,
+    HEAD_DIM, PAGE, _check_draft, _no_grad, _tree_attention, check_selection, decode_attention_store, decode_pages_into,
+    fp16_scale, prompt_attention, rotate_tokens, selected_attention,
 )
 from .runtime import TurboPolarKVCacheRuntime
 from .storage import pages_of
@@ -151,6 +151,51 @@ class TurboPolarFastCache:
         return decode_attention_store(q[:, :, 0], layout, pages, n_pages, rt._num_kv_heads, tail_k, tail_v,
                                       rt.actual_seq_len, scale)
 
+    # ------------------------------------------------------------------ rotated appends
+    def append_rotated(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                       interleaved: bool = False) -> torch.Tensor:
+        """Queries and keys turned by their positions, keys and values appended
+        (``TurboPolarKVCacheRuntime.append_rotated``).  Returns the queries, fp16 ``[B, H_q, T, 128]``."""
+        return self.runtime.append_rotated(q, k, v, cos, sin, interleaved)
+
+    def update_rotated(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                       interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``append_rotated`` of a prompt or a chunk, and the whole history decompressed, as ``update_and_fetch``
+        returns it: (queries, keys, values), all fp16."""
+        q, k, v = rotate_tokens(q, k, v, cos, sin, interleaved)
+        return (q, *self.update_and_fetch(k, v))
+
+    def decode_rotated(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, scale: float, interleaved: bool = False,
+                       defer_check: bool = False) -> torch.Tensor:
+        """``decode_attention`` of a token whose query and key are still to be turned by its position (``cos`` /
+        ``sin`` as for ``append_rotated``): two launches in all.  Returns fp16 ``[1, H_q, 128]``."""
+        self._validate_decode_shape(q, k_new, v_new, self.config)
+        q, k_new, v_new = rotate_tokens(q, k_new, v_new, cos, sin, interleaved)
+        return self.decode_attention(q, k_new, v_new, scale, defer_check)
+
+    # ------------------------------------------------------------------ selected pages
+    def selected_attention(self, q: torch.Tensor, scale: float, pages: int, first: int = 1, last: int = 1) -> torch.Tensor:
+        """One decode step's attention over part of the cache: the queries ``q`` ``[B, H_q, 1, 128]`` of the newest
+        tokens (appended before) over ``pages`` stored pages and the dense tail.  Of the pages each kv head takes the
+        first ``first``, the last ``last`` and those whose key bounds allow the largest scores to a query head of its
+        group (tp_select_pages); a cache of no more pages is attended whole, as by ``decode_attention``.  ``scale`` is
+        taken as fp16.  The bounds are kept with the cache (``runtime.page_bounds``).  Returns fp16 ``[B, H_q, 128]``."""
+        check_selection(pages, first, last)
+        _check_step_query(q, self)
+        rt = self.runtime
+        rt.resolve_deferred_check()
+        n_pages, H = rt.k_storage.block_count, rt._num_kv_heads
+        tail_k, tail_v = rt._tail_views()
+        scale, layout = fp16_scale(scale), rt.polar_encoder.layout
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
+        stored = self._store_pages() if n_pages else None
+        if n_pages <= pages:
+            return decode_attention_store(q[:, :, 0], layout, stored, n_pages, H, tail_k, tail_v, rt.actual_seq_len, scale)
+        return selected_attention(q[:, :, 0], layout, stored, n_pages, H, rt.page_bounds(), tail_k, tail_v, scale, pages,
+                                  first, last)[0]
+
     # ------------------------------------------------------------------ prompts, drafts, branches
     def prompt_attention(self, q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
                          causal: bool = True) -> torch.Tensor:
@@ -236,6 +281,25 @@ class TurboPolarFastCache:
 
     def empty(self) -> bool:
         return self.offset == 0
+
+
+def _check_step_query(q, cache: TurboPolarFastCache) -> None:
+    """The checks of a step's queries ``[B, H_q, 1, 128]`` against the tokens that ``cache`` holds."""
+    rt = cache.runtime
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[2] != 1 or q.shape[-1] != HEAD_DIM:
+        raise ValueError(f"q must be [B, H_q, 1, {HEAD_DIM}], got {tuple(getattr(q, 'shape', ()))}")
+    if not q.is_floating_point():
+        raise ValueError(f"q must be a float tensor, got {q.dtype}")
+    if not rt.actual_seq_len:
+        raise ValueError("nothing to attend: the cache holds no tokens")
+    if q.shape[0] != rt._batch_size:
+        raise ValueError(f"batch of q ({q.shape[0]}) and cache ({rt._batch_size}) differ")
+    if q.shape[1] < 1 or q.shape[1] % rt._num_kv_heads:
+        raise ValueError(f"H_q={q.shape[1]} is not a multiple of H_kv={rt._num_kv_heads}")
+    held = rt.k_storage.radii if rt.k_storage.block_count else rt._tail_k
+    if not q.is_cuda or held.device != q.device:
+        raise ValueError(f"q is on {q.device}, the cache on {held.device}; need one HIP device")
+    _no_grad(q)
 
 
 def make_turbo_caches(num_layers: int, num_q_heads: int, num_kv_heads: int, head_dim: int,

@@ -780,6 +780,208 @@ def take_tokens(k: torch.Tensor, v: torch.Tensor, index: Union[Sequence[int], Se
     check(st, "tp_take_tokens")
 
 
+# --------------------------------------------------------------------------
+# rotated appends
+# --------------------------------------------------------------------------
+
+_Strides2, _Strides3, _Strides9 = ctypes.c_int64 * 2, ctypes.c_int64 * 3, ctypes.c_int64 * 9
+_ROTATE_TYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+
+
+def _check_rotated(q, k, v, cos, sin) -> None:
+    """The checks of ``rotate_tokens``'s tensors against each other."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[-1] != HEAD_DIM:
+            raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ()))}")
+    if q.dtype not in _ROTATE_TYPES or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError(f"q, k and v must be of one type, float16, bfloat16 or float32, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, Hq, T, _ = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[2] != T:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match each other and q {tuple(q.shape)}")
+    if B < 1 or Hq < 1 or k.shape[1] < 1 or Hq % int(k.shape[1]):
+        raise ValueError(f"H_q={Hq} is not a multiple of H_kv={k.shape[1]}, or the batch is empty")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if not isinstance(t, torch.Tensor) or not t.is_floating_point():
+            raise ValueError(f"{name} must be a float tensor")
+        if t.dim() not in (2, 3) or t.shape[-2] != T or t.shape[-1] not in (HEAD_DIM // 2, HEAD_DIM) or (
+                t.dim() == 3 and t.shape[0] not in (1, B)):
+            raise ValueError(f"{name} must be [T, C] or [1 or B, T, C] for T={T} tokens of B={B} rows, C {HEAD_DIM} or "
+                             f"{HEAD_DIM // 2}, got {tuple(t.shape)}")
+    if cos.shape != sin.shape or cos.dtype is not sin.dtype:
+        raise ValueError(f"cos {tuple(cos.shape)} {cos.dtype} and sin {tuple(sin.shape)} {sin.dtype} differ")
+    require_hip(q, "q")
+    for name, t in (("k", k), ("v", v), ("cos", cos), ("sin", sin)):
+        if t.device != q.device:
+            raise ValueError(f"q is on {q.device}, {name} on {t.device}")
+    _no_grad(q, k, v, cos, sin)
+
+
+def _table(t: torch.Tensor, dtype) -> Tuple[torch.Tensor, int, int]:
+    """A table as the kernel reads it, and its batch and token strides."""
+    if t.dtype is not dtype and t.dtype is not torch.float32:
+        t = t.to(torch.float32)
+    b, tok = (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else 0), (t.stride(-2) if t.shape[-2] > 1 else 0)
+    if t.stride(-1) != 1 or (b | tok) & 7 or t.data_ptr() & 15:
+        t = _fresh(t)
+        b, tok = (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else 0), t.stride(-2)
+    return t, b, tok
+
+
+def rotate_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                  interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """tp_rotate_tokens: ``q`` ``[B, H_q, T, 128]`` and ``k`` ``[B, H_kv, T, 128]`` turned by their positions and
+    ``v`` cast, each fp16: q token by token, k and v contiguous, as an append takes them.  q, k and v are float16,
+    bfloat16 or float32, any strides with contiguous rows (others are copied).
+
+    ``cos`` / ``sin``: ``[T, C]`` or ``[1 or B, T, C]``, as a model's rotary embedding gives them: C = 128, a column a
+    dimension, or 64, a column a pair; of q's type or float32 (others are taken in float32).  Pairs are (d, d + 64), or
+    (2d, 2d + 1) where ``interleaved``."""
+    _check_rotated(q, k, v, cos, sin)
+    B, H, T, _ = k.shape
+    k_out, v_out = (torch.empty((B, H, T, HEAD_DIM), dtype=torch.float16, device=q.device) for _ in range(2))
+    return _rotate_tokens(q, k, v, cos, sin, interleaved, k_out, v_out, 0), k_out, v_out
+
+
+def _rotate_tokens(q, k, v, cos, sin, interleaved, k_out, v_out, pos, flag=None, epoch=0) -> torch.Tensor:
+    """``rotate_tokens`` of checked inputs into rows ``[pos, pos + T)`` of ``k_out`` / ``v_out`` ``[B, H, tokens, 128]``
+    (contiguous fp16); with ``flag`` and ``epoch`` (as for an append) the call waits for the verdict and raises the
+    append's ValueError.  Returns q turned."""
+    B, Hq, T, _ = q.shape
+    dev, kind = q.device, _ROTATE_TYPES[q.dtype]
+    out = _token_major(B, Hq, T, torch.float16, dev)
+    if T == 0:
+        return out
+    (q, qs), (k, ks), (v, vs) = _strided(q), _strided(k), _strided(v)
+    (cos, *table), (sin, *other) = _table(cos, q.dtype), _table(sin, q.dtype)
+    if table != other:
+        cos, sin = _fresh(cos), _fresh(sin)
+        table = [cos.stride(0) if cos.dim() == 3 and cos.shape[0] > 1 else 0, cos.stride(-2)]
+    st = call_on(
+        dev, lib().tp_rotate_tokens, q.data_ptr(), k.data_ptr(), v.data_ptr(), kind, B, Hq, int(k.shape[1]), T,
+        _Strides9(*qs, *ks, *vs), cos.data_ptr(), sin.data_ptr(), _ROTATE_TYPES[cos.dtype], int(cos.shape[-1]),
+        _Strides2(*table), 1 if interleaved else 0, out.data_ptr(), _Strides3(T * Hq * HEAD_DIM, HEAD_DIM, Hq * HEAD_DIM),
+        k_out.data_ptr(), v_out.data_ptr(), int(k_out.shape[2]), pos, 0 if flag is None else 2, ptr(flag),
+        0 if flag is None else flag.numel(), epoch, stream_handle(dev),
+    )
+    if st == _lib.TP_ERR_NONFINITE:
+        raise ValueError("append() inputs must contain finite values")
+    check(st, "tp_rotate_tokens")
+    return out
+
+
+# --------------------------------------------------------------------------
+# shared prefixes
+# --------------------------------------------------------------------------
+
+_Strides4 = ctypes.c_int64 * 4
+
+
+def shared_attention(q: torch.Tensor, layout, num_kv_heads: int, prefix, own, scale: float) -> torch.Tensor:
+    """tp_shared_attention: ``q`` ``[B, H_q, 128]`` over a prefix that every row shares and each row's own tokens.
+    ``prefix`` and ``own`` are (store's descriptor or None, stored pages, dense tail of keys or None, of values): of
+    one batch row, and of B.  Returns fp16 ``[B, H_q, 128]``."""
+    q16 = _q16(q)
+    B, Hq, _ = q16.shape
+    dev = q16.device
+    parts, tails = [], []
+    for pages, n_pages, tail_k, tail_v in (prefix, own):
+        length = 0 if tail_k is None else int(tail_k.shape[2])
+        tk = tv = None
+        stride = 0
+        if length:
+            tk, tv, stride = _tail_pair(tail_k, tail_v)
+        tails += [tk, tv]
+        parts.append((ctypes.byref(pages if pages is not None else _NO_PAGES), n_pages if pages is not None else 0,
+                      ptr(tk), ptr(tv), length, stride))
+    out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.float16, device=dev)
+    L = lib()
+    ws = _scratch(int(L.tp_shared_workspace_bytes(B, Hq, num_kv_heads, ctypes.byref(layout), parts[0][1], parts[0][4],
+                                                  parts[1][1], parts[1][4])), dev)
+    st = call_on(
+        dev, L.tp_shared_attention, q16.data_ptr(), out.data_ptr(), B, Hq, num_kv_heads, ctypes.byref(layout), *parts[0],
+        *parts[1], _Strides4(Hq * HEAD_DIM, HEAD_DIM, Hq * HEAD_DIM, HEAD_DIM), float(scale), ptr(ws),
+        0 if ws is None else ws.numel(), stream_handle(dev),
+    )
+    check(st, "tp_shared_attention")
+    return out
+
+
+# --------------------------------------------------------------------------
+# selected pages
+# --------------------------------------------------------------------------
+
+def page_bounds_into(layout, pages: TPPages, bh: int, page_begin: int, n_pages: int, bounds: torch.Tensor) -> None:
+    """tp_page_bounds: pages [page_begin, page_begin + n_pages) of every (batch, head) row into their places of
+    ``bounds`` (fp16 ``[B, H, capacity, 2, 128]``, contiguous)."""
+    dev = bounds.device
+    st = call_on(dev, lib().tp_page_bounds, ctypes.byref(layout), ctypes.byref(pages), bh, page_begin, n_pages,
+                 ptr(bounds), int(bounds.shape[2]), stream_handle(dev))
+    check(st, "tp_page_bounds")
+
+
+def _bounds_view(bounds: torch.Tensor, B: int, H: int, S: int, device) -> Tuple[torch.Tensor, int]:
+    """``bounds`` ``[B, H, S, 2, 128]`` as the kernel reads them, and the pages between its rows."""
+    if not isinstance(bounds, torch.Tensor) or tuple(bounds.shape) != (B, H, S, 2, HEAD_DIM) or bounds.dtype is not torch.float16:
+        raise ValueError(f"bounds must be float16 [{B}, {H}, {S}, 2, {HEAD_DIM}], got "
+                         f"{getattr(bounds, 'dtype', None)} {tuple(getattr(bounds, 'shape', ()))}")
+    if bounds.device != device:
+        raise ValueError(f"q is on {device}, bounds on {bounds.device}")
+    cap = _head_stride_pages(bounds, 2 * HEAD_DIM)
+    if cap == -1 or not _inner_ok(bounds, (2, HEAD_DIM)) or (cap is not None and cap < S) or bounds.data_ptr() & 15:
+        bounds = _fresh(bounds)
+        bounds = bounds if bounds.is_contiguous() else bounds.contiguous()
+        cap = S
+    return bounds, S if cap is None else cap
+
+
+def check_selection(pages: int, first: int, last: int) -> None:
+    for name, x in (("pages", pages), ("first", first), ("last", last)):
+        if isinstance(x, bool) or not isinstance(x, int):
+            raise TypeError(f"{name} must be an int, got {type(x).__name__}")
+    if pages < 1 or first < 0 or last < 0 or first + last > pages:
+        raise ValueError(f"cannot select {pages} pages, the first {first} and the last {last} among them")
+
+
+def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """The split-K workspace of the stream; one of its own inside a captured graph, whose replays may run beside
+    those of another graph or eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return _Workspace.get(device, nbytes, stream)
+
+
+def selected_attention(q: torch.Tensor, layout, pages: TPPages, n_pages: int, num_kv_heads: int, bounds: torch.Tensor,
+                       tail_k: Optional[torch.Tensor], tail_v: Optional[torch.Tensor], scale: float, count: int,
+                       first: int, last: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """tp_select_pages and tp_selected_attention: ``q`` ``[B, H_q, 128]`` over ``count`` of the ``n_pages`` stored
+    pages, each kv head its own, and the dense tail (``[B, H_kv, < 64, 128]`` or None).  ``bounds``: fp16 ``[B, H_kv,
+    n_pages, 2, 128]``.  Returns fp16 ``[B, H_q, 128]`` and the pages, int32 ``[B, H_kv, count]``, ascending."""
+    q16 = _q16(q)
+    B, Hq, _ = q16.shape
+    dev = q16.device
+    bounds, cap = _bounds_view(bounds, B, num_kv_heads, n_pages, dev)
+    tail_len = 0 if tail_k is None else int(tail_k.shape[2])
+    tk = tv = None
+    tail_stride = 0
+    if tail_len:
+        tk, tv, tail_stride = _tail_pair(tail_k, tail_v)
+    out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.float16, device=dev)
+    selected = torch.empty((B, num_kv_heads, count), dtype=torch.int32, device=dev)
+    L, stream = lib(), stream_handle(dev)
+    scores = _scratch(8 * B * num_kv_heads * n_pages, dev)
+    st = call_on(dev, L.tp_select_pages, q16.data_ptr(), B, Hq, num_kv_heads, bounds.data_ptr(), cap, n_pages, first, last,
+                 count, float(scale), selected.data_ptr(), scores.data_ptr(), scores.numel(), stream)
+    check(st, "tp_select_pages")
+    ws = _zeroed_workspace(_workspace_bytes(B, Hq, num_kv_heads, count, 0), dev, stream)
+    st = call_on(
+        dev, L.tp_selected_attention, q16.data_ptr(), B, Hq, num_kv_heads, ctypes.byref(layout), ctypes.byref(pages),
+        n_pages, selected.data_ptr(), count, ptr(tk), ptr(tv), tail_len, tail_stride, float(scale), ws.data_ptr(),
+        ws.numel(), out.data_ptr(), stream,
+    )
+    check(st, "tp_selected_attention")
+    return out, selected
+
+
 def copy_pages(buffers, batch: int, heads: int, batch_in: int, rows: Optional[list], src_capacity: int,
                dst_capacity: int, n_stored: int, page_index: Optional[list], keep: int,
                tails: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]], tail_tokens: int,

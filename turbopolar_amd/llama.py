@@ -18,7 +18,9 @@ Mirrors the reference's mlx_lm hook (benchmarks/turbopolar_fast_attention.py:
   compressed pages) and everything else through the original forward.  With
   ``prompt_kernel=True`` prompts and chunks of them go through
   ``TurboPolarFastCache.prompt_attention``, which forms no scores in memory (the
-  model's mask is still compared with the causal one).
+  model's mask is still compared with the causal one).  With ``rotary_kernel=True``
+  both kinds of step turn their queries and keys by one launch (tp_rotate_tokens)
+  instead of the model's own rotation.
 * The cache protocol's ``crop``, ``reorder_cache``, ``batch_select_indices`` and
   ``batch_repeat_interleave`` (assisted generation and beams) truncate and
   re-order the compressed cache.
@@ -35,6 +37,7 @@ import torch
 
 from .config import TurboPolarConfig
 from .fast_attention import TurboPolarFastCache, make_turbo_caches
+from .kernels import rotate_tokens
 
 try:  # transformers is an optional dependency of this module only
     from transformers.cache_utils import Cache, CacheLayerMixin
@@ -209,6 +212,9 @@ def _turbo_llama_attention_forward(
         if not _is_standard_causal_mask(attention_mask, L, fast.offset + L):
             raise NotImplementedError("TurboPolar fused decode only supports standard causal full-history masks.")
         cos, sin = position_embeddings
+        if _rotary_kernel and not torch.is_grad_enabled():
+            out = fast.decode_rotated(q, k, v, cos, sin, self.scaling, defer_check=_model_wrapped())
+            return self.o_proj(out.to(hidden_states.dtype).reshape(B, L, -1)), None
         q, k = _llama.apply_rotary_pos_emb(q, k, cos, sin)
         # The append's non-finite verdict is read once per forward, for every
         # layer together, by the model-forward wrapper (no stream drain per layer).
@@ -223,8 +229,11 @@ def _turbo_llama_attention_forward(
             proj(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2)
             for proj in (self.q_proj, self.k_proj, self.v_proj)
         )
-        q, k = _llama.apply_rotary_pos_emb(q, k, *position_embeddings)
-        out = past_key_values.fast(self.layer_idx).prompt_attention(q, k, v, self.scaling)
+        if _rotary_kernel:
+            q, k, v = rotate_tokens(q, k, v, *position_embeddings)
+        else:
+            q, k = _llama.apply_rotary_pos_emb(q, k, *position_embeddings)
+        out = past_key_values.fast(self.layer_idx).prompt_attention(q, k, v, self.scaling).to(hidden_states.dtype)
         past_key_values.layers[self.layer_idx].is_initialized = True
         return self.o_proj(out.transpose(1, 2).reshape(B, L, -1)), None
     return _orig_llama_attention_forward(
@@ -233,6 +242,7 @@ def _turbo_llama_attention_forward(
 
 
 _prompt_kernel = False
+_rotary_kernel = False
 
 
 def _takes_prompt(attention, hidden_states, mask, fast, asked) -> bool:
@@ -273,15 +283,18 @@ def _turbo_llama_model_forward(self, *args, **kwargs):
     return out
 
 
-def patch_llama_attention(model=None, prompt_kernel: bool = False) -> None:
+def patch_llama_attention(model=None, prompt_kernel: bool = False, rotary_kernel: bool = False) -> None:
     """Route Llama decode steps on a ``TurboPolarCache`` through the fused kernel
     (turbopolar_fast_attention.py:283-290).  Patches the class, like the
     reference; ``model`` is accepted for the same signature.  LlamaModel.forward
     is wrapped too, to read the steps' non-finite verdicts once per forward.
     ``prompt_kernel``: steps of several tokens run tp_prompt_attention over the
-    decompressed history instead of the model's own attention."""
-    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel
-    _prompt_kernel = bool(prompt_kernel)
+    decompressed history instead of the model's own attention.  ``rotary_kernel``: the
+    steps that go through a kernel (outside of gradients) turn queries and keys by
+    tp_rotate_tokens, which rounds a result once where the model's rotation in half
+    precision rounds its products too."""
+    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel, _rotary_kernel
+    _prompt_kernel, _rotary_kernel = bool(prompt_kernel), bool(rotary_kernel)
     if _orig_llama_attention_forward is None:
         _orig_llama_attention_forward = _llama.LlamaAttention.forward
     _llama.LlamaAttention.forward = _turbo_llama_attention_forward
@@ -292,8 +305,8 @@ def patch_llama_attention(model=None, prompt_kernel: bool = False) -> None:
 
 def unpatch_llama_attention(model=None) -> None:
     """Restore the original forward (turbopolar_fast_attention.py:293-298)."""
-    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel
-    _prompt_kernel = False
+    global _orig_llama_attention_forward, _orig_llama_model_forward, _prompt_kernel, _rotary_kernel
+    _prompt_kernel = _rotary_kernel = False
     if _orig_llama_attention_forward is not None:
         _llama.LlamaAttention.forward = _orig_llama_attention_forward
         _orig_llama_attention_forward = None

@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import copy
 import ctypes
-from typing import Any, Dict, Optional, Sequence, Tuple
+from typing import Any, Dict, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -31,7 +31,8 @@ from . import _lib
 from .codecs import GroupedVQuantizer, PolarQuantDecoder, PolarQuantEncoder
 from .config import TurboPolarConfig
 from .kernels import (
-    PAGE, copy_pages, decode_pages_gather, decode_pages_into, decode_step, encode_pages, step_flag_words, take_tokens,
+    HEAD_DIM, PAGE, _check_rotated, _rotate_tokens, copy_pages, decode_pages_gather, decode_pages_into, decode_step,
+    encode_pages, page_bounds_into, rotate_tokens, step_flag_words, take_tokens,
 )
 from .payload import PolarKeyBlock, QuantizedVBlock
 from .storage import Growth, PolarKBlockStorage, QuantVBlockStorage, capacity_for, pages_of
@@ -39,6 +40,13 @@ from .storage import Growth, PolarKBlockStorage, QuantVBlockStorage, capacity_fo
 
 def _nbytes(x: torch.Tensor) -> int:
     return int(x.numel() * x.element_size())
+
+
+class _Form(NamedTuple):
+    """Shape and type of an input that is stored in another type than it comes in."""
+
+    shape: Tuple[int, ...]
+    dtype: torch.dtype
 
 
 def _whole(x, name: str) -> int:
@@ -97,6 +105,8 @@ class TurboPolarKVCacheRuntime:
         self._flag: Optional[torch.Tensor] = None  # the launches' verdicts (pinned host memory)
         self._fused_views = None  # (block_count, storage buffers, (PolarKeyBlock, QuantizedVBlock))
         self._scratch = None  # one-page store for the padded tail when the storage is full
+        self._bounds: Optional[torch.Tensor] = None  # key bounds of the stored pages, [B, H, capacity, 2, 128]
+        self._bounds_pages = 0  # of how many
         self._epoch = 0
         # Appends whose non-finite verdict is deferred (append(..., defer_check=True)):
         # (epoch, state before the append), oldest first.
@@ -312,6 +322,42 @@ class TurboPolarKVCacheRuntime:
             self._tail_k = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
             self._tail_v = torch.empty((B, H, PAGE, D), dtype=dtype, device=device)
 
+    def append_rotated(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
+        """Turns ``q`` ``[B, H_q, T, 128]`` and ``k_new`` ``[B, H_kv, T, 128]`` by their positions and appends the keys
+        and ``v_new`` in fp16 (``kernels.rotate_tokens``, whose arguments these are).  Tokens that leave the dense tail
+        at a page at most are turned, checked and written to it by one launch; others are turned into a buffer and
+        appended.  Returns fp16 ``[B, H_q, T, 128]``.  Errors are ``append``'s and leave the cache unchanged."""
+        _check_rotated(q, k_new, v_new, cos, sin)
+        if self._pending:
+            self.resolve_deferred_check()
+        B, H, T, D = k_new.shape
+        if T < 1:
+            raise ValueError(f"input must have at least one token, got T={T}")
+        as_stored = _Form(k_new.shape, torch.float16)
+        err = self._invariant_error(as_stored)
+        if err is not None:
+            raise err
+        if not self._initialized:
+            self._tail_k = self._tail_v = None  # what a refused first append left, as for append
+        if self._tail_k is not None and self._tail_k.device != k_new.device:
+            raise ValueError(f"append() inputs moved from {self._tail_k.device} to {k_new.device}")
+        if self._tail_len + T > PAGE:
+            q, k16, v16 = rotate_tokens(q, k_new, v_new, cos, sin, interleaved)
+            self.append(k16, v16)
+            return q
+        self._make_tail(B, H, D, torch.float16, k_new.device)
+        self._epoch = ((self._epoch + 2) & 0xFFFFFFFE) or 2
+        q = _rotate_tokens(q, k_new, v_new, cos, sin, interleaved, self._tail_k, self._tail_v, self._tail_len, self._flag,
+                           self._epoch)
+        self._commit_invariants(as_stored)
+        self.actual_seq_len += T
+        self._tail_len += T
+        if self._tail_len == PAGE:
+            self._encode_into_storage(self._tail_k, self._tail_v, 0, 1)
+            self._tail_len = 0
+        return q
+
     def append_and_attend(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, scale: float, pages,
                           layout, defer_check: bool = False) -> Optional[torch.Tensor]:
         """``append`` of one token and the decode attention of ``q`` ``[B, H_q,
@@ -426,6 +472,7 @@ class TurboPolarKVCacheRuntime:
         (self.actual_seq_len, self._tail_len, self.k_storage.block_count, self.v_storage.block_count,
          self.total_blocks, self.bytes_written) = self._pending[0][1]
         self._fused_views = None
+        self._bounds_pages = min(self._bounds_pages, self.k_storage.block_count)
         self._pending.clear()
 
     def _stage(self, k, v, begin: int, n: int, dst: int, check: int) -> None:
@@ -607,6 +654,31 @@ class TurboPolarKVCacheRuntime:
         self.bytes_read += per_page * len(idx)
         return k
 
+    def page_bounds(self) -> torch.Tensor:
+        """The smallest and the largest of each decoded key component over every stored page: fp16 ``[B, H, pages, 2,
+        128]``, a view valid until the next append.  Kept (512 bytes a page and head), so a call reads only the pages
+        stored since the last one (tp_page_bounds).  No counterpart in the reference."""
+        if self._pending:
+            self.resolve_deferred_check()
+        ks = self.k_storage
+        n, held = ks.block_count, self._bounds_pages
+        if n == 0:
+            raise ValueError("the cache holds no pages")
+        if held < n and ks.radii.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the bounds of new pages cannot be taken inside a captured graph; call page_bounds() before it")
+        B, H = self._batch_size, self._num_kv_heads
+        if self._bounds is None or self._bounds.shape[2] < n:
+            grown = torch.empty((B, H, ks.capacity, 2, HEAD_DIM), dtype=torch.float16, device=ks.radii.device)
+            if held:
+                grown[:, :, :held] = self._bounds[:, :, :held]
+                # Its memory may be another stream's: not used again before the copy has read it.
+                self._bounds.record_stream(torch.cuda.current_stream(self._bounds.device))
+            self._bounds = grown
+        if held < n:
+            page_bounds_into(self.polar_encoder.layout, pages_of(ks, self.v_storage), B * H, held, n - held, self._bounds)
+            self._bounds_pages = n
+        return self._bounds[:, :, :n]
+
     def get_io_telemetry(self) -> Dict[str, Any]:
         """turbo_polar_cache.py:348-377 (same keys and closed forms)."""
         if self.k_storage.block_count == 0 and not self._tail_len:
@@ -697,6 +769,7 @@ class TurboPolarKVCacheRuntime:
             self.total_blocks = max(0, self.total_blocks - (S - pages))
             self.bytes_written = max(0, self.bytes_written - (S - pages) * self._page_bytes())
             self._fused_views = None
+            self._bounds_pages = min(self._bounds_pages, pages)
         self._tail_len = left
         self.actual_seq_len = tokens
 
@@ -795,7 +868,7 @@ class TurboPolarKVCacheRuntime:
         # The buffers replaced here were just read on the current stream, which need not be theirs: the
         # allocator hands their memory out again only after that copy.
         ks, vs = self.k_storage, self.v_storage
-        for t in (*ks._buffers(), vs.codes, vs.scales, self._tail_k, self._tail_v):
+        for t in (*ks._buffers(), vs.codes, vs.scales, self._tail_k, self._tail_v, self._bounds):
             if t is not None and t.is_cuda:
                 t.record_stream(torch.cuda.current_stream(t.device))
         read, spent = self.bytes_read, self.compression_time_ns
@@ -828,6 +901,8 @@ class TurboPolarKVCacheRuntime:
         self._tail_len = 0
         self._scratch = None
         self._fused_views = None
+        self._bounds = None
+        self._bounds_pages = 0
         self._pending = []
         self._initialized = False
         self._batch_size = None
