@@ -82,13 +82,12 @@ __device__ __forceinline__ float2v angle_pair(uint32_t code, int bits) {
 // A pair's key, r (cos a, sin a), each rounded once.
 __device__ __forceinline__ uint32_t key_pair(float r, float2v cs) { return F16::pack(r * cs.x, r * cs.y); }
 
-// Decodes half h of run n into a tile of keys: 4 pairs, 16 bytes.
+// Half h of run n, 4 pairs: their codes' (cos, sin) out of the table, and the keys, 16 bytes, into a tile.  Between
+// the two other work may go on, so that it does not wait for the table.
 template <int KIND, int N, int THREADS, class Pages>
-__device__ __forceinline__ void decode_keys(const Pages& a, const TreeLut& lut, const uint32_t* codes, int tid,
-                                            const PageRegs<KIND, N>& p, int n, int h, char* kt) {
+__device__ __forceinline__ void fetch_angles(const Pages& a, const TreeLut& lut, const uint32_t* codes, int tid,
+                                             const PageRegs<KIND, N>& p, int n, int h, float2v* cs) {
   const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
-  uint32_t e[4];
-  const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;  // rounded in fp32, as its products below
   int c0 = c;  // where a pair's code lies is computed anew: kept over the pages, it costs 30 registers
   if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
 #pragma unroll
@@ -107,14 +106,34 @@ __device__ __forceinline__ void decode_keys(const Pages& a, const TreeLut& lut, 
       const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
       code = (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
     }
+    cs[i] = lut.code[code];
+  }
+}
+
+template <int KIND, int N, int THREADS>
+__device__ __forceinline__ void store_keys(int tid, const PageRegs<KIND, N>& p, int n, int h, const float2v* cs,
+                                           char* kt) {
+  const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
+  const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;  // rounded in fp32, as its products below
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     float r;
     if constexpr (tree_i8(KIND))
       r = __builtin_amdgcn_exp2f((float)(int)(int8_t)(p.r8[n][h] >> (8 * i)) * ls);
     else
       r = h2f((uint16_t)(p.r[n][2 * h + (i >> 1)] >> (16 * (i & 1))));
-    e[i] = key_pair(r, lut.code[code]);
+    e[i] = key_pair(r, cs[i]);
   }
   *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + h)) = uint4v{e[0], e[1], e[2], e[3]};
+}
+
+template <int KIND, int N, int THREADS, class Pages>
+__device__ __forceinline__ void decode_keys(const Pages& a, const TreeLut& lut, const uint32_t* codes, int tid,
+                                            const PageRegs<KIND, N>& p, int n, int h, char* kt) {
+  float2v cs[4];
+  fetch_angles<KIND, N, THREADS>(a, lut, codes, tid, p, n, h, cs);
+  store_keys<KIND, N, THREADS>(tid, p, n, h, cs, kt);
 }
 
 // And into a tile of values: 8 codes.

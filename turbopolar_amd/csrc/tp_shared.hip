@@ -76,7 +76,10 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
   PageRegs<KIND, N> p;
   if (page < page_end) load_page<KIND, N, THREADS>(src, slot0 + page, tid, p);
 
-  const int rw = wave / TW, tw = wave % TW;
+  // Own rows fill a wave or two of the workgroup's; which ones goes round, so that those of neighbours lie on
+  // different SIMDs, and the others only decode.
+  const int tw = wave % TW, rw = (wave / TW + (own ? index : 0)) & (RW - 1);
+  const bool busy = (block * RW + rw) * kWaveRows < src.rows;
   const int row = (block * RW + rw) * kWaveRows + (lane & 31);
   const bool live = row < src.rows;
   const int at_row = min(row, src.rows - 1);  // loads of rows past the last repeat it
@@ -94,7 +97,7 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
   if (tid == 0) flag = 0;
   if (page < page_end) {
     build_tree_lut<KIND, THREADS>(src, lut, tid);
-    __syncthreads();
+    lds_barrier();
     float16v s[NB];
     if constexpr (BUFS == 1) {
       static_assert(!tree_any(KIND), "any layout's codes are staged in the other form");
@@ -102,18 +105,18 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i)
           decode_piece<KIND, N, THREADS>(src, lut, codes[0], tid, p, i, tiles[0][0], tiles[0][1]);
-        __syncthreads();
+        lds_barrier();
         // The last page again rather than none: a load under a branch is waited for at its join.
         load_page<KIND, N, THREADS>(src, slot0 + min(page + 1, page_end - 1), tid, p);
         score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s, [](int) {});
         finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, st);
-        __syncthreads();
+        lds_barrier();
       }
     } else {
       // The next page is decoded under this one's first products.
       if constexpr (tree_any(KIND)) {
         stage_rows<KIND, N, THREADS>(tid, p, codes[0]);
-        __syncthreads();
+        lds_barrier();
       }
 #pragma unroll
       for (int i = 0; i < 4 * N; ++i)
@@ -123,15 +126,23 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
         char *kt = tiles[buf ^ 1][0], *vt = tiles[buf ^ 1][1];
         const uint32_t* rows_of = codes[tree_any(KIND) ? buf ^ 1 : 0];
         stage_rows<KIND, N, THREADS>(tid, p, codes[tree_any(KIND) ? buf ^ 1 : 0]);
-        __syncthreads();
-        score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s, [&](int i) {
-          constexpr int kProducts = 8 * NB, kPieces = 4 * N;
+        lds_barrier();
+        if (busy) {
+          // Of each key piece the table is read, a piece of values decoded, and the keys then.
+          constexpr int kSlots = 8 * NB / (2 * N);
+          float2v cs[4];
+          score_tile<F16, NB>(tiles[buf][0], 32 * tw, at, qs, s, [&](int i) {
+            const int piece = i / kSlots, at_slot = i % kSlots, n = piece >> 1, h = piece & 1;
+            if (at_slot == 0) fetch_angles<KIND, N, THREADS>(src, lut, rows_of, tid, p, n, h, cs);
+            if (at_slot == kSlots / 2) decode_values<KIND, N, THREADS>(tid, p, n, h, vt);
+            if (at_slot == kSlots - 1) store_keys<KIND, N, THREADS>(tid, p, n, h, cs, kt);
+          });
+        } else {
 #pragma unroll
-          for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x)
-            decode_piece<KIND, N, THREADS>(src, lut, rows_of, tid, p, x, kt, vt);
-        });
+          for (int i = 0; i < 4 * N; ++i) decode_piece<KIND, N, THREADS>(src, lut, rows_of, tid, p, i, kt, vt);
+        }
         load_page<KIND, N, THREADS>(src, slot0 + min(page + 2, page_end - 1), tid, p);
-        finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, st);
+        if (busy) finish_tile<F16, NB>(tiles[buf][1], 32 * tw, at, a.c, s, st);
       }
     }
   }
@@ -139,19 +150,21 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
     const int count = src.tail_len;
     const uint16_t* k = src.tail_k + unit * src.tail_stride * kHeadDim;
     const uint16_t* v = src.tail_v + unit * src.tail_stride * kHeadDim;
-    __syncthreads();  // the tile before is read
+    lds_barrier();  // the tile before is read
     if (dense_tile<THREADS>(k, v, kHeadDim, kHeadDim, count, tid, tiles[0][0], tiles[0][1])) flag = 1;
-    __syncthreads();
-    float16v s[NB];
-    score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s, [](int) {});
-    mask_scores<NB>(s, count - 32 * tw - 4 * (lane >> 5));
-    finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, st);
-    if (flag)
-      add_nonfinite<F16>(st, lane, count, [&](int x) { return TW == 1 || (x >> 5) == tw; },
-                         [&](int x) { return v + x * kHeadDim; });
+    lds_barrier();
+    if (busy) {
+      float16v s[NB];
+      score_tile<F16, NB>(tiles[0][0], 32 * tw, at, qs, s, [](int) {});
+      mask_scores<NB>(s, count - 32 * tw - 4 * (lane >> 5));
+      finish_tile<F16, NB>(tiles[0][1], 32 * tw, at, a.c, s, st);
+      if (flag)
+        add_nonfinite<F16>(st, lane, count, [&](int x) { return TW == 1 || (x >> 5) == tw; },
+                           [&](int x) { return v + x * kHeadDim; });
+    }
   }
   if constexpr (TW == 2) {  // the second half's rows join the first's
-    __syncthreads();
+    lds_barrier();
     static_assert(RW * 64 * 64 * sizeof(float) <= sizeof(tiles), "the second half's rows lie over the tiles");
     float* side = reinterpret_cast<float*>(&tiles[0][0][0]) + rw * 64 * 64 + lane;
     if (tw == 1) {
@@ -162,7 +175,7 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
       side_ml[rw][0][lane] = st.m;
       side_ml[rw][1][lane] = st.l;
     }
-    __syncthreads();
+    lds_barrier();
     if (tw == 0) {
       const float m1 = side_ml[rw][0][lane], l1 = side_ml[rw][1][lane];
       const float m = fmaxf(st.m, m1), base = m == -INFINITY ? 0.0f : m;
@@ -185,9 +198,10 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
   }
 }
 
-// Rows of a workgroup by the prefix's rows, as the drafted-tree kernel takes them (see plan_tree), and the
-// tiles of a split: as few as let every workgroup, the prefix's and the rows' own, be on the GPU at once.
-constexpr int kSharedTarget = 2048;  // waves that fill the GPU, two a SIMD
+// Rows of a workgroup by the prefix's rows, as the drafted-tree kernel takes them (see plan_tree), and the tiles of
+// a split.
+constexpr int kSharedWaves = 2048;  // that fill the GPU, two a SIMD
+constexpr int kSharedCus = 256;
 
 struct SharedPlan {
   int32_t row_waves, tiles_per_split;
@@ -197,24 +211,32 @@ static SharedPlan plan_shared(int64_t batch, int32_t hkv, int32_t g, int64_t pre
   SharedPlan p;
   const int64_t rows[2] = {prefix_tiles ? batch * g : g, g};
   p.row_waves = rows[0] <= 32 && !any ? 1 : rows[0] <= 64 ? 2 : rows[0] <= 128 ? 4 : 8;
-  const int64_t target = kSharedTarget / (p.row_waves == 8 || (p.row_waves == 4 && any) ? 8 : p.row_waves == 1 ? 2 : 4);
+  const int64_t slots = kSharedWaves / (p.row_waves == 8 || (p.row_waves == 4 && any) ? 8 : p.row_waves == 1 ? 2 : 4);
   const int64_t units[2] = {hkv, batch * hkv}, tiles[2] = {prefix_tiles, own_tiles};
   int64_t total = 0;
   for (int i = 0; i < 2; ++i) {
     p.row_blocks[i] = (rows[i] + p.row_waves * kWaveRows - 1) / (p.row_waves * kWaveRows);
     total += units[i] * p.row_blocks[i] * tiles[i];
   }
-  int64_t each = std::max<int64_t>(1, (total + target - 1) / target);
-  const int64_t most = std::max(prefix_tiles, own_tiles);
-  for (;; ++each) {
-    int64_t groups = 0;
+  // In tiles: what a CU is dealt (workgroups go round the CUs, and two on one CU take twice as long: 32,805 tokens
+  // for 32 rows of 32/8 heads, 17 tiles each on 248 CUs 38.6 us, 9 on 456 places 39.1), four to start and end each
+  // round of workgroups (6 us), and the join's records at 3 TB/s.
+  const int64_t even = (total + kSharedCus - 1) / kSharedCus;
+  const int64_t step = std::max<int64_t>(1, even / 16);
+  double best = INFINITY;
+  for (int64_t each = std::max<int64_t>(1, even / 4); each <= 2 * even + 2; each += step) {
+    int64_t dealt = 0, groups = 0, records = 0;
     for (int i = 0; i < 2; ++i) {
-      p.records[i] = (tiles[i] + each - 1) / each;
-      groups += units[i] * p.row_blocks[i] * p.records[i];
+      const int64_t splits = (tiles[i] + each - 1) / each, n = units[i] * p.row_blocks[i] * splits;
+      dealt += (n + kSharedCus - 1) / kSharedCus * std::min(each, tiles[i]);
+      groups += n;
+      records += splits;
     }
-    if (groups <= target || each >= most) break;
+    const double cost = (double)dealt + 4.0 * (double)((groups + slots - 1) / slots) +
+                        (double)(batch * hkv * g * records) * (272.0 / 3.0e6 / 1.6);
+    if (cost < best) best = cost, p.tiles_per_split = (int32_t)each;
   }
-  p.tiles_per_split = (int32_t)each;
+  for (int i = 0; i < 2; ++i) p.records[i] = (tiles[i] + p.tiles_per_split - 1) / p.tiles_per_split;
   return p;
 }
 
