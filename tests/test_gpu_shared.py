@@ -213,3 +213,11 @@ def test_rotated_queries_feed_attention(device):
     q16 = cache.append_rotated(q, k, v, cos, sin)
     assert torch.equal(q16, want[0])
     check(cache.attention(q16, 0.1), q16, cache, 0.1, "rotated")
+
+
+@pytest.mark.parametrize("layout", ["default", "odd_split"])
+def test_own_tokens_by_a_launch_of_their_own(device, layout):
+    """More tiles of own tokens than go along with the prefix's, and a prefix of more rows than four waves hold."""
+    for B, hq, hkv, prefix, own in ((12, 32, 8, 70, 64 * 65), (33, 8, 1, 130, 200), (40, 16, 4, 64, 70)):
+        cache, q = made(device, layout, B, hq, hkv, prefix, own, seed=B)
+        check(cache.attention(q, 0.09), q, cache, 0.09, f"{layout} {B} {hq} {hkv} {prefix} {own}")

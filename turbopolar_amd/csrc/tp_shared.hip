@@ -5,9 +5,9 @@
 // over the tokens of the prefix (one cache, stored once) and those of row b's own cache.  The softmax of a
 // union is joined from the softmaxes of its parts, (m, l, o) each, so the prefix is attended by every row of
 // the batch together: its rows are the (sequence, head of the group) pairs of one kv head, up to 256 of them
-// for one read and one decode of a page.  A row's own pages are attended by its own heads.  Both go on in
-// one launch, split into runs of tiles (a page, or the dense tail) such that the workgroups fill the GPU once;
-// a second one joins the records.
+// for one read and one decode of a page.  A row's own pages are attended by its own heads.  Both are split into
+// runs of tiles (a page, or the dense tail) and go on in one launch, or one each (plan_shared); a last one joins
+// the records.
 #include <algorithm>
 
 #include "tp_page_tiles.h"
@@ -31,7 +31,7 @@ struct SharedPart {
   int32_t units;       // hkv, or batch * hkv
   int32_t rows;        // batch * g, or g
   int32_t row_blocks;  // of the workgroup's rows
-  int32_t records, first_record;
+  int32_t tiles_per_split, records, first_record;
   FastDiv div_units, div_blocks;
 };
 
@@ -42,8 +42,8 @@ struct SharedArgs {
   int32_t hkv, g, batch;
   FastDiv div_hkv, div_g;
   SharedPart part[2];  // the prefix, the rows' own
-  int32_t prefix_groups;
-  int32_t tiles_per_split, records;
+  int32_t prefix_groups;  // workgroups over the prefix, the launch's first
+  int32_t records;
   float c;
   uint32_t flip;
   uint16_t* part_o;
@@ -71,8 +71,8 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
   const int rest = fast_div(index, src.div_units), unit = index - rest * src.units;
   const int split = fast_div(rest, src.div_blocks), block = rest - split * src.row_blocks;
   const int64_t slot0 = (int64_t)unit * src.capacity;
-  int page = split * a.tiles_per_split;
-  const int page_end = min(page + a.tiles_per_split, src.n_pages);
+  int page = split * src.tiles_per_split;
+  const int page_end = min(page + src.tiles_per_split, src.n_pages);
   PageRegs<KIND, N> p;
   if (page < page_end) load_page<KIND, N, THREADS>(src, slot0 + page, tid, p);
 
@@ -198,45 +198,72 @@ __global__ __launch_bounds__((kSharedThreads<RW, TW>), 2) void shared_attention_
   }
 }
 
-// Rows of a workgroup by the prefix's rows, as the drafted-tree kernel takes them (see plan_tree), and the tiles of
-// a split.
 constexpr int kSharedWaves = 2048;  // that fill the GPU, two a SIMD
 constexpr int kSharedCus = 256;
 
 struct SharedPlan {
-  int32_t row_waves, tiles_per_split;
-  int64_t row_blocks[2], records[2];
+  int32_t row_waves[2];
+  int64_t tiles[2], row_blocks[2], tiles_per_split[2], records[2];
+  bool apart;  // a launch for either part
 };
-static SharedPlan plan_shared(int64_t batch, int32_t hkv, int32_t g, int64_t prefix_tiles, int64_t own_tiles, bool any) {
-  SharedPlan p;
-  const int64_t rows[2] = {prefix_tiles ? batch * g : g, g};
-  p.row_waves = rows[0] <= 32 && !any ? 1 : rows[0] <= 64 ? 2 : rows[0] <= 128 ? 4 : 8;
-  const int64_t slots = kSharedWaves / (p.row_waves == 8 || (p.row_waves == 4 && any) ? 8 : p.row_waves == 1 ? 2 : 4);
-  const int64_t units[2] = {hkv, batch * hkv}, tiles[2] = {prefix_tiles, own_tiles};
+
+// Splits of parts [begin, end), which are one launch.
+static void plan_splits(SharedPlan& p, const int64_t* units, int64_t rows, int begin, int end, bool any) {
+  const int rw = p.row_waves[begin];
+  const int64_t slots = kSharedWaves / (rw == 8 || (rw == 4 && any) ? 8 : rw == 1 ? 2 : 4);
   int64_t total = 0;
-  for (int i = 0; i < 2; ++i) {
-    p.row_blocks[i] = (rows[i] + p.row_waves * kWaveRows - 1) / (p.row_waves * kWaveRows);
-    total += units[i] * p.row_blocks[i] * tiles[i];
-  }
-  // In tiles: what a CU is dealt (workgroups go round the CUs, and two on one CU take twice as long: 32,805 tokens
-  // for 32 rows of 32/8 heads, 17 tiles each on 248 CUs 38.6 us, 9 on 456 places 39.1), four to start and end each
-  // round of workgroups (6 us), and the join's records at 3 TB/s.
+  for (int i = begin; i < end; ++i) total += units[i] * p.row_blocks[i] * p.tiles[i];
+  // In tiles of 1.7 us: a CU works on those it is dealt (workgroups go round the CUs) hardly faster for being two
+  // (32,805 tokens for 32 rows of 32/8 heads, 17 tiles each on 248 CUs 38.7 us, 9 on 456 places 42.0), small
+  // workgroups rather so (512 of two waves, 4 tiles each 16.8 us, 1,024 of 2 tiles 13.9); a round of workgroups
+  // starts and ends in 6 us; the records are written and read at 3 TB/s.
+  const double shared = rw == 1 ? 0.33 : 0.8, alone = rw == 1 ? 0.75 : 0.2;
   const int64_t even = (total + kSharedCus - 1) / kSharedCus;
   const int64_t step = std::max<int64_t>(1, even / 16);
   double best = INFINITY;
+  int64_t chosen = 1;
   for (int64_t each = std::max<int64_t>(1, even / 4); each <= 2 * even + 2; each += step) {
-    int64_t dealt = 0, groups = 0, records = 0;
-    for (int i = 0; i < 2; ++i) {
-      const int64_t splits = (tiles[i] + each - 1) / each, n = units[i] * p.row_blocks[i] * splits;
-      dealt += (n + kSharedCus - 1) / kSharedCus * std::min(each, tiles[i]);
+    int64_t dealt = 0, groups = 0, records = 0, longest = 0;
+    for (int i = begin; i < end; ++i) {
+      const int64_t splits = (p.tiles[i] + each - 1) / each, n = units[i] * p.row_blocks[i] * splits;
+      dealt += (n + kSharedCus - 1) / kSharedCus * std::min(each, p.tiles[i]);
+      longest = std::max(longest, std::min(each, p.tiles[i]));
       groups += n;
       records += splits;
     }
-    const double cost = (double)dealt + 4.0 * (double)((groups + slots - 1) / slots) +
-                        (double)(batch * hkv * g * records) * (272.0 / 3.0e6 / 1.6);
-    if (cost < best) best = cost, p.tiles_per_split = (int32_t)each;
+    const double cost = shared * (double)dealt + alone * (double)longest + 3.5 * (double)((groups + slots - 1) / slots) +
+                        (double)(rows * records) * (2.0 * 264.0 / 3.0e6 / 1.7);
+    if (cost < best) best = cost, chosen = each;
   }
-  for (int i = 0; i < 2; ++i) p.records[i] = (tiles[i] + p.tiles_per_split - 1) / p.tiles_per_split;
+  for (int i = begin; i < end; ++i) {
+    p.tiles_per_split[i] = chosen;
+    p.records[i] = (p.tiles[i] + chosen - 1) / chosen;
+  }
+}
+
+// Rows of a workgroup by the prefix's rows, as the drafted-tree kernel takes them (see plan_tree).  The rows' own
+// tokens go along in workgroups of that size, of which one wave multiplies, or get a launch of workgroups of their
+// size: where the prefix's have eight waves (us, one launch and two: 64 sequences of 32/8 heads, 1,000 tokens behind
+// 16,000, 77 and 59; of 64/8 heads, 200 behind 4,000, 38 both), or where they are more than 24 tiles a CU (32
+// sequences of 32/8 heads behind 16,000, 1,000 tokens each 41 and 42, 2,000 56 and 53, 4,000 92 and 81).
+static SharedPlan plan_shared(int64_t batch, int32_t hkv, int32_t g, int64_t prefix_tiles, int64_t own_tiles, bool any) {
+  SharedPlan p;
+  auto waves_for = [&](int64_t rows) { return rows <= 32 && !any ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; };
+  const int64_t units[2] = {hkv, batch * hkv}, rows[2] = {batch * g, g};
+  p.tiles[0] = prefix_tiles, p.tiles[1] = own_tiles;
+  p.row_waves[0] = p.row_waves[1] = waves_for(prefix_tiles ? rows[0] : rows[1]);
+  p.apart = prefix_tiles && own_tiles &&
+            (p.row_waves[0] == 8 || (p.row_waves[0] == 4 && any) ||
+             (p.row_waves[0] != waves_for(rows[1]) && units[1] * own_tiles > 24 * kSharedCus));
+  if (p.apart) p.row_waves[1] = waves_for(rows[1]);
+  for (int i = 0; i < 2; ++i)
+    p.row_blocks[i] = (rows[i] + p.row_waves[i] * kWaveRows - 1) / (p.row_waves[i] * kWaveRows);
+  if (p.apart) {
+    plan_splits(p, units, batch * hkv * g, 0, 1, any);
+    plan_splits(p, units, batch * hkv * g, 1, 2, any);
+  } else {
+    plan_splits(p, units, batch * hkv * g, 0, 2, any);
+  }
   return p;
 }
 
@@ -369,7 +396,7 @@ extern "C" int32_t tp_shared_attention(const void* q, void* out, int64_t batch, 
     SharedPart& x = a.part[i];
     groups[i] = units[i] * p.row_blocks[i] * p.records[i];
     x.units = (int32_t)units[i], x.rows = (int32_t)rows[i], x.row_blocks = (int32_t)p.row_blocks[i];
-    x.records = (int32_t)p.records[i];
+    x.tiles_per_split = (int32_t)p.tiles_per_split[i], x.records = (int32_t)p.records[i];
     x.div_units = make_fastdiv((uint32_t)units[i]), x.div_blocks = make_fastdiv((uint32_t)p.row_blocks[i]);
   }
   a.part[1].first_record = (int32_t)p.records[0];
@@ -382,8 +409,6 @@ extern "C" int32_t tp_shared_attention(const void* q, void* out, int64_t batch, 
   a.q_b = strides[0], a.q_h = strides[1], a.out_b = strides[2], a.out_h = strides[3];
   a.hkv = hkv, a.g = g, a.batch = (int32_t)batch;
   a.div_hkv = make_fastdiv((uint32_t)hkv), a.div_g = make_fastdiv((uint32_t)g);
-  a.prefix_groups = (int32_t)groups[0];
-  a.tiles_per_split = p.tiles_per_split;
   a.records = (int32_t)(p.records[0] + p.records[1]);
   a.c = std::max(fabsf(scale) * kLog2e, 1.17549435e-38f);  // 2^-126 stands for 0: see tp_prompt_attention
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
@@ -397,15 +422,18 @@ extern "C" int32_t tp_shared_attention(const void* q, void* out, int64_t batch, 
     a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)batch * hq * a.records * kHeadDim);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(groups[0] + groups[1]));
-  if (def)
-    launch_shared<kTreeDefault>(a, p.row_waves, grid, s);
-  else if (fast)
-    launch_shared<kTreeFast>(a, p.row_waves, grid, s);
-  else if (layout->int8_radii)
-    launch_shared<kTreeAnyI8>(a, p.row_waves, grid, s);
-  else
-    launch_shared<kTreeAnyF16>(a, p.row_waves, grid, s);
+  for (int i = 0; i < (p.apart ? 2 : 1); ++i) {
+    a.prefix_groups = i == 0 ? (int32_t)groups[0] : 0;
+    const dim3 grid((unsigned)(p.apart ? groups[i] : groups[0] + groups[1]));
+    if (def)
+      launch_shared<kTreeDefault>(a, p.row_waves[i], grid, s);
+    else if (fast)
+      launch_shared<kTreeFast>(a, p.row_waves[i], grid, s);
+    else if (layout->int8_radii)
+      launch_shared<kTreeAnyI8>(a, p.row_waves[i], grid, s);
+    else
+      launch_shared<kTreeAnyF16>(a, p.row_waves[i], grid, s);
+  }
   const int32_t st = launch_status("tp_shared_attention");
   if (st != TP_OK || a.records == 1) return st;
   JoinArgs j{};
