@@ -489,13 +489,14 @@ int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* pages, int6
  * the n_pages pages and those of the others with the largest scores, ties to the lower index.  Scores are fp64 sums
  * of exact products; one that is NaN counts as infinite.
  * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages.
- * workspace (tp_select_workspace_bytes) as for tp_prompt_attention.
+ * workspace: tp_select_workspace_bytes(...) bytes, 256-byte aligned, with the counter area of tp_decode_attention's
+ * (zero before and after a call), so that one workspace serves both.
  */
 int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int32_t hkv, const void* bounds,
                         int64_t bounds_capacity, int32_t n_pages, int32_t first, int32_t last, int32_t count,
                         float scale, int32_t* selected, void* workspace, size_t workspace_bytes, void* stream);
 
-size_t tp_select_workspace_bytes(int64_t batch, int32_t hkv, int32_t n_pages);
+size_t tp_select_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t n_pages);
 
 /*
  * tp_decode_attention over `count` of the n_pages stored pages, each (batch, kv head) its own (selected: device

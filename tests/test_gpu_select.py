@@ -14,7 +14,7 @@ from common import ATOL, LAYOUTS, PAGE, RTOL_L2, gen_kv, rel_l2, within_f16_ulp
 from test_gpu_rotate import draw, tables
 from test_gpu_tree import filled, pages64
 from turbopolar_amd import HipKernelBridge, TurboPolarConfig, TurboPolarFastCache
-from turbopolar_amd.kernels import fp16_scale, selected_attention
+from turbopolar_amd.kernels import fp16_scale, selected_attention, tail_args
 
 pytestmark = pytest.mark.gpu
 
@@ -192,8 +192,9 @@ def test_negative_scales_and_bounds_that_are_not_finite(device):
     q = queries(device, 1, 8, 4)
     bounds = cache.runtime.page_bounds()
     rt, lay = cache.runtime, cache.runtime.polar_encoder.layout
-    tail = rt._tail_views()
-    out, selected = selected_attention(q, lay, cache._store_pages(), 30, 2, bounds, *tail, -0.1, 6, 1, 1)
+    tail = tail_args(rt._tail_k, rt._tail_v, rt._tail_len)
+    out, selected = selected_attention(q, lay, cache._store_pages(), 30, 2, bounds, int(rt._bounds.shape[2]), tail, -0.1, 6,
+                                       1, 1)
     want = chosen64(scores64(q, bounds, -1)[0], 6, 1, 1)
     assert np.array_equal(selected.cpu().numpy(), want)
     close(out, attended(q, cache, want, np.float64(np.float32(-0.1))), "negative scale")

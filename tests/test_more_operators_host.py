@@ -100,7 +100,7 @@ def test_shared_layout_and_workspace():
 
 
 def select(**kw):
-    a = dict(q=P, batch=1, hq=4, hkv=2, bounds=P, cap=8, n=8, first=1, last=1, count=4, scale=0.1, out=P, ws=P, wsb=128)
+    a = dict(q=P, batch=1, hq=4, hkv=2, bounds=P, cap=8, n=8, first=1, last=1, count=4, scale=0.1, out=P, ws=P, wsb=65536 + 128)
     a.update(kw)
     st = _lib.lib().tp_select_pages(a["q"], a["batch"], a["hq"], a["hkv"], a["bounds"], a["cap"], a["n"], a["first"],
                                     a["last"], a["count"], a["scale"], a["out"], a["ws"], a["wsb"], None)
@@ -120,9 +120,9 @@ def test_select_refusals(change, message):
 
 
 def test_select_workspace():
-    assert select(wsb=127)[0] == select(ws=None)[0] == select(ws=P + 8)[0] == _lib.TP_ERR_WORKSPACE
+    assert select(wsb=65536 + 127)[0] == select(ws=None)[0] == select(ws=P + 8)[0] == _lib.TP_ERR_WORKSPACE
     size = _lib.lib().tp_select_workspace_bytes
-    assert size(1, 2, 8) == 128 and size(0, 2, 8) == 0 and size(3, 5, 100) == 12000
+    assert size(1, 4, 2, 8) == 65536 + 128 and size(0, 4, 2, 8) == 0 and size(3, 10, 5, 100) == 65536 + 12000
 
 
 def test_bounds_refusals():

@@ -214,7 +214,7 @@ _SIGNATURES = {
         c_i32,
         [c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_float, c_vp, c_vp, c_size, c_vp],
     ),
-    "tp_select_workspace_bytes": (c_size, [c_i64, c_i32, c_i32]),
+    "tp_select_workspace_bytes": (c_size, [c_i64, c_i32, c_i32, c_i32]),
     "tp_selected_attention": (
         c_i32,
         [

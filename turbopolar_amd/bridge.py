@@ -37,8 +37,8 @@ import torch
 from . import _lib
 from .draft import DraftTree
 from .kernels import (
-    HEAD_DIM, PageSet, _DEFAULT_LAYOUT, _no_grad, check_selection, decode_attention, decode_attention_dense_v, fp16_scale,
-    fused_qk, page_bounds_into, prompt_attention, selected_attention, tree_attention,
+    HEAD_DIM, PageSet, _DEFAULT_LAYOUT, _bounds_view, _no_grad, _tail_pair, check_selection, decode_attention,
+    decode_attention_dense_v, fp16_scale, fused_qk, page_bounds_into, prompt_attention, selected_attention, tree_attention,
 )
 from .payload import PolarKeyBlock, QuantizedVBlock, layout_from_metadata
 from .qjl import QJLPages
@@ -331,9 +331,13 @@ class HipKernelBridge:
         count = min(pages, held.S)
         if count < pages:  # every page: none needs a place of its own
             first = last = 0
-        out, selected = selected_attention(q, held.layout, held.pages, held.S, held.H, bounds, tail_k if tail_len else None,
-                                           tail_v if tail_len else None, fp16_scale(config.attention_scale), count, first,
-                                           last)
+        tail = (None, None, 0, 0)
+        if tail_len:
+            tk, tv, stride = _tail_pair(tail_k, tail_v)
+            tail = tk, tv, tail_len, stride
+        bounds, capacity = _bounds_view(bounds, held.B, held.H, held.S, dev)
+        out, selected = selected_attention(q, held.layout, held.pages, held.S, held.H, bounds, capacity, tail,
+                                           fp16_scale(config.attention_scale), count, first, last)
         trace = {
             "kernel_name": "selected_attention_quant_v_dense_tail",
             "hip_kernel": "tp_selected_attention",

@@ -218,6 +218,45 @@ __device__ __forceinline__ void build_lut(Lut& lut, const AttnArgs& a, int tid) 
   }
 }
 
+// What the fp16 tables leave of the cosines and sines, for keys in two parts (split_pair).
+struct LutRest {
+  uint32_t code[512];
+  uint2 pair[256];
+};
+
+__device__ __forceinline__ uint32_t make_cs_rest(uint32_t code, int bits) {
+  const float th = code_angle(code, bits), c = cosf(th), s = sinf(th);
+  const half2v cs = {(f16)c, (f16)s};
+  return pack_h2(half2v{(f16)(c - (float)cs.x), (f16)(s - (float)cs.y)});
+}
+
+template <int KIND>
+__device__ __forceinline__ void build_lut_rest(LutRest& lut, const AttnArgs& a, int tid) {
+  const uint32_t c = (uint32_t)tid;
+  if constexpr (KIND == kKindDefault || KIND == kKindDefaultHR) {
+    lut.pair[c] = make_uint2(make_cs_rest(c & 15u, 4), make_cs_rest(c >> 4, 4));
+  } else if constexpr (KIND == kKindFast) {
+    lut.code[kLutDeep + c] = make_cs_rest(c, 8);
+  } else if constexpr (any_kind(KIND)) {
+    if (c < (1u << a.l1_bits)) lut.code[c] = make_cs_rest(c, a.l1_bits);
+    if (c < (1u << a.deep_bits)) lut.code[kLutDeep + c] = make_cs_rest(c, a.deep_bits);
+  }
+}
+
+// r (cos, sin) as a rounded fp16 pair and the fp16 pair of what that rounding, the table's and the radius's
+// left (r = r16 + r_rest): the products' errors come out of the FMA exactly, so that the two parts are off by
+// 2^-21 of the key.  An infinite radius leaves infinity less infinity: the rest is bounded, its sum with the
+// rounded part then is what that is (half a step of the largest fp16 number is 16).
+__device__ __forceinline__ uint32_t split_pair(half2v r, half2v r_rest, uint32_t cs, uint32_t cs_rest, uint32_t& rest) {
+  const half2v c = __builtin_bit_cast(half2v, cs), most = {(f16)32.0f, (f16)32.0f};
+  const half2v k = r * c;
+  half2v x = __builtin_elementwise_fma(r, c, -k);
+  x = __builtin_elementwise_fma(r, __builtin_bit_cast(half2v, cs_rest), x);
+  x = __builtin_elementwise_fma(r_rest, c, x);
+  rest = pack_h2(__builtin_elementwise_min(__builtin_elementwise_max(x, -most), most));
+  return pack_h2(k);
+}
+
 // Word 3 of a raw buffer resource on gfx9-family GPUs: DATA_FORMAT 32-bit
 // (bits 18:15 = 4), every other field 0 (untyped loads, no swizzle).
 constexpr int kRawBufferWord3 = 0x00020000;
@@ -650,6 +689,7 @@ __device__ __forceinline__ void fold_halves(const float4v& acc, float4v& s, int 
 // streams and picks per pair.
 constexpr int kAnyCodeBytes = 16 * (64 * kAnyChunks + 2);  // the chunks, and what a stream reads past them
 constexpr int kAnyWaveBytes = kAnyCodeBytes + 256 * 2;      // and, for int8 log radii, the page's radii by code
+constexpr int kAnySplitBytes = kAnyWaveBytes + 256 * 2;     // and what fp16 leaves of them
 
 __device__ __forceinline__ void code_stream(const uint32_t* words, int bit, uint32_t (&s)[4]) {
   const uint32_t* d = words + (bit >> 5);
@@ -670,9 +710,12 @@ __device__ __forceinline__ uint32_t stream_codes(const uint32_t (&s)[4], int kk,
 
 // QK over one compressed page: s[mt][i] = score(token score_token(mt, i, l4,
 // KIND == kKindDefaultHR), head l16).
-template <int KIND>
+// SPLIT: keys in two fp16 parts (split_pair), each multiplied; otherwise one, rounded from rounded factors.
+template <int KIND, bool SPLIT = false>
 __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const KRegs<KIND>& k,
-                                        const half8v* qb, int l16, int l4, float4v* s, void* wave_lds) {
+                                        const half8v* qb, int l16, int l4, float4v* s, void* wave_lds,
+                                        const LutRest* lut_rest = nullptr) {
+  [[maybe_unused]] const half2v zero = {(f16)0.0f, (f16)0.0f};
   if constexpr (KIND == kKindDefaultHR) {
     // Load g: 8 pairs of one token half (A operand row l16 = (8g + l16/2,
     // half l16&1)); k-step kk takes its pairs 4kk .. 4kk+3, code bytes 2kk
@@ -687,10 +730,21 @@ __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const
         const uint2 cs01 = lut.pair[(cw >> (16 * kk)) & 0xffu];
         const uint2 cs23 = lut.pair[(cw >> (16 * kk + 8)) & 0xffu];
         uint32_t e[4];
-        e[0] = pack_h2(lo_lo(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.x));
-        e[1] = pack_h2(hi_hi(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.y));
-        e[2] = pack_h2(lo_lo(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.x));
-        e[3] = pack_h2(hi_hi(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.y));
+        if constexpr (SPLIT) {
+          const uint2 rest01 = lut_rest->pair[(cw >> (16 * kk)) & 0xffu];
+          const uint2 rest23 = lut_rest->pair[(cw >> (16 * kk + 8)) & 0xffu];
+          uint32_t x[4];
+          e[0] = split_pair(lo_lo(rw[2 * kk]), zero, cs01.x, rest01.x, x[0]);
+          e[1] = split_pair(hi_hi(rw[2 * kk]), zero, cs01.y, rest01.y, x[1]);
+          e[2] = split_pair(lo_lo(rw[2 * kk + 1]), zero, cs23.x, rest23.x, x[2]);
+          e[3] = split_pair(hi_hi(rw[2 * kk + 1]), zero, cs23.y, rest23.y, x[3]);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(x[0], x[1], x[2], x[3]), qb[kk], acc, 0, 0, 0);
+        } else {
+          e[0] = pack_h2(lo_lo(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.x));
+          e[1] = pack_h2(hi_hi(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.y));
+          e[2] = pack_h2(lo_lo(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.x));
+          e[3] = pack_h2(hi_hi(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.y));
+        }
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(e[0], e[1], e[2], e[3]), qb[kk], acc, 0, 0, 0);
       }
       fold_halves(acc, s[g >> 1], 2 * (g & 1));
@@ -710,10 +764,21 @@ __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const
         const uint2 cs01 = lut.pair[b0];
         const uint2 cs23 = lut.pair[b1];
         uint32_t e[4];
-        e[0] = pack_h2(lo_lo(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.x));
-        e[1] = pack_h2(hi_hi(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.y));
-        e[2] = pack_h2(lo_lo(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.x));
-        e[3] = pack_h2(hi_hi(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.y));
+        if constexpr (SPLIT) {
+          const uint2 rest01 = lut_rest->pair[b0];
+          const uint2 rest23 = lut_rest->pair[b1];
+          uint32_t x[4];
+          e[0] = split_pair(lo_lo(rw[2 * kk]), zero, cs01.x, rest01.x, x[0]);
+          e[1] = split_pair(hi_hi(rw[2 * kk]), zero, cs01.y, rest01.y, x[1]);
+          e[2] = split_pair(lo_lo(rw[2 * kk + 1]), zero, cs23.x, rest23.x, x[2]);
+          e[3] = split_pair(hi_hi(rw[2 * kk + 1]), zero, cs23.y, rest23.y, x[3]);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(x[0], x[1], x[2], x[3]), qb[kk], acc, 0, 0, 0);
+        } else {
+          e[0] = pack_h2(lo_lo(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.x));
+          e[1] = pack_h2(hi_hi(rw[2 * kk]) * __builtin_bit_cast(half2v, cs01.y));
+          e[2] = pack_h2(lo_lo(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.x));
+          e[3] = pack_h2(hi_hi(rw[2 * kk + 1]) * __builtin_bit_cast(half2v, cs23.y));
+        }
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(e[0], e[1], e[2], e[3]), qb[kk], acc, 0, 0, 0);
       }
       s[mt] = acc;
@@ -731,14 +796,24 @@ __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t e[4];
+        [[maybe_unused]] uint32_t x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int rc = (int)(int8_t)((rw[kk] >> (8 * i)) & 0xffu);
           const uint32_t code = (cw[kk] >> (8 * i)) & 0xffu;
-          const f16 r = (f16)__builtin_amdgcn_exp2f((float)rc * ls2);
-          const half2v cs = __builtin_bit_cast(half2v, lut.code[kLutDeep + code]);
-          e[i] = pack_h2(half2v{r, r} * cs);
+          const float r32 = __builtin_amdgcn_exp2f((float)rc * ls2);
+          const f16 r = (f16)r32;
+          if constexpr (SPLIT) {
+            const f16 rest = (f16)(r32 - (float)r);
+            e[i] = split_pair(half2v{r, r}, half2v{rest, rest}, lut.code[kLutDeep + code],
+                              lut_rest->code[kLutDeep + code], x[i]);
+          } else {
+            const half2v cs = __builtin_bit_cast(half2v, lut.code[kLutDeep + code]);
+            e[i] = pack_h2(half2v{r, r} * cs);
+          }
         }
+        if constexpr (SPLIT)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(x[0], x[1], x[2], x[3]), qb[kk], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(e[0], e[1], e[2], e[3]), qb[kk], acc, 0, 0, 0);
       }
       s[mt] = acc;
@@ -759,9 +834,15 @@ __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const
       const float ls = h2f((uint16_t)k.ls_bits);
       const int c0 = 4 * (16 * l4 + l16);
       half2v x[2];
+      [[maybe_unused]] half2v rest[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i >> 1][i & 1] = (f16)expf((float)(int8_t)(c0 + i) * ls);
+      for (int i = 0; i < 4; ++i) {
+        const float r32 = expf((float)(int8_t)(c0 + i) * ls);
+        x[i >> 1][i & 1] = (f16)r32;
+        if constexpr (SPLIT) rest[i >> 1][i & 1] = (f16)(r32 - (float)(f16)r32);
+      }
       *reinterpret_cast<uint2*>(radius + c0) = make_uint2(pack_h2(x[0]), pack_h2(x[1]));
+      if constexpr (SPLIT) *reinterpret_cast<uint2*>(radius + 256 + c0) = make_uint2(pack_h2(rest[0]), pack_h2(rest[1]));
     }
     wave_lds_sync();
     // The lane's stream: the row that its run starts in.
@@ -796,22 +877,33 @@ __device__ __forceinline__ void qk_regs(const AttnArgs& a, const Lut& lut, const
           }
         }
         uint32_t e[4];
+        [[maybe_unused]] uint32_t rest[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           half2v r;
+          [[maybe_unused]] half2v r_rest = zero;
           if constexpr (KIND == kKindAnyI8) {
             const uint4 q = k.r[mt];
             const uint32_t w = kk == 0 ? q.x : kk == 1 ? q.y : kk == 2 ? q.z : q.w;
             const f16 x = radius[(w >> (8 * i)) & 0xffu];
             r = half2v{x, x};
+            if constexpr (SPLIT) {
+              const f16 y = radius[256 + ((w >> (8 * i)) & 0xffu)];
+              r_rest = half2v{y, y};
+            }
           } else {
             const uint4 q = k.r[mt][kk >> 1];
             const uint32_t w = (kk & 1) ? ((i & 2) ? q.w : q.z) : ((i & 2) ? q.y : q.x);
             r = (i & 1) ? hi_hi(w) : lo_lo(w);
           }
           const uint32_t cs = lut.code[entry[i]];
-          e[i] = pack_h2(r * __builtin_bit_cast(half2v, cs));
+          if constexpr (SPLIT)
+            e[i] = split_pair(r, r_rest, cs, lut_rest->code[entry[i]], rest[i]);
+          else
+            e[i] = pack_h2(r * __builtin_bit_cast(half2v, cs));
         }
+        if constexpr (SPLIT)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(rest[0], rest[1], rest[2], rest[3]), qb[kk], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(e[0], e[1], e[2], e[3]), qb[kk], acc, 0, 0, 0);
       }
       s[mt] = acc;
@@ -851,24 +943,30 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, int64_t slot, int l16,
 // acc[j] += Vhat^T tile j x P, Vhat = f16(code * scale) exactly: codes become
 // fp16 pairs (tokens e, e+1) by SDWA converts, then one packed multiply by the
 // pair's scales.
-template <int J>
+// SPLIT: with what that rounding leaves, which the FMA gives exactly, as a second product.
+template <int J, bool SPLIT>
 __device__ __forceinline__ void pv_tile(const VRegs& v, int ks, const half2v* sp, const half8v& pb,
                                         float4v& acc) {
   uint32_t e[4];
+  [[maybe_unused]] uint32_t x[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const uint2 wa = v.w[8 * ks + 2 * q];
     const uint2 wb = v.w[8 * ks + 2 * q + 1];
     const uint32_t c = (J < 4) ? i8pair_f16<J & 3>(wa.x, wb.x) : i8pair_f16<J & 3>(wa.y, wb.y);
-    e[q] = pack_h2(__builtin_bit_cast(half2v, c) * sp[q]);
+    const half2v value = __builtin_bit_cast(half2v, c) * sp[q];
+    e[q] = pack_h2(value);
+    if constexpr (SPLIT) x[q] = pack_h2(__builtin_elementwise_fma(__builtin_bit_cast(half2v, c), sp[q], -value));
   }
+  if constexpr (SPLIT)
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(x[0], x[1], x[2], x[3]), pb, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(e[0], e[1], e[2], e[3]), pb, acc, 0, 0, 0);
 }
 
 // sbase4: byte index of the lane holding the scale dword of token
 // v_token(0, l4, 0, HR) of the lane's group g (4 * (2 * that token + g/2));
 // ssel: v_perm selector taking half g & 1 of two dwords.
-template <bool HR>
+template <bool HR, bool SPLIT = false>
 __device__ __forceinline__ void pv_regs(const VRegs& v, int sbase4, uint32_t ssel, const half8v* pb,
                                         float4v* acc) {
 #pragma unroll
@@ -885,14 +983,14 @@ __device__ __forceinline__ void pv_regs(const VRegs& v, int sbase4, uint32_t sse
       const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(sbase4 + 8 * t0 + 8, (int)v.sd[ks]);
       sp[q] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(hi, lo, ssel));
     }
-    pv_tile<0>(v, ks, sp, pb[ks], acc[0]);
-    pv_tile<1>(v, ks, sp, pb[ks], acc[1]);
-    pv_tile<2>(v, ks, sp, pb[ks], acc[2]);
-    pv_tile<3>(v, ks, sp, pb[ks], acc[3]);
-    pv_tile<4>(v, ks, sp, pb[ks], acc[4]);
-    pv_tile<5>(v, ks, sp, pb[ks], acc[5]);
-    pv_tile<6>(v, ks, sp, pb[ks], acc[6]);
-    pv_tile<7>(v, ks, sp, pb[ks], acc[7]);
+    pv_tile<0, SPLIT>(v, ks, sp, pb[ks], acc[0]);
+    pv_tile<1, SPLIT>(v, ks, sp, pb[ks], acc[1]);
+    pv_tile<2, SPLIT>(v, ks, sp, pb[ks], acc[2]);
+    pv_tile<3, SPLIT>(v, ks, sp, pb[ks], acc[3]);
+    pv_tile<4, SPLIT>(v, ks, sp, pb[ks], acc[4]);
+    pv_tile<5, SPLIT>(v, ks, sp, pb[ks], acc[5]);
+    pv_tile<6, SPLIT>(v, ks, sp, pb[ks], acc[6]);
+    pv_tile<7, SPLIT>(v, ks, sp, pb[ks], acc[7]);
   }
 }
 
@@ -1086,7 +1184,7 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, int64_t slot, int l16,
   }
 }
 
-template <bool HR>
+template <bool HR, bool SPLIT = false>
 __device__ __forceinline__ void pv_regs(const DenseVRegs& v, int sbase4, uint32_t ssel, const half8v* pb,
                                         float4v* acc) {
   (void)sbase4;
@@ -1103,7 +1201,9 @@ __device__ __forceinline__ void pv_regs(const DenseVRegs& v, int sbase4, uint32_
 // enough in fp16) and the 32-register accumulator rescale is rare.
 constexpr float kLazyRescale = 8.0f;
 
-template <bool HR>
+// HEADROOM: weights lie 2^7 higher than the largest being 1 (2^15 at most), so that what is 2^-32 of it still
+// counts in fp16 (2^-25 otherwise); sums and results carry the same factor, which the division takes out.
+template <bool HR, bool HEADROOM = false>
 __device__ __forceinline__ void softmax_page(const float4v* s, int valid, float scale_log2, int l4,
                                              float& m_run, float& l_run, float4v* acc, half8v* pb) {
   float x[16];
@@ -1137,7 +1237,7 @@ __device__ __forceinline__ void softmax_page(const float4v* s, int valid, float 
   }
   // m_run is still -inf only if every score of this page is -inf or NaN: then
   // -inf scores weigh 0 and NaN scores stay NaN, as in the reference's softmax.
-  const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+  const float m_use = (m_run == -INFINITY ? 0.0f : m_run) - (HEADROOM ? 7.0f : 0.0f);
   float lsum = 0.0f;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
@@ -1840,7 +1940,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
   // V: the page store's codes, or the dense V planes' rows (DV).
   typename std::conditional<DV, DenseVRegs, VRegs>::type vr;
   void* wave_lds = &sh.acc[wave][0];  // this wave's merge area, free until finish_unit
-  static_assert(sizeof(sh.acc[0]) >= kAnyWaveBytes, "a page's code rows fit the merge area");
+  static_assert(sizeof(sh.acc[0]) >= (LIST ? kAnySplitBytes : kAnyWaveBytes), "a page's code rows fit the merge area");
   if constexpr (KIND != kKindNone) {
     // A launch with pages has one in every split (p_begin < n_pages).  A wave
     // without a page of its own issues the same loads with every lane on the
@@ -1864,6 +1964,12 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
   if constexpr (KIND != kKindNone) {
     if (tid < 256) build_lut<KIND>(sh.lut, a, tid);
   }
+  __shared__ typename std::conditional<LIST, LutRest, int>::type lut_rest;
+  if constexpr (LIST) {
+    if (tid < 256) build_lut_rest<KIND>(lut_rest, a, tid);
+  }
+  const LutRest* rest = nullptr;
+  if constexpr (LIST) rest = &lut_rest;
   TP_STAMP(3);
   __shared__ float qjl_sin[QJL != kQjlOff ? kQjlMaxBits + 1 : 1];
   __shared__ uint32_t qjl_qw[QJL == kQjlAny ? 16 * kQjlMaxWords : 1];
@@ -1894,7 +2000,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
   if constexpr (KIND != kKindNone) {
     for (int it = 0; page + WAVES < p_end; page += WAVES, ++it) {
       float4v s[4];
-      qk_regs<KIND>(a, sh.lut, kr, qb, l16, l4, s, wave_lds);
+      qk_regs<KIND, LIST>(a, sh.lut, kr, qb, l16, l4, s, wave_lds, rest);
       if constexpr (QJL == kQjl64) qjl_correct<HR>(a, bkv * a.qjl_capacity + page, l4, qsig, qnorm, qjl_sin, s);
       if constexpr (QJL == kQjlAny)
         qjl_correct_any<HR>(a, bkv * a.qjl_capacity + page, l4, qjl_qw, HR ? (l16 & 7) : l16, qnorm, qjl_sin, s);
@@ -1902,8 +2008,8 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
       const int at_next = LIST ? next_page : page + WAVES;
       load_k<KIND>(a, bkv * a.capacity + at_next, l16, l4, kr);
       half8v pb[2];
-      softmax_page<HR>(s, kPageTokens, a.scale_log2, l4, m_run, l_run, acc, pb);
-      pv_regs<HR>(vr, sbase4, ssel, pb, acc);
+      softmax_page<HR, LIST>(s, kPageTokens, a.scale_log2, l4, m_run, l_run, acc, pb);
+      pv_regs<HR, LIST>(vr, sbase4, ssel, pb, acc);
       if constexpr (DV)
         load_v<HR>(a, bkv * a.v_capacity + page + WAVES, l16, l4, lane, vr);
       else
@@ -1913,13 +2019,13 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
     }
     if (page < p_end) {
       float4v s[4];
-      qk_regs<KIND>(a, sh.lut, kr, qb, l16, l4, s, wave_lds);
+      qk_regs<KIND, LIST>(a, sh.lut, kr, qb, l16, l4, s, wave_lds, rest);
       if constexpr (QJL == kQjl64) qjl_correct<HR>(a, bkv * a.qjl_capacity + page, l4, qsig, qnorm, qjl_sin, s);
       if constexpr (QJL == kQjlAny)
         qjl_correct_any<HR>(a, bkv * a.qjl_capacity + page, l4, qjl_qw, HR ? (l16 & 7) : l16, qnorm, qjl_sin, s);
       const int valid = (int)min((int64_t)kPageTokens, a.seq_len - (int64_t)page * kPageTokens);
       half8v pb[2];
-      softmax_page<HR>(s, valid, a.scale_log2, l4, m_run, l_run, acc, pb);
+      softmax_page<HR, LIST>(s, valid, a.scale_log2, l4, m_run, l_run, acc, pb);
       if constexpr (DV) {
         // Dense V rows of masked tokens get P = 0, but 0 * NaN is NaN in the
         // MFMA: rows at or past `valid` are zeroed, so whatever a caller's
@@ -1935,7 +2041,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
           }
         }
       }
-      pv_regs<HR>(vr, sbase4, ssel, pb, acc);
+      pv_regs<HR, LIST>(vr, sbase4, ssel, pb, acc);
     }
   }
 
@@ -1953,7 +2059,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
         float4v s[4];
         qk_tail<HR>(tr, qb, s);
         half8v pb[2];
-        softmax_page<HR>(s, valid, a.scale_log2, l4, m_run, l_run, acc, pb);
+        softmax_page<HR, LIST>(s, valid, a.scale_log2, l4, m_run, l_run, acc, pb);
         pv_tail(tr, pb, acc);
       }
     }
@@ -2294,6 +2400,7 @@ template <int KIND, int W, int QJL, bool DV = false>
 static void launch_decode_w(const AttnArgs& a, dim3 grid, hipStream_t s) {
   const dim3 block(W * 64);
   if constexpr (QJL == kQjlOff && !DV) {
+#ifndef TP_TIMELINE  // the measurement library has no use for them
     if (a.list) {
       if (a.tier_splits > 0)
         hipLaunchKernelGGL((decode_attention_kernel<KIND, W, kFlList | kFlTiers>), grid, block, 0, s, a);
@@ -2301,6 +2408,7 @@ static void launch_decode_w(const AttnArgs& a, dim3 grid, hipStream_t s) {
         hipLaunchKernelGGL((decode_attention_kernel<KIND, W, kFlList>), grid, block, 0, s, a);
       return;
     }
+#endif
     if (a.new_k) {  // a step: one z layer more, for stage_new_rows
       const dim3 g(grid.x, grid.y, grid.z + 1);
       if (a.tier_splits > 0)
@@ -2653,6 +2761,10 @@ int32_t tp_selected_attention(const void* q, int64_t batch, int32_t hq, int32_t 
     set_error("scale must be finite");
     return TP_ERR_INVALID;
   }
+#ifdef TP_TIMELINE
+  set_error("the measurement library has no kernels for selected pages");
+  return TP_ERR_UNSUPPORTED;
+#endif
   // The same page may be listed more than once (its tokens then count as often), but not more pages than are stored.
   if (count > n_pages) {
     set_error("%d pages selected of %d", count, n_pages);

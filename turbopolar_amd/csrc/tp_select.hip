@@ -93,17 +93,20 @@ __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs 
   reinterpret_cast<half2v*>(a.bounds + (bh * a.bounds_capacity + page) * 2 * kHeadDim)[tid] = x;
 }
 
-struct ScoreArgs {
+struct SelectArgs {
   const uint16_t* q;       // [units][g][128]
   const uint16_t* bounds;  // [units][capacity][2][128]
   uint64_t* keys;          // [units][count]
+  uint32_t* tickets;       // [units], 0 before and after
+  int32_t* selected;       // [units][first + take + last]
   int64_t capacity;
-  int32_t g, first, count;  // scored: pages [first, first + count)
-  uint32_t flip;            // negative scales: the queries' signs turned
+  int32_t g, first, last, count, take, n_pages;  // scored: pages [first, first + count), of which `take` are selected
+  uint32_t flip;                                 // negative scales: the queries' signs turned
 };
 
-constexpr int kScoreThreads = 256;
-constexpr int kScorePages = kScoreThreads / 8;
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kScorePages = kSelectThreads / 8;
 constexpr int kScoreHeads = 16;
 
 // A score as a whole number of the same order.
@@ -113,13 +116,9 @@ __device__ __forceinline__ uint64_t score_key(double s) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// 8 lanes a page, 16 dimensions a lane, the group's queries in LDS.
-__global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(ScoreArgs a) {
-  __shared__ __align__(16) float qs[kScoreHeads][kHeadDim];
-  const int tid = threadIdx.x, c = tid & 7;
-  const int64_t unit = blockIdx.y;
-  const int i = (int)blockIdx.x * kScorePages + (tid >> 3);
-  const int page = a.first + min(i, a.count - 1);  // those past the last repeat it
+// The key of the thread's page: 8 lanes a page, 16 dimensions a lane, the group's queries in LDS.
+__device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, int page, int tid, float (*qs)[kHeadDim]) {
+  const int c = tid & 7;
   const uint16_t* b = a.bounds + (unit * a.capacity + page) * 2 * kHeadDim + 16 * c;
   uint4v w[4];
 #pragma unroll
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(ScoreArgs a)
   for (int h0 = 0; h0 < a.g; h0 += kScoreHeads) {
     const int heads = min(kScoreHeads, a.g - h0);
     __syncthreads();
-    for (int x = tid; x < heads * kHeadDim; x += kScoreThreads)
+    for (int x = tid; x < heads * kHeadDim; x += kSelectThreads)
       qs[0][x] = h2f((uint16_t)(a.q[(unit * a.g + h0) * kHeadDim + x] ^ a.flip));
     __syncthreads();
     for (int h = 0; h < heads; ++h) {
@@ -147,29 +146,37 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(ScoreArgs a)
       best = s > best ? s : best;
     }
   }
-  if (c == 0 && i < a.count) a.keys[unit * a.count + i] = score_key(any_nan ? (double)INFINITY : best);
+  return score_key(any_nan ? (double)INFINITY : best);
 }
 
-struct SelectArgs {
-  const uint64_t* keys;  // [units][count]
-  int32_t* selected;     // [units][first + take + last]
-  int32_t first, last, count, take, n_pages;
-};
-
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
-
-// A workgroup a (batch, kv head): the `take`-th largest key by its digits of 8 bits from the first in which the
-// keys differ, then the pages above it, and the first of those that equal it, in their order.
+// A workgroup of each 64 pages of a (batch, kv head) scores them; the last of them to be done selects: the `take`-th
+// largest key by its digits of 8 bits from the first in which the keys differ, then the pages above it, and the first
+// of those that equal it, in their order.  PER: keys of a thread, held in registers (0: more, read anew each time).
+// Keys go out and come back past the caches of the XCDs (agent scope), between them a ticket.
+template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs a) {
+  __shared__ __align__(16) float qs[kScoreHeads][kHeadDim];
   __shared__ uint32_t hist[256];
   __shared__ uint64_t ends[2][kSelectWaves];
   __shared__ uint64_t found;
-  __shared__ int32_t found_rest, found_all;
+  __shared__ int32_t found_rest, found_all, is_last;
   __shared__ int32_t counts[2][kSelectWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint64_t* keys = a.keys + (int64_t)blockIdx.x * a.count;
-  int32_t* out = a.selected + (int64_t)blockIdx.x * (a.first + a.take + a.last);
+  const int64_t unit = blockIdx.y;
+  uint64_t* keys = a.keys + unit * a.count;
+  int32_t* out = a.selected + unit * (a.first + a.take + a.last);
+  if (a.take > 0 && a.take < a.count) {
+    const int i = (int)blockIdx.x * kScorePages + (tid >> 3);
+    const uint64_t key = page_key(a, unit, a.first + min(i, a.count - 1), tid, qs);  // those past the last repeat it
+    if ((tid & 7) == 0 && i < a.count) __hip_atomic_store(keys + i, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores are where every XCD sees them
+    __syncthreads();
+    if (tid == 0)
+      is_last = __hip_atomic_fetch_add(a.tickets + unit, 1u, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
+    __syncthreads();
+    if (!is_last) return;
+    if (tid == 0) __hip_atomic_store(a.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   for (int i = tid; i < a.first; i += kSelectThreads) out[i] = i;
   for (int i = tid; i < a.last; i += kSelectThreads) out[a.first + a.take + i] = a.n_pages - a.last + i;
   if (a.take == 0) return;
@@ -178,12 +185,25 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     for (int i = tid; i < a.count; i += kSelectThreads) out[i] = a.first + i;
     return;
   }
+  auto load = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  uint64_t mine[PER ? PER : 1];
+  if constexpr (PER)
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine[j] = load(min(tid + kSelectThreads * j, a.count - 1));
+  auto each_key = [&](auto use) {
+    if constexpr (PER) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (tid + kSelectThreads * j < a.count) use(mine[j]);
+    } else {
+      for (int i = tid; i < a.count; i += kSelectThreads) use(load(i));
+    }
+  };
   uint64_t low = ~0ull, high = 0;
-  for (int i = tid; i < a.count; i += kSelectThreads) {
-    const uint64_t k = keys[i];
+  each_key([&](uint64_t k) {
     low = k < low ? k : low;
     high = k > high ? k : high;
-  }
+  });
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint64_t x = __shfl_xor((unsigned long long)low, d), y = __shfl_xor((unsigned long long)high, d);
@@ -196,7 +216,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     low = ends[0][w] < low ? ends[0][w] : low;
     high = ends[1][w] > high ? ends[1][w] : high;
   }
-  // Keys agree above bit `top`; the digits found so far are `prefix`, the keys' bits from `shift` on.
+  // Keys agree above bit `shift`; the digits found so far are `prefix`, the keys' bits from there on.
   int shift = low == high ? 0 : 64 - __builtin_clzll(low ^ high);
   uint64_t prefix = shift == 64 ? 0 : high >> shift;
   int32_t rest = a.take;
@@ -205,10 +225,9 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     const int width = min(shift, 8), next = shift - width;
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < a.count; i += kSelectThreads) {
-      const uint64_t k = keys[i];
+    each_key([&](uint64_t k) {
       if (shift == 64 || (k >> shift) == prefix) atomicAdd(&hist[(uint32_t)(k >> next) & ((1u << width) - 1u)], 1u);
-    }
+    });
     __syncthreads();
     if (wave == 0) {  // the digit in which the rest-th key from the top lies
       uint32_t n[4], sum = 0;
@@ -239,9 +258,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
   }
   // Above the prefix: taken; equal to it: the first `rest` of them (all of them where `all`).
   int32_t base = 0, equal_base = 0;
-  for (int i0 = 0; i0 < a.count; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const uint64_t k = i < a.count ? keys[i] >> shift : 0;
+  auto place = [&](int i, uint64_t key) {
+    const uint64_t k = key >> shift;
     const bool over = i < a.count && k > prefix, equal = i < a.count && k == prefix;
     const uint64_t equals = __ballot(equal), below = (1ull << lane) - 1ull;
     if (lane == 0) counts[0][wave] = __popcll(equals);
@@ -263,6 +281,12 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     if (taken) out[at] = a.first + i;
     base += taken_all;
     equal_base += equal_all;
+  };
+  if constexpr (PER) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) place(tid + kSelectThreads * j, mine[j]);
+  } else {
+    for (int i0 = 0; i0 < a.count; i0 += kSelectThreads) place(i0 + tid, load(min(i0 + tid, a.count - 1)));
   }
 }
 
@@ -311,9 +335,9 @@ extern "C" int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* 
   return launch_status("tp_page_bounds");
 }
 
-extern "C" size_t tp_select_workspace_bytes(int64_t batch, int32_t hkv, int32_t n_pages) {
-  if (batch < 1 || hkv < 1 || n_pages < 0) return 0;
-  return (size_t)batch * hkv * n_pages * sizeof(uint64_t);
+extern "C" size_t tp_select_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t n_pages) {
+  if (batch < 1 || hkv < 1 || hq < hkv || n_pages < 0) return 0;
+  return tp_decode_counter_bytes(batch, hq, hkv) + (size_t)batch * hkv * n_pages * sizeof(uint64_t);
 }
 
 extern "C" int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int32_t hkv, const void* bounds,
@@ -342,30 +366,29 @@ extern "C" int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int
     set_error("q, bounds (16-byte aligned) and selected must be non-NULL buffers");
     return TP_ERR_INVALID;
   }
-  const size_t need = tp_select_workspace_bytes(batch, hkv, n_pages);
+  const size_t need = tp_select_workspace_bytes(batch, hq, hkv, n_pages);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u)) {
     set_error("workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace_bytes);
     return TP_ERR_WORKSPACE;
   }
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned units = (unsigned)(batch * hkv);
-  const int32_t middle = n_pages - first - last, take = count - first - last;
-  uint64_t* keys = static_cast<uint64_t*>(workspace);
-  if (take > 0 && take < middle) {
-    ScoreArgs a{};
-    a.q = static_cast<const uint16_t*>(q);
-    a.bounds = static_cast<const uint16_t*>(bounds);
-    a.keys = keys;
-    a.capacity = bounds_capacity;
-    a.g = hq / hkv, a.first = first, a.count = middle;
-    a.flip = scale < 0.0f ? 0x8000u : 0u;
-    hipLaunchKernelGGL(page_scores_kernel, dim3((unsigned)((middle + kScorePages - 1) / kScorePages), units),
-                       dim3(kScoreThreads), 0, s, a);
-  }
   SelectArgs a{};
-  a.keys = keys;
+  a.q = static_cast<const uint16_t*>(q);
+  a.bounds = static_cast<const uint16_t*>(bounds);
+  a.tickets = static_cast<uint32_t*>(workspace);
+  a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + tp_decode_counter_bytes(batch, hq, hkv));
   a.selected = selected;
-  a.first = first, a.last = last, a.count = middle, a.take = take, a.n_pages = n_pages;
-  hipLaunchKernelGGL(select_pages_kernel, dim3(units), dim3(kSelectThreads), 0, s, a);
+  a.capacity = bounds_capacity;
+  a.g = hq / hkv, a.first = first, a.last = last, a.count = n_pages - first - last, a.take = count - first - last;
+  a.n_pages = n_pages;
+  a.flip = scale < 0.0f ? 0x8000u : 0u;
+  const bool scored = a.take > 0 && a.take < a.count;
+  const dim3 grid(scored ? (unsigned)((a.count + kScorePages - 1) / kScorePages) : 1u, (unsigned)(batch * hkv));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.count <= kSelectThreads)
+    hipLaunchKernelGGL(select_pages_kernel<1>, grid, dim3(kSelectThreads), 0, s, a);
+  else if (a.count <= 4 * kSelectThreads)
+    hipLaunchKernelGGL(select_pages_kernel<4>, grid, dim3(kSelectThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(select_pages_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
   return launch_status("tp_select_pages");
 }

@@ -36,7 +36,7 @@ from .config import TurboPolarConfig
 from .draft import DraftTree
 from .kernels import (
     HEAD_DIM, PAGE, _check_draft, _no_grad, _tree_attention, check_selection, decode_attention_store, decode_pages_into,
-    fp16_scale, prompt_attention, rotate_tokens, selected_attention,
+    fp16_scale, prompt_attention, rotate_tokens, selected_attention, tail_args,
 )
 from .runtime import TurboPolarKVCacheRuntime
 from .storage import pages_of
@@ -186,15 +186,16 @@ class TurboPolarFastCache:
         rt = self.runtime
         rt.resolve_deferred_check()
         n_pages, H = rt.k_storage.block_count, rt._num_kv_heads
-        tail_k, tail_v = rt._tail_views()
         scale, layout = fp16_scale(scale), rt.polar_encoder.layout
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
         stored = self._store_pages() if n_pages else None
         if n_pages <= pages:
+            tail_k, tail_v = rt._tail_views()
             return decode_attention_store(q[:, :, 0], layout, stored, n_pages, H, tail_k, tail_v, rt.actual_seq_len, scale)
-        return selected_attention(q[:, :, 0], layout, stored, n_pages, H, rt.page_bounds(), tail_k, tail_v, scale, pages,
-                                  first, last)[0]
+        bounds = rt.page_bounds()
+        return selected_attention(q[:, :, 0], layout, stored, n_pages, H, bounds, int(rt._bounds.shape[2]),
+                                  tail_args(rt._tail_k, rt._tail_v, rt._tail_len), scale, pages, first, last)[0]
 
     # ------------------------------------------------------------------ prompts, drafts, branches
     def prompt_attention(self, q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,

@@ -876,30 +876,55 @@ def _rotate_tokens(q, k, v, cos, sin, interleaved, k_out, v_out, pos, flag=None,
 _Strides4 = ctypes.c_int64 * 4
 
 
+def tail_args(tail_k: Optional[torch.Tensor], tail_v: Optional[torch.Tensor], tokens: int) -> tuple:
+    """The first ``tokens`` rows of a cache's tail buffers ``[B, H, 64, 128]`` as an attention call takes them: (keys,
+    values, tokens, tokens between rows), pointers or, where the buffers are not fp16, converted tensors."""
+    if not tokens:
+        return None, None, 0, 0
+    if tail_k.dtype is torch.float16:  # contiguous, as the runtime makes them
+        return tail_k.data_ptr(), tail_v.data_ptr(), tokens, int(tail_k.shape[2])
+    k, v, stride = _tail_pair(tail_k[:, :, :tokens], tail_v[:, :, :tokens])
+    return k, v, tokens, stride
+
+
+def _pointer(x):
+    return x.data_ptr() if isinstance(x, torch.Tensor) else x
+
+
+@lru_cache(maxsize=1024)
+def _shared_workspace(B: int, Hq: int, Hkv: int, layout: tuple, prefix_pages: int, prefix_tail: bool, n_pages: int,
+                      tail: bool) -> int:
+    return int(lib().tp_shared_workspace_bytes(B, Hq, Hkv, ctypes.byref(_lib.make_layout(*layout)), prefix_pages,
+                                               int(prefix_tail), n_pages, int(tail)))
+
+
+def _step_query(q: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """A step's queries ``[B, H_q, 1, 128]`` as a kernel reads them in place, and their batch and head strides."""
+    if q.dtype is not torch.float16:
+        q = q.to(torch.float16)
+    s0, s1, _, s3 = q.stride()
+    if s3 != 1 or (s0 | s1) & 7 or q.data_ptr() & 15:
+        q = _fresh(q)
+        s0, s1, _, _ = q.stride()
+    return q, s0, s1
+
+
 def shared_attention(q: torch.Tensor, layout, num_kv_heads: int, prefix, own, scale: float) -> torch.Tensor:
-    """tp_shared_attention: ``q`` ``[B, H_q, 128]`` over a prefix that every row shares and each row's own tokens.
-    ``prefix`` and ``own`` are (store's descriptor or None, stored pages, dense tail of keys or None, of values): of
-    one batch row, and of B.  Returns fp16 ``[B, H_q, 128]``."""
-    q16 = _q16(q)
-    B, Hq, _ = q16.shape
-    dev = q16.device
-    parts, tails = [], []
-    for pages, n_pages, tail_k, tail_v in (prefix, own):
-        length = 0 if tail_k is None else int(tail_k.shape[2])
-        tk = tv = None
-        stride = 0
-        if length:
-            tk, tv, stride = _tail_pair(tail_k, tail_v)
-        tails += [tk, tv]
-        parts.append((ctypes.byref(pages if pages is not None else _NO_PAGES), n_pages if pages is not None else 0,
-                      ptr(tk), ptr(tv), length, stride))
+    """tp_shared_attention: ``q`` ``[B, H_q, 1, 128]`` over a prefix that every row shares and each row's own tokens.
+    ``prefix`` and ``own`` are (store's descriptor or None, stored pages, ``tail_args``): of one batch row, and of B.
+    Returns fp16 ``[B, H_q, 128]``."""
+    q, q_b, q_h = _step_query(q)
+    B, Hq, _, _ = q.shape
+    dev = q.device
+    (pages0, n0, (k0, v0, tail0, stride0)), (pages1, n1, (k1, v1, tail1, stride1)) = prefix, own
     out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.float16, device=dev)
-    L = lib()
-    ws = _scratch(int(L.tp_shared_workspace_bytes(B, Hq, num_kv_heads, ctypes.byref(layout), parts[0][1], parts[0][4],
-                                                  parts[1][1], parts[1][4])), dev)
+    form = layout.int8_radii, layout.l1_bits, layout.deep_bits, layout.split_dim
+    ws = _scratch(_shared_workspace(B, Hq, num_kv_heads, form, n0, tail0 > 0, n1, tail1 > 0), dev)
     st = call_on(
-        dev, L.tp_shared_attention, q16.data_ptr(), out.data_ptr(), B, Hq, num_kv_heads, ctypes.byref(layout), *parts[0],
-        *parts[1], _Strides4(Hq * HEAD_DIM, HEAD_DIM, Hq * HEAD_DIM, HEAD_DIM), float(scale), ptr(ws),
+        dev, lib().tp_shared_attention, q.data_ptr(), out.data_ptr(), B, Hq, num_kv_heads, ctypes.byref(layout),
+        ctypes.byref(_NO_PAGES if pages0 is None else pages0), n0, _pointer(k0), _pointer(v0), tail0, stride0,
+        ctypes.byref(_NO_PAGES if pages1 is None else pages1), n1, _pointer(k1), _pointer(v1), tail1, stride1,
+        _Strides4(q_b, q_h, Hq * HEAD_DIM, HEAD_DIM), float(scale), None if ws is None else ws.data_ptr(),
         0 if ws is None else ws.numel(), stream_handle(dev),
     )
     check(st, "tp_shared_attention")
@@ -921,6 +946,9 @@ def page_bounds_into(layout, pages: TPPages, bh: int, page_begin: int, n_pages: 
 
 def _bounds_view(bounds: torch.Tensor, B: int, H: int, S: int, device) -> Tuple[torch.Tensor, int]:
     """``bounds`` ``[B, H, S, 2, 128]`` as the kernel reads them, and the pages between its rows."""
+    if isinstance(bounds, torch.Tensor) and bounds.shape == (B, H, S, 2, HEAD_DIM) and bounds.dtype is torch.float16 and (
+            bounds.device == device and bounds.is_contiguous() and not bounds.data_ptr() & 15):
+        return bounds, S
     if not isinstance(bounds, torch.Tensor) or tuple(bounds.shape) != (B, H, S, 2, HEAD_DIM) or bounds.dtype is not torch.float16:
         raise ValueError(f"bounds must be float16 [{B}, {H}, {S}, 2, {HEAD_DIM}], got "
                          f"{getattr(bounds, 'dtype', None)} {tuple(getattr(bounds, 'shape', ()))}")
@@ -942,6 +970,12 @@ def check_selection(pages: int, first: int, last: int) -> None:
         raise ValueError(f"cannot select {pages} pages, the first {first} and the last {last} among them")
 
 
+@lru_cache(maxsize=1024)
+def _selection_workspace(B: int, Hq: int, Hkv: int, n_pages: int, count: int) -> int:
+    """What tp_select_pages and tp_selected_attention take, one after the other."""
+    return max(int(lib().tp_select_workspace_bytes(B, Hq, Hkv, n_pages)), _workspace_bytes(B, Hq, Hkv, count, 0))
+
+
 def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
     """The split-K workspace of the stream; one of its own inside a captured graph, whose replays may run beside
     those of another graph or eager calls."""
@@ -951,32 +985,27 @@ def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.T
 
 
 def selected_attention(q: torch.Tensor, layout, pages: TPPages, n_pages: int, num_kv_heads: int, bounds: torch.Tensor,
-                       tail_k: Optional[torch.Tensor], tail_v: Optional[torch.Tensor], scale: float, count: int,
-                       first: int, last: int) -> Tuple[torch.Tensor, torch.Tensor]:
+                       capacity: int, tail: tuple, scale: float, count: int, first: int,
+                       last: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """tp_select_pages and tp_selected_attention: ``q`` ``[B, H_q, 128]`` over ``count`` of the ``n_pages`` stored
-    pages, each kv head its own, and the dense tail (``[B, H_kv, < 64, 128]`` or None).  ``bounds``: fp16 ``[B, H_kv,
-    n_pages, 2, 128]``.  Returns fp16 ``[B, H_q, 128]`` and the pages, int32 ``[B, H_kv, count]``, ascending."""
+    pages, each kv head its own, and the dense tail (``tail_args``).  ``bounds``: fp16 ``[B, H_kv, n_pages, 2, 128]``,
+    rows ``capacity`` pages apart.  Returns fp16 ``[B, H_q, 128]`` and the pages, int32 ``[B, H_kv, count]``,
+    ascending."""
     q16 = _q16(q)
     B, Hq, _ = q16.shape
     dev = q16.device
-    bounds, cap = _bounds_view(bounds, B, num_kv_heads, n_pages, dev)
-    tail_len = 0 if tail_k is None else int(tail_k.shape[2])
-    tk = tv = None
-    tail_stride = 0
-    if tail_len:
-        tk, tv, tail_stride = _tail_pair(tail_k, tail_v)
+    tk, tv, tail_len, tail_stride = tail
     out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.float16, device=dev)
     selected = torch.empty((B, num_kv_heads, count), dtype=torch.int32, device=dev)
     L, stream = lib(), stream_handle(dev)
-    scores = _scratch(8 * B * num_kv_heads * n_pages, dev)
-    st = call_on(dev, L.tp_select_pages, q16.data_ptr(), B, Hq, num_kv_heads, bounds.data_ptr(), cap, n_pages, first, last,
-                 count, float(scale), selected.data_ptr(), scores.data_ptr(), scores.numel(), stream)
+    ws = _zeroed_workspace(_selection_workspace(B, Hq, num_kv_heads, n_pages, count), dev, stream)
+    q_ptr, list_ptr, ws_ptr, ws_bytes, scale = q16.data_ptr(), selected.data_ptr(), ws.data_ptr(), ws.numel(), float(scale)
+    st = call_on(dev, L.tp_select_pages, q_ptr, B, Hq, num_kv_heads, bounds.data_ptr(), capacity, n_pages, first, last,
+                 count, scale, list_ptr, ws_ptr, ws_bytes, stream)
     check(st, "tp_select_pages")
-    ws = _zeroed_workspace(_workspace_bytes(B, Hq, num_kv_heads, count, 0), dev, stream)
     st = call_on(
-        dev, L.tp_selected_attention, q16.data_ptr(), B, Hq, num_kv_heads, ctypes.byref(layout), ctypes.byref(pages),
-        n_pages, selected.data_ptr(), count, ptr(tk), ptr(tv), tail_len, tail_stride, float(scale), ws.data_ptr(),
-        ws.numel(), out.data_ptr(), stream,
+        dev, L.tp_selected_attention, q_ptr, B, Hq, num_kv_heads, ctypes.byref(layout), ctypes.byref(pages), n_pages,
+        list_ptr, count, _pointer(tk), _pointer(tv), tail_len, tail_stride, scale, ws_ptr, ws_bytes, out.data_ptr(), stream,
     )
     check(st, "tp_selected_attention")
     return out, selected

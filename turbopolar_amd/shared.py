@@ -13,7 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from .fast_attention import TurboPolarFastCache
-from .kernels import HEAD_DIM, _no_grad, fp16_scale, shared_attention
+from .kernels import HEAD_DIM, _no_grad, fp16_scale, shared_attention, tail_args
 
 
 def _layout_of(cache: TurboPolarFastCache) -> tuple:
@@ -100,14 +100,13 @@ class SharedPrefixCache:
             rt.resolve_deferred_check()
             if rt.actual_seq_len and rt._batch_size != rows:
                 raise ValueError(f"batch of q ({B}) and of the {name} ({rt._batch_size}) do not match")
-            n_pages = rt.k_storage.block_count
-            tail_k, tail_v = rt._tail_views()
-            held = rt.k_storage.radii if n_pages else tail_k
-            if held is not None and (held.device != q.device or not q.is_cuda):
+            n_pages, tokens = rt.k_storage.block_count, rt._tail_len
+            held = rt.k_storage.radii if n_pages else rt._tail_k
+            if (n_pages or tokens) and (held.device != q.device or not q.is_cuda):
                 raise ValueError(f"q is on {q.device}, the {name} on {held.device}; need one HIP device")
-            parts.append((cache._store_pages() if n_pages else None, n_pages, tail_k, tail_v))
+            parts.append((cache._store_pages() if n_pages else None, n_pages, tail_args(rt._tail_k, rt._tail_v, tokens)))
         _no_grad(q)
-        return shared_attention(q[:, :, 0], self.prefix.runtime.polar_encoder.layout, heads, *parts, fp16_scale(scale))
+        return shared_attention(q, self.prefix.runtime.polar_encoder.layout, heads, *parts, fp16_scale(scale))
 
     def decode_attention(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, scale: float) -> torch.Tensor:
         """Appends a token to each sequence (``[B, H_kv, 1, 128]``) and attends."""
