@@ -14,6 +14,7 @@
 // their scores differ by less than 2^-46 of their terms, whatever the order of the sum: which pages are attended
 // does not depend on rounding.
 #include <algorithm>
+#include <type_traits>
 
 #include "tp_page_tiles.h"
 
@@ -25,72 +26,129 @@ struct BoundsArgs {
   const uint8_t* angle_l1;
   const uint8_t* angle_deep;
   int64_t capacity, bounds_capacity;
-  int32_t page_begin, l1_bits, deep_bits, split_half, l1_row, deep_row;
+  int32_t page_begin, n_pages, l1_bits, deep_bits, split_half, l1_row, deep_row;
   uint16_t* bounds;  // [bh][bounds_capacity][2][128]
 };
 
 constexpr int kBoundsThreads = 256;
 
-// A workgroup a page.  Thread (c, t0) decodes pairs 8 c .. + 7 of tokens t0 and t0 + 32; the running bounds are
-// joined over the wave's tokens by shuffles and over the waves in LDS.  Bound by the reads of the key fields.
-template <bool I8>
-__global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
-  __shared__ float2v lut[512];
-  __shared__ half2v side[4][2][kPairs];
-  __shared__ float radius[I8 ? 256 : 1];  // of int8 codes, from -128 on, as the page decoder computes them
-  const int tid = threadIdx.x, c = tid & 7, lane = tid & 63, wave = tid >> 6;
-  const int64_t bh = blockIdx.y, page = (int64_t)a.page_begin + blockIdx.x, slot = bh * a.capacity + page;
-  if (tid < (1 << a.l1_bits)) lut[tid] = angle_pair(tid, a.l1_bits);
-  if (tid < (1 << a.deep_bits)) lut[256 + tid] = angle_pair(tid, a.deep_bits);
-  if constexpr (I8) radius[tid] = expf((float)(tid - 128) * h2f(a.radii_scales[slot]));
-  half2v lo[8], hi[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) lo[i] = half2v{(f16)INFINITY, (f16)INFINITY}, hi[i] = -lo[i];
-  __syncthreads();
+// A thread's part of a page's key fields: pairs 8 c .. + 7 of tokens t0 and t0 + 32.
+template <int KIND>
+struct BoundsRegs {
+  uint4v r[tree_i8(KIND) ? 1 : 2];
+  uint2v r8[tree_i8(KIND) ? 2 : 1];
+  uint2v codes[2];  // the run's 8 codes, as bytes, or as nibbles in the first word
+  uint32_t ls;
+};
+
+template <int KIND>
+__device__ __forceinline__ void load_bounds(const BoundsArgs& a, int64_t slot, int tid, BoundsRegs<KIND>& p) {
+  const int c = tid & 7;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int64_t row = slot * kPageTokens + (tid >> 3) + 32 * n;
-    float r[8];
-    if constexpr (I8) {
-      const uint2v w = *reinterpret_cast<const uint2v*>(static_cast<const int8_t*>(a.radii) + row * kPairs + 8 * c);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = radius[((w[i >> 2] >> (8 * (i & 3))) + 128u) & 0xffu];
+    if constexpr (tree_i8(KIND))
+      p.r8[n] = *reinterpret_cast<const uint2v*>(static_cast<const int8_t*>(a.radii) + row * kPairs + 8 * c);
+    else
+      p.r[n] = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(a.radii) + row * kPairs + 8 * c);
+    if constexpr (KIND == kTreeDefault) {
+      p.codes[n].x = *reinterpret_cast<const uint32_t*>((c < 4 ? a.angle_l1 : a.angle_deep) + row * 16 + 4 * (c & 3));
+    } else if constexpr (KIND == kTreeFast) {
+      p.codes[n] = *reinterpret_cast<const uint2v*>(a.angle_deep + row * kPairs + 8 * c);
     } else {
-      const uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(a.radii) + row * kPairs + 8 * c);
+      uint32_t w[2] = {0u, 0u};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = h2f((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int pair = 8 * c + i;
-      const bool l1 = pair < a.split_half;
-      const int bits = l1 ? a.l1_bits : a.deep_bits, bit = (l1 ? pair : pair - a.split_half) * bits;
-      const uint32_t byte = l1 ? a.angle_l1[row * a.l1_row + (bit >> 3)] : a.angle_deep[row * a.deep_row + (bit >> 3)];
-      const float2v cs = lut[(l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u))];
-      // Rounded to fp16 before they are compared: rounding keeps the order.
-      const half2v k = __builtin_convertvector((float2v{r[i] * cs.x, r[i] * cs.y}), half2v);
-      lo[i] = __builtin_elementwise_min(lo[i], k), hi[i] = __builtin_elementwise_max(hi[i], k);
+      for (int i = 0; i < 8; ++i) {
+        const int pair = 8 * c + i;
+        const bool l1 = pair < a.split_half;
+        const int bits = l1 ? a.l1_bits : a.deep_bits, bit = (l1 ? pair : pair - a.split_half) * bits;
+        const uint32_t byte = l1 ? a.angle_l1[row * a.l1_row + (bit >> 3)] : a.angle_deep[row * a.deep_row + (bit >> 3)];
+        w[i >> 2] |= ((byte >> (bit & 7)) & ((1u << bits) - 1u)) << (8 * (i & 3));
+      }
+      p.codes[n] = uint2v{w[0], w[1]};
     }
   }
-  auto other = [](half2v x, int d) { return __builtin_bit_cast(half2v, __shfl_xor(__builtin_bit_cast(int, x), d)); };
+  if constexpr (tree_i8(KIND)) p.ls = a.radii_scales[slot];
+}
+
+// The smallest of a wave's lanes of one c (lane % 8) for 16 registers: a swap of half of the lanes of two registers
+// joins them in one, which then holds the one's result in some lanes and the other's in the rest.  Register m of the
+// four that remain holds, in row r = lane / 16, that of x[4 m + joined_register(r)].
+__device__ __forceinline__ int joined_register(int row) { return ((row & 1) << 1) | (row >> 1); }
+__device__ __forceinline__ void smallest_of_tokens(const half2v (&x)[16], half2v (&z)[4]) {
+  auto smaller = [](uint32_t u, uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(half2v, u), __builtin_bit_cast(half2v, w)));
+  };
+  uint32_t y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int k = 0; k < 8; ++k) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x[2 * k]),
+                                                    __builtin_bit_cast(uint32_t, x[2 * k + 1]), false, false);
+    y[k] = smaller(p[0], p[1]);
+  }
 #pragma unroll
-    for (int d = 8; d < 64; d <<= 1) {
-      lo[i] = __builtin_elementwise_min(lo[i], other(lo[i], d));
-      hi[i] = __builtin_elementwise_max(hi[i], other(hi[i], d));
+  for (int m = 0; m < 4; ++m) {
+    const auto p = __builtin_amdgcn_permlane16_swap(y[2 * m], y[2 * m + 1], false, false);
+    const uint32_t w = smaller(p[0], p[1]);
+    z[m] = __builtin_bit_cast(half2v, smaller(w, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, true)));  // row_ror:8
+  }
+}
+
+// A workgroup walks over pages of a (batch, head) row, one ahead in registers; the bounds are joined over the wave's
+// tokens in registers and over the waves in LDS.  Bound by the reads of the key fields: 4,096 pages of the default
+// layout, 42 MB.
+template <int KIND>
+__global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
+  __shared__ TreeLut lut;
+  __shared__ half2v side[2][4][2 * kPairs];  // smallest keys, then smallest negated keys
+  __shared__ float radius[tree_i8(KIND) ? 2 : 1][tree_i8(KIND) ? 256 : 1];  // of int8 codes, from -128 on
+  const int tid = threadIdx.x, c = tid & 7, lane = tid & 63, wave = tid >> 6;
+  const int64_t bh = blockIdx.y;
+  const int step = (int)gridDim.x;
+  BoundsRegs<KIND> next;
+  load_bounds<KIND>(a, bh * a.capacity + a.page_begin + blockIdx.x, tid, next);
+  build_tree_lut<KIND, kBoundsThreads>(a, lut, tid);
+  for (int i = blockIdx.x, buf = 0; i < a.n_pages; i += step, buf ^= 1) {
+    const BoundsRegs<KIND> p = next;
+    load_bounds<KIND>(a, bh * a.capacity + a.page_begin + min(i + step, a.n_pages - 1), tid, next);
+    if constexpr (tree_i8(KIND)) radius[buf][tid] = expf((float)(tid - 128) * h2f((uint16_t)p.ls));
+    if (tree_i8(KIND) || i == (int)blockIdx.x) lds_barrier();
+    half2v x[16];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float r;
+        if constexpr (tree_i8(KIND))
+          r = radius[buf][((p.r8[n][j >> 2] >> (8 * (j & 3))) + 128u) & 0xffu];
+        else
+          r = h2f((uint16_t)(p.r[n][j >> 1] >> (16 * (j & 1))));
+        uint32_t code;
+        if constexpr (KIND == kTreeDefault)
+          code = (p.codes[n].x >> (4 * j)) & 15u;
+        else
+          code = (KIND == kTreeFast || 8 * c + j >= a.split_half ? 256u : 0u) + ((p.codes[n][j >> 2] >> (8 * (j & 3))) & 0xffu);
+        const float2v cs = lut.code[code];
+        // Rounded to fp16 before they are compared: rounding keeps the order.
+        const half2v k = __builtin_convertvector((float2v{r * cs.x, r * cs.y}), half2v);
+        x[j] = n ? __builtin_elementwise_min(x[j], k) : k;
+        x[8 + j] = n ? __builtin_elementwise_min(x[8 + j], -k) : -k;
+      }
+    half2v z[4];
+    smallest_of_tokens(x, z);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int at = 4 * m + joined_register(lane >> 4);
+      if (!(lane & 8)) side[buf][wave][(at & 8) * (kPairs / 8) + 8 * c + (at & 7)] = z[m];
     }
-  if (lane < 8)
+    lds_barrier();
+    if (tid < 2 * kPairs) {
+      half2v y = side[buf][0][tid];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) side[wave][0][8 * c + i] = lo[i], side[wave][1][8 * c + i] = hi[i];
-  __syncthreads();
-  if (tid >= 128) return;
-  const int which = tid >> 6, d = tid & 63;
-  half2v x = side[0][which][d];
-#pragma unroll
-  for (int w = 1; w < 4; ++w)
-    x = which ? __builtin_elementwise_max(x, side[w][1][d]) : __builtin_elementwise_min(x, side[w][0][d]);
-  reinterpret_cast<half2v*>(a.bounds + (bh * a.bounds_capacity + page) * 2 * kHeadDim)[tid] = x;
+      for (int w = 1; w < 4; ++w) y = __builtin_elementwise_min(y, side[buf][w][tid]);
+      reinterpret_cast<half2v*>(a.bounds + (bh * a.bounds_capacity + a.page_begin + i) * 2 * kHeadDim)[tid] = tid < kPairs ? y : -y;
+    }
+  }
 }
 
 struct SelectArgs {
@@ -149,6 +207,33 @@ __device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, 
   return score_key(any_nan ? (double)INFINITY : best);
 }
 
+// The sum over lanes 0 .. this one.
+__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // row_shr:1, 2, 4, 8
+  add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // row_bcast:15, to rows 1 and 3
+  add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // row_bcast:31, to rows 2 and 3
+  return x;
+}
+
+// All lanes' bits, in every lane.
+__device__ __forceinline__ uint32_t wave_or(uint32_t x) {
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true);  // row_ror:1, 2, 4, 8
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true);
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = p[0] | p[1];
+  const auto q = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return q[0] | q[1];
+}
+
 // A workgroup of each 64 pages of a (batch, kv head) scores them; the last of them to be done selects: the `take`-th
 // largest key by its digits of 8 bits from the first in which the keys differ, then the pages above it, and the first
 // of those that equal it, in their order.  PER: keys of a thread, held in registers (0: more, read anew each time).
@@ -157,10 +242,10 @@ template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs a) {
   __shared__ __align__(16) float qs[kScoreHeads][kHeadDim];
   __shared__ uint32_t hist[256];
-  __shared__ uint64_t ends[2][kSelectWaves];
+  __shared__ uint32_t ends[2][kSelectWaves];
   __shared__ uint64_t found;
   __shared__ int32_t found_rest, found_all, is_last;
-  __shared__ int32_t counts[2][kSelectWaves];
+  __shared__ int32_t counts[2][PER ? PER : 2][kSelectWaves];  // pages above the prefix, and equal to it
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t unit = blockIdx.y;
   uint64_t* keys = a.keys + unit * a.count;
@@ -177,6 +262,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     if (!is_last) return;
     if (tid == 0) __hip_atomic_store(a.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
+  if (tid < 256) hist[tid] = 0;
   for (int i = tid; i < a.first; i += kSelectThreads) out[i] = i;
   for (int i = tid; i < a.last; i += kSelectThreads) out[a.first + a.take + i] = a.n_pages - a.last + i;
   if (a.take == 0) return;
@@ -185,6 +271,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     for (int i = tid; i < a.count; i += kSelectThreads) out[i] = a.first + i;
     return;
   }
+  __syncthreads();
   auto load = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
   uint64_t mine[PER ? PER : 1];
   if constexpr (PER)
@@ -199,32 +286,21 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
       for (int i = tid; i < a.count; i += kSelectThreads) use(load(i));
     }
   };
-  uint64_t low = ~0ull, high = 0;
-  each_key([&](uint64_t k) {
-    low = k < low ? k : low;
-    high = k > high ? k : high;
-  });
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t x = __shfl_xor((unsigned long long)low, d), y = __shfl_xor((unsigned long long)high, d);
-    low = x < low ? x : low;
-    high = y > high ? y : high;
-  }
-  if (lane == 0) ends[0][wave] = low, ends[1][wave] = high;
+  const uint64_t one = load(0);
+  uint64_t differ = 0;
+  each_key([&](uint64_t k) { differ |= k ^ one; });
+  const uint32_t differ_lo = wave_or((uint32_t)differ), differ_hi = wave_or((uint32_t)(differ >> 32));
+  if (lane == 0) ends[0][wave] = differ_lo, ends[1][wave] = differ_hi;
   __syncthreads();
-  for (int w = 0; w < kSelectWaves; ++w) {
-    low = ends[0][w] < low ? ends[0][w] : low;
-    high = ends[1][w] > high ? ends[1][w] : high;
-  }
+  differ = 0;
+  for (int w = 0; w < kSelectWaves; ++w) differ |= (uint64_t)ends[1][w] << 32 | ends[0][w];
   // Keys agree above bit `shift`; the digits found so far are `prefix`, the keys' bits from there on.
-  int shift = low == high ? 0 : 64 - __builtin_clzll(low ^ high);
-  uint64_t prefix = shift == 64 ? 0 : high >> shift;
+  int shift = differ ? 64 - __builtin_clzll(differ) : 0;
+  uint64_t prefix = shift == 64 ? 0 : one >> shift;
   int32_t rest = a.take;
   bool all = false;  // whether every key with the prefix is taken
   while (shift > 0 && !all) {
     const int width = min(shift, 8), next = shift - width;
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
     each_key([&](uint64_t k) {
       if (shift == 64 || (k >> shift) == prefix) atomicAdd(&hist[(uint32_t)(k >> next) & ((1u << width) - 1u)], 1u);
     });
@@ -233,12 +309,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
       uint32_t n[4], sum = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) n[j] = hist[255 - 4 * lane - j], sum += n[j];
-      uint32_t above = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t x = __shfl_up(above, d);
-        above += lane >= d ? x : 0u;
-      }
+      uint32_t above = wave_sum_up_to(sum);
       above -= sum;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -255,38 +326,59 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     rest = found_rest;
     all = found_all != 0;
     shift = next;
+    if (shift > 0 && !all) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+    }
   }
   // Above the prefix: taken; equal to it: the first `rest` of them (all of them where `all`).
-  int32_t base = 0, equal_base = 0;
-  auto place = [&](int i, uint64_t key) {
+  const uint64_t below = (1ull << lane) - 1ull;
+  auto compare = [&](int i, uint64_t key, uint64_t& over, uint64_t& equal) {
     const uint64_t k = key >> shift;
-    const bool over = i < a.count && k > prefix, equal = i < a.count && k == prefix;
-    const uint64_t equals = __ballot(equal), below = (1ull << lane) - 1ull;
-    if (lane == 0) counts[0][wave] = __popcll(equals);
-    __syncthreads();
-    int32_t rank = equal_base + __popcll(equals & below), equal_all = 0;
-    for (int w = 0; w < kSelectWaves; ++w) {
-      rank += w < wave ? counts[0][w] : 0;
-      equal_all += counts[0][w];
-    }
-    const bool taken = over || (equal && rank < rest);
-    const uint64_t takes = __ballot(taken);
-    if (lane == 0) counts[1][wave] = __popcll(takes);
-    __syncthreads();
-    int32_t at = base + __popcll(takes & below), taken_all = 0;
-    for (int w = 0; w < kSelectWaves; ++w) {
-      at += w < wave ? counts[1][w] : 0;
-      taken_all += counts[1][w];
-    }
-    if (taken) out[at] = a.first + i;
-    base += taken_all;
-    equal_base += equal_all;
+    over = __ballot(i < a.count && k > prefix);
+    equal = __ballot(i < a.count && k == prefix);
+  };
+  // Page i, with `over` and `equal` the wave's, and how many of either lie before the wave.
+  auto place = [&](int i, uint64_t over, uint64_t equal, int32_t overs, int32_t equals) {
+    overs += __popcll(over & below);
+    equals += __popcll(equal & below);
+    const bool is_equal = (equal >> lane) & 1u;
+    if (((over >> lane) & 1u) || (is_equal && equals < rest)) out[overs + min(equals, rest)] = a.first + i;
   };
   if constexpr (PER) {
+    uint64_t over[PER], equal[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) place(tid + kSelectThreads * j, mine[j]);
+    for (int j = 0; j < PER; ++j) {
+      compare(tid + kSelectThreads * j, mine[j], over[j], equal[j]);
+      if (lane == 0) counts[0][j][wave] = __popcll(over[j]), counts[1][j][wave] = __popcll(equal[j]);
+    }
+    __syncthreads();
+    int32_t overs = 0, equals = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      int32_t before[2] = {overs, equals};
+      for (int w = 0; w < kSelectWaves; ++w) {
+        const int32_t x = counts[0][j][w], y = counts[1][j][w];
+        before[0] += w < wave ? x : 0, before[1] += w < wave ? y : 0;
+        overs += x, equals += y;
+      }
+      place(tid + kSelectThreads * j, over[j], equal[j], before[0], before[1]);
+    }
   } else {
-    for (int i0 = 0; i0 < a.count; i0 += kSelectThreads) place(i0 + tid, load(min(i0 + tid, a.count - 1)));
+    int32_t overs = 0, equals = 0;
+    for (int i0 = 0, buf = 0; i0 < a.count; i0 += kSelectThreads, buf ^= 1) {
+      uint64_t over, equal;
+      compare(i0 + tid, load(min(i0 + tid, a.count - 1)), over, equal);
+      if (lane == 0) counts[0][buf][wave] = __popcll(over), counts[1][buf][wave] = __popcll(equal);
+      __syncthreads();
+      int32_t before[2] = {overs, equals};
+      for (int w = 0; w < kSelectWaves; ++w) {
+        const int32_t x = counts[0][buf][w], y = counts[1][buf][w];
+        before[0] += w < wave ? x : 0, before[1] += w < wave ? y : 0;
+        overs += x, equals += y;
+      }
+      place(i0 + tid, over, equal, before[0], before[1]);
+    }
   }
 }
 
@@ -326,12 +418,23 @@ extern "C" int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* 
   a.l1_bits = layout->l1_bits, a.deep_bits = layout->deep_bits, a.split_half = layout->split_dim / 2;
   a.l1_row = l1_row, a.deep_row = deep_row;
   a.bounds = static_cast<uint16_t*>(bounds);
-  const dim3 grid((unsigned)n_pages, (unsigned)bh);
+  a.n_pages = n_pages;
+  // As many workgroups as the GPU holds, eight a CU.
+  const int64_t most = std::max<int64_t>(1, 2048 / bh);
+  const dim3 grid((unsigned)std::min<int64_t>(n_pages, most), (unsigned)bh);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (layout->int8_radii)
-    hipLaunchKernelGGL(page_bounds_kernel<true>, grid, dim3(kBoundsThreads), 0, s, a);
+  // The runtime's two layouts; their code words are read whole.
+  const bool def = !layout->int8_radii && layout->l1_bits == 4 && layout->deep_bits == 4 && layout->split_dim == 64 &&
+                   !(((uintptr_t)pages->angle_l1 | (uintptr_t)pages->angle_deep) & 3u);
+  const bool fast = layout->int8_radii && layout->deep_bits == 8 && layout->split_dim == 0 && !((uintptr_t)pages->angle_deep & 7u);
+  if (def)
+    hipLaunchKernelGGL(page_bounds_kernel<kTreeDefault>, grid, dim3(kBoundsThreads), 0, s, a);
+  else if (fast)
+    hipLaunchKernelGGL(page_bounds_kernel<kTreeFast>, grid, dim3(kBoundsThreads), 0, s, a);
+  else if (layout->int8_radii)
+    hipLaunchKernelGGL(page_bounds_kernel<kTreeAnyI8>, grid, dim3(kBoundsThreads), 0, s, a);
   else
-    hipLaunchKernelGGL(page_bounds_kernel<false>, grid, dim3(kBoundsThreads), 0, s, a);
+    hipLaunchKernelGGL(page_bounds_kernel<kTreeAnyF16>, grid, dim3(kBoundsThreads), 0, s, a);
   return launch_status("tp_page_bounds");
 }
 
