@@ -341,5 +341,79 @@ def test_streams_and_graphs(device):
     assert call(1).shape == (1, 32, 128)
 
 
+def test_bounds_taken_on_another_stream(device):
+    """A call on one stream takes the bounds of all pages behind other work; one on a second stream, right after it,
+    waits for them."""
+    cache = filled(device, "default", 2, 8, 2, 64 * 300 + 9, seed=1)
+    twin = cache.fork()
+    q = queries(device, 2, 8, 1)[:, :, None]
+    want = twin.selected_attention(q, 0.1, 20, 1, 2)
+    x = torch.randn(4096, 4096, device=device)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    with torch.cuda.stream(streams[0]):
+        for _ in range(20):
+            x = x @ x * 1e-3
+        outs.append(cache.selected_attention(q, 0.1, 20, 1, 2))
+    with torch.cuda.stream(streams[1]):
+        outs.append(cache.selected_attention(q, 0.1, 20, 1, 2))
+    torch.cuda.synchronize()
+    # Grown and extended on the second stream, read on the first and on the default one.
+    k, v = (torch.from_numpy(t).to(device) for t in gen_kv(3, 2, 2, 64 * 400))
+    cache.runtime.append(k, v), twin.runtime.append(k, v)
+    later = twin.selected_attention(q, 0.1, 20, 1, 2)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[1]):
+        for _ in range(20):
+            x = x @ x * 1e-3
+        outs.append(cache.selected_attention(q, 0.1, 20, 1, 2))
+    with torch.cuda.stream(streams[0]):
+        outs.append(cache.selected_attention(q, 0.1, 20, 1, 2))
+    outs.append(cache.selected_attention(q, 0.1, 20, 1, 2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs[:2]) and all(torch.equal(o, later) for o in outs[2:])
+
+
+def test_graphs_of_whole_caches(device):
+    """Caches of no more pages than a call takes are attended whole; two graphs of such calls share no workspace."""
+    caches = [filled(device, "default", 2, 8, 2, 64 * 200 + 9, seed=1), filled(device, "fast", 1, 32, 8, 64 * 150, seed=2)]
+    qs = [queries(device, 2, 8, 1)[:, :, None], queries(device, 1, 32, 2)[:, :, None]]
+    call = lambda i: caches[i].selected_attention(qs[i], 0.1, 500, 1, 2)  # noqa: E731
+    for i in (0, 1):
+        call(i)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in (0, 1):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([call(i) for _ in range(4)])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed in range(4):
+        for i in (0, 1):
+            qs[i].copy_(queries(device, qs[i].shape[0], qs[i].shape[1], 10 + seed)[:, :, None])
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            want = call(i)
+            assert all(torch.equal(o, want) for o in outs[i])
+
+
+def test_float32_caches(device):
+    """Tokens appended in float32 stay so in the dense tail: attended as their rounding to fp16, which these are."""
+    cache = TurboPolarFastCache(TurboPolarConfig(num_q_heads=8, num_kv_heads=2))
+    k, v = (torch.from_numpy(t).to(device) for t in gen_kv(3, 2, 2, 64 * 20 + 33))
+    cache.runtime.append(k.float(), v.float())
+    assert cache.runtime._tail_k.dtype is torch.float32 and torch.equal(k.half().float(), k.float())
+    q = queries(device, 2, 8, 4)
+    scale = cache.config.attention_scale
+    want = chosen64(scores64(q, cache.runtime.page_bounds())[0], 6, 1, 1)
+    close(cache.selected_attention(q[:, :, None], scale, 6), attended(q, cache, want, fp16_scale(scale)), "float32")
+
+
 def test_oracle_layouts_are_all_covered():
     assert {c[0] for c in CASES} == set(LAYOUTS) and oracle is not None

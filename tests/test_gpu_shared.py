@@ -221,3 +221,31 @@ def test_own_tokens_by_a_launch_of_their_own(device, layout):
     for B, hq, hkv, prefix, own in ((12, 32, 8, 70, 64 * 65), (33, 8, 1, 130, 200), (40, 16, 4, 64, 70)):
         cache, q = made(device, layout, B, hq, hkv, prefix, own, seed=B)
         check(cache.attention(q, 0.09), q, cache, 0.09, f"{layout} {B} {hq} {hkv} {prefix} {own}")
+
+
+def test_a_refused_step_leaves_the_sequences(device):
+    cache, q = made(device, "default", 3, 8, 2, 100, 70)
+    new = torch.ones(3, 2, 1, 128, device=device).half()
+    for args in ((q[:, :7], new, new, 0.1), (q, new, new, float("inf")), (q.clone().requires_grad_(), new, new, 0.1),
+                 (q.cpu(), new, new, 0.1), (q[..., :64], new, new, 0.1), (q.long(), new, new, 0.1)):
+        with pytest.raises(ValueError):
+            cache.decode_attention(*args)
+        assert cache.offset == 170
+    with pytest.raises(ValueError):  # the first step's batch too
+        SharedPrefixCache(cache.prefix).decode_attention(q[:, :7], new, new, 0.1)
+    with pytest.raises(ValueError, match="one HIP device"):
+        SharedPrefixCache(cache.prefix).decode_attention(q, new.cpu(), new.cpu(), 0.1)
+    assert cache.decode_attention(q, new, new, 0.1).shape == (3, 8, 128) and cache.offset == 171
+
+
+def test_float32_caches(device):
+    """Tokens appended in float32 stay so in the dense tail: attended as their rounding to fp16, which these are."""
+    cache, q = made(device, "default", 3, 8, 2, 100, 70, seed=4)
+    wide = SharedPrefixCache(TurboPolarFastCache(cache.config), TurboPolarFastCache(cache.config))
+    for seed, c, B, T in ((5, wide.prefix, 1, 100), (6, wide.own, 3, 70)):
+        k, v = (torch.from_numpy(t).to(device) for t in gen_kv(seed, B, 2, T))
+        assert torch.equal(k.half().float(), k.float())
+        c.runtime.append(k.float(), v.float())
+    wide = SharedPrefixCache(wide.prefix, wide.own)  # counts the prefix's tokens
+    assert wide.own.runtime._tail_k.dtype is torch.float32
+    check(wide.attention(q, 0.1), q, wide, 0.1, "float32")

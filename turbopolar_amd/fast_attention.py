@@ -192,7 +192,8 @@ class TurboPolarFastCache:
         stored = self._store_pages() if n_pages else None
         if n_pages <= pages:
             tail_k, tail_v = rt._tail_views()
-            return decode_attention_store(q[:, :, 0], layout, stored, n_pages, H, tail_k, tail_v, rt.actual_seq_len, scale)
+            return decode_attention_store(q[:, :, 0], layout, stored, n_pages, H, tail_k, tail_v, rt.actual_seq_len, scale,
+                                          own_workspace=True)
         bounds = rt.page_bounds()
         return selected_attention(q[:, :, 0], layout, stored, n_pages, H, bounds, int(rt._bounds.shape[2]),
                                   tail_args(rt._tail_k, rt._tail_v, rt._tail_len), scale, pages, first, last)[0]

@@ -324,6 +324,18 @@ class _Workspace:
         return buf
 
 
+def _stream_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    return _Workspace.get(device, nbytes, stream)
+
+
+def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """The split-K workspace of the stream; one of its own inside a captured graph, whose replays may run beside
+    those of another graph or eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return _Workspace.get(device, nbytes, stream)
+
+
 @lru_cache(maxsize=1024)
 def _workspace_bytes(B: int, Hq: int, Hkv: int, n_pages: int, pps: int) -> int:
     """tp_decode_workspace_bytes (its size does not depend on the tail)."""
@@ -382,7 +394,7 @@ _NO_PAGES = TPPages()
 
 
 def _launch_decode(q16, Hkv, layout, pages, n_pages, tk, tv, tail_len, tail_stride, seq_len, scale, pps, out,
-                   qjl=None):
+                   qjl=None, workspace=_stream_workspace):
     B, Hq, _ = q16.shape
     dev = q16.device
     if out is None:
@@ -390,7 +402,7 @@ def _launch_decode(q16, Hkv, layout, pages, n_pages, tk, tv, tail_len, tail_stri
     L = lib()
     pps = int(pps)  # 0: the library's default
     stream = stream_handle(dev)
-    ws = _Workspace.get(dev, _workspace_bytes(B, Hq, Hkv, n_pages, pps), stream)
+    ws = workspace(_workspace_bytes(B, Hq, Hkv, n_pages, pps), dev, stream)
     head = (ptr(q16), B, Hq, Hkv, ctypes.byref(layout), ctypes.byref(pages), n_pages)
     rest = (None if tk is None else tk.data_ptr(), None if tv is None else tv.data_ptr(), tail_len, tail_stride,
             int(seq_len), float(scale), pps, ws.data_ptr(), ws.numel(), ptr(out), stream)
@@ -461,11 +473,12 @@ def decode_attention_dense_v(
 
 def decode_attention_store(q: torch.Tensor, layout, pages: TPPages, n_pages: int, num_kv_heads: int,
                            tail_k: Optional[torch.Tensor], tail_v: Optional[torch.Tensor], seq_len: int,
-                           scale: float) -> torch.Tensor:
+                           scale: float, own_workspace: bool = False) -> torch.Tensor:
     """A cache's decode step: ``tp_decode_attention`` over the first ``n_pages``
     slots of a page store used in place (``pages`` carries its capacity) and a
     dense tail given as ``[B, H_kv, T, 128]`` views of a token-major buffer
-    (``T`` < 64).  ``q`` is ``[B, H_q, 128]``."""
+    (``T`` < 64).  ``q`` is ``[B, H_q, 128]``.  ``own_workspace``: inside a captured
+    graph the workspace is the graph's (``_zeroed_workspace``)."""
     q16 = _q16(q)
     tail_len = 0 if tail_k is None else int(tail_k.shape[2])
     tk = tv = None
@@ -475,7 +488,7 @@ def decode_attention_store(q: torch.Tensor, layout, pages: TPPages, n_pages: int
     if pages is None:
         pages, n_pages = _NO_PAGES, 0
     return _launch_decode(q16, num_kv_heads, layout, pages, n_pages, tk, tv, tail_len, tail_stride, seq_len, scale,
-                          0, None)
+                          0, None, workspace=_zeroed_workspace if own_workspace else _stream_workspace)
 
 
 @lru_cache(maxsize=1024)
@@ -974,14 +987,6 @@ def check_selection(pages: int, first: int, last: int) -> None:
 def _selection_workspace(B: int, Hq: int, Hkv: int, n_pages: int, count: int) -> int:
     """What tp_select_pages and tp_selected_attention take, one after the other."""
     return max(int(lib().tp_select_workspace_bytes(B, Hq, Hkv, n_pages)), _workspace_bytes(B, Hq, Hkv, count, 0))
-
-
-def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    """The split-K workspace of the stream; one of its own inside a captured graph, whose replays may run beside
-    those of another graph or eager calls."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return _Workspace.get(device, nbytes, stream)
 
 
 def selected_attention(q: torch.Tensor, layout, pages: TPPages, n_pages: int, num_kv_heads: int, bounds: torch.Tensor,

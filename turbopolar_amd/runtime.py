@@ -28,6 +28,7 @@ from typing import Any, Dict, NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
+from ._lib import stream_handle
 from .codecs import GroupedVQuantizer, PolarQuantDecoder, PolarQuantEncoder
 from .config import TurboPolarConfig
 from .kernels import (
@@ -107,6 +108,7 @@ class TurboPolarKVCacheRuntime:
         self._scratch = None  # one-page store for the padded tail when the storage is full
         self._bounds: Optional[torch.Tensor] = None  # key bounds of the stored pages, [B, H, capacity, 2, 128]
         self._bounds_pages = 0  # of how many
+        self._bounds_on: Optional[tuple] = None  # the stream that wrote the last of them, an event behind it
         self._epoch = 0
         # Appends whose non-finite verdict is deferred (append(..., defer_check=True)):
         # (epoch, state before the append), oldest first.
@@ -657,7 +659,8 @@ class TurboPolarKVCacheRuntime:
     def page_bounds(self) -> torch.Tensor:
         """The smallest and the largest of each decoded key component over every stored page: fp16 ``[B, H, pages, 2,
         128]``, a view valid until the next append.  Kept (512 bytes a page and head), so a call reads only the pages
-        stored since the last one (tp_page_bounds).  No counterpart in the reference."""
+        stored since the last one (tp_page_bounds); a call on another stream than theirs waits there for what is still
+        under way.  No counterpart in the reference."""
         if self._pending:
             self.resolve_deferred_check()
         ks = self.k_storage
@@ -667,6 +670,10 @@ class TurboPolarKVCacheRuntime:
         if held < n and ks.radii.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the bounds of new pages cannot be taken inside a captured graph; call page_bounds() before it")
         B, H = self._batch_size, self._num_kv_heads
+        if held and self._bounds_on[0] != stream_handle(ks.radii.device) and not torch.cuda.is_current_stream_capturing():
+            # A call that only reads the cache wrote them, so its user knows of nothing to wait for.
+            torch.cuda.current_stream(ks.radii.device).wait_event(self._bounds_on[1])
+            self._bounds.record_stream(torch.cuda.current_stream(ks.radii.device))
         if self._bounds is None or self._bounds.shape[2] < n:
             grown = torch.empty((B, H, ks.capacity, 2, HEAD_DIM), dtype=torch.float16, device=ks.radii.device)
             if held:
@@ -677,6 +684,8 @@ class TurboPolarKVCacheRuntime:
         if held < n:
             page_bounds_into(self.polar_encoder.layout, pages_of(ks, self.v_storage), B * H, held, n - held, self._bounds)
             self._bounds_pages = n
+            stream = torch.cuda.current_stream(ks.radii.device)
+            self._bounds_on = stream.cuda_stream, stream.record_event()
         return self._bounds[:, :, :n]
 
     def get_io_telemetry(self) -> Dict[str, Any]:
@@ -903,6 +912,7 @@ class TurboPolarKVCacheRuntime:
         self._fused_views = None
         self._bounds = None
         self._bounds_pages = 0
+        self._bounds_on = None
         self._pending = []
         self._initialized = False
         self._batch_size = None

@@ -8,6 +8,7 @@ batch B).  No counterpart in the reference, which keeps one line of tokens per c
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -84,6 +85,21 @@ class SharedPrefixCache:
         """One decode step's attention: the queries ``q`` ``[B, H_q, 1, 128]`` over the prefix and each sequence's own
         tokens (tp_shared_attention; ``scale`` taken as fp16, as for ``TurboPolarFastCache.decode_attention``).
         Returns fp16 ``[B, H_q, 128]``."""
+        scale = self._check_step(q, scale)
+        if not self.offset:
+            raise ValueError("nothing to attend: the prefix and the sequences hold no tokens")
+        return self._attend(q, scale)
+
+    def _attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
+        parts = []
+        for cache in (self.prefix, self.own):
+            rt = cache.runtime
+            n_pages, tokens = rt.k_storage.block_count, rt._tail_len
+            parts.append((cache._store_pages() if n_pages else None, n_pages, tail_args(rt._tail_k, rt._tail_v, tokens)))
+        return shared_attention(q, self.prefix.runtime.polar_encoder.layout, self.config.num_kv_heads, *parts, scale)
+
+    def _check_step(self, q: torch.Tensor, scale: float) -> float:
+        """The checks of a step's queries against what is held; ``scale`` in fp16."""
         if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[2] != 1 or q.shape[-1] != HEAD_DIM:
             raise ValueError(f"q must be [B, H_q, 1, {HEAD_DIM}], got {tuple(getattr(q, 'shape', ()))}")
         if not q.is_floating_point():
@@ -92,25 +108,27 @@ class SharedPrefixCache:
         if B < 1 or Hq < 1 or Hq % heads:
             raise ValueError(f"H_q={Hq} is not a multiple of H_kv={heads}, or the batch is empty")
         self._check_prefix()
-        if not self.offset:
-            raise ValueError("nothing to attend: the prefix and the sequences hold no tokens")
-        parts = []
+        scale = fp16_scale(scale)
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
         for name, cache, rows in (("prefix", self.prefix, 1), ("own cache", self.own, B)):
             rt = cache.runtime
             rt.resolve_deferred_check()
             if rt.actual_seq_len and rt._batch_size != rows:
                 raise ValueError(f"batch of q ({B}) and of the {name} ({rt._batch_size}) do not match")
-            n_pages, tokens = rt.k_storage.block_count, rt._tail_len
-            held = rt.k_storage.radii if n_pages else rt._tail_k
-            if (n_pages or tokens) and (held.device != q.device or not q.is_cuda):
+            held = rt.k_storage.radii if rt.k_storage.block_count else rt._tail_k
+            if rt.actual_seq_len and (held.device != q.device or not q.is_cuda):
                 raise ValueError(f"q is on {q.device}, the {name} on {held.device}; need one HIP device")
-            parts.append((cache._store_pages() if n_pages else None, n_pages, tail_args(rt._tail_k, rt._tail_v, tokens)))
         _no_grad(q)
-        return shared_attention(q, self.prefix.runtime.polar_encoder.layout, heads, *parts, fp16_scale(scale))
+        return scale
 
     def decode_attention(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, scale: float) -> torch.Tensor:
-        """Appends a token to each sequence (``[B, H_kv, 1, 128]``) and attends."""
+        """Appends a token to each sequence (``[B, H_kv, 1, 128]``) and attends; a refused call leaves the sequences as
+        they were."""
         if k_new.dim() != 4 or k_new.shape[2] != 1 or q.dim() != 4 or q.shape[0] != k_new.shape[0]:
             raise ValueError("decode_attention only supports a single query/key/value token")
+        scale = self._check_step(q, scale)
+        if k_new.device != q.device or not q.is_cuda:
+            raise ValueError(f"q is on {q.device}, the new token on {k_new.device}; need one HIP device")
         self.append(k_new, v_new)
-        return self.attention(q, scale)
+        return self._attend(q, scale)
