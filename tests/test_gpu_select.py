@@ -13,7 +13,7 @@ import oracle
 from common import ATOL, LAYOUTS, PAGE, RTOL_L2, gen_kv, rel_l2, within_f16_ulp
 from test_gpu_rotate import draw, tables
 from test_gpu_tree import filled, pages64
-from turbopolar_amd import HipKernelBridge, TurboPolarConfig, TurboPolarFastCache
+from turbopolar_amd import HipKernelBridge, TurboPolarConfig, TurboPolarFastCache, _lib
 from turbopolar_amd.kernels import fp16_scale, selected_attention, tail_args
 
 pytestmark = pytest.mark.gpu
@@ -185,6 +185,33 @@ def test_many_equal_scores_among_others(device):
         for n in (1, 999, 1000, 1024, 1025, 2500, 2999):
             got = bridge_call(cache, q, bounds, n, 0, 0)[1]
             assert np.array_equal(got.cpu().numpy(), chosen64(scores, n, 0, 0)), (values, n)
+
+
+@pytest.mark.parametrize("S", [1, 64, 65, 511, 512, 513, 2047, 2048, 2049, 4096, 4097, 8191, 8192, 8193, 9001])
+def test_any_number_of_pages(device, S):
+    """The entry point alone, around the numbers of pages at which the kernel takes another form, and one call right
+    behind another in one workspace."""
+    B, hq, hkv = 2, 6, 2
+    g = torch.Generator(device=device).manual_seed(S)
+    bounds = torch.randn((B, hkv, S, 2, 128), generator=g, device=device).sort(dim=3).values.half().contiguous()
+    q = queries(device, B, hq, S)
+    scores, err = scores64(q, bounds)
+    L = _lib.lib()
+    ws = torch.zeros(int(L.tp_select_workspace_bytes(B, hq, hkv, S)), dtype=torch.uint8, device=device)
+    asked = [(min(S, n), min(f, S), min(la, S - min(f, S))) for n, f, la in ((1, 0, 0), (33, 1, 2), (S // 3 + 3, 2, 1), (S, 0, 1))]
+    outs = []
+    for n, first, last in asked:
+        outs.append(torch.full((B, hkv, n), -1, dtype=torch.int32, device=device))
+        st = L.tp_select_pages(q.data_ptr(), B, hq, hkv, bounds.data_ptr(), S, S, first, min(last, n - first), n, 0.1,
+                               outs[-1].data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        assert st == 0
+    for (n, first, last), got in zip(asked, outs):
+        last = min(last, n - first)
+        between = np.sort(scores[:, :, first:S - last], axis=-1)[..., ::-1]
+        take = n - first - last
+        if 0 < take < between.shape[-1]:  # no score within rounding of the border: as the input was drawn
+            assert np.all(between[..., take - 1] - between[..., take] > 2 * err.max())
+        assert np.array_equal(got.cpu().numpy(), chosen64(scores, n, first, last)), (n, first, last)
 
 
 def test_negative_scales_and_bounds_that_are_not_finite(device):

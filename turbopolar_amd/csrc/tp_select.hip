@@ -95,8 +95,10 @@ __device__ __forceinline__ void smallest_of_tokens(const half2v (&x)[16], half2v
 }
 
 // A workgroup walks over pages of a (batch, head) row, one ahead in registers; the bounds are joined over the wave's
-// tokens in registers and over the waves in LDS.  Bound by the reads of the key fields: 4,096 pages of the default
-// layout, 42 MB.
+// tokens in registers and over the waves in LDS.  Every key field is read once, 10 KB a page of the default layout, and
+// 512 bytes are written: 4,096 pages (512 of 8 rows, 44 MB) take 11.6 us, 3.8 TB/s, 5.1 of a copy's; bound by that and
+// by the arithmetic, 8,192 products, roundings and comparisons a page (20.6 us with bytes read one by one and joined by
+// shuffles, 16 with whole words and a page ahead).  128 pages take 3.3 us, mostly a launch.
 template <int KIND>
 __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
   __shared__ TreeLut lut;
@@ -174,7 +176,17 @@ __device__ __forceinline__ uint64_t score_key(double s) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The key of the thread's page: 8 lanes a page, 16 dimensions a lane, the group's queries in LDS.
+template <int CTRL>
+__device__ __forceinline__ double moved(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The key of the thread's page: 8 lanes a page, 16 dimensions a lane, the group's queries in LDS.  Two heads at a time,
+// whose sums are chains of their own, joined by lane moves: 16 rows of 32/8 heads and 2,045 pages (134 MB of bounds) 57
+// us against 68 with one head and shuffles.
 __device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, int page, int tid, float (*qs)[kHeadDim]) {
   const int c = tid & 7;
   const uint16_t* b = a.bounds + (unit * a.capacity + page) * 2 * kHeadDim + 16 * c;
@@ -189,6 +201,7 @@ __device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, 
     for (int x = tid; x < heads * kHeadDim; x += kSelectThreads)
       qs[0][x] = h2f((uint16_t)(a.q[(unit * a.g + h0) * kHeadDim + x] ^ a.flip));
     __syncthreads();
+#pragma unroll 2
     for (int h = 0; h < heads; ++h) {
       double s = 0.0;
 #pragma unroll
@@ -198,8 +211,9 @@ __device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, 
         const uint32_t hi = (w[2 + (j >> 3)][(j >> 1) & 3] >> (16 * (j & 1))) & 0xffffu;
         s += (double)fmaxf(x * h2f((uint16_t)lo), x * h2f((uint16_t)hi));
       }
-#pragma unroll
-      for (int d = 1; d < 8; d <<= 1) s += __shfl_xor(s, d);
+      s += moved<0xb1>(s);   // quad_perm 1 0 3 2
+      s += moved<0x4e>(s);   // quad_perm 2 3 0 1
+      s += moved<0x141>(s);  // row_half_mirror: a lane of the other four
       any_nan = any_nan || s != s;
       best = s > best ? s : best;
     }
@@ -238,6 +252,10 @@ __device__ __forceinline__ uint32_t wave_or(uint32_t x) {
 // largest key by its digits of 8 bits from the first in which the keys differ, then the pages above it, and the first
 // of those that equal it, in their order.  PER: keys of a thread, held in registers (0: more, read anew each time).
 // Keys go out and come back past the caches of the XCDs (agent scope), between them a ticket.
+// Bound by its latencies: for one sequence of 32/8 heads 513 pages take 6.7 us, 2,045 pages (8.4 MB of bounds, 1.6 us
+// of a copy's time) 10.7, 4,096 17.5 and 8,192 30.6, of which the last workgroup's selection is 2 us a thousand pages;
+// two launches, one to score and one to select, took 11.2 and 14.8 us for the first two.  Keys in registers against
+// PER 0, us: 4,096 pages 17.5 (PER 8), 20.8 (16), 21.9; 8,192 30.6 (16), 41.0; 2,100 13.2 (8), 16.1 (16).
 template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs a) {
   __shared__ __align__(16) float qs[kScoreHeads][kHeadDim];
@@ -491,6 +509,10 @@ extern "C" int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int
     hipLaunchKernelGGL(select_pages_kernel<1>, grid, dim3(kSelectThreads), 0, s, a);
   else if (a.count <= 4 * kSelectThreads)
     hipLaunchKernelGGL(select_pages_kernel<4>, grid, dim3(kSelectThreads), 0, s, a);
+  else if (a.count <= 8 * kSelectThreads)
+    hipLaunchKernelGGL(select_pages_kernel<8>, grid, dim3(kSelectThreads), 0, s, a);
+  else if (a.count <= 16 * kSelectThreads)
+    hipLaunchKernelGGL(select_pages_kernel<16>, grid, dim3(kSelectThreads), 0, s, a);
   else
     hipLaunchKernelGGL(select_pages_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
   return launch_status("tp_select_pages");
