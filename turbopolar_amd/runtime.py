@@ -570,9 +570,11 @@ class TurboPolarKVCacheRuntime:
         else:
             sc = self._scratch
             if sc is None or sc["radii"].shape[:2] != (B, H) or sc["radii"].device != dev:
-                sc = self.polar_encoder.alloc_pages(B, H, 1, dev)
-                sc["v_codes"] = torch.zeros((B, H, 1, PAGE, self._head_dim), dtype=torch.int8, device=dev)
-                sc["v_scales"] = torch.zeros((B, H, 1, PAGE, self._head_dim // 32), dtype=torch.float16, device=dev)
+                # Not cleared: the encoder writes whole pages, as into the store's fresh slots.
+                sc = {name: None if spec is None else torch.empty((*spec[0], 1, *spec[1]), dtype=spec[2], device=dev)
+                      for name, spec in self.polar_encoder.page_shapes(B, H).items()}
+                sc["v_codes"] = torch.empty((B, H, 1, PAGE, self._head_dim), dtype=torch.int8, device=dev)
+                sc["v_scales"] = torch.empty((B, H, 1, PAGE, self._head_dim // 32), dtype=torch.float16, device=dev)
                 sc["pages"] = _lib.TPPages(
                     _lib.ptr(sc["radii"]), _lib.ptr(sc["radii_scales"]), _lib.ptr(sc["angle_codes_l1"]),
                     _lib.ptr(sc["angle_codes_deep"]), _lib.ptr(sc["v_codes"]), _lib.ptr(sc["v_scales"]), 1,
