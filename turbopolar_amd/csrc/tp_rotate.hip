@@ -79,7 +79,10 @@ __device__ __forceinline__ bool any_nonfinite(uint4v w) {
 }
 
 // A workgroup a token: 8 lanes share a head's row, each with 8 dimensions of either half of it (or 16 in a row),
-// and walk over the heads, 32 at a time, so that the token's tables are read once.
+// and walk over the heads, 32 at a time, so that the token's tables are read once.  Every element is read and written
+// once: bound by that.  4,100 tokens of 32/8 heads in bf16 (103 MB) take 18.2 us, 5.65 TB/s (partly in the caches);
+// 32,773 in fp16 with fp32 tables (839 MB) 175 us, 4.8 TB/s, where a copy reaches 5.1; a token 4 us, a launch's.  No faster:
+// accesses past the caches (187 us), runs of neighbouring tokens on one XCD (172 to 177).
 constexpr int kRotThreads = 256;
 constexpr int kRotRows = kRotThreads / 8;
 

@@ -89,13 +89,16 @@ class TurboPolarFastCache:
         v_out = torch.empty_like(k_out)
         layout = rt.polar_encoder.layout
         run = n_pages
+        full = n_pages == rt.k_storage.capacity
+        if run and full:  # the tail page has no free slot: the long launch goes first, the host's work runs under it
+            decode_pages_into(layout, self._store_pages(), B * H, 0, run, k_out, v_out, 0)
         if tail:
             pages, slot, in_storage = rt._partial_page_store()
             if in_storage:  # the tail page sits in the store's next free slot
                 run = n_pages + 1
             else:
                 decode_pages_into(layout, pages, B * H, slot, 1, k_out, v_out, n_pages * PAGE)
-        if run:
+        if run and not full:
             decode_pages_into(layout, self._store_pages(), B * H, 0, run, k_out, v_out, 0)
         k, v = k_out[:, :, : rt.actual_seq_len], v_out[:, :, : rt.actual_seq_len]
         if want != torch.float16:
