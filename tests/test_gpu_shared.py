@@ -249,3 +249,10 @@ def test_float32_caches(device):
     wide = SharedPrefixCache(wide.prefix, wide.own)  # counts the prefix's tokens
     assert wide.own.runtime._tail_k.dtype is torch.float32
     check(wide.attention(q, 0.1), q, wide, 0.1, "float32")
+
+
+def test_a_large_batch(device):
+    """More (sequence, head) rows than a workgroup takes, many times over."""
+    case = ("default", 700, 8, 2, 70, 3)
+    cache, q = made(device, *case, seed=8)
+    check(cache.attention(q, 0.1), q, cache, 0.1, f"{case}")
