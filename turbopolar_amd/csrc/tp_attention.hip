@@ -1240,7 +1240,8 @@ __device__ __forceinline__ void softmax_page(const float4v* s, int valid, float 
   }
   // m_run is still -inf only if every score of this page is -inf or NaN: then
   // -inf scores weigh 0 and NaN scores stay NaN, as in the reference's softmax.
-  const float m_use = (m_run == -INFINITY ? 0.0f : m_run) - (HEADROOM ? 7.0f : 0.0f);
+  float m_use = m_run == -INFINITY ? 0.0f : m_run;
+  if constexpr (HEADROOM) m_use -= 7.0f;
   float lsum = 0.0f;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
@@ -2008,15 +2009,19 @@ __global__ __launch_bounds__(WAVES * 64) void decode_attention_kernel(AttnArgs a
       if constexpr (QJL == kQjlAny)
         qjl_correct_any<HR>(a, bkv * a.qjl_capacity + page, l4, qjl_qw, HR ? (l16 & 7) : l16, qnorm, qjl_sin, s);
       if (it < 12) TP_STAMP(4 + 4 * it);
-      const int at_next = LIST ? next_page : page + WAVES;
-      load_k<KIND>(a, bkv * a.capacity + at_next, l16, l4, kr);
+      if constexpr (LIST)
+        load_k<KIND>(a, bkv * a.capacity + next_page, l16, l4, kr);
+      else
+        load_k<KIND>(a, bkv * a.capacity + page + WAVES, l16, l4, kr);
       half8v pb[2];
       softmax_page<HR, LIST>(s, kPageTokens, a.scale_log2, l4, m_run, l_run, acc, pb);
       pv_regs<HR, LIST>(vr, sbase4, ssel, pb, acc);
       if constexpr (DV)
         load_v<HR>(a, bkv * a.v_capacity + page + WAVES, l16, l4, lane, vr);
+      else if constexpr (LIST)
+        load_v<HR>(a, bkv * a.capacity + next_page, l16, l4, lane, vr);
       else
-        load_v<HR>(a, bkv * a.capacity + at_next, l16, l4, lane, vr);
+        load_v<HR>(a, bkv * a.capacity + page + WAVES, l16, l4, lane, vr);
       if constexpr (LIST) next_page = stored_page(a, bkv, min(page + 2 * WAVES, a.n_pages - 1));
       if (it < 12) TP_STAMP(5 + 4 * it);
     }

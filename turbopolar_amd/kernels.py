@@ -324,10 +324,6 @@ class _Workspace:
         return buf
 
 
-def _stream_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    return _Workspace.get(device, nbytes, stream)
-
-
 def _zeroed_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
     """The split-K workspace of the stream; one of its own inside a captured graph, whose replays may run beside
     those of another graph or eager calls."""
@@ -394,7 +390,7 @@ _NO_PAGES = TPPages()
 
 
 def _launch_decode(q16, Hkv, layout, pages, n_pages, tk, tv, tail_len, tail_stride, seq_len, scale, pps, out,
-                   qjl=None, workspace=_stream_workspace):
+                   qjl=None, own_workspace=False):
     B, Hq, _ = q16.shape
     dev = q16.device
     if out is None:
@@ -402,7 +398,8 @@ def _launch_decode(q16, Hkv, layout, pages, n_pages, tk, tv, tail_len, tail_stri
     L = lib()
     pps = int(pps)  # 0: the library's default
     stream = stream_handle(dev)
-    ws = workspace(_workspace_bytes(B, Hq, Hkv, n_pages, pps), dev, stream)
+    nbytes = _workspace_bytes(B, Hq, Hkv, n_pages, pps)
+    ws = _zeroed_workspace(nbytes, dev, stream) if own_workspace else _Workspace.get(dev, nbytes, stream)
     head = (ptr(q16), B, Hq, Hkv, ctypes.byref(layout), ctypes.byref(pages), n_pages)
     rest = (None if tk is None else tk.data_ptr(), None if tv is None else tv.data_ptr(), tail_len, tail_stride,
             int(seq_len), float(scale), pps, ws.data_ptr(), ws.numel(), ptr(out), stream)
@@ -488,7 +485,7 @@ def decode_attention_store(q: torch.Tensor, layout, pages: TPPages, n_pages: int
     if pages is None:
         pages, n_pages = _NO_PAGES, 0
     return _launch_decode(q16, num_kv_heads, layout, pages, n_pages, tk, tv, tail_len, tail_stride, seq_len, scale,
-                          0, None, workspace=_zeroed_workspace if own_workspace else _stream_workspace)
+                          0, None, own_workspace=own_workspace)
 
 
 @lru_cache(maxsize=1024)
