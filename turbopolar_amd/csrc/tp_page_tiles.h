@@ -82,6 +82,32 @@ __device__ __forceinline__ float2v angle_pair(uint32_t code, int bits) {
 // A pair's key, r (cos a, sin a), each rounded once.
 __device__ __forceinline__ uint32_t key_pair(float r, float2v cs) { return F16::pack(r * cs.x, r * cs.y); }
 
+// Of pair i of half h of run n: its code's place in the table, and its radius.  c is the thread's column, tid & 7.
+template <int KIND, int N, class Pages>
+__device__ __forceinline__ uint32_t pair_code(const Pages& a, const uint32_t* codes, const PageRegs<KIND, N>& p, int n,
+                                              int h, int i, int c, int t) {
+  if constexpr (KIND == kTreeDefault) {
+    return (p.c4[n] >> (16 * h + 4 * i)) & 15u;
+  } else if constexpr (KIND == kTreeFast) {
+    return 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
+  } else {
+    const int pair = 8 * c + 4 * h + i;
+    const bool l1 = pair < a.split_half;
+    const int bits = l1 ? a.l1_bits : a.deep_bits;
+    const int bit = (l1 ? pair : pair - a.split_half) * bits;
+    const int row = l1 ? t * a.l1_row : kPageTokens * a.l1_row + t * a.deep_row;
+    const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
+    return (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
+  }
+}
+template <int KIND, int N>
+__device__ __forceinline__ float pair_radius(const PageRegs<KIND, N>& p, int n, int h, int i, float ls) {
+  if constexpr (tree_i8(KIND))
+    return __builtin_amdgcn_exp2f((float)(int)(int8_t)(p.r8[n][h] >> (8 * i)) * ls);
+  else
+    return h2f((uint16_t)(p.r[n][2 * h + (i >> 1)] >> (16 * (i & 1))));
+}
+
 // Half h of run n, 4 pairs: their codes' (cos, sin) out of the table, and the keys, 16 bytes, into a tile.  Between
 // the two other work may go on, so that it does not wait for the table.
 template <int KIND, int N, int THREADS, class Pages>
@@ -91,23 +117,7 @@ __device__ __forceinline__ void fetch_angles(const Pages& a, const TreeLut& lut,
   int c0 = c;  // where a pair's code lies is computed anew: kept over the pages, it costs 30 registers
   if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t code;
-    if constexpr (KIND == kTreeDefault) {
-      code = (p.c4[n] >> (16 * h + 4 * i)) & 15u;
-    } else if constexpr (KIND == kTreeFast) {
-      code = 256 + ((p.c8[n][h] >> (8 * i)) & 0xffu);
-    } else {
-      const int pair = 8 * c0 + 4 * h + i;
-      const bool l1 = pair < a.split_half;
-      const int bits = l1 ? a.l1_bits : a.deep_bits;
-      const int bit = (l1 ? pair : pair - a.split_half) * bits;
-      const int row = l1 ? t * a.l1_row : kPageTokens * a.l1_row + t * a.deep_row;
-      const uint32_t byte = reinterpret_cast<const uint8_t*>(codes)[row + (bit >> 3)];
-      code = (l1 ? 0u : 256u) + ((byte >> (bit & 7)) & ((1u << bits) - 1u));
-    }
-    cs[i] = lut.code[code];
-  }
+  for (int i = 0; i < 4; ++i) cs[i] = lut.code[pair_code<KIND, N>(a, codes, p, n, h, i, c0, t)];
 }
 
 template <int KIND, int N, int THREADS>
@@ -117,23 +127,24 @@ __device__ __forceinline__ void store_keys(int tid, const PageRegs<KIND, N>& p, 
   const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;  // rounded in fp32, as its products below
   uint32_t e[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float r;
-    if constexpr (tree_i8(KIND))
-      r = __builtin_amdgcn_exp2f((float)(int)(int8_t)(p.r8[n][h] >> (8 * i)) * ls);
-    else
-      r = h2f((uint16_t)(p.r[n][2 * h + (i >> 1)] >> (16 * (i & 1))));
-    e[i] = key_pair(r, cs[i]);
-  }
+  for (int i = 0; i < 4; ++i) e[i] = key_pair(pair_radius<KIND, N>(p, n, h, i, ls), cs[i]);
   *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + h)) = uint4v{e[0], e[1], e[2], e[3]};
 }
 
 template <int KIND, int N, int THREADS, class Pages>
 __device__ __forceinline__ void decode_keys(const Pages& a, const TreeLut& lut, const uint32_t* codes, int tid,
                                             const PageRegs<KIND, N>& p, int n, int h, char* kt) {
-  float2v cs[4];
-  fetch_angles<KIND, N, THREADS>(a, lut, codes, tid, p, n, h, cs);
-  store_keys<KIND, N, THREADS>(tid, p, n, h, cs, kt);
+  const int c = tid & 7, t = (tid >> 3) + (THREADS / 8) * n;
+  int c0 = c;  // as in fetch_angles
+  if constexpr (tree_any(KIND)) asm volatile("" : "+v"(c0));
+  const float ls = tree_i8(KIND) ? h2f((uint16_t)p.ls) * kLog2e : 0.0f;
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2v cs = lut.code[pair_code<KIND, N>(a, codes, p, n, h, i, c0, t)];
+    e[i] = key_pair(pair_radius<KIND, N>(p, n, h, i, ls), cs);
+  }
+  *reinterpret_cast<uint4v*>(kt + tile_at(t, 2 * c + h)) = uint4v{e[0], e[1], e[2], e[3]};
 }
 
 // And into a tile of values: 8 codes.
