@@ -2,7 +2,7 @@
 
 Scores are float64 sums of 128 exact products, off by 127 2^-53 of the sum of their sizes on either side, so the
 selection has to be the definition's wherever the last page taken and the first one left differ by more than that
-(asserted for the inputs used).  Attention's error as in test_gpu_attention: BASELINE's tolerances, max-abs 2e-3 (for
+(asserted for the inputs used).  Attention's error as in test_gpu_attention: max-abs 2e-3 (for
 results of about 1) and relative L2 1e-3."""
 
 import numpy as np
