@@ -490,7 +490,8 @@ int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* pages, int6
  * of exact products; one that is NaN counts as infinite.
  * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages.
  * workspace: tp_select_workspace_bytes(...) bytes, 256-byte aligned, with the counter area of tp_decode_attention's
- * (zero before and after a call), so that one workspace serves both.
+ * (zero before and after a call), so that one workspace serves both.  Of that area the first 64 KiB are used, whatever
+ * the rows: more than 16,384 (batch, kv head) rows take a launch for each 16,384.
  */
 int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int32_t hkv, const void* bounds,
                         int64_t bounds_capacity, int32_t n_pages, int32_t first, int32_t last, int32_t count,

@@ -157,9 +157,10 @@ struct SelectArgs {
   const uint16_t* q;       // [units][g][128]
   const uint16_t* bounds;  // [units][capacity][2][128]
   uint64_t* keys;          // [units][count]
-  uint32_t* tickets;       // [units], 0 before and after
+  uint32_t* tickets;       // one of each row of the launch, 0 before and after
   int32_t* selected;       // [units][first + take + last]
   int64_t capacity;
+  int32_t first_unit;
   int32_t g, first, last, count, take, n_pages;  // scored: pages [first, first + count), of which `take` are selected
   uint32_t flip;                                 // negative scales: the queries' signs turned
 };
@@ -168,6 +169,9 @@ constexpr int kSelectThreads = 512;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kScorePages = kSelectThreads / 8;
 constexpr int kScoreHeads = 16;
+// Rows of a launch: as many as the counter area of the smallest workspace has tickets for.  What lies behind it is other
+// calls' keys and records, so a row's ticket never does.
+constexpr int64_t kTicketRows = 65536 / sizeof(uint32_t);
 
 // A score as a whole number of the same order.
 __device__ __forceinline__ uint64_t score_key(double s) {
@@ -265,7 +269,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
   __shared__ int32_t found_rest, found_all, is_last;
   __shared__ int32_t counts[2][PER ? PER : 2][kSelectWaves];  // pages above the prefix, and equal to it
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t unit = blockIdx.y;
+  const int64_t unit = a.first_unit + (int64_t)blockIdx.y;
+  uint32_t* ticket = a.tickets + blockIdx.y;
   uint64_t* keys = a.keys + unit * a.count;
   int32_t* out = a.selected + unit * (a.first + a.take + a.last);
   if (a.take > 0 && a.take < a.count) {
@@ -275,10 +280,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages_kernel(SelectArgs
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores are where every XCD sees them
     __syncthreads();
     if (tid == 0)
-      is_last = __hip_atomic_fetch_add(a.tickets + unit, 1u, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
+      is_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
     __syncthreads();
     if (!is_last) return;
-    if (tid == 0) __hip_atomic_store(a.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (tid < 256) hist[tid] = 0;
   for (int i = tid; i < a.first; i += kSelectThreads) out[i] = i;
@@ -503,17 +508,23 @@ extern "C" int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int
   a.n_pages = n_pages;
   a.flip = scale < 0.0f ? 0x8000u : 0u;
   const bool scored = a.take > 0 && a.take < a.count;
-  const dim3 grid(scored ? (unsigned)((a.count + kScorePages - 1) / kScorePages) : 1u, (unsigned)(batch * hkv));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.count <= kSelectThreads)
-    hipLaunchKernelGGL(select_pages_kernel<1>, grid, dim3(kSelectThreads), 0, s, a);
-  else if (a.count <= 4 * kSelectThreads)
-    hipLaunchKernelGGL(select_pages_kernel<4>, grid, dim3(kSelectThreads), 0, s, a);
-  else if (a.count <= 8 * kSelectThreads)
-    hipLaunchKernelGGL(select_pages_kernel<8>, grid, dim3(kSelectThreads), 0, s, a);
-  else if (a.count <= 16 * kSelectThreads)
-    hipLaunchKernelGGL(select_pages_kernel<16>, grid, dim3(kSelectThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL(select_pages_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
-  return launch_status("tp_select_pages");
+  int32_t st = TP_OK;
+  for (int64_t unit = 0; unit < batch * hkv && st == TP_OK; unit += kTicketRows) {
+    a.first_unit = (int32_t)unit;
+    const dim3 grid(scored ? (unsigned)((a.count + kScorePages - 1) / kScorePages) : 1u,
+                    (unsigned)std::min(kTicketRows, batch * hkv - unit));
+    if (a.count <= kSelectThreads)
+      hipLaunchKernelGGL(select_pages_kernel<1>, grid, dim3(kSelectThreads), 0, s, a);
+    else if (a.count <= 4 * kSelectThreads)
+      hipLaunchKernelGGL(select_pages_kernel<4>, grid, dim3(kSelectThreads), 0, s, a);
+    else if (a.count <= 8 * kSelectThreads)
+      hipLaunchKernelGGL(select_pages_kernel<8>, grid, dim3(kSelectThreads), 0, s, a);
+    else if (a.count <= 16 * kSelectThreads)
+      hipLaunchKernelGGL(select_pages_kernel<16>, grid, dim3(kSelectThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL(select_pages_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
+    st = launch_status("tp_select_pages");
+  }
+  return st;
 }
