@@ -146,7 +146,9 @@ int32_t tp_fused_qk(const void* q, int64_t batch, int32_t hq, int32_t hkv,
  *   reference's mask does).
  * pages_per_split: pages per workgroup (0 = library default); the grid is
  *   (hkv, batch x ceil(hq / hkv / 16), ceil(n_pages / pages_per_split))
- *   workgroups, and its second and third sizes must not exceed 65535.
+ *   workgroups, and its second and third sizes must not exceed 65535.  More than
+ *   16384 units (batch x hkv x ceil(hq / hkv / 16)) take all pages in one workgroup
+ *   each, whatever is asked for.
  * workspace: device memory of at least tp_decode_workspace_bytes(...) bytes.
  *   Its counter area (the first tp_decode_counter_bytes(batch, hq, hkv) bytes)
  *   must be zero before the first call; every call leaves it zero again.  One
@@ -212,8 +214,9 @@ size_t tp_decode_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t
 
 /* Size of the zero-initialised counter area at the start of the workspace:
  * 64 KiB for up to 16384 units (batch x hkv x ceil(hq / hkv / 16)), 4 bytes
- * per unit beyond.  Up to that size it is the same for every shape, so one
- * workspace, zeroed once, serves calls of any shape. */
+ * per unit beyond, of which the first 64 KiB are used.  No shape's counters lie
+ * where another's records do, so one workspace, zeroed once, serves calls of any
+ * shape. */
 size_t tp_decode_counter_bytes(int64_t batch, int32_t hq, int32_t hkv);
 
 /* Host-side bounds check of the decode kernels (no GPU work, no counterpart in

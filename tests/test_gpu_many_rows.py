@@ -9,7 +9,7 @@ from common import PAGE
 from test_gpu_select import attended, bridge_call, chosen64, close, queries, scores64
 from test_gpu_tree import filled
 from turbopolar_amd import _lib
-from turbopolar_amd.kernels import fp16_scale
+from turbopolar_amd.kernels import PageSet, decode_attention, fp16_scale
 
 pytestmark = pytest.mark.gpu
 AREA = 65536 // 4  # words of the counter area
@@ -102,3 +102,24 @@ def test_any_number_of_rows(device):
         want = scores64(q, bounds)[0].argmax(-1)[..., None]
         for out in got:
             assert np.array_equal(out.cpu().numpy(), want), rows
+
+
+def test_decode_of_many_rows_in_splits(device):
+    """Splits asked for where one workgroup a row is the default."""
+    small = filled(device, "default", 3, 8, 4, PAGE * 6, seed=4)
+    q = queries(device, 3, 8, 2)
+    scale = fp16_scale(small.config.attention_scale)
+    result = attended(q, small, np.broadcast_to(np.arange(6), (3, 4, 6)), scale)
+    step = split_step(device)
+    big, at = repeated(small, 4200)
+    block, values, *_ = big.runtime.get_fused_attention_inputs()
+    pages, many = PageSet(block, values), q[at].contiguous()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        outs = []
+        for splits in (1, 2, 1):
+            outs.append(decode_attention(many, pages, None, None, PAGE * 6, scale, pages_per_split=splits))
+            step()
+    torch.cuda.synchronize()
+    for out in outs:
+        close(out, result[at], "decode")

@@ -1293,7 +1293,8 @@ constexpr int kRedStride = 132;  // padded LDS row of one head's 128 accumulator
 // shared by calls of different shapes never finds records where counters
 // belong.  Counters sit 256 bytes apart while the units fit (the tickets of all
 // units arrive within a few microseconds, and one shared cache line serialises
-// them), closer beyond 256 units; beyond 16384 units the area grows.
+// them), closer beyond 256 units; beyond 16384 units nothing is split
+// (pages_per_split_of), so no counter lies behind the area.
 constexpr size_t kCounterArea = 65536;
 static inline int32_t counter_stride_of(int64_t units) {
   int32_t w = 64;
@@ -2170,6 +2171,14 @@ static int32_t n_splits_of(int32_t n_pages, int32_t pps) {
   return n_pages <= 0 ? 1 : (n_pages + pps - 1) / pps;
 }
 
+// The pages a workgroup takes where `asked` for (0: the default).  More units than the counter area has words take one
+// split: their counters would lie where other calls' records do, and so many units fill the GPU many times over.
+static int32_t pages_per_split_of(int64_t batch, int32_t hq, int32_t hkv, int32_t n_pages, int32_t asked) {
+  const bool shape = batch > 0 && hq > 0 && hkv > 0;  // a bad one is refused later
+  if (shape && (size_t)batch * hkv * head_blocks_of(hq, hkv) * sizeof(uint32_t) > kCounterArea) return std::max(n_pages, 1);
+  return asked > 0 ? asked : tp_default_pages_per_split(batch, hq, hkv, n_pages);
+}
+
 // Two-tier combine: above kTierMinSplits splits per unit, the splits form
 // groups of kTierSplits whose last workgroup combines the group, and the last
 // group combines the groups, so no workgroup folds more than max(kTierSplits,
@@ -2305,7 +2314,7 @@ size_t tp_decode_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv, int32_t
                                  int32_t tail_len, int32_t pages_per_split) {
   (void)tail_len;
   if (batch < 1 || hq < 1 || hkv < 1) return 0;
-  if (pages_per_split <= 0) pages_per_split = tp_default_pages_per_split(batch, hq, hkv, n_pages);
+  pages_per_split = pages_per_split_of(batch, hq, hkv, n_pages, pages_per_split);
   const size_t units = (size_t)batch * hkv * head_blocks_of(hq, hkv);
   const size_t splits = (size_t)n_splits_of(n_pages, pages_per_split);
   const size_t groups = (size_t)tiers_of((int64_t)units, (int32_t)splits).groups;
@@ -2595,7 +2604,7 @@ static int32_t decode_attention_impl(const void* q, int64_t batch, int32_t hq, i
     return TP_ERR_INVALID;
   }
   if (actual_seq_len > total) actual_seq_len = total;
-  if (pages_per_split <= 0) pages_per_split = tp_default_pages_per_split(batch, hq, hkv, n_pages);
+  pages_per_split = pages_per_split_of(batch, hq, hkv, n_pages, pages_per_split);
   const int32_t n_splits = n_splits_of(n_pages, pages_per_split);
   // The grid is (hkv, batch * head_blocks, n_splits); y and z are at most 65535.
   const int64_t n_rows = (int64_t)batch * a.head_blocks;
@@ -2836,8 +2845,7 @@ extern "C" unsigned long long tp_selftest_decode_bounds(const tp_bounds_case* c,
   const int n_pages = c->n_pages;
   const int64_t cap = c->capacity;
   const bool int8r = c->layout.int8_radii != 0;
-  const int pps = c->pages_per_split > 0 ? c->pages_per_split
-                                         : tp_default_pages_per_split(c->batch, c->hq, c->hkv, n_pages);
+  const int pps = pages_per_split_of(c->batch, c->hq, c->hkv, n_pages, c->pages_per_split);
   const int S = n_splits_of(n_pages, pps);
   const int64_t units = BH * head_blocks;
   const int64_t total = (int64_t)n_pages * kPageTokens + c->tail_len;
@@ -3236,7 +3244,7 @@ extern "C" int32_t tp_decode_attention_noalloc(const void* q, int64_t batch, int
                                                int32_t tail_len, int64_t tail_stride, int64_t actual_seq_len,
                                                float scale, int32_t pages_per_split, void* out, void* stream) {
   clear_error();
-  if (pages_per_split <= 0) pages_per_split = tp_default_pages_per_split(batch, hq, hkv, n_pages);
+  pages_per_split = pages_per_split_of(batch, hq, hkv, n_pages, pages_per_split);
   const bool split = n_pages > 0 && n_splits_of(n_pages, pages_per_split) > 1;
   void* ws = nullptr;
   size_t ws_bytes = 0;
