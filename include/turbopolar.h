@@ -491,7 +491,7 @@ int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* pages, int6
  * larger product with q.  selected: int32 [batch][hkv][count], ascending: the first `first` and the last `last` of
  * the n_pages pages and those of the others with the largest scores, ties to the lower index.  Scores are fp64 sums
  * of exact products; one that is NaN counts as infinite.
- * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages.
+ * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages < 2^28.
  * workspace: tp_select_workspace_bytes(...) bytes, 256-byte aligned, with the counter area of tp_decode_attention's
  * (zero before and after a call), so that one workspace serves both.  Of that area the first 64 KiB are used, whatever
  * the rows: more than 16,384 (batch, kv head) rows take a launch for each 16,384.

@@ -56,3 +56,17 @@ def test_far_rotated_tokens(device):
     for a, b in ((0, 40), (2 ** 18 - 3, 2 ** 18 + 3), (2 ** 19 - 20, T)):
         want = rotate_tokens(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], cos[a:b], sin[a:b])
         assert all(torch.equal(x[:, :, a:b], y) for x, y in zip(got, want))
+
+
+def test_more_rotated_tokens_than_a_grid_holds(device):
+    """2^24 tokens and more, a workgroup each, every row of the batch the same one in memory."""
+    B, T = 4099, 4097
+    assert B * T > 2 ** 24
+    q, k, v = (torch.randn((1, 1, T, 128), dtype=torch.float16, device=device) for _ in range(3))
+    cos, sin = tables(device, 0, T, 64, False, torch.float32)
+    want = rotate_tokens(q, k, v, cos, sin)
+    got = rotate_tokens(*(t.expand(B, -1, -1, -1) for t in (q, k, v)), cos, sin)
+    for x, y in zip(got, want):
+        assert x.shape[0] == B
+        for b in range(0, B, 512):
+            assert torch.equal(x[b:b + 512], y.expand(min(512, B - b), -1, -1, -1)), b

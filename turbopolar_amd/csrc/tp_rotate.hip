@@ -33,6 +33,7 @@ struct RotateArgs {
   int64_t kv_row, kv_pos;  // tokens between (batch, head) rows of k_out and v_out, and of their first one
   int32_t hq, hkv, columns;
   int64_t tokens;
+  int64_t first;  // token of the launch's first workgroup, rows counted one behind the other
   uint32_t* flag;
   uint32_t epoch;
   int32_t check, reports;
@@ -85,12 +86,13 @@ __device__ __forceinline__ bool any_nonfinite(uint4v w) {
 // accesses past the caches (187 us), runs of neighbouring tokens on one XCD (172 to 177).
 constexpr int kRotThreads = 256;
 constexpr int kRotRows = kRotThreads / 8;
+constexpr int64_t kRotLaunch = 1 << 23;  // tokens of a launch: a grid holds less than 2^32 threads
 
 template <int TYPE, int TABLE, bool INTER>
 __global__ __launch_bounds__(kRotThreads) void rotate_tokens_kernel(RotateArgs a) {
   constexpr bool WIDE = TYPE == kRotF32 || TABLE == kRotF32;
   const int c = threadIdx.x & 7, slot = threadIdx.x >> 3;
-  const int64_t b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens;
+  const int64_t index = a.first + blockIdx.x, b = index / a.tokens, t = index - b * a.tokens;
   const int lo = INTER ? 16 * c : 8 * c, hi = INTER ? 16 * c + 8 : kHeadDim / 2 + 8 * c;
   float cl[8], ch[8], sl[8], sh[8];
   const int64_t row = b * a.c_b + t * a.c_t;
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(kRotThreads) void rotate_tokens_kernel(RotateArgs a
   }
   if (!a.check) return;
   // Each workgroup reports its verdict on a line of its own once its reads and writes are issued, and the host
-  // polls them; or, where there are more than lines, only a non-finite value.
+  // polls them; or, where there are more than lines or than a launch's, only a non-finite value.
   const bool any_bad = __syncthreads_or(bad);
   if (threadIdx.x != 0) return;
   if (a.reports)
@@ -262,21 +264,24 @@ extern "C" int32_t tp_rotate_tokens(const void* q, const void* k, const void* v,
   a.hq = hq, a.hkv = hkv, a.columns = columns, a.tokens = tokens;
   a.flag = flag, a.epoch = epoch, a.check = check;
   const int64_t groups = batch * tokens;
-  a.reports = groups <= flag_words / kReportStride;
-  const dim3 grid((unsigned)groups);
+  a.reports = groups <= std::min(flag_words / kReportStride, kRotLaunch);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool inter = interleaved != 0;
-  if (dtype == kRotF32)
-    launch_rotate<kRotF32, kRotF32>(a, inter, grid, s);
-  else if (dtype == kRotF16 && table_dtype == kRotF16)
-    launch_rotate<kRotF16, kRotF16>(a, inter, grid, s);
-  else if (dtype == kRotF16)
-    launch_rotate<kRotF16, kRotF32>(a, inter, grid, s);
-  else if (table_dtype == kRotBF16)
-    launch_rotate<kRotBF16, kRotBF16>(a, inter, grid, s);
-  else
-    launch_rotate<kRotBF16, kRotF32>(a, inter, grid, s);
-  const int32_t st = launch_status("tp_rotate_tokens");
+  int32_t st = TP_OK;
+  for (; a.first < groups && st == TP_OK; a.first += kRotLaunch) {
+    const dim3 grid((unsigned)std::min(kRotLaunch, groups - a.first));
+    if (dtype == kRotF32)
+      launch_rotate<kRotF32, kRotF32>(a, inter, grid, s);
+    else if (dtype == kRotF16 && table_dtype == kRotF16)
+      launch_rotate<kRotF16, kRotF16>(a, inter, grid, s);
+    else if (dtype == kRotF16)
+      launch_rotate<kRotF16, kRotF32>(a, inter, grid, s);
+    else if (table_dtype == kRotBF16)
+      launch_rotate<kRotBF16, kRotBF16>(a, inter, grid, s);
+    else
+      launch_rotate<kRotBF16, kRotF32>(a, inter, grid, s);
+    st = launch_status("tp_rotate_tokens");
+  }
   if (st != TP_OK || !check) return st;
   return a.reports ? wait_reports(flag, epoch, groups, s) : wait_verdict(flag, epoch, s, false, "tp_rotate_tokens");
 }

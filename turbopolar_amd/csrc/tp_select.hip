@@ -476,8 +476,8 @@ extern "C" int32_t tp_select_pages(const void* q, int64_t batch, int32_t hq, int
               (long long)batch, hq, hkv);
     return TP_ERR_INVALID;
   }
-  if (n_pages < 1 || bounds_capacity < n_pages || n_pages > INT32_MAX / 2) {
-    set_error("n_pages=%d is not within the bounds' capacity", n_pages);
+  if (n_pages < 1 || bounds_capacity < n_pages || n_pages > INT32_MAX / 8) {  // 8 threads a page, less than 2^32 a launch
+    set_error("n_pages=%d is not within the bounds' capacity, or past 2^28", n_pages);
     return TP_ERR_INVALID;
   }
   if (first < 0 || last < 0 || count < 1 || count > n_pages || first > count || last > count - first) {

@@ -405,8 +405,9 @@ extern "C" int32_t tp_shared_attention(const void* q, void* out, int64_t batch, 
     x.div_units = make_fastdiv((uint32_t)units[i]), x.div_blocks = make_fastdiv((uint32_t)p.row_blocks[i]);
   }
   a.part[1].first_record = (int32_t)p.records[0];
-  if (groups[0] + groups[1] > INT32_MAX) {
-    set_error("too many workgroups for one launch");
+  const int rw = std::max(p.row_waves[0], p.row_waves[1]);
+  if ((groups[0] + groups[1]) * (rw == 8 ? 512 : 128 * rw) > (int64_t)UINT32_MAX) {
+    set_error("too many workgroups for one launch, whose threads are less than 2^32");
     return TP_ERR_INVALID;
   }
   a.q = static_cast<const uint16_t*>(q);
