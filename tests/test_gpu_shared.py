@@ -256,3 +256,28 @@ def test_a_large_batch(device):
     case = ("default", 700, 8, 2, 70, 3)
     cache, q = made(device, *case, seed=8)
     check(cache.attention(q, 0.1), q, cache, 0.1, f"{case}")
+
+
+def test_compacted_prefixes_are_refused(device):
+    """Pages in another order, or others, are another prefix of the same length; the same ones in place are not."""
+    cache, q = made(device, "default", 2, 8, 2, 64 * 3 + 9, 5)
+    want = cache.attention(q, 0.1)
+    cache.prefix.keep_pages([0, 1, 2])
+    assert torch.equal(cache.attention(q, 0.1), want)
+    cache.prefix.keep_pages(torch.tensor([0, 2, 1]))
+    assert cache.prefix.offset == cache.prefix_tokens
+    with pytest.raises(ValueError, match="tokens are others"):
+        cache.attention(q, 0.1)
+    # What an append that is refused later leaves is what was there.
+    cache, q = made(device, "default", 2, 8, 2, 64 * 3 + 9, 5)
+    k, v = (torch.from_numpy(t).to(device) for t in gen_kv(3, 1, 2, 1))
+    bad = torch.full_like(k, float("nan"))
+    cache.prefix.runtime.append(bad, v, defer_check=True)
+    with pytest.raises(ValueError, match="finite"):
+        cache.prefix.runtime.resolve_deferred_check()
+    assert torch.equal(cache.attention(q, 0.1), want)
+    # Cut inside of its pages and filled again, and only a few of its pages shared.
+    cache.prefix.truncate(64 * 2 + 3)
+    cache.prefix.runtime.append(*(t.expand(-1, -1, 70, -1) for t in (k, v)))
+    with pytest.raises(ValueError, match="tokens are others"):
+        cache.attention(q, 0.1)

@@ -256,6 +256,47 @@ def test_shared_prefix_bookkeeping():
         SharedPrefixCache(small()).attention(q, 0.1)
 
 
+def test_a_prefix_of_other_tokens_is_refused():
+    """Cut below its length and filled up to it again, or emptied: the length alone does not tell."""
+    q = torch.zeros(2, 4, 1, 128).half()
+
+    def shared_cache():
+        prefix = small()
+        prefix.runtime.append(*kv(1, 20))
+        return prefix, SharedPrefixCache(prefix)
+
+    prefix, cache = shared_cache()
+    prefix.truncate(12)
+    prefix.runtime.append(*kv(1, 8, 3))
+    assert prefix.offset == 20
+    for call in (lambda: cache.attention(q, 0.1), cache.fork, lambda: cache.decode_attention(q, *kv(2, 1), 0.1)):
+        with pytest.raises(ValueError, match="tokens are others"):
+            call()
+    again = SharedPrefixCache(prefix)  # of the tokens held now
+    with pytest.raises(ValueError, match="HIP device"):
+        again.attention(q, 0.1)
+    prefix.runtime.append(*kv(1, 9, 4))  # longer, and back: the same tokens
+    prefix.truncate(25)
+    prefix.truncate(20)
+    assert again.fork().offset == 20
+    prefix.select_rows([0])
+    assert again.fork().offset == 20
+    with pytest.raises(ValueError, match="tokens are others"):
+        cache.fork()
+    prefix.runtime.reset()
+    prefix.runtime.append(*kv(1, 20))
+    with pytest.raises(ValueError, match="tokens are others"):
+        again.fork()
+    prefix, cache = shared_cache()
+    branch = prefix.fork()
+    branch.truncate(3)
+    assert cache.fork().offset == 20  # a branch's cuts are its own
+    prefix.runtime = branch.runtime
+    branch.runtime.append(*kv(1, 17))
+    with pytest.raises(ValueError, match="tokens are others"):
+        cache.fork()
+
+
 def test_selected_attention_host_refusals():
     cache = small()
     q = torch.zeros(1, 4, 1, 128).half()

@@ -113,6 +113,7 @@ class TurboPolarKVCacheRuntime:
         # Appends whose non-finite verdict is deferred (append(..., defer_check=True)):
         # (epoch, state before the append), oldest first.
         self._pending: list = []
+        self._cuts: Optional[list] = None  # the lengths that cuts left, recorded from the first mark() on
 
         self._initialized = False
         self._batch_size: Optional[int] = None
@@ -476,6 +477,7 @@ class TurboPolarKVCacheRuntime:
         self._fused_views = None
         self._bounds_pages = min(self._bounds_pages, self.k_storage.block_count)
         self._pending.clear()
+        self._cut_to(self.actual_seq_len)
 
     def _stage(self, k, v, begin: int, n: int, dst: int, check: int) -> None:
         B, H, T, _ = k.shape
@@ -783,6 +785,22 @@ class TurboPolarKVCacheRuntime:
             self._bounds_pages = min(self._bounds_pages, pages)
         self._tail_len = left
         self.actual_seq_len = tokens
+        self._cut_to(tokens)
+
+    def mark(self) -> int:
+        """This moment, for ``kept_since``."""
+        if self._cuts is None:
+            self._cuts = []
+        return len(self._cuts)
+
+    def kept_since(self, mark: int) -> int:
+        """The first tokens that are still those of a ``mark``, or of later appends: fewer than were there then if the
+        cache was cut below that, even where others have taken their places since."""
+        return min(self._cuts[mark:], default=self.actual_seq_len)
+
+    def _cut_to(self, tokens: int) -> None:
+        if self._cuts is not None:
+            self._cuts.append(tokens)
 
     def _decode_to_tail(self, source: "TurboPolarKVCacheRuntime", page: int) -> None:
         """``source``'s stored page decoded into the dense tail's buffers."""
@@ -849,7 +867,7 @@ class TurboPolarKVCacheRuntime:
         vars(other).update(vars(self))
         # The encoder's layout follows its attributes, which may have been set: a copy of it.
         other.polar_encoder = copy.copy(self.polar_encoder)
-        other._flag, other._epoch = None, 0
+        other._flag, other._epoch, other._cuts = None, 0, None
         other.reset()
         return other
 
@@ -885,20 +903,32 @@ class TurboPolarKVCacheRuntime:
         read, spent = self.bytes_read, self.compression_time_ns
         flag = self._flag if other._batch_size == self._batch_size else None
         vars(self).update({**vars(other), "bytes_read": read, "compression_time_ns": spent, "_epoch": self._epoch,
-                           "polar_encoder": self.polar_encoder, "_flag": flag if flag is not None else other._flag})
+                           "polar_encoder": self.polar_encoder, "_flag": flag if flag is not None else other._flag,
+                           "_cuts": self._cuts})
 
     def select_rows(self, rows: Sequence[int]) -> None:
         """Makes batch row i what row ``rows[i]`` was (beams re-ordered, or a batch that grows or
         shrinks)."""
+        alone = self._batch_size in (None, 1)  # whose rows are all the one that there was
         self._adopt(self.fork(rows=rows))
+        if not alone:
+            self._cut_to(0)
 
     def keep_pages(self, pages: Sequence[int]) -> None:
         """Compacts the cache to the stored pages ``pages``, in that order, and the tail; the
         others' memory is freed.  ``actual_seq_len`` becomes the tokens held."""
+        if self._pending:
+            self.resolve_deferred_check()
+        pages = _indices(pages, self.k_storage.block_count, "pages", "stored pages")
+        same = next((i for i, page in enumerate(pages) if page != i), len(pages))
+        whole = same == len(pages) == self.k_storage.block_count
         self._adopt(self.fork(pages=pages))
+        if not whole:
+            self._cut_to(same * PAGE)
 
     def reset(self) -> None:
         """turbo_polar_cache.py:379-395."""
+        self._cut_to(0)
         self.k_storage = PolarKBlockStorage()
         self.v_storage = QuantVBlockStorage()
         self.qjl_blocks = []

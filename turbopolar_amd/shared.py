@@ -24,8 +24,9 @@ def _layout_of(cache: TurboPolarFastCache) -> tuple:
 
 class SharedPrefixCache:
     """``prefix``: the cache of the common tokens, of batch 1; it is not copied and must not change while branches
-    read it.  ``own``: the sequences' own tokens, a cache of the same layout and heads (a new one by default, whose
-    batch the first append fixes)."""
+    read it: where its length is another, or others took the place of tokens that were cut from it, calls raise.  ``own``:
+    the sequences' own tokens, a cache of the same layout and heads (a new one by default, whose batch the first append
+    fixes)."""
 
     def __init__(self, prefix: TurboPolarFastCache, own: Optional[TurboPolarFastCache] = None):
         for name, cache in (("prefix", prefix), ("own", own)):
@@ -41,6 +42,7 @@ class SharedPrefixCache:
             raise ValueError("the prefix and the sequences' own cache must have one layout and number of KV heads")
         self.prefix, self.own, self.config = prefix, own, prefix.config
         self.prefix_tokens = prefix.offset
+        self._shared = prefix.runtime, prefix.runtime.mark()
 
     @property
     def offset(self) -> int:
@@ -80,6 +82,9 @@ class SharedPrefixCache:
         if self.prefix.offset != self.prefix_tokens:
             raise ValueError(f"the prefix held {self.prefix_tokens} tokens when it was shared and holds "
                              f"{self.prefix.offset} now")
+        runtime, mark = self._shared
+        if self.prefix.runtime is not runtime or runtime.kept_since(mark) < self.prefix_tokens:
+            raise ValueError("the prefix was cut and filled again after it was shared: its tokens are others")
 
     def attention(self, q: torch.Tensor, scale: float) -> torch.Tensor:
         """One decode step's attention: the queries ``q`` ``[B, H_q, 1, 128]`` over the prefix and each sequence's own
