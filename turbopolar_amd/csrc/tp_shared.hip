@@ -39,7 +39,7 @@ struct SharedArgs {
   const uint16_t* q;
   uint16_t* out;
   int64_t q_b, q_h, out_b, out_h;
-  int32_t hkv, g, batch;
+  int32_t hkv, g;
   FastDiv div_hkv, div_g;
   SharedPart part[2];  // the prefix, the rows' own
   int32_t prefix_groups;  // workgroups over the prefix, the launch's first
@@ -413,7 +413,7 @@ extern "C" int32_t tp_shared_attention(const void* q, void* out, int64_t batch, 
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
   a.q_b = strides[0], a.q_h = strides[1], a.out_b = strides[2], a.out_h = strides[3];
-  a.hkv = hkv, a.g = g, a.batch = (int32_t)batch;
+  a.hkv = hkv, a.g = g;
   a.div_hkv = make_fastdiv((uint32_t)hkv), a.div_g = make_fastdiv((uint32_t)g);
   a.records = (int32_t)(p.records[0] + p.records[1]);
   a.c = std::max(fabsf(scale) * kLog2e, 1.17549435e-38f);  // 2^-126 stands for 0: see tp_prompt_attention
