@@ -487,10 +487,12 @@ int32_t tp_page_bounds(const tp_page_layout* layout, const tp_pages* pages, int6
 
 /*
  * The pages that a query is likely to need.  A page's score for (batch, kv head) is the largest of
- * sum_d max(q_d lo_d, q_d hi_d) over the query heads of the group (of -q where scale < 0): no key of the page has a
- * larger product with q.  selected: int32 [batch][hkv][count], ascending: the first `first` and the last `last` of
- * the n_pages pages and those of the others with the largest scores, ties to the lower index.  Scores are fp64 sums
- * of exact products; one that is NaN counts as infinite.
+ * sum_d max(q_d lo_d, q_d hi_d) over the query heads of the group (of -q where scale < 0): no key of the page, rounded
+ * as the bounds' are, has a larger product with q; one that tp_selected_attention multiplies is rounded less, and its
+ * product may exceed the score by half a step of fp16 of each component.  selected: int32 [batch][hkv][count],
+ * ascending: the first `first` and the last `last` of the n_pages pages and those of the others with the largest scores,
+ * ties to the lower index.  Scores are fp64 sums of exact products; one that is NaN counts as infinite, and a NaN beside
+ * a number in a maximum (0 times one infinite bound) as that number.
  * q: fp16 [batch][hq][128]; bounds as tp_page_bounds writes them; first + last <= count <= n_pages < 2^28.
  * workspace: tp_select_workspace_bytes(...) bytes, 256-byte aligned, with the counter area of tp_decode_attention's
  * (zero before and after a call), so that one workspace serves both.  Of that area the first 64 KiB are used, whatever

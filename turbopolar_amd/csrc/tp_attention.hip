@@ -244,12 +244,14 @@ __device__ __forceinline__ void build_lut_rest(LutRest& lut, const AttnArgs& a, 
 }
 
 // r (cos, sin) as a rounded fp16 pair and the fp16 pair of what that rounding, the table's and the radius's
-// left (r = r16 + r_rest): the products' errors come out of the FMA exactly, so that the two parts are off by
-// 2^-21 of the key.  tp_selected_attention takes keys and values so, an extra matrix product of each: few pages are
-// read, so that the scores' errors are most of the result's (relative L2 8.4e-4 to 9.6e-4 of it with one part, 2.8e-4 to
-// 3.0e-4 with two), and most of its time is a launch's and the first loads': 64 pages of one sequence of 32/8 heads
-// 10.9 us against 9.3, 128 of the fast layout 10.5 against 8.8, 48 of each of 8 sequences (53 MB) 18.0 against 14.7.  An infinite radius leaves infinity less infinity: the rest is bounded, its sum with the
-// rounded part then is what that is (half a step of the largest fp16 number is 16).
+// left (r = r16 + r_rest).  The two parts are off by 2^-21 of the key, or, where the rests are below fp16's normal
+// numbers (of keys below 2^-4, of small cosines), by 2^-25 (4 + r): three roundings, the table's and the radius's.
+// tp_selected_attention takes keys and values so, an extra matrix product of each: few pages are read, so that the
+// scores' errors are most of the result's (relative L2 8.4e-4 to 9.6e-4 of it with one part, 2.5e-4 to 3.0e-4 with two),
+// and most of its time is a launch's and the first loads': 64 pages of one sequence of 32/8 heads 10.9 us against 9.3,
+// 128 of the fast layout 10.5 against 8.8, 48 of each of 8 sequences (53 MB) 18.0 against 14.7.  An infinite radius
+// leaves infinity less infinity: the rest is bounded, its sum with the rounded part then is what that is (half a step
+// of the largest fp16 number is 16).
 __device__ __forceinline__ uint32_t split_pair(half2v r, half2v r_rest, uint32_t cs, uint32_t cs_rest, uint32_t& rest) {
   const half2v c = __builtin_bit_cast(half2v, cs), most = {(f16)32.0f, (f16)32.0f};
   const half2v k = r * c;

@@ -2,13 +2,15 @@
 //
 // The bounds of a page are the smallest and the largest of each key component over its 64 tokens,
 // lo_d <= k_d <= hi_d (of the keys r (cos a, sin a), fp32 products rounded to fp16; the page decoder rounds
-// them in one step, which differs in the last bit where the fp32 product is a tie).  So no key of the page has a larger
+// them in one step, which differs in the last bit where the fp32 product is a tie).  So none of these keys has a larger
 // product with q than
 //
-//   u(q, page) = sum_d max(q_d lo_d, q_d hi_d),
+//   u(q, page) = sum_d max(q_d lo_d, q_d hi_d)
 //
-// and a page's score is the largest u over the query heads of its group.  Selected are the first and the last
-// pages asked for and those of the others with the largest scores, ties to the lower index, in ascending order.
+// (those that tp_selected_attention multiplies are not rounded so far, and their products may exceed it by half a step of
+// fp16 of each component), and a page's score is the largest u over the query heads of its group.  Selected are the
+// first and the last pages asked for and those of the others with the largest scores, ties to the lower index, in
+// ascending order.
 //
 // Scores are sums of exact products (fp16 by fp16 fits fp32) in fp64, so that two pages change places only if
 // their scores differ by less than 2^-46 of their terms, whatever the order of the sum: which pages are attended
@@ -213,7 +215,7 @@ __device__ __forceinline__ uint64_t page_key(const SelectArgs& a, int64_t unit, 
         const float x = qs[h][16 * c + j];
         const uint32_t lo = (w[j >> 3][(j >> 1) & 3] >> (16 * (j & 1))) & 0xffffu;
         const uint32_t hi = (w[2 + (j >> 3)][(j >> 1) & 3] >> (16 * (j & 1))) & 0xffffu;
-        s += (double)fmaxf(x * h2f((uint16_t)lo), x * h2f((uint16_t)hi));
+        s += (double)fmaxf(x * h2f((uint16_t)lo), x * h2f((uint16_t)hi));  // of 0 times infinity, NaN, and a number: that
       }
       s += moved<0xb1>(s);   // quad_perm 1 0 3 2
       s += moved<0x4e>(s);   // quad_perm 2 3 0 1
