@@ -442,5 +442,27 @@ def test_float32_caches(device):
     close(cache.selected_attention(q[:, :, None], scale, 6), attended(q, cache, want, fp16_scale(scale)), "float32")
 
 
+@pytest.mark.parametrize("layout", sorted(LAYOUTS))
+@pytest.mark.parametrize("hq", [8, 40])
+def test_values_past_the_largest_fp16_number(device, layout, hq):
+    """A value of 65504 is stored as 127 times 516, which fp16 holds as infinity: attended as what it is decoded to,
+    here as by the decode step's own kernel."""
+    k, v = gen_kv(5, 1, 2, PAGE * 8)
+    v[0, 0, 70, 3], v[0, 1, 200, 90] = 65504, -65504
+    cache = TurboPolarFastCache(filled(device, layout, 1, hq, 2, 0).config)
+    cache.runtime.append(torch.from_numpy(k).to(device), torch.from_numpy(v).to(device))
+    _, v64 = pages64(cache.runtime)
+    assert np.isposinf(v64[0, 0, 70, 3]) and np.isneginf(v64[0, 1, 200, 90])
+    q = queries(device, 1, hq, 4)
+    got, selected = bridge_call(cache, q, cache.runtime.page_bounds(), 7, 5, 1)
+    want = attended(q, cache, selected.cpu().numpy(), fp16_scale(cache.config.attention_scale))
+    got = got.double().cpu().numpy()
+    assert np.isinf(want).any() and not np.isnan(want).any()
+    finite = np.isfinite(want)
+    assert np.array_equal(got[~finite], want[~finite])
+    # The rest of the dimensions of those tokens' groups are of the coarse scale, and rounded as any other.
+    assert np.all(np.abs(got - want)[finite] <= ATOL + 2.0 ** -11 * np.abs(want[finite]))
+
+
 def test_oracle_layouts_are_all_covered():
     assert {c[0] for c in CASES} == set(LAYOUTS) and oracle is not None

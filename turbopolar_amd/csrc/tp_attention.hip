@@ -948,10 +948,11 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, int64_t slot, int l16,
 // acc[j] += Vhat^T tile j x P, Vhat = f16(code * scale) exactly: codes become
 // fp16 pairs (tokens e, e+1) by SDWA converts, then one packed multiply by the
 // pair's scales.
-// SPLIT: with what that rounding leaves, which the FMA gives exactly, as a second product.
+// SPLIT: with what that rounding leaves, which the FMA gives exactly, as a second product.  keep: all bits, or none for a
+// page with a scale of 512 or more, whose largest codes are infinite in fp16: infinity less infinity is no rest.
 template <int J, bool SPLIT>
 __device__ __forceinline__ void pv_tile(const VRegs& v, int ks, const half2v* sp, const half8v& pb,
-                                        float4v& acc) {
+                                        float4v& acc, [[maybe_unused]] uint32_t keep) {
   uint32_t e[4];
   [[maybe_unused]] uint32_t x[4];
 #pragma unroll
@@ -961,7 +962,7 @@ __device__ __forceinline__ void pv_tile(const VRegs& v, int ks, const half2v* sp
     const uint32_t c = (J < 4) ? i8pair_f16<J & 3>(wa.x, wb.x) : i8pair_f16<J & 3>(wa.y, wb.y);
     const half2v value = __builtin_bit_cast(half2v, c) * sp[q];
     e[q] = pack_h2(value);
-    if constexpr (SPLIT) x[q] = pack_h2(__builtin_elementwise_fma(__builtin_bit_cast(half2v, c), sp[q], -value));
+    if constexpr (SPLIT) x[q] = keep & pack_h2(__builtin_elementwise_fma(__builtin_bit_cast(half2v, c), sp[q], -value));
   }
   if constexpr (SPLIT)
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(x[0], x[1], x[2], x[3]), pb, acc, 0, 0, 0);
@@ -974,6 +975,11 @@ __device__ __forceinline__ void pv_tile(const VRegs& v, int ks, const half2v* sp
 template <bool HR, bool SPLIT = false>
 __device__ __forceinline__ void pv_regs(const VRegs& v, int sbase4, uint32_t ssel, const half8v* pb,
                                         float4v* acc) {
+  uint32_t keep = 0;
+  if constexpr (SPLIT) {
+    const uint32_t from_512 = ((v.sd[0] & (v.sd[0] << 1)) | (v.sd[1] & (v.sd[1] << 1))) & 0x40004000u;
+    keep = __any(from_512 != 0) ? 0u : ~0u;
+  }
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     // Scales of tokens (2q, 2q+1) of this k-step as fp16 pairs: tokens
@@ -988,14 +994,14 @@ __device__ __forceinline__ void pv_regs(const VRegs& v, int sbase4, uint32_t sse
       const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(sbase4 + 8 * t0 + 8, (int)v.sd[ks]);
       sp[q] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(hi, lo, ssel));
     }
-    pv_tile<0, SPLIT>(v, ks, sp, pb[ks], acc[0]);
-    pv_tile<1, SPLIT>(v, ks, sp, pb[ks], acc[1]);
-    pv_tile<2, SPLIT>(v, ks, sp, pb[ks], acc[2]);
-    pv_tile<3, SPLIT>(v, ks, sp, pb[ks], acc[3]);
-    pv_tile<4, SPLIT>(v, ks, sp, pb[ks], acc[4]);
-    pv_tile<5, SPLIT>(v, ks, sp, pb[ks], acc[5]);
-    pv_tile<6, SPLIT>(v, ks, sp, pb[ks], acc[6]);
-    pv_tile<7, SPLIT>(v, ks, sp, pb[ks], acc[7]);
+    pv_tile<0, SPLIT>(v, ks, sp, pb[ks], acc[0], keep);
+    pv_tile<1, SPLIT>(v, ks, sp, pb[ks], acc[1], keep);
+    pv_tile<2, SPLIT>(v, ks, sp, pb[ks], acc[2], keep);
+    pv_tile<3, SPLIT>(v, ks, sp, pb[ks], acc[3], keep);
+    pv_tile<4, SPLIT>(v, ks, sp, pb[ks], acc[4], keep);
+    pv_tile<5, SPLIT>(v, ks, sp, pb[ks], acc[5], keep);
+    pv_tile<6, SPLIT>(v, ks, sp, pb[ks], acc[6], keep);
+    pv_tile<7, SPLIT>(v, ks, sp, pb[ks], acc[7], keep);
   }
 }
 
