@@ -55,10 +55,12 @@ constexpr int kSharedThreads = 64 * RW * TW;
 
 // RW waves of 32 rows each; TW waves share a row block and take a tile's tokens in TW parts (as the
 // drafted-tree kernel's).  Roundings: a key component once, from fp32 angles and radii, a value, a weight, a
-// record and the result once each; sums in 32 bits.  The keys' is most of the result's error (relative L2 6.0e-4 to
-// 6.9e-4 over a long prefix): in two parts it would be 3.5e-4, and the kernel below 49 us long, of 38.7.
+// record and the result once each; sums in 32 bits.  The keys', which makes them the page decoder's, is most of the
+// result's error (relative L2 5.7e-4 to 7.1e-4 over a long prefix): with keys in two parts it was 3.5e-4, and the kernel
+// took 49 us where it took 38.7.
 // A page is decoded in 1.7 us a workgroup on its own CU, under the products of the page before: 32 sequences of 32/8
-// heads, 300 tokens each behind 32,805 (103 MB, 17.4 GFLOP) take 38.7 us and the join of the records 5.3: bound by the
+// heads, 300 tokens each behind 32,805 (103 MB, 17.4 GFLOP) take 40.4 us and the join of the records 5.7 (42.9 in all,
+// pass behind pass): bound by the
 // decode, vector operations and table reads, rather than by the bytes (20 us of a copy's time) or the products (14.5 at
 // a large product's rate).
 template <int KIND, int RW, int TW>
